@@ -257,6 +257,104 @@ int kf_kv_cache_append(const void* k_new, const void* v_new, const float* rope_c
                        const float* rope_sin, void* k_cache, void* v_cache, int start, int B,
                        int Snew, int Hkv, int Smax, int D, int dtype, void* stream);
 
+/* ---- Speculative decoding: several drafted tokens per sequence are scored in
+ * one step.  No counterpart in the reference (its generate decodes one token
+ * per step).  A step is kf_attn_tree in every layer, kf_verify_drafts on the
+ * logits, kf_kv_cache_keep on the caches. */
+
+/* Most nodes (drafted tokens, the last emitted one included) per sequence. */
+#define KF_TREE_MAX_NODES 256
+
+/* Workspace bytes kf_attn_tree needs; max_len bounds lens[b] + N. */
+int kf_attn_tree_workspace_size(int B, int N, int Hq, int Hkv, int D, int max_len, int dtype,
+                                size_t* bytes);
+
+/* Appends N drafted tokens per sequence to a KV cache and attends each to the
+ * cached prefix, itself and its ancestors.
+ *   q_new [B, N, Hq, D], k_new, v_new [B, N, Hkv, D] contiguous, before RoPE
+ *   k_cache, v_cache [B, Hkv, Smax, D] contiguous; on return rows lens[b] + i of
+ *       sequence b hold node i's rotated key and its value (i < counts[b])
+ *   lens  [B] int32 on the device: tokens cached before the step (the prefix)
+ *   parents  int32 on the device: the parent of each node, -1 for a node that
+ *       follows the prefix directly; a parent comes before its children.  Row b
+ *       at parents + b * parents_stride: N for a tree per sequence, 0 for one
+ *       tree for all.  NULL: a chain (node i follows node i - 1)
+ *   counts  [B] int32 on the device, nodes in use per sequence, 0 .. N, or NULL
+ *       for N: the others' rows of out are zero and their cache rows stay
+ *   rope_cos/sin [rope_rows, D/2]: a node at depth d (0 with parent -1) is at
+ *       position lens[b] + d and uses row lens[b] + d - rope_row_offset
+ *   out  [B, N, Hq, D]
+ *   max_len  an upper bound on lens[b] + counts[b] (<= Smax)
+ *   q_norm_weight, k_norm_weight, norm_eps  as for kf_attn_decode
+ * lens is not modified; kf_kv_cache_keep advances it.  N <= KF_TREE_MAX_NODES.
+ * Inf and NaN in rows a node does not see do not reach its output.
+ * lens, parents and counts live on the device, so they cannot be validated
+ * before the launch: a sequence with a count outside 0 .. N, lens[b] +
+ * counts[b] beyond max_len, a parent that does not come before its child, or a
+ * table row outside [0, rope_rows) gets NaN outputs and no cache write. */
+int kf_attn_tree(const void* q_new, const void* k_new, const void* v_new, void* k_cache,
+                 void* v_cache, const int32_t* lens, const int32_t* parents,
+                 int64_t parents_stride, const int32_t* counts, const float* rope_cos,
+                 const float* rope_sin, int64_t rope_row_offset, int64_t rope_rows, void* out,
+                 void* workspace, size_t workspace_bytes, int B, int N, int Smax, int Hq, int Hkv,
+                 int D, int max_len, const float* q_norm_weight, const float* k_norm_weight,
+                 float norm_eps, int dtype, void* stream);
+
+/* Largest vocabulary of kf_verify_drafts. */
+#define KF_VERIFY_MAX_VOCAB 1048576
+
+/* Verifies drafted tokens against the target's distributions with given random
+ * numbers; the emitted tokens (the path's, then next) have the target's
+ * distribution.
+ *   logits  [B, N, V], row (b, i) at b * logits_stride_b + i * logits_stride_n:
+ *       softmax(row / temperature) is the target's distribution of the token
+ *       after node i.  -inf is probability 0 (a filtered token)
+ *   tokens  [B, N] int64, node i's token; node 0 is the last emitted token (its
+ *       token is not read), every other node has a parent 0 <= parent < i
+ *   parents, parents_stride, counts  as for kf_attn_tree, parents[0] = -1
+ *   draft_logits  NULL: the drafts are tried as they are.  Otherwise row i is
+ *       what the draft model drew node i + 1 from (softmax at the same
+ *       temperature), i < N - 1; needs a chain (parents NULL)
+ *   uniforms  [B, N] float32 in [0, 1): entry i > 0 tests node i, entry 0 draws
+ *       next
+ *   temperature  0: a node is accepted if its token is its parent's most likely
+ *       (the lowest of equals), next is the last node's most likely token
+ *   path  [B, N] int32: the accepted nodes in order, node 0 first, -1 behind
+ *   kept  [B] int32: how many they are
+ *   next  [B] int64: the token after the path
+ * From node 0 on, a node's children are tried in index order.  Without
+ * draft_logits a child with token c is accepted if u W < p(c), W the mass its
+ * refused elder siblings leave (a token refused before is refused again); next
+ * is drawn from p without the refused tokens.  With them it is accepted if
+ * u q(c) < p(c), and after a refusal next is drawn from max(p - q, 0).  next is
+ * the smallest v at which the running sum of the weights, in 64 bits, passes
+ * uniforms[b][0] times their total.
+ * counts[b] = 0, a count outside 0 .. N or a parent out of range: kept 0, next
+ * -1.  A row on the path that is no distribution (NaN, +inf, or -inf
+ * throughout) ends the path, and next is -1.  Reads only rows on the path. */
+int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_n,
+                     const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
+                     const int32_t* counts, const void* draft_logits, int64_t draft_stride_b,
+                     int64_t draft_stride_n, const float* uniforms, double temperature,
+                     int32_t* path, int32_t* kept, int64_t* next, int B, int N, int V, int dtype,
+                     void* stream);
+
+/* Moves the accepted path's rows together in n_caches KV caches (the layers of
+ * a model): row lens[b] + path[b][j] to row lens[b] + j, j < kept[b], and writes
+ * lens_out[b] = lens[b] + kept[b].
+ *   k_caches, v_caches  host arrays of n_caches device pointers to caches
+ *       [B, Hkv, Smax, D] contiguous
+ *   lens, lens_out  host arrays of n_caches device pointers to [B] int32;
+ *       lens_out[c] may be lens[c] where no other cache reads it
+ *   path [B, N], kept [B]  what kf_verify_drafts returned
+ * Other rows stay as they are.  A sequence with kept[b] outside 0 .. N, or a
+ * path that does not rise or leaves the nodes or the cache, is left alone
+ * (lens_out[b] = lens[b]). */
+int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t* const* lens,
+                     int32_t* const* lens_out, int n_caches, const int32_t* path,
+                     const int32_t* kept, int N, int B, int Hkv, int Smax, int D, int dtype,
+                     void* stream);
+
 /* Workspace bytes kf_attn_capture needs. */
 int kf_attn_capture_workspace_size(int B, int Sq, int Sk, int Hq, int Hkv, int D, int dtype,
                                    size_t* bytes);

@@ -8,6 +8,7 @@
 #include "kf_internal.h"
 
 #include <atomic>
+#include <climits>
 
 namespace kf {
 
@@ -461,6 +462,121 @@ int kf_kv_cache_append(const void* k_new, const void* v_new, const float* rope_c
                "cache overflow: start %d + %d new tokens > capacity %d", start, Snew, Smax);
   return cache_append(k_new, v_new, rope_cos, rope_sin, k_cache, v_cache, start, B, Snew, Hkv,
                       Smax, D, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"
+
+namespace {
+int check_tree(int B, int N, int max_len, int Hq, int Hkv, int D, int dtype) {
+  int rc = check_common(B, N, max_len, Hq, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(N <= KF_TREE_MAX_NODES, "at most %d nodes per sequence (got %d)",
+               KF_TREE_MAX_NODES, N);
+  KF_CHECK_ARG(B <= 65535, "at most 65535 sequences (got %d)", B);
+  KF_CHECK_ARG((int64_t)B * N * Hq <= INT_MAX, "B * N * n_heads exceeds 2^31 (%d, %d, %d)", B, N,
+               Hq);
+  return KF_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int kf_attn_tree_workspace_size(int B, int N, int Hq, int Hkv, int D, int max_len, int dtype,
+                                size_t* bytes) {
+  int rc = check_tree(B, N, max_len, Hq, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(bytes != nullptr, "bytes is null");
+  TreeArgs a = {};
+  a.B = B; a.N = N; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_len = max_len; a.dtype = dtype;
+  *bytes = tree_workspace(a);
+  return KF_OK;
+}
+
+int kf_attn_tree(const void* q_new, const void* k_new, const void* v_new, void* k_cache,
+                 void* v_cache, const int32_t* lens, const int32_t* parents,
+                 int64_t parents_stride, const int32_t* counts, const float* rope_cos,
+                 const float* rope_sin, int64_t rope_row_offset, int64_t rope_rows, void* out,
+                 void* workspace, size_t workspace_bytes, int B, int N, int Smax, int Hq, int Hkv,
+                 int D, int max_len, const float* q_norm_weight, const float* k_norm_weight,
+                 float norm_eps, int dtype, void* stream) {
+  int rc = check_tree(B, N, max_len, Hq, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(q_new && k_new && v_new && k_cache && v_cache && lens && rope_cos && rope_sin &&
+                   out,
+               "null tensor pointer");
+  KF_CHECK_ARG(!q_norm_weight == !k_norm_weight,
+               "QK-norm needs both q_norm_weight and k_norm_weight (or neither)");
+  KF_CHECK_ARG(max_len <= Smax, "max_len (%d) exceeds the cache length (%d)", max_len, Smax);
+  KF_CHECK_ARG(rope_rows > 0, "rope tables must have at least one row");
+  KF_CHECK_ARG(parents_stride == 0 || parents_stride >= N,
+               "parents_stride must be 0 or at least N (got %lld)", (long long)parents_stride);
+  TreeArgs a;
+  a.q_new = q_new; a.k_new = k_new; a.v_new = v_new; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.lens = lens; a.parents = parents; a.parents_stride = parents_stride; a.counts = counts;
+  a.cos = rope_cos; a.sin = rope_sin; a.rope_row_offset = rope_row_offset;
+  a.rope_rows = rope_rows; a.out = out;
+  a.B = B; a.N = N; a.Smax = Smax; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_len = max_len;
+  a.q_norm_w = q_norm_weight; a.k_norm_w = k_norm_weight; a.norm_eps = norm_eps;
+  a.dtype = dtype; a.scale = 1.0f / sqrtf((float)D); a.stream = (hipStream_t)stream;
+  const size_t need = tree_workspace(a);
+  if (workspace_bytes < need || !workspace) {
+    set_error("workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return KF_ERR_WORKSPACE;
+  }
+  return tree_attention(a, workspace);
+}
+
+int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_n,
+                     const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
+                     const int32_t* counts, const void* draft_logits, int64_t draft_stride_b,
+                     int64_t draft_stride_n, const float* uniforms, double temperature,
+                     int32_t* path, int32_t* kept, int64_t* next, int B, int N, int V, int dtype,
+                     void* stream) {
+  KF_CHECK_ARG(B > 0 && N > 0 && V > 0, "B, N, V must be positive (got %d, %d, %d)", B, N, V);
+  KF_CHECK_ARG(N <= KF_TREE_MAX_NODES, "at most %d nodes per sequence (got %d)",
+               KF_TREE_MAX_NODES, N);
+  KF_CHECK_ARG(V <= KF_VERIFY_MAX_VOCAB, "at most %d tokens in the vocabulary (got %d)",
+               KF_VERIFY_MAX_VOCAB, V);
+  KF_CHECK_ARG(dtype == F32 || dtype == BF16 || dtype == F16, "unsupported dtype code %d", dtype);
+  KF_CHECK_ARG(logits && tokens && uniforms && path && kept && next, "null tensor pointer");
+  KF_CHECK_ARG(temperature >= 0.0 && temperature < INFINITY,
+               "temperature must be finite and not negative (got %g)", temperature);
+  KF_CHECK_ARG(!draft_logits || (!parents && temperature > 0.0),
+               "draft_logits need a chain of drafts (parents NULL) and a temperature above 0");
+  KF_CHECK_ARG(parents_stride == 0 || parents_stride >= N,
+               "parents_stride must be 0 or at least N (got %lld)", (long long)parents_stride);
+  VerifyArgs a;
+  a.logits = logits; a.logits_sb = logits_stride_b; a.logits_sn = logits_stride_n;
+  a.tokens = tokens; a.parents = parents; a.parents_stride = parents_stride; a.counts = counts;
+  a.drafts = N > 1 ? draft_logits : nullptr;
+  a.drafts_sb = draft_stride_b; a.drafts_sn = draft_stride_n;
+  a.uniforms = uniforms; a.temperature = temperature;
+  a.path = path; a.kept = kept; a.next = next;
+  a.B = B; a.N = N; a.V = V; a.dtype = dtype; a.stream = (hipStream_t)stream;
+  return verify_drafts(a);
+}
+
+int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t* const* lens,
+                     int32_t* const* lens_out, int n_caches, const int32_t* path,
+                     const int32_t* kept, int N, int B, int Hkv, int Smax, int D, int dtype,
+                     void* stream) {
+  int rc = check_tree(B, N, Smax, Hkv, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(n_caches > 0, "n_caches must be positive (got %d)", n_caches);
+  KF_CHECK_ARG(k_caches && v_caches && lens && lens_out && path && kept, "null tensor pointer");
+  for (int c = 0; c < n_caches; ++c) {
+    KF_CHECK_ARG(k_caches[c] && v_caches[c] && lens[c] && lens_out[c],
+                 "null tensor pointer (cache %d)", c);
+    // the workgroups of one cache know nothing of the others': none may write
+    // what another reads or writes
+    KF_CHECK_ARG(k_caches[c] != v_caches[c], "cache %d has one tensor for K and V", c);
+    for (int d = 0; d < n_caches; ++d)
+      KF_CHECK_ARG(d == c || (lens_out[c] != lens[d] && k_caches[c] != k_caches[d] &&
+                              v_caches[c] != v_caches[d] && k_caches[c] != v_caches[d]),
+                   "caches %d and %d share a tensor that one of them writes", c, d);
+  }
+  return cache_keep(k_caches, v_caches, lens, lens_out, n_caches, path, kept, N, B, Hkv, Smax, D,
+                    dtype, (hipStream_t)stream);
 }
 
 int kf_attn_capture_workspace_size(int B, int Sq, int Sk, int Hq, int Hkv, int D, int dtype,

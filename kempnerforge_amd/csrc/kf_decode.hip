@@ -23,6 +23,7 @@
 #include "kf_internal.h"
 #include "kf_merge.h"
 #include "kf_mfma.h"
+#include "kf_split.h"
 
 #include <algorithm>
 #include <atomic>
@@ -169,72 +170,8 @@ struct DecodeSched {
     const int len = lens[b];
     return decode_len_ok(len, max_len, row_offset, rope_rows) ? (len + KC) / KC : 0;
   }
+  __device__ __forceinline__ int chunks(int b) const { return nck(b) * Hkv; }
 };
-
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return __builtin_amdgcn_readfirstlane(v);
-}
-
-// Total chunks C over all pairs (wavefront-uniform).
-__device__ __forceinline__ int total_chunks(const DecodeSched& s, int lane) {
-  int tot = 0;
-  for (int b0 = 0; b0 < s.B; b0 += 64) tot += wave_sum_int(b0 + lane < s.B ? s.nck(b0 + lane) : 0);
-  return tot * s.Hkv;
-}
-
-// Sequence holding global chunk c (0 <= c < C) and the index of its first
-// chunk, Hkv * (chunks of the sequences before it).  Wavefront-uniform.
-__device__ __forceinline__ void locate_chunk(const DecodeSched& s, int c, int lane, int& b_out,
-                                             int& base_out) {
-  int run = 0;
-  b_out = 0;
-  base_out = 0;
-  for (int b0 = 0; b0 < s.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = (b < s.B ? s.nck(b) : 0) * s.Hkv;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += y;
-    }
-    const uint64_t m = __builtin_amdgcn_ballot_w64(n > 0 && run + incl - n <= c && c < run + incl);
-    if (m) {
-      const int l = (int)__builtin_ctzll(m);
-      b_out = b0 + l;
-      base_out = run + __shfl(incl - n, l, 64);
-      b_out = __builtin_amdgcn_readfirstlane(b_out);
-      base_out = __builtin_amdgcn_readfirstlane(base_out);
-      return;
-    }
-    run += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
-  }
-}
-
-// floor(x / d) for 0 <= x < 2^53 and 0 < d < 2^31: the double quotient is
-// within one of the exact one (its relative error is below 2^-52 and x / d <
-// 2^53), so one correction step either way makes it exact, in far fewer
-// instructions than a 64-bit integer division.
-__device__ __forceinline__ int64_t floor_div(int64_t x, int64_t d) {
-  int64_t q = (int64_t)((double)x / (double)d);
-  if (q * d > x)
-    --q;
-  else if ((q + 1) * d <= x)
-    ++q;
-  return q;
-}
-
-// First chunk of wavefront w's range, floor(w C / NW).
-__device__ __forceinline__ int range_start(int w, int C, int NW) {
-  return (int)floor_div((int64_t)w * C, NW);
-}
-
-// The wavefront whose range holds chunk c: the largest w with w C / NW <= c.
-__device__ __forceinline__ int chunk_owner(int c, int C, int NW) {
-  return (int)floor_div(((int64_t)c + 1) * NW - 1, C);
-}
 
 // Position in the chunk list: pair (b, g), local chunk lc of nck, new-token
 // position len (keys 0 .. len are attended).

@@ -182,4 +182,49 @@ int cache_append(const void* k_new, const void* v_new, const float* cos, const f
                  void* k_cache, void* v_cache, int start, int B, int Snew, int Hkv, int Smax,
                  int D, int dtype, hipStream_t stream);
 
+// attention of a tree of drafted tokens over a cache (kf_tree.hip)
+struct TreeArgs {
+  const void *q_new, *k_new, *v_new;  // [B, N, Hq, D], [B, N, Hkv, D] contiguous, pre-RoPE
+  void *k_cache, *v_cache;            // [B, Hkv, Smax, D] contiguous
+  const int32_t* lens;                // [B] cached tokens per sequence
+  const int32_t* parents;             // [N] or [B, N] (parents_stride 0 or N), null: a chain
+  int64_t parents_stride;
+  const int32_t* counts;              // [B] nodes in use, null: N
+  const float *cos, *sin;             // table; row = position - rope_row_offset
+  int64_t rope_row_offset, rope_rows;
+  void* out;                          // [B, N, Hq, D]
+  int B, N, Smax, Hq, Hkv, D, max_len;
+  const float *q_norm_w, *k_norm_w;
+  float norm_eps;
+  int dtype;
+  float scale;
+  hipStream_t stream;
+};
+size_t tree_workspace(const TreeArgs& a);
+int tree_attention(const TreeArgs& a, void* workspace);
+
+// verification of drafted tokens, and the move of the accepted cache rows
+// (kf_spec.hip)
+struct VerifyArgs {
+  const void* logits;   // row (b, i) at b * logits_sb + i * logits_sn, V contiguous values
+  const void* drafts;   // row (b, i) the distribution that node i + 1 was drawn from, or null
+  int64_t logits_sb, logits_sn, drafts_sb, drafts_sn;
+  const int64_t* tokens;     // [B, N]
+  const float* uniforms;     // [B, N]
+  const int32_t* parents;    // as TreeArgs
+  int64_t parents_stride;
+  const int32_t* counts;     // as TreeArgs
+  int32_t *path, *kept;      // [B, N], [B]
+  int64_t* next;             // [B]
+  int B, N, V;
+  double temperature;
+  int dtype;
+  hipStream_t stream;
+};
+int verify_drafts(const VerifyArgs& a);
+constexpr int KEEP_CACHES = 64;  // caches per launch: their pointers are kernel arguments
+int cache_keep(void* const* k, void* const* v, const int32_t* const* lens,
+               int32_t* const* lens_out, int n_caches, const int32_t* path, const int32_t* kept,
+               int N, int B, int Hkv, int Smax, int D, int dtype, hipStream_t stream);
+
 }  // namespace kf

@@ -14,6 +14,7 @@ only accept GPU tensors: there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import weakref
@@ -482,6 +483,232 @@ def cache_append_raw(k_new, v_new, cos, sin, k_cache, v_cache, start: int) -> No
                                       _ptr(k_cache), _ptr(v_cache), int(start), B, Snew, Hkv,
                                       Smax, D, _dtype_code(k_new), _stream(k_new)),
                "kf_kv_cache_append")
+
+
+# --------------------------------------------------------------------------- speculative decoding
+TREE_MAX_NODES = 256  # KF_TREE_MAX_NODES
+
+
+def _on_device(t: torch.Tensor):
+    """The context in which the library sees ``t``'s device as the current one."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(t: torch.Tensor, **others) -> None:
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise RuntimeError(f"{name} must be on the same device as the others ({t.device}, "
+                               f"got {o.device})")
+
+
+def _tree_args(parents, counts, B: int, N: int, device):
+    """``parents`` (``[N]`` or ``[B, N]``, None for a chain) and ``counts`` (``[B]`` or
+    None) as the contiguous int32 tensors the kernels read, and the parents' row stride."""
+    stride = 0
+    for name, t in (("parents", parents), ("counts", counts)):
+        if t is None:
+            continue
+        if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+            raise TypeError(f"{name} must be an integer tensor (got {t.dtype})")
+        if t.device != device:
+            raise RuntimeError(f"{name} must be on the same device as the others")
+    if parents is not None:
+        if tuple(parents.shape) not in ((N,), (B, N)):
+            raise ValueError(f"parents must be [{N}] or [{B}, {N}] (got {tuple(parents.shape)})")
+        stride = N if parents.dim() == 2 else 0
+        parents = parents.to(torch.int32).contiguous()
+    if counts is not None:
+        if tuple(counts.shape) != (B,):
+            raise ValueError(f"counts must be [{B}] (got {tuple(counts.shape)})")
+        counts = counts.to(torch.int32).contiguous()
+    return parents, stride, counts
+
+
+def tree_decode_raw(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, *,
+                    rope_row_offset: int, max_len: int, parents=None, counts=None,
+                    q_norm_weight=None, k_norm_weight=None, norm_eps: float = 1e-5):
+    """Attention of a tree of drafted tokens over a KV cache (``kf_attn_tree``).
+
+    ``q_new [B,N,Hq,D]``, ``k_new`` and ``v_new`` ``[B,N,Hkv,D]`` are the N nodes
+    of each sequence (at most 256), before RoPE.  ``parents`` (``[N]`` for one tree
+    for all sequences or ``[B,N]``, integers on the device) names each node's
+    parent, which comes before it, or -1 for a node that follows the cached
+    prefix directly; None is a chain.  Node i is rotated at position ``lens[b] +
+    depth``, written to cache row ``lens[b] + i``, and attends the prefix, itself
+    and its ancestors.  ``counts [B]`` are the nodes in use (None: all); the
+    others give zeros and leave their cache rows.  ``max_len`` bounds ``lens[b] +
+    counts[b]``.  ``lens`` is not modified: :func:`cache_keep_raw` moves the
+    accepted rows together and advances it.  Returns out ``[B,N,Hq,D]``.
+
+    As in :func:`decode_raw`, what lies on the device is checked there: a
+    sequence whose length, count, parents or RoPE rows are out of range gets NaN
+    outputs and no cache write."""
+    _require_gpu(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin)
+    lib = _lib.load()
+    if q_new.dim() != 4 or k_new.dim() != 4 or k_cache.dim() != 4:
+        raise ValueError("q_new, k_new, v_new and the caches must have four dimensions")
+    B, N, Hq, D = q_new.shape
+    Hkv, Smax = k_cache.shape[1], k_cache.shape[2]
+    if tuple(k_new.shape) != (B, N, Hkv, D) or k_new.shape != v_new.shape:
+        raise ValueError(f"k_new and v_new must be [{B}, {N}, {Hkv}, {D}] "
+                         f"(got {tuple(k_new.shape)}, {tuple(v_new.shape)})")
+    if tuple(k_cache.shape) != (B, Hkv, Smax, D) or k_cache.shape != v_cache.shape:
+        raise ValueError(f"the KV caches must be [{B}, n_kv_heads, max_seq_len, {D}] "
+                         f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
+    if any(t.dtype != q_new.dtype for t in (k_new, v_new, k_cache, v_cache)):
+        raise TypeError("q_new, k_new, v_new and the caches must share a dtype")
+    if not 1 <= N <= TREE_MAX_NODES:
+        raise ValueError(f"1 to {TREE_MAX_NODES} nodes per sequence (got {N})")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim]")
+    if lens.dtype != torch.int32 or not lens.is_contiguous() or tuple(lens.shape) != (B,):
+        raise TypeError(f"lens must be a contiguous int32 tensor [{B}]")
+    _same_device(q_new, k_new=k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, lens=lens,
+                 rope_cos=cos, rope_sin=sin)
+    q_new, k_new, v_new = (t.contiguous() for t in (q_new, k_new, v_new))
+    cos = _rope_table(cos, 1, D // 2, "rope_cos")
+    sin = _rope_table(sin, 1, D // 2, "rope_sin")
+    if cos.shape != sin.shape:
+        raise ValueError("rope_cos and rope_sin must have the same shape")
+    parents, stride, counts = _tree_args(parents, counts, B, N, q_new.device)
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("QK-norm needs both q_norm_weight and k_norm_weight")
+    qnw = knw = None
+    dt = _dtype_code(q_new)
+    with _on_device(q_new):
+        if q_norm_weight is not None:
+            qnw, knw = (_norm_weight(w, D, q_new.device) for w in (q_norm_weight, k_norm_weight))
+        out = torch.empty_like(q_new)
+        # (max_len grows from step to step: asked per step, not kept)
+        nbytes = _lib.size_out()
+        _lib.check(lib.kf_attn_tree_workspace_size(B, N, Hq, Hkv, D, max_len, dt,
+                                                   ctypes.byref(nbytes)),
+                   "kf_attn_tree_workspace_size")
+        ws = _workspace(nbytes.value, q_new.device)
+        _lib.check(lib.kf_attn_tree(_ptr(q_new), _ptr(k_new), _ptr(v_new), _ptr(k_cache),
+                                    _ptr(v_cache), _ptr(lens), _ptr(parents), stride,
+                                    _ptr(counts), _ptr(cos), _ptr(sin), int(rope_row_offset),
+                                    cos.shape[0], _ptr(out), _ptr(ws), ws.numel(), B, N, Smax, Hq,
+                                    Hkv, D, int(max_len), _ptr(qnw), _ptr(knw), float(norm_eps),
+                                    dt, _stream(q_new)),
+                   "kf_attn_tree")
+    return out
+
+
+def verify_drafts_raw(logits, tokens, uniforms, *, temperature: float = 1.0, parents=None,
+                      counts=None, draft_logits=None):
+    """Verification of drafted tokens against the target's distributions
+    (``kf_verify_drafts``); returns path ``[B,N]`` int32, kept ``[B]`` int32 and the
+    next token ``[B]`` int64, all on the device.
+
+    ``logits [B,N,V]`` are the target's at every node (contiguous values; any row
+    strides), ``tokens [B,N]`` the nodes' tokens, ``uniforms [B,N]`` float32 random
+    numbers in [0, 1).  Node 0 is the token emitted last, so its row verifies its
+    children; ``parents`` and ``counts`` as in :func:`tree_decode_raw` (``parents[0]``
+    is -1, no other).  From node 0 a node's children are tried in index order; the
+    path is the accepted nodes, node 0 first (-1 behind the last of ``kept``), and
+    ``next`` the token after it.  Without ``draft_logits`` a child with token c is
+    accepted with probability p(c) over what its refused elder siblings leave, p
+    being ``softmax(logits / temperature)``, and next is drawn from p without the
+    refused tokens.  ``draft_logits [B,N-1,V]`` (a chain only) are what the draft
+    model drew nodes 1 .. N-1 from, at the same temperature: accepted with
+    probability min(1, p / q), next then from max(p - q, 0).  Either way the
+    emitted tokens follow the target.  Filtered tokens (top-k, top-p) are logits of
+    -inf.  ``temperature`` 0: a node is accepted if its token is the most likely.
+
+    Unused sequences (``counts[b]`` 0) and counts or parents out of range give kept
+    0 and next -1; a row on the path that is no distribution (NaN, +inf, all -inf)
+    ends the path with next -1."""
+    _require_gpu(logits, tokens, uniforms)
+    lib = _lib.load()
+    if logits.dim() != 3 or logits.stride(-1) != 1:
+        raise ValueError("logits must be [B, N, V] with contiguous values "
+                         f"(got {tuple(logits.shape)}, strides {logits.stride()})")
+    B, N, V = logits.shape
+    if not 1 <= N <= TREE_MAX_NODES:
+        raise ValueError(f"1 to {TREE_MAX_NODES} nodes per sequence (got {N})")
+    if tuple(tokens.shape) != (B, N) or tuple(uniforms.shape) != (B, N):
+        raise ValueError(f"tokens and uniforms must be [{B}, {N}] "
+                         f"(got {tuple(tokens.shape)}, {tuple(uniforms.shape)})")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be int64 or int32 (got {tokens.dtype})")
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"uniforms must be float32 (got {uniforms.dtype})")
+    _same_device(logits, tokens=tokens, uniforms=uniforms, draft_logits=draft_logits)
+    parents, stride, counts = _tree_args(parents, counts, B, N, logits.device)
+    dsb = dsn = 0
+    if draft_logits is not None:
+        if parents is not None:
+            raise ValueError("draft_logits need a chain of drafts (parents=None)")
+        if temperature == 0:
+            raise ValueError("draft_logits need a temperature above 0")
+        if tuple(draft_logits.shape) != (B, N - 1, V) or draft_logits.dtype != logits.dtype:
+            raise ValueError(f"draft_logits must be [{B}, {N - 1}, {V}] of the logits' dtype "
+                             f"(got {tuple(draft_logits.shape)}, {draft_logits.dtype})")
+        if N == 1:
+            draft_logits = None
+        elif draft_logits.stride(-1) != 1:
+            raise ValueError("draft_logits must have contiguous values")
+        else:
+            dsb, dsn = draft_logits.stride(0), draft_logits.stride(1)
+    dt = _dtype_code(logits)
+    tokens, uniforms = tokens.to(torch.int64).contiguous(), uniforms.contiguous()
+    with _on_device(logits):
+        path = torch.empty(B, N, dtype=torch.int32, device=logits.device)
+        kept = torch.empty(B, dtype=torch.int32, device=logits.device)
+        token = torch.empty(B, dtype=torch.int64, device=logits.device)
+        _lib.check(lib.kf_verify_drafts(_ptr(logits), logits.stride(0), logits.stride(1),
+                                        _ptr(tokens), _ptr(parents), stride, _ptr(counts),
+                                        _ptr(draft_logits), dsb, dsn, _ptr(uniforms),
+                                        float(temperature), _ptr(path), _ptr(kept), _ptr(token),
+                                        B, N, V, dt, _stream(logits)),
+                   "kf_verify_drafts")
+    return path, kept, token
+
+
+def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> None:
+    """Moves an accepted path's rows together in the KV caches of all layers
+    (``kf_kv_cache_keep``): row ``lens[c][b] + path[b, j]`` of cache c to row
+    ``lens[c][b] + j`` for ``j < kept[b]``, and ``lens_out[c][b] = lens[c][b] +
+    kept[b]``.  ``k_caches``, ``v_caches`` and ``lens`` are lists with one tensor per
+    cache (``[B, n_kv_heads, max_seq_len, head_dim]`` contiguous, ``[B]`` int32);
+    ``lens_out`` (None: ``lens``, in place) likewise, and then no two caches may
+    share a ``lens`` tensor.  ``path [B,N]`` and ``kept [B]`` int32 are
+    :func:`verify_drafts_raw`'s.  Other rows stay as they are.  A sequence whose
+    path does not rise or leaves the cache is left alone."""
+    k_caches, v_caches, lens = list(k_caches), list(v_caches), list(lens)
+    lens_out = lens if lens_out is None else list(lens_out)
+    if not k_caches or not len(k_caches) == len(v_caches) == len(lens) == len(lens_out):
+        raise ValueError("k_caches, v_caches, lens and lens_out need one tensor per cache "
+                         f"(got {len(k_caches)}, {len(v_caches)}, {len(lens)}, {len(lens_out)})")
+    k0 = k_caches[0]
+    _require_gpu(*k_caches, *v_caches, *lens, *lens_out, path, kept)
+    if k0.dim() != 4:
+        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
+    B, Hkv, Smax, D = k0.shape
+    for t in k_caches + v_caches:
+        if t.shape != k0.shape or t.dtype != k0.dtype or not t.is_contiguous():
+            raise ValueError("KV caches must be contiguous, of one shape and one dtype")
+    for t in lens + lens_out:
+        if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != (B,):
+            raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
+    for t in k_caches + v_caches + lens + lens_out:
+        _same_device(k0, a_cache=t, path=path, kept=kept)
+    if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= TREE_MAX_NODES:
+        raise ValueError(f"path must be [{B}, N] with N from 1 to {TREE_MAX_NODES} "
+                         f"(got {tuple(path.shape)})")
+    if tuple(kept.shape) != (B,) or path.dtype != torch.int32 or kept.dtype != torch.int32:
+        raise TypeError(f"path [{B}, N] and kept [{B}] must be int32")
+    path, kept = path.contiguous(), kept.contiguous()
+    n = len(k_caches)
+    arr = ctypes.c_void_p * n
+    ptrs = [arr(*(t.data_ptr() for t in ts)) for ts in (k_caches, v_caches, lens, lens_out)]
+    with _on_device(k0):
+        _lib.check(_lib.load().kf_kv_cache_keep(*ptrs, n, _ptr(path), _ptr(kept), path.shape[1], B,
+                                                Hkv, Smax, D, _dtype_code(k0), _stream(k0)),
+                   "kf_kv_cache_keep")
 
 
 def capture_raw(q, k, v, cos, sin, *, causal: bool, k_rotated: bool, k_layout: str = "bshd",
