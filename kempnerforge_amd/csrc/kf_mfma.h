@@ -150,11 +150,14 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 // rows and 2 per transposed read on 256-byte rows).
 // R = 4 (64-byte rows, only read one row per lane with ds_read_b128): the row's
 // 4-row group index, so 16 consecutive rows of one chunk meet 16 distinct
-// 16-byte slots of a 256-byte window.
+// 16-byte slots of a 256-byte window.  R = 32 (512-byte rows, float32): the row
+// within 16, for the same reason; 4-byte reads along a row are conflict-free
+// under any swizzle.
 template <int R>
 __device__ __forceinline__ int swz(int row) {
-  return R == 16  ? (((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1))
-         : R == 8 ? (((row << 1) & 4) | ((row >> 1) & 2) | ((row >> 3) & 1))
+  return R == 32  ? (row & 15)
+         : R == 16 ? (((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1))
+         : R == 8  ? (((row << 1) & 4) | ((row >> 1) & 2) | ((row >> 3) & 1))
                   : ((row >> 2) & 3);
 }
 

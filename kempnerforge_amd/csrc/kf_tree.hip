@@ -4,14 +4,31 @@
 // its ancestors in the tree:
 //   s_ij = q_i . k_j / sqrt(D),  j in prefix or anc(i);  o_i = softmax(s_i) V
 // Its key is rotated at position lens[b] + depth(i) and stored in cache row
-// lens[b] + i, so that the rows of all nodes lie behind the prefix in node order.
+// lens[b] + i, so that the rows of all nodes lie behind the prefix in node order
+// and are read like it, under a mask.
 //
 //  1. prep    the ancestors of every node (as bit masks), the rotated queries,
 //             and the nodes' rows of the caches
-//  2. rows    one wavefront per (node, query head)
+//  2. stream  split-K attention on the matrix cores: a workgroup takes up to 128
+//             (node, query head) rows of a KV head and an equal share of all key
+//             chunks; a row tile that more than one workgroup met leaves float32
+//             partials
+//  3. merge   joins the partials; rows of unused nodes and refused sequences
+// Head sizes other than 64 and 128 run as one wavefront per row (tree_rows).
+//
+// Rounding: the norm and the rotation of q and k are formed in 32 bits.  k is
+// rounded once, where it is stored.  q is not rounded to 16 bits: it goes
+// through the 16-bit matrix instructions as the sum of two numbers of the input
+// type (hi = q rounded, lo = q - hi rounded), which keeps 16 of its bits for
+// half as many more products.  P is rounded to the input type before it
+// multiplies V; the sums, the row maxima and the row sums stay in 32 bits.
 #include "kf_common.h"
 #include "kf_internal.h"
+#include "kf_merge.h"
+#include "kf_mfma.h"
+#include "kf_split.h"
 
+#include <algorithm>
 #include <climits>
 
 namespace kf {
@@ -21,29 +38,23 @@ namespace {
 constexpr int MAXN = KF_TREE_MAX_NODES;
 constexpr int MAXW = MAXN / 32;  // 32-bit words of an ancestor mask
 
-// RMSNorm of one element given its row's sum of squares (rms_scale of
-// kf_decode.hip: float32, rounded to the storage type).
-template <typename T>
-__device__ __forceinline__ float rms_scale(float x, float ss, int D, float eps, float w) {
-  const float r = rsqrtf(ss / (float)D + eps);
-  return round_to<T>((x * r) * w);
-}
-
 template <typename T>
 __device__ __forceinline__ bool finite(T x) {
   return fabsf(to_f32(x)) < INFINITY;  // false for NaN too
 }
 
-// One workgroup: sequence blockIdx.y, `per` of its N * (Hq + 2 Hkv) rows.
+// One workgroup: sequence blockIdx.y, `per` of its N * (Hq + 2 Hkv) rows.  The
+// queries go to `qrot` scaled by D^-1/2 log2(e), as [B][Hkv][node, head of the
+// group][D]: float32, or (SPLIT) hi and, `qlo` elements behind, lo.
 //
 // The ancestor masks come from pointer doubling: after round r, mask[i] holds
 // the 2^r nearest of i and its ancestors and ptr[i] the next one beyond, so 8
 // rounds cover 256 nodes whatever their depth (a walk up a chain of 200 would
 // take 200 dependent reads).  Every workgroup of a sequence forms them again
 // (under a microsecond, no launch of its own); the first one stores them.
-template <typename T>
-__global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, T* __restrict__ qrot,
-                                                        uint32_t* __restrict__ anc,
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __restrict__ qrot,
+                                                        int64_t qlo, uint32_t* __restrict__ anc,
                                                         int2* __restrict__ seq,
                                                         uint8_t* __restrict__ vbad, int W,
                                                         int per) {
@@ -125,24 +136,39 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, T* __restric
     const int g = is_q ? h / n_rep : h - a.Hq;
     const T* src = is_q ? (const T*)a.q_new + (node * a.Hq + h) * D
                         : (const T*)a.k_new + (node * a.Hkv + g) * D;
-    T* dst = is_q ? qrot + (((int64_t)b * a.Hkv + g) * N * n_rep + (int64_t)i * n_rep + h % n_rep) * D
-                  : (T*)a.k_cache + (((int64_t)b * a.Hkv + g) * a.Smax + L + i) * D;
+    const int64_t qrow =
+        (((int64_t)b * a.Hkv + g) * N * n_rep + (int64_t)i * n_rep + h % n_rep) * D;
+    T* kdst = (T*)a.k_cache + (((int64_t)b * a.Hkv + g) * a.Smax + L + i) * D;
     const float* nw = is_q ? a.q_norm_w : a.k_norm_w;
-    float ss = 0.f;
+    float rs = 1.f;
     if (nw != nullptr) {
+      float ss = 0.f;
       for (int d = lane; d < D; d += 64) ss += to_f32(src[d]) * to_f32(src[d]);
-      ss = wave_sum(ss);
+      rs = rsqrtf(wave_sum(ss) / (float)D + a.norm_eps);
     }
     const int64_t row = ((int64_t)L + sdepth[i] - a.rope_row_offset) * half;
     for (int d = lane; d < half; d += 64) {
-      float x1 = to_f32(src[d]), x2 = to_f32(src[d + half]), y1, y2;
+      float x1 = to_f32(src[d]), x2 = to_f32(src[d + half]);
       if (nw != nullptr) {
-        x1 = rms_scale<T>(x1, ss, D, a.norm_eps, nw[d]);
-        x2 = rms_scale<T>(x2, ss, D, a.norm_eps, nw[d + half]);
+        x1 = x1 * rs * nw[d];
+        x2 = x2 * rs * nw[d + half];
       }
-      rope_pair<T>(x1, x2, a.cos[row + d], a.sin[row + d], y1, y2);
-      dst[d] = from_f32<T>(y1);
-      dst[d + half] = from_f32<T>(y2);
+      const float c = a.cos[row + d], s = a.sin[row + d];
+      const float y[2] = {x1 * c - x2 * s, x2 * c + x1 * s};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = d + e * half;
+        if (!is_q) {
+          kdst[at] = from_f32<T>(y[e]);
+        } else if constexpr (SPLIT) {
+          const float z = y[e] * (a.scale * kLog2e);
+          const T hi = from_f32<T>(z);
+          ((T*)qrot)[qrow + at] = hi;
+          ((T*)qrot)[qlo + qrow + at] = from_f32<T>(z - to_f32(hi));
+        } else {
+          ((float*)qrot)[qrow + at] = y[e] * (a.scale * kLog2e);
+        }
+      }
     }
   }
 }
@@ -150,7 +176,7 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, T* __restric
 // One wavefront per (b, node, query head), any D <= 256: the prefix and the
 // node's own row and ancestors, one key at a time.  Masked keys are not read.
 template <typename T>
-__global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const T* __restrict__ qrot,
+__global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const float* __restrict__ qrot,
                                                         const uint32_t* __restrict__ anc,
                                                         const int2* __restrict__ seq, int W) {
   const int lane = threadIdx.x & 63;
@@ -165,22 +191,22 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const T* __r
     return;
   }
   const int L = s.y;
-  const T* q = qrot + (((int64_t)b * a.Hkv + g) * a.N * n_rep + (int64_t)i * n_rep + hq % n_rep) * D;
+  const float* q = qrot + (((int64_t)b * a.Hkv + g) * a.N * n_rep + (int64_t)i * n_rep + hq % n_rep) * D;
   const T* kb = (const T*)a.k_cache + ((int64_t)b * a.Hkv + g) * a.Smax * D;
   const T* vb = (const T*)a.v_cache + ((int64_t)b * a.Hkv + g) * a.Smax * D;
   float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) qv[e] = lane + 64 * e < D ? to_f32(q[lane + 64 * e]) : 0.f;
+  for (int e = 0; e < 4; ++e) qv[e] = lane + 64 * e < D ? q[lane + 64 * e] : 0.f;
   float m = -INFINITY, l = 0.f;
   auto key = [&](int j) {
     float x = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (lane + 64 * e < D) x += qv[e] * to_f32(kb[(int64_t)j * D + lane + 64 * e]);
-    x = wave_sum(x) * a.scale;
+    x = wave_sum(x);
     const float mn = fmaxf(m, x);
     const float ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = expf(m - ref), p = expf(x - ref);
+    const float alpha = fast_exp2(m - ref), p = fast_exp2(x - ref);
     l = l * alpha + p;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -197,32 +223,529 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const T* __r
     if (lane + 64 * e < D) out[lane + 64 * e] = from_f32<T>(acc[e] / l);
 }
 
+// ---- split-K attention on the matrix cores -------------------------------------
+// Row tile t of pair (b, g) holds rows t ROWS .. of the pair's n_b n_rep rows
+// (node-major: the heads of a node side by side); every tile meets the nck(b) =
+// ceil((lens[b] + n_b) / KC) key chunks of its pair.
+struct TreeSched {
+  const int2* seq;
+  int B, Hkv, n_rep, rows, kc;
+  __device__ __forceinline__ int nck(int2 s) const { return (s.x + s.y + kc - 1) / kc; }
+  __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
+  __device__ __forceinline__ int chunks(int b) const {
+    const int2 s = seq[b];
+    return s.x > 0 ? Hkv * tiles(s) * nck(s) : 0;
+  }
+};
+
+// Place in the chunk list: sequence b (s: its nodes in use and prefix length),
+// KV head g, row tile t, chunk c of nck.
+struct TreeCursor {
+  int b, g, t, c, nck, tiles;
+  int2 s;
+  __device__ __forceinline__ void at(const TreeSched& sched, int b_) {
+    b = b_;
+    s = sched.seq[b];
+    s.x = __builtin_amdgcn_readfirstlane(s.x);
+    s.y = __builtin_amdgcn_readfirstlane(s.y);
+    nck = sched.nck(s);
+    tiles = sched.tiles(s);
+  }
+  __device__ __forceinline__ void seek(const TreeSched& sched, int chunk, int lane) {
+    int sb, base;
+    locate_chunk(sched, chunk, lane, sb, base);
+    at(sched, sb);
+    const int rem = chunk - base;
+    c = rem % nck;
+    t = rem / nck % tiles;
+    g = rem / nck / tiles;
+  }
+  __device__ __forceinline__ void next(const TreeSched& sched) {
+    if (++c < nck) return;
+    c = 0;
+    if (++t < tiles) return;
+    t = 0;
+    if (++g < sched.Hkv) return;
+    g = 0;
+    for (int nb = b + 1; nb < sched.B; ++nb) {
+      if (sched.seq[nb].x > 0) {
+        at(sched, nb);
+        return;
+      }
+    }
+    b = sched.B;  // behind the last chunk
+  }
+};
+
+// What depends on the element type: the products on 32 x 32 tiles.
+//   S^T (keys x rows) += K q^T: lane l supplies row l % 32 of both operands, dims
+//       of its half h = l / 32 in 16-byte pieces
+//   O^T (dims x rows) += V^T P^T: P^T straight from the S registers (lane l holds
+//       row l % 32, register i key 8 (i / 4) + 4 h + i % 4)
+template <typename T, int D>
+struct Tile {
+  static constexpr int R = D / 8;     // 16-byte chunks per cache row
+  static constexpr int KS = D / 16;   // pieces of a lane's half row
+  static constexpr int QP = 2;        // q as hi and lo
+  typedef mfma::TrOffsets<D> VOff;
+  static __device__ __forceinline__ VOff v_off(int lane) { return mfma::tr_offsets<D>(lane); }
+  static __device__ __forceinline__ void scores(const T* k, int row0, const u32x4 (*q)[KS],
+                                                f32x16& s, int lane) {
+    using namespace mfma;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const bf16x8& a = lds_frag<R>(k, row0 + (lane & 31), 2 * ks + (lane >> 5));
+      s = mfma32<T>(a, as_bf16x8(q[0][ks]), s);
+      s = mfma32<T>(a, as_bf16x8(q[1][ks]), s);
+    }
+  }
+  static __device__ __forceinline__ void values(const T* v, int row0, const VOff& off,
+                                                const f32x16& p, f32x16* acc, int lane) {
+    using namespace mfma;
+    bf16x8 pb[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = p[8 * c + j];
+      pb[c] = as_bf16x8(pack8<T>(f));
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        acc[dt] = mfma32<T>(lds_frag_t<D>(v + row0 * D, off, c, dt), pb[c], acc[dt]);
+    __builtin_amdgcn_sched_barrier(0);  // the next block's reads stay behind these products
+  }
+};
+template <int D>
+struct Tile<float, D> {
+  static constexpr int R = D / 4;
+  static constexpr int KS = D / 8;
+  static constexpr int QP = 1;
+  struct VOff {};
+  static __device__ __forceinline__ VOff v_off(int) { return {}; }
+  static __device__ __forceinline__ f32x16 mma(float a, float b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void scores(const float* k, int row0, const u32x4 (*q)[KS],
+                                                f32x16& s, int lane) {
+    const int row = row0 + (lane & 31), sw = mfma::swz<R>(row);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const f32x4 a = *(const f32x4*)(k + (row * R + ((2 * ks + (lane >> 5)) ^ sw)) * 4);
+      const f32x4 b = __builtin_bit_cast(f32x4, q[0][ks]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = mma(a[e], b[e], s);
+    }
+  }
+  static __device__ __forceinline__ void values(const float* v, int row0, const VOff&,
+                                                const f32x16& p, f32x16* acc, int lane) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = row0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4, sw = mfma::swz<R>(row);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const int ch = 8 * dt + ((lane & 31) >> 2);
+        acc[dt] = mma(v[(row * R + (ch ^ sw)) * 4 + (lane & 3)], p[i], acc[dt]);
+      }
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // later rows' reads stay behind
+    }
+  }
+};
+
+// A workgroup of four wavefronts: RW of them side by side over the rows (32
+// each), KW = 4 / RW over the keys of a chunk (BKW each).  A chunk's K and V rows
+// go straight from the cache to one of two LDS stages while the other one is
+// computed; one barrier per chunk.
+template <typename T, int D, int RW, int BKW>
+struct Shape {
+  static constexpr int KW = 4 / RW, ROWS = 32 * RW, KC = BKW * KW;
+  static constexpr int TILE = KC * D;                  // elements of a K (or V) tile
+  static constexpr size_t STAGE = 2 * TILE * sizeof(T);
+  static constexpr size_t LDS = 2 * STAGE + (KW - 1) * ROWS * 2 * sizeof(float);
+  // (float32 rows of 128: q, the sums and a block's scores leave no room for two
+  // wavefronts per SIMD)
+  static constexpr int PER_CU = LDS * 2 <= 160 * 1024 && D * sizeof(T) <= 256 ? 2 : 1;
+  static_assert((KW - 1) * ROWS * D * sizeof(float) <= STAGE, "the key waves' exchange");
+};
+
+template <typename T, int D, int RW, int BKW>
+__global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stream_kernel(
+    TreeArgs a, const T* __restrict__ qrot, int64_t qlo, const uint32_t* __restrict__ anc,
+    const int2* __restrict__ seq, const uint8_t* __restrict__ vbad, int W,
+    float* __restrict__ opart, float* __restrict__ mlpart, int tiles_max) {
+  using namespace mfma;
+  using X = Tile<T, D>;
+  using Sh = Shape<T, D, RW, BKW>;
+  constexpr int KW = Sh::KW, ROWS = Sh::ROWS, KC = Sh::KC, NB = BKW / 32, DT = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int w = wave_id(), lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
+  const int rw = w % RW, kw = w / RW;
+  const int N = a.N, n_rep = a.Hq / a.Hkv;
+  const TreeSched sched{seq, a.B, a.Hkv, n_rep, ROWS, KC};
+  const int C = total_chunks(sched, lane), NW = min((int)gridDim.x, C);
+  const int gw = blockIdx.x;
+  if (gw >= NW) return;
+  const int c_lo = range_start(gw, C, NW), c_hi = range_start(gw + 1, C, NW);
+
+  auto stage_k = [&](int i) { return (T*)(lds + (i & 1) * Sh::STAGE); };
+  auto issue = [&](const TreeCursor& p, int i) {
+    const int64_t row = ((int64_t)p.b * a.Hkv + p.g) * a.Smax + (int64_t)p.c * KC;
+    const int rows = p.s.x + p.s.y - p.c * KC;  // >= 1; rows past the last repeat it
+    uint16_t* dst = (uint16_t*)stage_k(i);
+    constexpr int U = sizeof(T) / 2;
+    tile_to_lds<KC, X::R>((const uint16_t*)((const T*)a.k_cache + row * D), D * U, dst, w, lane,
+                          rows);
+    tile_to_lds<KC, X::R>((const uint16_t*)((const T*)a.v_cache + row * D), D * U,
+                          dst + Sh::TILE * U, w, lane, rows);
+  };
+
+  const typename X::VOff voff = X::v_off(lane);
+  u32x4 q[X::QP][X::KS];
+  f32x16 acc[DT];
+  float m = -INFINITY, lsum = 0.f;
+  TreeCursor cc, ic;
+  cc.seek(sched, c_lo, lane);
+  ic = cc;
+  issue(ic, c_lo);
+  bool whole = false;  // this workgroup holds all of the row tile's chunks
+  int row = 0, node = 0;
+
+  for (int i = c_lo; i < c_hi; ++i) {
+    const bool first = i == c_lo || cc.c == 0;
+    if (first) {
+      whole = cc.c == 0;
+      const int nrows = cc.s.x * n_rep;
+      row = min(cc.t * ROWS + 32 * rw + l31, nrows - 1);
+      node = row / n_rep;
+      const T* qr = qrot + ((((int64_t)cc.b * a.Hkv + cc.g) * N * n_rep + row) * D);
+#pragma unroll
+      for (int p = 0; p < X::QP; ++p)
+#pragma unroll
+        for (int ks = 0; ks < X::KS; ++ks)
+          q[p][ks] = *(const u32x4*)(qr + p * qlo + (2 * ks + h) * (16 / (int)sizeof(T)));
+      m = -INFINITY;
+      lsum = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+    }
+    lds_copy_wait();
+    __syncthreads();  // chunk i has landed for all; the other stage is free
+    const bool more = i + 1 < c_hi;
+    if (more) {
+      ic.next(sched);
+      issue(ic, i + 1);
+    }
+    T* kt = stage_k(i);
+    T* vt = kt + Sh::TILE;
+    const int L = cc.s.y, keys = L + cc.s.x;
+    const int k0 = cc.c * KC + kw * BKW;  // the wavefront's first key
+    // Blocks that hold nodes' keys, or places behind the last one (the loads repeat
+    // the last row there): which of the block's 32 keys the lane's row sees, and
+    // which have Inf or NaN in their V row.
+    auto sees = [&](int t0) -> uint32_t {  // t0: node of the block's first key, > -32
+      const uint32_t* words = anc + ((int64_t)cc.b * N + node) * W;
+      const int idx = t0 >> 5, sh = t0 & 31;
+      const uint32_t w0 = idx < 0 ? ~0u : idx < W ? words[idx] : 0u;
+      const uint32_t w1 = idx + 1 < W ? words[idx + 1] : 0u;
+      return sh ? (w0 >> sh) | (w1 << (32 - sh)) : w0;
+    };
+    auto unclean = [&](int t0) -> uint32_t {
+      const uint8_t* flag = vbad + ((int64_t)cc.b * a.Hkv + cc.g) * N;
+      const int kn = t0 + l31;
+      return (uint32_t)__builtin_amdgcn_ballot_w64(
+          kn >= 0 && flag[max(min(kn, cc.s.x - 1), 0)] != 0);
+    };
+    f32x16 s[NB];
+    bool bad = false;
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[nb][e] = 0.f;
+      X::scores(kt, kw * BKW + 32 * nb, q, s[nb], lane);
+      const int t0 = k0 + 32 * nb - L;
+      if (t0 > -32) {  // (uniform)
+        const uint32_t bits = sees(t0) >> (4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[nb][e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[nb][e] : -INFINITY;
+        bad |= unclean(t0) != 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[nb][e]);
+    }
+    const float mnew = fmaxf(m, pair_max32(tmax));
+    const float ref = mnew == -INFINITY ? 0.f : mnew;  // a row that has met no key yet
+    const float alpha = fast_exp2(m - ref);
+    m = mnew;
+    lsum *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[nb][e] = fast_exp2(s[nb][e] - ref);
+        lsum += s[nb][e];
+      }
+      const int row0 = kw * BKW + 32 * nb;
+      const int t0 = k0 + 32 * nb - L;
+      if (bad && t0 > -32) {  // 0 x Inf must not reach the rows that do not see the key
+        for (uint32_t x = unclean(t0); x; x &= x - 1) {
+          const int r = row0 + __builtin_ctz(x);
+          if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      X::values(vt, row0, voff, s[nb], acc, lane);
+      if (bad && t0 > -32) {  // those keys one by one, for the rows that see them
+        const uint32_t bits = sees(t0);
+        for (uint32_t x = unclean(t0); x; x &= x - 1) {
+          const int kk = __builtin_ctz(x), key = k0 + 32 * nb + kk;
+          if (key >= keys) break;
+          float p = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (8 * (e / 4) + 4 * h + e % 4 == kk) p = s[nb][e];
+          p = pair_sum32(p);
+          if ((bits >> kk) & 1) {
+            const T* vr = (const T*)a.v_cache +
+                          (((int64_t)cc.b * a.Hkv + cc.g) * a.Smax + key) * D + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                acc[dt][e] += p * to_f32(vr[32 * dt + 8 * (e / 4) + e % 4]);
+          }
+        }
+      }
+    }
+    const bool last = cc.c == cc.nck - 1;
+    if (last || !more) {
+      // the row tile's part of this workgroup ends: the key waves' sums joined in
+      // the stage just computed, then the output, or a partial in slot gw + tile
+      whole = whole && last;
+      float l = pair_sum32(lsum);
+      if constexpr (KW > 1) {
+        __syncthreads();  // all wavefronts are done with the stage
+        float* xo = (float*)kt;                    // [KW - 1][ROWS][D]
+        float* xm = (float*)(lds + 2 * Sh::STAGE);  // [KW - 1][ROWS][2]
+        const int r = 32 * rw + l31;
+        if (kw > 0) {
+          float* o = xo + ((kw - 1) * ROWS + r) * D + 4 * h;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              // (a lane's pieces rotated by its row: the rows lie D floats apart)
+              const int ch = ((8 * dt + 2 * (e / 4)) ^ (2 * (r & 3))) * 4;
+              *(f32x4*)(o + ch) = f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
+            }
+          if (h == 0) *(float2*)(xm + ((kw - 1) * ROWS + r) * 2) = make_float2(m, l);
+        }
+        __syncthreads();
+        if (kw == 0) {
+#pragma unroll
+          for (int x = 0; x < KW - 1; ++x) {
+            const float2 ml = *(const float2*)(xm + (x * ROWS + r) * 2);
+            const float mj = fmaxf(m, ml.x), rj = mj == -INFINITY ? 0.f : mj;
+            const float f0 = fast_exp2(m - rj), f1 = fast_exp2(ml.x - rj);
+            m = mj;
+            l = l * f0 + ml.y * f1;
+            const float* o = xo + (x * ROWS + r) * D + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                const int ch = ((8 * dt + 2 * (e / 4)) ^ (2 * (r & 3))) * 4;
+                const f32x4 y = *(const f32x4*)(o + ch);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[dt][e + j] = acc[dt][e + j] * f0 + y[j] * f1;
+              }
+          }
+        }
+      }
+      const int r = cc.t * ROWS + 32 * rw + l31;
+      if (kw == 0 && r < cc.s.x * n_rep) {
+        if (whole) {
+          const float inv = 1.f / l;
+          T* o = (T*)a.out + (((int64_t)cc.b * N + r / n_rep) * a.Hq + cc.g * n_rep + r % n_rep) * D +
+                 4 * h;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              T y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] = from_f32<T>(acc[dt][e + j] * inv);
+              __builtin_memcpy(__builtin_assume_aligned(o + 32 * dt + 2 * e, 4 * sizeof(T)), y,
+                               sizeof(y));
+            }
+        } else {
+          const int64_t slot = (int64_t)gw + ((int64_t)cc.b * a.Hkv + cc.g) * tiles_max + cc.t;
+          float* o = opart + (slot * ROWS + 32 * rw + l31) * D + 4 * h;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *(f32x4*)(o + 32 * dt + 2 * e) =
+                  f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
+          if (h == 0)
+            *(float2*)(mlpart + (slot * ROWS + 32 * rw + l31) * 2) = make_float2(m, l);
+        }
+      }
+    }
+    cc.next(sched);
+  }
+}
+
+// One row (b, node, query head) per WPR wavefronts: the partials of the
+// workgroups that met its row tile (kf_merge.h); rows that one workgroup
+// finished are left alone.
+template <typename T, int D, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void tree_merge_kernel(
+    TreeArgs a, const int2* __restrict__ seq, const float* __restrict__ opart,
+    const float* __restrict__ mlpart, int rows, int kc, int NWmax, int tiles_max) {
+  __shared__ __attribute__((aligned(16))) float sO[WPR > 1 ? WPR * D : 4];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t at = WPR == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
+  if (at >= (int64_t)a.B * a.N * a.Hq) return;
+  const int hq = (int)(at % a.Hq), i = (int)(at / a.Hq % a.N), b = (int)(at / a.Hq / a.N);
+  const int n_rep = a.Hq / a.Hkv, g = hq / n_rep;
+  const TreeSched sched{seq, a.B, a.Hkv, n_rep, rows, kc};
+  T* orow = (T*)a.out + at * D + 4 * lane;
+  const bool writer = lane < D / 4 && (WPR == 1 || w == 0);
+  const int2 s = seq[b];
+  if (s.x < 0 || i >= s.x) {  // a refused sequence, or an unused node
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (writer) orow[e] = from_f32<T>(s.x < 0 ? NAN : 0.f);
+    return;
+  }
+  int tot = 0, pre = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? sched.chunks(b0 + lane) : 0;
+    tot += wave_sum_int(n);
+    pre += wave_sum_int(b0 + lane < b ? n : 0);
+  }
+  const int NW = min(NWmax, tot), nck = sched.nck(s);
+  const int r = i * n_rep + hq % n_rep, t = r / rows;
+  const int c0 = pre + (g * sched.tiles(s) + t) * nck;
+  const int w0 = chunk_owner(c0, tot, NW), ns = chunk_owner(c0 + nck - 1, tot, NW) - w0 + 1;
+  if (ns == 1) return;
+  const int64_t first =
+      ((int64_t)w0 + ((int64_t)b * a.Hkv + g) * tiles_max + t) * rows + r % rows;
+  const f32x4 o = merge_row<D, WPR>(opart + first * D, mlpart + first * 2, (int64_t)rows * D,
+                                    (int64_t)rows * 2, ns, sO, WPR == 1 ? 0 : w, lane);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (writer) orow[e] = from_f32<T>(o[e]);
+}
+
+// ---- host ----------------------------------------------------------------------
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// workspace: rotated queries, ancestor masks, per sequence (nodes in use or -1,
-// prefix length), per (b, KV head, node) whether its V row holds Inf or NaN
+// The stream kernel's shape for a call: row waves (0: one wavefront per row) and
+// what follows from it.
+struct Plan {
+  int rw, bkw, rows, kc, tiles, grid, per_cu;
+};
+Plan plan_of(const TreeArgs& a) {
+  Plan p = {};
+  const int n_rep = a.Hq / a.Hkv, m = a.N * n_rep;
+  if (a.D != 64 && a.D != 128) return p;
+  // enough row waves for the pair's rows; float32 has no LDS for four key waves
+  p.rw = m <= 32 && a.dtype != F32 ? 1 : m <= 64 ? 2 : 4;
+  p.bkw = p.rw == 4 && a.dtype != F32 ? 64 : 32;
+  p.rows = 32 * p.rw;
+  p.kc = p.bkw * 4 / p.rw;
+  p.tiles = (m + p.rows - 1) / p.rows;
+  const size_t lds = (size_t)4 * p.kc * a.D * (a.dtype == F32 ? 4 : 2) +
+                     (size_t)(4 / p.rw - 1) * p.rows * 8;  // Shape::LDS
+  p.per_cu = 2 * lds <= 160 * 1024 && !(a.dtype == F32 && a.D == 128) ? 2 : 1;  // Shape::PER_CU
+  const int64_t chunks = (int64_t)a.B * a.Hkv * p.tiles * ((a.max_len + p.kc - 1) / p.kc);
+  if (chunks >= INT_MAX) return Plan{};
+  p.grid = (int)std::min<int64_t>(p.per_cu * std::min(device_cu_count(), 512), chunks);
+  return p;
+}
+
+// workspace: rotated queries (hi and lo, or float32: four bytes an element at
+// the most), ancestor masks, per sequence (nodes in use or -1, prefix length),
+// per (b, KV head, node) whether its V row holds Inf or NaN, the partials
 struct Ws {
   void* qrot;
   uint32_t* anc;
   int2* seq;
   uint8_t* vbad;
+  float *opart, *mlpart;
   size_t bytes;
 };
 Ws carve(const TreeArgs& a, void* p) {
-  const size_t el = a.dtype == F32 ? 4 : 2;
   const size_t W = (a.N + 31) / 32;
   char* c = (char*)p;
   Ws w;
   w.qrot = c;
-  c += up256((size_t)a.B * a.N * a.Hq * a.D * el);
+  c += up256((size_t)a.B * a.N * a.Hq * a.D * 4);
   w.anc = (uint32_t*)c;
   c += up256((size_t)a.B * a.N * W * 4);
   w.seq = (int2*)c;
   c += up256((size_t)a.B * sizeof(int2));
   w.vbad = (uint8_t*)c;
   c += up256((size_t)a.B * a.Hkv * a.N);
+  const Plan pl = plan_of(a);
+  const size_t prow = pl.rw ? ((size_t)pl.grid + (size_t)a.B * a.Hkv * pl.tiles) * pl.rows : 0;
+  w.opart = (float*)c;
+  c += up256(prow * a.D * 4);
+  w.mlpart = (float*)c;
+  c += up256(prow * 2 * 4);
   w.bytes = (size_t)(c - (char*)p);
   return w;
+}
+
+template <typename T, int D, int RW, int BKW>
+int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
+  using Sh = Shape<T, D, RW, BKW>;
+  auto kernel = tree_stream_kernel<T, D, RW, BKW>;
+  if (Sh::LDS > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(
+        (const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::LDS);
+    if (e != hipSuccess) {
+      set_error("tree attention: %s", hipGetErrorString(e));
+      return KF_ERR_HIP;
+    }
+  }
+  KF_LAUNCH("tree_stream", kernel, dim3(p.grid), dim3(256), Sh::LDS, a.stream, a,
+            (const T*)w.qrot, qlo, w.anc, w.seq, w.vbad, (a.N + 31) / 32, w.opart, w.mlpart,
+            p.tiles);
+  KF_CHECK_LAUNCH();
+  return KF_OK;
+}
+
+template <typename T, int D>
+int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
+  int rc;
+  if constexpr (std::is_same<T, float>::value)
+    rc = p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p, qlo) : launch_stream<T, D, 4, 32>(a, w, p, qlo);
+  else
+    rc = p.rw == 1   ? launch_stream<T, D, 1, 32>(a, w, p, qlo)
+         : p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p, qlo)
+                     : launch_stream<T, D, 4, 64>(a, w, p, qlo);
+  if (rc) return rc;
+  const int rows = a.B * a.N * a.Hq;
+  const int64_t tiles = (int64_t)a.B * a.Hkv * p.tiles, nck = (a.max_len + p.kc - 1) / p.kc;
+  const int wpr = merge_waves((int)std::min(nck, p.grid / tiles + 1));
+  KF_LAUNCH("tree_merge",
+            (wpr == 1   ? tree_merge_kernel<T, D, 1>
+             : wpr == 4 ? tree_merge_kernel<T, D, 4>
+                        : tree_merge_kernel<T, D, 16>),
+            dim3(wpr == 1 ? (rows + 3) / 4 : rows), dim3(wpr == 1 ? 256 : 64 * wpr), 0, a.stream,
+            a, w.seq, w.opart, w.mlpart, p.rows, p.kc, p.grid, p.tiles);
+  KF_CHECK_LAUNCH();
+  return KF_OK;
 }
 
 template <typename T>
@@ -230,12 +753,26 @@ int tree_typed(const TreeArgs& a, void* workspace) {
   const Ws w = carve(a, workspace);
   const int W = (a.N + 31) / 32, per = 16;
   const int64_t rows = (int64_t)a.N * (a.Hq + 2 * a.Hkv);
-  KF_LAUNCH("tree_prep", tree_prep_kernel<T>, dim3((unsigned)((rows + per - 1) / per), a.B),
-            dim3(256), 0, a.stream, a, (T*)w.qrot, w.anc, w.seq, w.vbad, W, per);
+  const dim3 grid((unsigned)((rows + per - 1) / per), a.B);
+  Plan p = plan_of(a);
+  // (the stream kernel's direct loads and vector stores need aligned buffers)
+  if (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.out) % 16 != 0) p = Plan{};
+  const int64_t qlo = (int64_t)a.B * a.N * a.Hq * a.D;
+  if (p.rw && !std::is_same<T, float>::value) {
+    if constexpr (!std::is_same<T, float>::value)
+      KF_LAUNCH("tree_prep", (tree_prep_kernel<T, true>), grid, dim3(256), 0, a.stream, a, w.qrot,
+                qlo, w.anc, w.seq, w.vbad, W, per);
+  } else {
+    KF_LAUNCH("tree_prep", (tree_prep_kernel<T, false>), grid, dim3(256), 0, a.stream, a, w.qrot,
+              qlo, w.anc, w.seq, w.vbad, W, per);
+  }
   KF_CHECK_LAUNCH();
+  if (p.rw)
+    return a.D == 128 ? stream_and_merge<T, 128>(a, w, p, qlo)
+                      : stream_and_merge<T, 64>(a, w, p, qlo);
   KF_LAUNCH("tree_rows", tree_rows_kernel<T>,
             dim3((unsigned)(((int64_t)a.B * a.N * a.Hq + 3) / 4)), dim3(256), 0, a.stream, a,
-            (const T*)w.qrot, w.anc, w.seq, W);
+            (const float*)w.qrot, w.anc, w.seq, W);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }

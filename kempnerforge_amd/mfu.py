@@ -171,7 +171,8 @@ _ATTN_KEYS = ("fwd_mfma", "fwd32_kernel", "bwd_dkdv", "dkdv_reduce_kernel", "bwd
               "capture_f32_kernel", "fwd_generic", "fwd_f32_kernel", "rows_f32_kernel",
               "stats_f32_kernel", "mask_prep_f32_kernel", "dkdv_parts_f32_kernel",
               "widen_kernel", "narrow_kernel", "cache_append", "append_kernel",
-              "append_rows_kernel", "tree_prep_kernel", "tree_rows_kernel", "verify_kernel",
+              "append_rows_kernel", "tree_prep_kernel", "tree_rows_kernel", "tree_stream_kernel",
+              "tree_merge_kernel", "verify_kernel",
               "cache_keep_kernel", "kf::attn", "flash", "fmha", "attention")
 _MATMUL_KEYS = ("gemm", "mm", "matmul", "dot", "bmm", "cublas", "nvjet", "cutlass",
                 "cijk_", "hipblaslt", "rocblas", "ck_tile", "wvsplitk")

@@ -3,14 +3,12 @@
 The reference has no counterpart (its ``generate`` decodes one token per step,
 ``kempnerforge/model/generate.py:60-131``); the attention it restates is the decode
 of ``kempnerforge/model/attention.py:165-175,229-231`` with a mask among the new
-tokens, RoPE rounded as the reference's eager ``apply_rope`` rounds it.
+tokens.
 """
 
 from __future__ import annotations
 
 import torch
-
-from oracle import attention_ref as ref
 
 
 def ancestors(parents: list[int]) -> list[list[int]]:
@@ -22,47 +20,49 @@ def ancestors(parents: list[int]) -> list[list[int]]:
     return out
 
 
-def rms_norm(x, w, eps):
-    """RMSNorm over the last dimension in float32, rounded to x's dtype
-    (``kempnerforge/model/norm.py:22-27``)."""
-    f = x.float()
-    f = f * torch.rsqrt(f.pow(2).mean(-1, keepdim=True) + eps)
-    return (f * w.float()).to(x.dtype)
+def _rotate(x, cos, sin):
+    """Half-split RoPE of ``x [..., D]`` by one row of the tables, in 64 bits."""
+    half = x.shape[-1] // 2
+    c, s = cos.double(), sin.double()
+    x1, x2 = x[..., :half], x[..., half:]
+    return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
-def tree_step(q, k, v, kc, vc, lens, cos, sin, parents, counts=None, row_offset=0,
-              q_norm=None, k_norm=None, eps=1e-5):
-    """out (float64), the caches after the step, and per output element the sum
-    of p |v| (what errors of the probabilities multiply).  ``parents``: one list
-    per sequence.  Unused nodes: zeros, cache rows as they were."""
+def rotated(x, lens, cos, sin, parents, counts=None, row_offset=0, norm=None, eps=1e-5):
+    """``x [B, N, H, D]`` (RMS-normalised first with ``norm``) rotated at each
+    node's position, in 64 bits; unused nodes are left zero."""
+    y = torch.zeros(x.shape, dtype=torch.float64)
+    for b in range(x.shape[0]):
+        n = x.shape[1] if counts is None else int(counts[b])
+        for i, anc in enumerate(ancestors(parents[b][:n])):
+            r = x[b, i].double()
+            if norm is not None:
+                r = r / (r.pow(2).mean(-1, keepdim=True) + eps).sqrt() * norm.double()
+            at = int(lens[b]) + len(anc) - 1 - row_offset
+            y[b, i] = _rotate(r, cos[at], sin[at])
+    return y
+
+
+def tree_attention(q, kc, vc, lens, parents, counts=None):
+    """out (float64) of rotated queries ``q [B, N, Hq, D]`` over caches that hold the
+    nodes' rows behind the prefix, and per output element the sum of p |v| (what
+    errors of the probabilities multiply).  Unused nodes: zeros."""
     B, N, Hq, D = q.shape
-    Hkv = k.shape[2]
+    Hkv = kc.shape[1]
     rep = Hq // Hkv
-    kc, vc = kc.clone(), vc.clone()
     out = torch.zeros(B, N, Hq, D, dtype=torch.float64)
     mag = torch.zeros_like(out)
     for b in range(B):
         n = N if counts is None else int(counts[b])
         L = int(lens[b])
-        anc = ancestors(parents[b][:n])
-        qb, kb = q[b, :n], k[b, :n]
-        if q_norm is not None:
-            qb, kb = rms_norm(qb, q_norm, eps), rms_norm(kb, k_norm, eps)
-        for i in range(n):
-            at = L + len(anc[i]) - 1 - row_offset
-            c, s = cos[at:at + 1], sin[at:at + 1]
-            kc[b, :, L + i] = ref.apply_rope(kb[i][None, :, None], c, s)[0, :, 0]
-            vc[b, :, L + i] = v[b, i]
-        for i in range(n):
-            at = L + len(anc[i]) - 1 - row_offset
-            qi = ref.apply_rope(qb[i][None, :, None], cos[at:at + 1], sin[at:at + 1])[0, :, 0]
-            rows = list(range(L)) + [L + j for j in anc[i]]
+        for i, anc in enumerate(ancestors(parents[b][:n])):
+            rows = list(range(L)) + [L + j for j in anc]
             kk, vv = kc[b][:, rows].double(), vc[b][:, rows].double()
             p = torch.softmax(
-                (qi.double().view(Hkv, rep, D) @ kk.transpose(1, 2)) * D ** -0.5, dim=-1)
+                (q[b, i].double().view(Hkv, rep, D) @ kk.transpose(1, 2)) * D ** -0.5, dim=-1)
             out[b, i] = (p @ vv).view(Hq, D)
             mag[b, i] = (p @ vv.abs()).view(Hq, D)
-    return out, kc, vc, mag
+    return out, mag
 
 
 def verify(logits, tokens, uniforms, temperature, parents, counts=None, draft_logits=None):

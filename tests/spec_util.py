@@ -36,19 +36,42 @@ def tree_inputs(dtype, B, N, Hq, Hkv, D, Smax, seed=0):
     return q, k, v, kc, vc, cos, sin
 
 
+# what is left of q when it is the sum of two numbers of the type (float32: q itself)
+Q_LEFT = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}
+
+
+def check_rows(kcd, kc, k64, lens, counts, dtype, more=0.0):
+    """The nodes' keys in the cache: the rotation in 32 bits (two products and a
+    sum, 3 steps of 2^-24 of their magnitude, below 8 for N(0, 1) rows), rounded
+    once; all other rows as they were.  ``more``: relative error before the
+    rotation."""
+    got, want = kcd.cpu(), kc.clone()
+    for b, L in enumerate(lens):
+        n = k64.shape[1] if counts is None else counts[b]
+        rows = k64[b, :n].transpose(0, 1)
+        new = got[b, :, L:L + n].double()
+        bound = (half_ulp(rows, dtype) + 8 * (3 * U32 + more)) * (1 + 2.0 ** -7)
+        assert ((new - rows).abs() <= bound).all(), b
+        want[b, :, L:L + n] = got[b, :, L:L + n]
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
 def tree_bound(want, mag, dtype, D, keys, dot=12.0, moved=0.0):
-    """Per element, how far an output may be from the 64-bit one.
+    """Per element, how far an output may be from the 64-bit one over the same
+    cache rows.
 
     Scores are sums of D products in 32 bits, each rounded at most once more than
-    exactly (D + 4 steps of 2^-24 of the products' magnitudes, whose sum times
-    D^-1/2 is at most ``dot``: the rows are N(0, 1), so it is below |q| |k| D^-1/2,
-    about D^1/2 = 11.3 with the spread of the norms); a hardware exponential adds
-    2^-22.  Numerator and denominator both carry that, so the probabilities are
-    off by twice it, relatively; sums over the keys add one step each, and P is
-    rounded to the storage type before it multiplies V (half a step).  All of it
-    multiplies sum p |v| = ``mag``.  The result is rounded once more.  ``moved``:
-    what the scores are off by beyond that (operands rounded elsewhere)."""
-    rel = (2 * ((D + 4) * U32 * dot + moved) + 2 ** -21 + 2 * (keys + 8) * U32 + P_STEP[dtype])
+    exactly (D + 8 steps of 2^-24 of the products' magnitudes, the rotation's
+    among them, whose sum times D^-1/2 is at most ``dot``: the rows are N(0, 1), so
+    it is below |q| |k| D^-1/2, about D^1/2 = 11.3 with the spread of the norms), and q
+    enters them to Q_LEFT; a hardware exponential adds 2^-22.  Numerator and
+    denominator both carry that, so the probabilities are off by twice it,
+    relatively; sums over the keys add one step each, and P is rounded to the
+    storage type before it multiplies V (half a step).  All of it multiplies sum
+    p |v| = ``mag``.  The result is rounded once more.  ``moved``: what the scores
+    are off by beyond that."""
+    rel = (2 * (((D + 8) * U32 + Q_LEFT[dtype]) * dot + moved) + 2 ** -21
+           + 2 * (keys + 8) * U32 + P_STEP[dtype])
     return rel * mag + half_ulp(want, dtype)
 
 
@@ -84,4 +107,5 @@ def verify_inputs(dtype, B, N, V, seed=0, parents=None, temperature=1.0, drafts=
     return logits, tokens, torch.rand(B, N, generator=g), draft
 
 
-__all__ = ["trees", "tree_inputs", "tree_bound", "check_tree", "verify_inputs", "spec_ref"]
+__all__ = ["trees", "tree_inputs", "check_rows", "tree_bound", "check_tree", "verify_inputs",
+           "spec_ref"]
