@@ -24,11 +24,11 @@
 // multiplies V; the sums, the row maxima and the row sums stay in 32 bits.
 #include "kf_common.h"
 #include "kf_internal.h"
-#include "kf_merge.h"
 #include "kf_mfma.h"
 #include "kf_split.h"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 namespace kf {
@@ -43,6 +43,31 @@ __device__ __forceinline__ bool finite(T x) {
   return fabsf(to_f32(x)) < INFINITY;  // false for NaN too
 }
 
+// One piece of a row: E = 16 / sizeof(T) elements of each RoPE half, 16-byte
+// loads and stores.
+template <typename T>
+struct Piece {
+  static constexpr int E = 16 / sizeof(T);
+  u32x4 a, b;
+  __device__ __forceinline__ void load(const T* row, int d, int half) {
+    a = *(const u32x4*)(row + d);
+    b = *(const u32x4*)(row + d + half);
+  }
+  static __device__ __forceinline__ void unpack(const u32x4& u, float* f) {
+    if constexpr (sizeof(T) == 4)
+      __builtin_memcpy(f, &u, 16);
+    else
+      unpack8<T>(u, f);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    if constexpr (sizeof(T) == 4)
+      return u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                   __float_as_uint(f[3])};
+    else
+      return pack8<T>(f);
+  }
+};
+
 // One workgroup: sequence blockIdx.y, `per` of its N * (Hq + 2 Hkv) rows.  The
 // queries go to `qrot` scaled by D^-1/2 log2(e), as [B][Hkv][node, head of the
 // group][D]: float32, or (SPLIT) hi and, `qlo` elements behind, lo.
@@ -52,7 +77,13 @@ __device__ __forceinline__ bool finite(T x) {
 // rounds cover 256 nodes whatever their depth (a walk up a chain of 200 would
 // take 200 dependent reads).  Every workgroup of a sequence forms them again
 // (under a microsecond, no launch of its own); the first one stores them.
-template <typename T, bool SPLIT>
+//
+// DV > 0: the head size, rows of 16-byte pieces (G lanes a row, per = 256 / G
+// rows, one per lane group): bound by the latency of three dependent loads (the
+// lengths and parents, the table row, the stores), so a row's own loads are
+// issued before the masks are formed.  DV = 0: any head size, one wavefront a
+// row and element by element.
+template <typename T, bool SPLIT, int DV>
 __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __restrict__ qrot,
                                                         int64_t qlo, uint32_t* __restrict__ anc,
                                                         int2* __restrict__ seq,
@@ -61,7 +92,22 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __rest
   __shared__ uint32_t smask[MAXN][MAXW + 1];
   __shared__ int sptr[MAXN], sdepth[MAXN];
   const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int N = a.N, D = a.D, half = D / 2;
+  const int N = a.N, D = DV > 0 ? DV : a.D, half = D / 2;
+  const int heads = a.Hq + 2 * a.Hkv, n_rep = a.Hq / a.Hkv;
+  // the lane group's row: node vi, head vh (queries, keys, values)
+  constexpr int G = DV > 0 ? DV / 2 / Piece<T>::E : 1;
+  const int vr = blockIdx.x * per + t / G;
+  const int vi = vr / heads, vh = vr % heads, vd = t % G * Piece<T>::E;
+  Piece<T> x;
+  if constexpr (DV > 0) {
+    if (vi < N) {
+      const int64_t node = (int64_t)b * N + vi;
+      const T* src = vh < a.Hq            ? (const T*)a.q_new + (node * a.Hq + vh) * D
+                     : vh < a.Hq + a.Hkv ? (const T*)a.k_new + (node * a.Hkv + vh - a.Hq) * D
+                                         : (const T*)a.v_new + (node * a.Hkv + vh - a.Hq - a.Hkv) * D;
+      x.load(src, vd, half);
+    }
+  }
   const int L = a.lens[b], n = a.counts ? a.counts[b] : N;
   bool bad = n < 0 || n > N || L < 0 || (int64_t)L + n > a.max_len;
   const int used = bad ? 0 : n;
@@ -113,7 +159,86 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __rest
       for (int k = 0; k < W; ++k) anc[((int64_t)b * N + t) * W + k] = smask[t][k];
   }
   if (bad) return;
-  const int heads = a.Hq + 2 * a.Hkv, n_rep = a.Hq / a.Hkv;
+  if constexpr (DV > 0) {
+    constexpr int E = Piece<T>::E;
+    if (vi >= n) return;
+    const int64_t slot = (int64_t)L + vi;
+    float f1[E], f2[E];
+    Piece<T>::unpack(x.a, f1);
+    Piece<T>::unpack(x.b, f2);
+    if (vh >= a.Hq + a.Hkv) {
+      const int g = vh - a.Hq - a.Hkv;
+      T* dst = (T*)a.v_cache + (((int64_t)b * a.Hkv + g) * a.Smax + slot) * D + vd;
+      *(u32x4*)dst = x.a;
+      *(u32x4*)(dst + half) = x.b;
+      bool fin = true;
+#pragma unroll
+      for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(!fin);
+      const uint64_t mine = ((1ull << G) - 1) << (lane / G * G);
+      if (t % G == 0) vbad[((int64_t)b * a.Hkv + g) * N + vi] = (m & mine) != 0;
+      return;
+    }
+    const bool is_q = vh < a.Hq;
+    const float* nw = is_q ? a.q_norm_w : a.k_norm_w;
+    const int64_t row = ((int64_t)L + sdepth[vi] - a.rope_row_offset) * half + vd;
+    float c[E], sn[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      c[e] = a.cos[row + e];
+      sn[e] = a.sin[row + e];
+    }
+    if (nw != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss += f1[e] * f1[e] + f2[e] * f2[e];
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) ss += __shfl_xor(ss, o, 64);
+      const float rs = rsqrtf(ss / (float)D + a.norm_eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        f1[e] = f1[e] * rs * nw[vd + e];
+        f2[e] = f2[e] * rs * nw[vd + half + e];
+      }
+    }
+    float y1[E], y2[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      y1[e] = f1[e] * c[e] - f2[e] * sn[e];
+      y2[e] = f2[e] * c[e] + f1[e] * sn[e];
+    }
+    if (!is_q) {
+      const int g = vh - a.Hq;
+      T* dst = (T*)a.k_cache + (((int64_t)b * a.Hkv + g) * a.Smax + slot) * D + vd;
+      *(u32x4*)dst = Piece<T>::pack(y1);
+      *(u32x4*)(dst + half) = Piece<T>::pack(y2);
+      return;
+    }
+    const int g = vh / n_rep;
+    const float sc = a.scale * kLog2e;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      y1[e] *= sc;
+      y2[e] *= sc;
+    }
+    T* dst = (T*)qrot +
+             (((int64_t)b * a.Hkv + g) * N * n_rep + (int64_t)vi * n_rep + vh % n_rep) * D + vd;
+    const u32x4 h1 = Piece<T>::pack(y1), h2 = Piece<T>::pack(y2);
+    *(u32x4*)dst = h1;
+    *(u32x4*)(dst + half) = h2;
+    if constexpr (SPLIT) {
+      Piece<T>::unpack(h1, f1);
+      Piece<T>::unpack(h2, f2);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        y1[e] -= f1[e];
+        y2[e] -= f2[e];
+      }
+      *(u32x4*)(dst + qlo) = Piece<T>::pack(y1);
+      *(u32x4*)(dst + qlo + half) = Piece<T>::pack(y2);
+    }
+    return;
+  }
   const int64_t r1 = min((int64_t)n * heads, (int64_t)(blockIdx.x + 1) * per);
   for (int64_t r = (int64_t)blockIdx.x * per + w; r < r1; r += 4) {
     const int i = (int)(r / heads), h = (int)(r % heads);
@@ -603,47 +728,74 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   }
 }
 
-// One row (b, node, query head) per WPR wavefronts: the partials of the
-// workgroups that met its row tile (kf_merge.h); rows that one workgroup
-// finished are left alone.
-template <typename T, int D, int WPR>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void tree_merge_kernel(
+// The rows of tile blockIdx.x, 16 bytes of a row per thread and
+// blockIdx.y's share of them: the partials of the workgroups that met the tile
+// rescaled to a common maximum and summed; a tile that one workgroup finished is
+// left alone.  The schedule's divisions are the workgroup's, not each row's:
+// one wavefront per row took 14.5 us where this takes ... (tree_batch's sizes).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(
     TreeArgs a, const int2* __restrict__ seq, const float* __restrict__ opart,
     const float* __restrict__ mlpart, int rows, int kc, int NWmax, int tiles_max) {
-  __shared__ __attribute__((aligned(16))) float sO[WPR > 1 ? WPR * D : 4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t at = WPR == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
-  if (at >= (int64_t)a.B * a.N * a.Hq) return;
-  const int hq = (int)(at % a.Hq), i = (int)(at / a.Hq % a.N), b = (int)(at / a.Hq / a.N);
-  const int n_rep = a.Hq / a.Hkv, g = hq / n_rep;
-  const TreeSched sched{seq, a.B, a.Hkv, n_rep, rows, kc};
-  T* orow = (T*)a.out + at * D + 4 * lane;
-  const bool writer = lane < D / 4 && (WPR == 1 || w == 0);
+  constexpr int LPR = D / 4;  // lanes of a row
+  const int lane = threadIdx.x & 63, n_rep = a.Hq / a.Hkv;
+  const int item = blockIdx.x, t = item % tiles_max, bg = item / tiles_max, b = bg / a.Hkv,
+            g = bg % a.Hkv;
+  const int r = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+  const int row = t * rows + r, i = row / n_rep, hq = g * n_rep + row % n_rep;
   const int2 s = seq[b];
-  if (s.x < 0 || i >= s.x) {  // a refused sequence, or an unused node
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (writer) orow[e] = from_f32<T>(s.x < 0 ? NAN : 0.f);
-    return;
-  }
+  const TreeSched sched{seq, a.B, a.Hkv, n_rep, rows, kc};
   int tot = 0, pre = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int n = b0 + lane < a.B ? sched.chunks(b0 + lane) : 0;
     tot += wave_sum_int(n);
     pre += wave_sum_int(b0 + lane < b ? n : 0);
   }
+  if (i >= a.N || r >= rows) return;
+  T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + hq) * D + col;
+  T y[4];
+  if (s.x < 0 || i >= s.x) {  // a refused sequence, or an unused node
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(s.x < 0 ? NAN : 0.f);
+    __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
+    return;
+  }
   const int NW = min(NWmax, tot), nck = sched.nck(s);
-  const int r = i * n_rep + hq % n_rep, t = r / rows;
   const int c0 = pre + (g * sched.tiles(s) + t) * nck;
   const int w0 = chunk_owner(c0, tot, NW), ns = chunk_owner(c0 + nck - 1, tot, NW) - w0 + 1;
   if (ns == 1) return;
-  const int64_t first =
-      ((int64_t)w0 + ((int64_t)b * a.Hkv + g) * tiles_max + t) * rows + r % rows;
-  const f32x4 o = merge_row<D, WPR>(opart + first * D, mlpart + first * 2, (int64_t)rows * D,
-                                    (int64_t)rows * 2, ns, sO, WPR == 1 ? 0 : w, lane);
+  const int64_t first = ((int64_t)w0 + item) * rows + r;
+  const float* ob = opart + first * D + col;
+  const float2* mb = (const float2*)mlpart + first;
+  // (m, l) of all partials are read twice: for the maximum, then with the sums
+  float M = -INFINITY;
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < ns; j0 += U) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (writer) orow[e] = from_f32<T>(o[e]);
+    for (int u = 0; u < U; ++u) M = fmaxf(M, mb[(int64_t)min(j0 + u, ns - 1) * rows].x);
+  }
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < ns; j0 += U) {
+    f32x4 po[U];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = min(j0 + u, ns - 1);
+      ml[u] = mb[j * rows];
+      po[u] = *(const f32x4*)(ob + j * rows * D);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = j0 + u < ns ? fast_exp2(ml[u].x - M) : 0.f;
+      l += w != 0.f ? w * ml[u].y : 0.f;  // (a partial of weight 0 is left out)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += w != 0.f ? w * po[u][e] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[e] / l);
+  __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -710,9 +862,16 @@ template <typename T, int D, int RW, int BKW>
 int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
   using Sh = Shape<T, D, RW, BKW>;
   auto kernel = tree_stream_kernel<T, D, RW, BKW>;
-  if (Sh::LDS > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(
-        (const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::LDS);
+  if (Sh::LDS > 64 * 1024) {  // asked for once per device
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (e == hipSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)Sh::LDS);
+      if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    }
     if (e != hipSuccess) {
       set_error("tree attention: %s", hipGetErrorString(e));
       return KF_ERR_HIP;
@@ -735,15 +894,10 @@ int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo)
          : p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p, qlo)
                      : launch_stream<T, D, 4, 64>(a, w, p, qlo);
   if (rc) return rc;
-  const int rows = a.B * a.N * a.Hq;
-  const int64_t tiles = (int64_t)a.B * a.Hkv * p.tiles, nck = (a.max_len + p.kc - 1) / p.kc;
-  const int wpr = merge_waves((int)std::min(nck, p.grid / tiles + 1));
-  KF_LAUNCH("tree_merge",
-            (wpr == 1   ? tree_merge_kernel<T, D, 1>
-             : wpr == 4 ? tree_merge_kernel<T, D, 4>
-                        : tree_merge_kernel<T, D, 16>),
-            dim3(wpr == 1 ? (rows + 3) / 4 : rows), dim3(wpr == 1 ? 256 : 64 * wpr), 0, a.stream,
-            a, w.seq, w.opart, w.mlpart, p.rows, p.kc, p.grid, p.tiles);
+  const int rpw = 256 / (D / 4);  // rows of a workgroup
+  KF_LAUNCH("tree_merge", (tree_merge_kernel<T, D>),
+            dim3(a.B * a.Hkv * p.tiles, (p.rows + rpw - 1) / rpw), dim3(256), 0, a.stream, a,
+            w.seq, w.opart, w.mlpart, p.rows, p.kc, p.grid, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
@@ -751,21 +905,21 @@ int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo)
 template <typename T>
 int tree_typed(const TreeArgs& a, void* workspace) {
   const Ws w = carve(a, workspace);
-  const int W = (a.N + 31) / 32, per = 16;
-  const int64_t rows = (int64_t)a.N * (a.Hq + 2 * a.Hkv);
-  const dim3 grid((unsigned)((rows + per - 1) / per), a.B);
   Plan p = plan_of(a);
-  // (the stream kernel's direct loads and vector stores need aligned buffers)
-  if (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.out) % 16 != 0) p = Plan{};
+  // (the stream kernel's direct loads and the vector rows need aligned buffers)
+  if (((uintptr_t)a.q_new | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_cache |
+       (uintptr_t)a.v_cache | (uintptr_t)a.out) % 16 != 0)
+    p = Plan{};
   const int64_t qlo = (int64_t)a.B * a.N * a.Hq * a.D;
-  if (p.rw && !std::is_same<T, float>::value) {
-    if constexpr (!std::is_same<T, float>::value)
-      KF_LAUNCH("tree_prep", (tree_prep_kernel<T, true>), grid, dim3(256), 0, a.stream, a, w.qrot,
-                qlo, w.anc, w.seq, w.vbad, W, per);
-  } else {
-    KF_LAUNCH("tree_prep", (tree_prep_kernel<T, false>), grid, dim3(256), 0, a.stream, a, w.qrot,
-              qlo, w.anc, w.seq, w.vbad, W, per);
-  }
+  constexpr bool SPLIT = !std::is_same<T, float>::value;
+  auto prep = p.rw == 0     ? tree_prep_kernel<T, false, 0>
+              : a.D == 128 ? tree_prep_kernel<T, SPLIT, 128>
+                           : tree_prep_kernel<T, SPLIT, 64>;
+  const int W = (a.N + 31) / 32;
+  const int per = p.rw ? 256 / (a.D / 2 / Piece<T>::E) : 16;
+  const int64_t rows = (int64_t)a.N * (a.Hq + 2 * a.Hkv);
+  KF_LAUNCH("tree_prep", prep, dim3((unsigned)((rows + per - 1) / per), a.B), dim3(256), 0,
+            a.stream, a, w.qrot, qlo, w.anc, w.seq, w.vbad, W, per);
   KF_CHECK_LAUNCH();
   if (p.rw)
     return a.D == 128 ? stream_and_merge<T, 128>(a, w, p, qlo)

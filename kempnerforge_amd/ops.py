@@ -14,9 +14,11 @@ only accept GPU tensors: there is no CPU path.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import functools
+import operator
 import weakref
 from typing import Optional
 
@@ -489,38 +491,43 @@ def cache_append_raw(k_new, v_new, cos, sin, k_cache, v_cache, start: int) -> No
 TREE_MAX_NODES = 256  # KF_TREE_MAX_NODES
 
 
-def _on_device(t: torch.Tensor):
-    """The context in which the library sees ``t``'s device as the current one."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_SAME = contextlib.nullcontext()
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
-def _same_device(t: torch.Tensor, **others) -> None:
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise RuntimeError(f"{name} must be on the same device as the others ({t.device}, "
-                               f"got {o.device})")
+def _on_device(index: int):
+    """The context in which the library sees device ``index`` as the current one."""
+    return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _tree_args(parents, counts, B: int, N: int, device):
+def _one_device(*ts) -> int:
+    """The one GPU that all tensors (None: absent) lie on."""
+    dev = {t.get_device() for t in ts if t is not None}
+    if len(dev) != 1 or -1 in dev:
+        _require_gpu(*(t for t in ts if t is not None))
+        raise RuntimeError(f"the tensors must lie on one device (got {sorted(dev)})")
+    return dev.pop()
+
+
+_INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _tree_args(parents, counts, B: int, N: int):
     """``parents`` (``[N]`` or ``[B, N]``, None for a chain) and ``counts`` (``[B]`` or
     None) as the contiguous int32 tensors the kernels read, and the parents' row stride."""
     stride = 0
-    for name, t in (("parents", parents), ("counts", counts)):
-        if t is None:
-            continue
-        if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-            raise TypeError(f"{name} must be an integer tensor (got {t.dtype})")
-        if t.device != device:
-            raise RuntimeError(f"{name} must be on the same device as the others")
     if parents is not None:
-        if tuple(parents.shape) not in ((N,), (B, N)):
+        if parents.dtype not in _INTS:
+            raise TypeError(f"parents must be an integer tensor (got {parents.dtype})")
+        if parents.shape == (B, N):
+            stride = N
+        elif parents.shape != (N,):
             raise ValueError(f"parents must be [{N}] or [{B}, {N}] (got {tuple(parents.shape)})")
-        stride = N if parents.dim() == 2 else 0
         parents = parents.to(torch.int32).contiguous()
     if counts is not None:
-        if tuple(counts.shape) != (B,):
+        if counts.dtype not in _INTS:
+            raise TypeError(f"counts must be an integer tensor (got {counts.dtype})")
+        if counts.shape != (B,):
             raise ValueError(f"counts must be [{B}] (got {tuple(counts.shape)})")
         counts = counts.to(torch.int32).contiguous()
     return parents, stride, counts
@@ -545,55 +552,54 @@ def tree_decode_raw(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, *,
     As in :func:`decode_raw`, what lies on the device is checked there: a
     sequence whose length, count, parents or RoPE rows are out of range gets NaN
     outputs and no cache write."""
-    _require_gpu(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin)
     lib = _lib.load()
-    if q_new.dim() != 4 or k_new.dim() != 4 or k_cache.dim() != 4:
+    qs, ks, cs, dtype = q_new.shape, k_new.shape, k_cache.shape, q_new.dtype
+    if len(qs) != 4 or len(ks) != 4 or len(cs) != 4:
         raise ValueError("q_new, k_new, v_new and the caches must have four dimensions")
-    B, N, Hq, D = q_new.shape
-    Hkv, Smax = k_cache.shape[1], k_cache.shape[2]
-    if tuple(k_new.shape) != (B, N, Hkv, D) or k_new.shape != v_new.shape:
+    B, N, Hq, D = qs
+    Hkv, Smax = cs[1], cs[2]
+    if ks != (B, N, Hkv, D) or v_new.shape != ks:
         raise ValueError(f"k_new and v_new must be [{B}, {N}, {Hkv}, {D}] "
-                         f"(got {tuple(k_new.shape)}, {tuple(v_new.shape)})")
-    if tuple(k_cache.shape) != (B, Hkv, Smax, D) or k_cache.shape != v_cache.shape:
+                         f"(got {tuple(ks)}, {tuple(v_new.shape)})")
+    if cs[0] != B or cs[3] != D or v_cache.shape != cs:
         raise ValueError(f"the KV caches must be [{B}, n_kv_heads, max_seq_len, {D}] "
-                         f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
-    if any(t.dtype != q_new.dtype for t in (k_new, v_new, k_cache, v_cache)):
+                         f"(got {tuple(cs)}, {tuple(v_cache.shape)})")
+    if not dtype == k_new.dtype == v_new.dtype == k_cache.dtype == v_cache.dtype:
         raise TypeError("q_new, k_new, v_new and the caches must share a dtype")
     if not 1 <= N <= TREE_MAX_NODES:
         raise ValueError(f"1 to {TREE_MAX_NODES} nodes per sequence (got {N})")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim]")
-    if lens.dtype != torch.int32 or not lens.is_contiguous() or tuple(lens.shape) != (B,):
+    if lens.dtype != torch.int32 or not lens.is_contiguous() or lens.shape != (B,):
         raise TypeError(f"lens must be a contiguous int32 tensor [{B}]")
-    _same_device(q_new, k_new=k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, lens=lens,
-                 rope_cos=cos, rope_sin=sin)
-    q_new, k_new, v_new = (t.contiguous() for t in (q_new, k_new, v_new))
+    dev = _one_device(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, parents, counts)
+    q_new, k_new, v_new = q_new.contiguous(), k_new.contiguous(), v_new.contiguous()
     cos = _rope_table(cos, 1, D // 2, "rope_cos")
     sin = _rope_table(sin, 1, D // 2, "rope_sin")
     if cos.shape != sin.shape:
         raise ValueError("rope_cos and rope_sin must have the same shape")
-    parents, stride, counts = _tree_args(parents, counts, B, N, q_new.device)
+    parents, stride, counts = _tree_args(parents, counts, B, N)
     if (q_norm_weight is None) != (k_norm_weight is None):
         raise ValueError("QK-norm needs both q_norm_weight and k_norm_weight")
     qnw = knw = None
-    dt = _dtype_code(q_new)
-    with _on_device(q_new):
+    dt, max_len = _dtype_code(q_new), int(max_len)
+    with _on_device(dev):
         if q_norm_weight is not None:
             qnw, knw = (_norm_weight(w, D, q_new.device) for w in (q_norm_weight, k_norm_weight))
         out = torch.empty_like(q_new)
         # (max_len grows from step to step: asked per step, not kept)
         nbytes = _lib.size_out()
-        _lib.check(lib.kf_attn_tree_workspace_size(B, N, Hq, Hkv, D, max_len, dt,
-                                                   ctypes.byref(nbytes)),
-                   "kf_attn_tree_workspace_size")
-        ws = _workspace(nbytes.value, q_new.device)
-        _lib.check(lib.kf_attn_tree(_ptr(q_new), _ptr(k_new), _ptr(v_new), _ptr(k_cache),
-                                    _ptr(v_cache), _ptr(lens), _ptr(parents), stride,
-                                    _ptr(counts), _ptr(cos), _ptr(sin), int(rope_row_offset),
-                                    cos.shape[0], _ptr(out), _ptr(ws), ws.numel(), B, N, Smax, Hq,
-                                    Hkv, D, int(max_len), _ptr(qnw), _ptr(knw), float(norm_eps),
-                                    dt, _stream(q_new)),
-                   "kf_attn_tree")
+        rc = lib.kf_attn_tree_workspace_size(B, N, Hq, Hkv, D, max_len, dt, ctypes.byref(nbytes))
+        if rc == 0:
+            ws = _workspace(nbytes.value, q_new.device)
+            rc = lib.kf_attn_tree(q_new.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+                                  k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr(),
+                                  _ptr(parents), stride, _ptr(counts), cos.data_ptr(),
+                                  sin.data_ptr(), int(rope_row_offset), cos.shape[0],
+                                  out.data_ptr(), ws.data_ptr(), ws.numel(), B, N, Smax, Hq, Hkv,
+                                  D, max_len, _ptr(qnw), _ptr(knw), float(norm_eps), dt,
+                                  _stream(q_new))
+        _lib.check(rc, "kf_attn_tree")
     return out
 
 
@@ -621,41 +627,41 @@ def verify_drafts_raw(logits, tokens, uniforms, *, temperature: float = 1.0, par
     Unused sequences (``counts[b]`` 0) and counts or parents out of range give kept
     0 and next -1; a row on the path that is no distribution (NaN, +inf, all -inf)
     ends the path with next -1."""
-    _require_gpu(logits, tokens, uniforms)
     lib = _lib.load()
-    if logits.dim() != 3 or logits.stride(-1) != 1:
+    ls = logits.shape
+    if len(ls) != 3 or (logits.stride(2) != 1 and ls[2] != 1):
         raise ValueError("logits must be [B, N, V] with contiguous values "
-                         f"(got {tuple(logits.shape)}, strides {logits.stride()})")
-    B, N, V = logits.shape
+                         f"(got {tuple(ls)}, strides {logits.stride()})")
+    B, N, V = ls
     if not 1 <= N <= TREE_MAX_NODES:
         raise ValueError(f"1 to {TREE_MAX_NODES} nodes per sequence (got {N})")
-    if tuple(tokens.shape) != (B, N) or tuple(uniforms.shape) != (B, N):
+    if tokens.shape != (B, N) or uniforms.shape != (B, N):
         raise ValueError(f"tokens and uniforms must be [{B}, {N}] "
                          f"(got {tuple(tokens.shape)}, {tuple(uniforms.shape)})")
     if tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"tokens must be int64 or int32 (got {tokens.dtype})")
     if uniforms.dtype != torch.float32:
         raise TypeError(f"uniforms must be float32 (got {uniforms.dtype})")
-    _same_device(logits, tokens=tokens, uniforms=uniforms, draft_logits=draft_logits)
-    parents, stride, counts = _tree_args(parents, counts, B, N, logits.device)
+    dev = _one_device(logits, tokens, uniforms, draft_logits, parents, counts)
+    parents, stride, counts = _tree_args(parents, counts, B, N)
     dsb = dsn = 0
     if draft_logits is not None:
         if parents is not None:
             raise ValueError("draft_logits need a chain of drafts (parents=None)")
         if temperature == 0:
             raise ValueError("draft_logits need a temperature above 0")
-        if tuple(draft_logits.shape) != (B, N - 1, V) or draft_logits.dtype != logits.dtype:
+        if draft_logits.shape != (B, N - 1, V) or draft_logits.dtype != logits.dtype:
             raise ValueError(f"draft_logits must be [{B}, {N - 1}, {V}] of the logits' dtype "
                              f"(got {tuple(draft_logits.shape)}, {draft_logits.dtype})")
         if N == 1:
             draft_logits = None
-        elif draft_logits.stride(-1) != 1:
+        elif draft_logits.stride(2) != 1 and V != 1:
             raise ValueError("draft_logits must have contiguous values")
         else:
             dsb, dsn = draft_logits.stride(0), draft_logits.stride(1)
     dt = _dtype_code(logits)
     tokens, uniforms = tokens.to(torch.int64).contiguous(), uniforms.contiguous()
-    with _on_device(logits):
+    with _on_device(dev):
         path = torch.empty(B, N, dtype=torch.int32, device=logits.device)
         kept = torch.empty(B, dtype=torch.int32, device=logits.device)
         token = torch.empty(B, dtype=torch.int64, device=logits.device)
@@ -680,34 +686,44 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
     path does not rise or leaves the cache is left alone."""
     k_caches, v_caches, lens = list(k_caches), list(v_caches), list(lens)
     lens_out = lens if lens_out is None else list(lens_out)
-    if not k_caches or not len(k_caches) == len(v_caches) == len(lens) == len(lens_out):
+    n = len(k_caches)
+    if n == 0 or not n == len(v_caches) == len(lens) == len(lens_out):
         raise ValueError("k_caches, v_caches, lens and lens_out need one tensor per cache "
-                         f"(got {len(k_caches)}, {len(v_caches)}, {len(lens)}, {len(lens_out)})")
+                         f"(got {n}, {len(v_caches)}, {len(lens)}, {len(lens_out)})")
+    # (a model has tens of layers: one C-level pass over the tensors per property)
+    caches, lengths = k_caches + v_caches, lens + lens_out if lens_out is not lens else lens
+    T = torch.Tensor
+    dev = set(map(T.get_device, caches))
+    dev.update(map(T.get_device, lengths))
+    dev.update((path.get_device(), kept.get_device()))
+    if len(dev) != 1 or -1 in dev:
+        _require_gpu(*caches, *lengths, path, kept)
+        raise RuntimeError(f"the tensors must lie on one device (got {sorted(dev)})")
+    shapes = set(map(T.size, caches))
     k0 = k_caches[0]
-    _require_gpu(*k_caches, *v_caches, *lens, *lens_out, path, kept)
-    if k0.dim() != 4:
-        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
+    if len(shapes) != 1 or k0.dim() != 4 or not all(map(T.is_contiguous, caches)) \
+            or len(set(map(_DTYPE_OF, caches))) != 1:
+        raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim], of "
+                         "one shape and one dtype")
     B, Hkv, Smax, D = k0.shape
-    for t in k_caches + v_caches:
-        if t.shape != k0.shape or t.dtype != k0.dtype or not t.is_contiguous():
-            raise ValueError("KV caches must be contiguous, of one shape and one dtype")
-    for t in lens + lens_out:
-        if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != (B,):
-            raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
-    for t in k_caches + v_caches + lens + lens_out:
-        _same_device(k0, a_cache=t, path=path, kept=kept)
+    if set(map(T.size, lengths)) != {(B,)} or set(map(_DTYPE_OF, lengths)) != {torch.int32} \
+            or not all(map(T.is_contiguous, lengths)):
+        raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= TREE_MAX_NODES:
         raise ValueError(f"path must be [{B}, N] with N from 1 to {TREE_MAX_NODES} "
                          f"(got {tuple(path.shape)})")
-    if tuple(kept.shape) != (B,) or path.dtype != torch.int32 or kept.dtype != torch.int32:
+    if kept.shape != (B,) or path.dtype != torch.int32 or kept.dtype != torch.int32:
         raise TypeError(f"path [{B}, N] and kept [{B}] must be int32")
     path, kept = path.contiguous(), kept.contiguous()
-    n = len(k_caches)
-    arr = ctypes.c_void_p * n
-    ptrs = [arr(*(t.data_ptr() for t in ts)) for ts in (k_caches, v_caches, lens, lens_out)]
-    with _on_device(k0):
-        _lib.check(_lib.load().kf_kv_cache_keep(*ptrs, n, _ptr(path), _ptr(kept), path.shape[1], B,
-                                                Hkv, Smax, D, _dtype_code(k0), _stream(k0)),
+    # one host array of the pointers: keys' caches, values' caches, lengths in and out
+    ptrs = array.array("Q", map(T.data_ptr, caches))
+    ptrs.extend(map(T.data_ptr, lens))
+    ptrs.extend(map(T.data_ptr, lens_out))
+    at = ptrs.buffer_info()[0]
+    with _on_device(dev.pop()):
+        _lib.check(_lib.load().kf_kv_cache_keep(at, at + 8 * n, at + 16 * n, at + 24 * n, n,
+                                                path.data_ptr(), kept.data_ptr(), path.shape[1],
+                                                B, Hkv, Smax, D, _dtype_code(k0), _stream(k0)),
                    "kf_kv_cache_keep")
 
 
