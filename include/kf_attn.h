@@ -303,6 +303,11 @@ int kf_attn_tree(const void* q_new, const void* k_new, const void* v_new, void* 
 /* Largest vocabulary of kf_verify_drafts. */
 #define KF_VERIFY_MAX_VOCAB 1048576
 
+/* Workspace bytes kf_verify_drafts needs (with_drafts: whether draft_logits will
+ * be passed). */
+int kf_verify_drafts_workspace_size(int B, int N, int V, int with_drafts, int dtype,
+                                    size_t* bytes);
+
 /* Verifies drafted tokens against the target's distributions with given random
  * numbers; the emitted tokens (the path's, then next) have the target's
  * distribution.
@@ -331,13 +336,13 @@ int kf_attn_tree(const void* q_new, const void* k_new, const void* v_new, void* 
  * uniforms[b][0] times their total.
  * counts[b] = 0, a count outside 0 .. N or a parent out of range: kept 0, next
  * -1.  A row on the path that is no distribution (NaN, +inf, or -inf
- * throughout) ends the path, and next is -1.  Reads only rows on the path. */
+ * throughout) ends the path, and next is -1. */
 int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_n,
                      const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
                      const int32_t* counts, const void* draft_logits, int64_t draft_stride_b,
                      int64_t draft_stride_n, const float* uniforms, double temperature,
-                     int32_t* path, int32_t* kept, int64_t* next, int B, int N, int V, int dtype,
-                     void* stream);
+                     int32_t* path, int32_t* kept, int64_t* next, void* workspace,
+                     size_t workspace_bytes, int B, int N, int V, int dtype, void* stream);
 
 /* Moves the accepted path's rows together in n_caches KV caches (the layers of
  * a model): row lens[b] + path[b][j] to row lens[b] + j, j < kept[b], and writes

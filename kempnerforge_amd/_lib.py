@@ -8,6 +8,7 @@ no fallback: if the library is missing, every attention call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -50,7 +51,8 @@ SIGNATURES = {
     "kf_attn_tree": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _vp, _fp, _fp, _c_i64, _c_i64, _vp,
                       _vp, _c_sz] + [_c_int] * 7 + [_fp, _fp, ctypes.c_float, _c_int, _vp], _c_int),
     "kf_verify_drafts": ([_vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _fp,
-                          ctypes.c_double, _vp, _vp, _vp] + [_c_int] * 4 + [_vp], _c_int),
+                          ctypes.c_double, _vp, _vp, _vp, _vp, _c_sz] + [_c_int] * 4 + [_vp], _c_int),
+    "kf_verify_drafts_workspace_size": ([_c_int] * 5 + [_szp], _c_int),
     "kf_kv_cache_keep": ([_vp] * 4 + [_c_int] + [_vp] * 2 + [_c_int] * 6 + [_vp], _c_int),
     "kf_attn_capture_workspace_size": ([_c_int] * 7 + [_szp], _c_int),
     "kf_attn_capture": ([_vp, _vp, _vp, _fp, _fp, _fp, _vp, _fp, _vp, _c_sz] + [_c_int] * 6
@@ -90,6 +92,25 @@ def load() -> ctypes.CDLL:
                 fn.restype = restype
             _lib = lib
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The Python module over torch's headers (``csrc/kf_torch.cpp``), loaded once;
+    raises if it has not been built."""
+    global _native
+    if _native is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "kf_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"kempnerforge_amd: native module not found at {path}; build it "
+                               "with `python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("kf_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _native = module
+    return _native
 
 
 def check(rc: int, what: str) -> None:

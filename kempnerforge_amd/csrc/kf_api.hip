@@ -526,18 +526,43 @@ int kf_attn_tree(const void* q_new, const void* k_new, const void* v_new, void* 
   return tree_attention(a, workspace);
 }
 
+}  // extern "C"
+
+namespace {
+int check_verify(int B, int N, int V, int dtype) {
+  KF_CHECK_ARG(B > 0 && N > 0 && V > 0, "B, N, V must be positive (got %d, %d, %d)", B, N, V);
+  KF_CHECK_ARG(N <= KF_TREE_MAX_NODES, "at most %d nodes per sequence (got %d)",
+               KF_TREE_MAX_NODES, N);
+  KF_CHECK_ARG(B <= 65535, "at most 65535 sequences (got %d)", B);
+  KF_CHECK_ARG(V <= KF_VERIFY_MAX_VOCAB, "at most %d tokens in the vocabulary (got %d)",
+               KF_VERIFY_MAX_VOCAB, V);
+  KF_CHECK_ARG(dtype == F32 || dtype == BF16 || dtype == F16, "unsupported dtype code %d", dtype);
+  return KF_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int kf_verify_drafts_workspace_size(int B, int N, int V, int with_drafts, int dtype,
+                                    size_t* bytes) {
+  int rc = check_verify(B, N, V, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(bytes != nullptr, "bytes is null");
+  VerifyArgs a = {};
+  a.B = B; a.N = N; a.V = V; a.dtype = dtype;
+  a.drafts = with_drafts && N > 1 ? bytes : nullptr;  // only whether there are any
+  *bytes = verify_workspace(a);
+  return KF_OK;
+}
+
 int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_n,
                      const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
                      const int32_t* counts, const void* draft_logits, int64_t draft_stride_b,
                      int64_t draft_stride_n, const float* uniforms, double temperature,
-                     int32_t* path, int32_t* kept, int64_t* next, int B, int N, int V, int dtype,
-                     void* stream) {
-  KF_CHECK_ARG(B > 0 && N > 0 && V > 0, "B, N, V must be positive (got %d, %d, %d)", B, N, V);
-  KF_CHECK_ARG(N <= KF_TREE_MAX_NODES, "at most %d nodes per sequence (got %d)",
-               KF_TREE_MAX_NODES, N);
-  KF_CHECK_ARG(V <= KF_VERIFY_MAX_VOCAB, "at most %d tokens in the vocabulary (got %d)",
-               KF_VERIFY_MAX_VOCAB, V);
-  KF_CHECK_ARG(dtype == F32 || dtype == BF16 || dtype == F16, "unsupported dtype code %d", dtype);
+                     int32_t* path, int32_t* kept, int64_t* next, void* workspace,
+                     size_t workspace_bytes, int B, int N, int V, int dtype, void* stream) {
+  int rc = check_verify(B, N, V, dtype);
+  if (rc) return rc;
   KF_CHECK_ARG(logits && tokens && uniforms && path && kept && next, "null tensor pointer");
   KF_CHECK_ARG(temperature >= 0.0 && temperature < INFINITY,
                "temperature must be finite and not negative (got %g)", temperature);
@@ -550,10 +575,17 @@ int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits
   a.tokens = tokens; a.parents = parents; a.parents_stride = parents_stride; a.counts = counts;
   a.drafts = N > 1 ? draft_logits : nullptr;
   a.drafts_sb = draft_stride_b; a.drafts_sn = draft_stride_n;
-  a.uniforms = uniforms; a.temperature = temperature;
+  a.uniforms = uniforms;
+  a.greedy = !(temperature > 0.0);
+  a.inv_t = a.greedy ? 1.0 : 1.0 / temperature;
   a.path = path; a.kept = kept; a.next = next;
   a.B = B; a.N = N; a.V = V; a.dtype = dtype; a.stream = (hipStream_t)stream;
-  return verify_drafts(a);
+  const size_t need = verify_workspace(a);
+  if (workspace_bytes < need || !workspace) {
+    set_error("workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return KF_ERR_WORKSPACE;
+  }
+  return verify_drafts(a, workspace);
 }
 
 int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t* const* lens,

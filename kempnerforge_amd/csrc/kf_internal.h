@@ -217,11 +217,13 @@ struct VerifyArgs {
   int32_t *path, *kept;      // [B, N], [B]
   int64_t* next;             // [B]
   int B, N, V;
-  double temperature;
+  int greedy;    // temperature 0
+  double inv_t;  // 1 / temperature (1 if greedy)
   int dtype;
   hipStream_t stream;
 };
-int verify_drafts(const VerifyArgs& a);
+size_t verify_workspace(const VerifyArgs& a);
+int verify_drafts(const VerifyArgs& a, void* workspace);
 constexpr int KEEP_CACHES = 64;  // caches per launch: their pointers are kernel arguments
 int cache_keep(void* const* k, void* const* v, const int32_t* const* lens,
                int32_t* const* lens_out, int n_caches, const int32_t* path, const int32_t* kept,

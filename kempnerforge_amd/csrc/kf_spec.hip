@@ -29,13 +29,19 @@ constexpr int MAXN = KF_TREE_MAX_NODES;
 // is the most likely one (the lowest of equals), and that token follows the
 // path.
 //
-// One workgroup of 16 wavefronts per sequence: the walk reads only the rows on
-// its path, and the next row is known only after the last.
-constexpr int VT = 1024, VW = VT / 64;
+// Two ways to the path, then the draw.  A row's softmax costs a pass over V
+// values, and the next row of a path is known only after the last:
+//   all rows  (stats) the sums of every row at once, over the whole chip, then
+//             (draw) the walk over them, which is short
+//   walk      (walk) one workgroup per sequence, row by row down the path
+// The first reads every row once at the chip's rate, the second only the path's,
+// at one CU's; verify_drafts says which is taken.  The draw's weights are formed by
+// all workgroups of a sequence, a slice of the row each, and the last one to
+// arrive picks the token.
 
 // 16 bytes of a row as floats: granule k of the row's aligned granules, the
-// row's first element at place `lead` of granule 0.  Places outside the row get
-// -inf.
+// row's first element at place `lead` of granule 0.  Places outside the row are
+// -inf, and never read.
 template <typename T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);
@@ -46,299 +52,577 @@ struct Row {
   }
   __device__ __forceinline__ int granules() const { return (lead + V + E - 1) / E; }
   __device__ __forceinline__ int first(int k) const { return k * E - lead; }
-  __device__ __forceinline__ void load(int k, float* f) const {
+  __device__ __forceinline__ u32x4 raw(int k) const {
     const int v0 = first(k);
-    if (v0 >= 0 && v0 + E <= V) {
-      T t[E];
-      *(u32x4*)t = *(const u32x4*)(x + v0);
+    if (v0 >= 0 && v0 + E <= V) return *(const u32x4*)(x + v0);
+    T t[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = to_f32(t[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        f[e] = v0 + e >= 0 && v0 + e < V ? to_f32(x[v0 + e]) : -INFINITY;
-    }
+    for (int e = 0; e < E; ++e)
+      t[e] = v0 + e >= 0 && v0 + e < V ? x[v0 + e] : from_f32<T>(-INFINITY);
+    u32x4 u;
+    __builtin_memcpy(&u, t, 16);
+    return u;
+  }
+  static __device__ __forceinline__ void unpack(const u32x4& u, float* f) {
+    if constexpr (sizeof(T) == 4)
+      __builtin_memcpy(f, &u, 16);
+    else
+      unpack8<T>(u, f);
   }
 };
+
+// 2^x for x <= 0 in 64 bits: 2^round(x) times the Taylor polynomial of 2^r, |r| <=
+// 1/2, whose first term left out is (ln 2 / 2)^12 / 12! = 6e-15.
+__device__ __forceinline__ double exp2_64(double x) {
+  const double n = __builtin_rint(x), r = x - n;
+  constexpr double L = 0.69314718055994530942;
+  constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5,
+                   c6 = c5 * L / 6, c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9,
+                   c10 = c9 * L / 10, c11 = c10 * L / 11;
+  double p = c11;
+  p = fma(p, r, c10);
+  p = fma(p, r, c9);
+  p = fma(p, r, c8);
+  p = fma(p, r, c7);
+  p = fma(p, r, c6);
+  p = fma(p, r, c5);
+  p = fma(p, r, c4);
+  p = fma(p, r, c3);
+  p = fma(p, r, c2);
+  p = fma(p, r, L);
+  p = fma(p, r, 1.0);
+  // (below 2^-1070 nothing is left; -inf has no r)
+  return x > -1070.0 ? __builtin_ldexp(p, (int)n) : x <= -1070.0 ? 0.0 : x;
+}
 
 struct Stat {
   float m;   // maximum
-  double s;  // sum of exp((x - m) / T); not positive and finite: no distribution
   int at;    // first place of the maximum
+  double s;  // sum of 2^((x - m) c); not positive and finite: no distribution
 };
-
-// Maximum, its first place and (SUM) the sum of exp((x - m) / T) of a row, by
-// the whole workgroup.  A row holding NaN gets s = NaN.
-// Each exponential is one float32 instruction (relative error 2^-22 and that of
-// its argument); their sum is kept in 64 bits.
-template <typename T>
-__device__ Stat row_stats(const Row<T>& r, double inv_t, float* sf, double* sd, int* si) {
-  constexpr int E = Row<T>::E;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const float c = (float)(inv_t * 1.4426950408889634);
-  float m = -INFINITY;
-  int at = INT_MAX;
-  double s = 0.0;
-  bool nan = false;
-  for (int k = t; k < r.granules(); k += VT) {
-    float f[E];
-    r.load(k, f);
-    float gm = f[0];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      nan |= f[e] != f[e];
-      gm = fmaxf(gm, f[e]);
-    }
-    if (gm > m) {
-      s *= (double)exp2f((m - gm) * c);  // (m = -inf: s is 0)
-      m = gm;
-#pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (f[e] == gm) at = r.first(k) + e;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float gs = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) gs += exp2f((f[e] - ref) * c);
-    s += (double)gs;
-  }
-  if (at == INT_MAX && t < r.V) at = t;  // a share without a finite value
-  if (nan) s = NAN;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float m2 = __shfl_xor(m, o, 64);
-    const double s2 = __shfl_xor(s, o, 64);
-    const int a2 = __shfl_xor(at, o, 64);
-    const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * (double)exp2f((m - ref) * c) + s2 * (double)exp2f((m2 - ref) * c);
-    at = m > m2 ? at : m2 > m ? a2 : min(at, a2);
-    m = mn;
-  }
-  __syncthreads();  // the previous use of the exchange arrays is over
-  if (lane == 0) {
-    sf[w] = m;
-    sd[w] = s;
-    si[w] = at;
-  }
-  __syncthreads();
-  Stat o{-INFINITY, 0.0, INT_MAX};
-  for (int j = 0; j < VW; ++j) o.m = fmaxf(o.m, sf[j]);
-  const float ref = o.m == -INFINITY ? 0.f : o.m;
-  for (int j = 0; j < VW; ++j) {
-    o.s += sd[j] * (double)exp2f((sf[j] - ref) * c);
-    if (sf[j] == o.m) o.at = min(o.at, si[j]);
-  }
-  return o;
-}
-
 __device__ __forceinline__ bool has_mass(double s) { return s > 0.0 && s < INFINITY; }
 
-// p(x) of a row in 64 bits.
-__device__ __forceinline__ double prob(float x, const Stat& st, double inv_t) {
-  return exp(((double)x - (double)st.m) * inv_t) / st.s;
+// 2^((a - b) c) for two maxima, 1 where both are -inf
+template <bool DP>
+__device__ __forceinline__ double weight_of(float a, float b, double c) {
+  if (a == b) return 1.0;
+  return DP ? exp2_64(((double)a - (double)b) * c) : (double)exp2f((float)((a - b) * (float)c));
 }
 
-// V <= KF_VERIFY_MAX_VOCAB: segments of 64 granules of at least 4 values
-constexpr int MAXSEG = KF_VERIFY_MAX_VOCAB / 256 + 2;
+// Joins a statistic of other values of the row.  Equal maxima: the lower place.
+template <bool DP>
+__device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
+  const float m = fmaxf(x.m, y.m);
+  x.s = x.s * weight_of<DP>(x.m, m, c) + y.s * weight_of<DP>(y.m, m, c);
+  x.at = x.m > y.m ? x.at : y.m > x.m ? y.at : min(x.at, y.at);
+  x.m = m;
+}
 
-template <typename T>
-__global__ __launch_bounds__(VT) void verify_kernel(VerifyArgs a) {
+// Adds granules k, k + stride, ... (U of them, below `end`) to a thread's share:
+// the maximum of the batch first, then (SUM) one exponential a value; without SUM
+// the place of the maximum.  s becomes NaN where a value is NaN or (SUM) +inf.
+// DP: exponentials in 64 bits; else one float32 instruction each (relative error
+// 2^-22 and that of its argument), summed in 64 bits a batch at a time.
+template <typename T, int U>
+__device__ __forceinline__ void load_batch(const Row<T>& r, int k, int stride, int end,
+                                           u32x4* raw) {
   constexpr int E = Row<T>::E;
-  __shared__ int spar[MAXN], stok[MAXN], spath[MAXN];
-  __shared__ float su[MAXN];
-  __shared__ double sp[MAXN];
-  __shared__ int srefused[MAXN];  // tokens of the last node's refused children
-  __shared__ float sf[VW];
-  __shared__ double sd[VW];
-  __shared__ int si[VW];
-  __shared__ int step, token, nref;
-  __shared__ double seg[MAXSEG];
-  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int N = a.N, V = a.V;
-  const int n = a.counts ? a.counts[b] : N;
-  const bool greedy = !(a.temperature > 0.0);
-  const double inv_t = greedy ? 1.0 : 1.0 / a.temperature;
-  bool bad = n < 0 || n > N;
-  if (t < N) {
-    int par = t - 1;
-    if (a.parents != nullptr) par = a.parents[(int64_t)b * a.parents_stride + t];
-    const int64_t tok = a.tokens[(int64_t)b * N + t];
-    spar[t] = par;
-    stok[t] = tok >= 0 && tok < V ? (int)tok : -1;
-    su[t] = a.uniforms[(int64_t)b * N + t];
-    spath[t] = -1;
-    if (t < n && (t == 0 ? par != -1 : par < 0 || par >= t)) bad = true;
-  }
-  bad = __syncthreads_or(bad);
-  int cur = 0, len = 0;
-  int64_t next = -1;
-  if (!bad && n > 0) {
-    while (true) {
-      if (t == 0) {
-        spath[len] = cur;
-        step = -1;
-        token = -1;
-        nref = 0;
-      }
-      ++len;
-      const Row<T> row((const T*)a.logits + b * a.logits_sb + cur * a.logits_sn, V);
-      const Stat st = row_stats<T>(row, inv_t, sf, sd, si);
-      if (greedy ? st.s != st.s : !has_mass(st.s)) break;  // no distribution: next stays -1
-      const bool drafted = a.drafts != nullptr && cur + 1 < n;
-      const Row<T> drow(drafted ? (const T*)a.drafts + b * a.drafts_sb + cur * a.drafts_sn : row.x,
-                        V);
-      Stat dst{0.f, 1.0, 0};
-      if (drafted) dst = row_stats<T>(drow, inv_t, sf, sd, si);
-      // every child's probability, then the children in order
-      if (t < n && spar[t] == cur && t > 0) {
-        const int c = stok[t];
-        double p = -1.0;  // a token outside the vocabulary, or a sibling's: refused
-        if (c >= 0) {
-          if (greedy) {
-            p = c == st.at;
-          } else {
-            p = prob(to_f32(row.x[c]), st, inv_t);
-            if (!drafted)
-              for (int j = cur + 1; j < t; ++j)
-                if (spar[j] == cur && stok[j] == c) p = -1.0;
-          }
-        }
-        sp[t] = p;
-      }
-      __syncthreads();
-      if (t == 0) {
-        double left = 1.0;
-        for (int i = cur + 1; i < n; ++i) {
-          if (spar[i] != cur) continue;
-          const double p = sp[i];
-          bool take;
-          if (greedy)
-            take = p > 0.0;
-          else if (drafted)
-            take = p >= 0.0 && (double)su[i] * prob(to_f32(drow.x[stok[i]]), dst, inv_t) < p;
-          else
-            take = p >= 0.0 && (double)su[i] * left < p;
-          if (take) {
-            step = i;
-            break;
-          }
-          if (p > 0.0) {
-            left -= p;
-            srefused[nref++] = stok[i];
-          }
-        }
-      }
-      __syncthreads();
-      const int to = step;
-      if (to >= 0) {
-        cur = to;
-        __syncthreads();  // step is read before it is written again
-        continue;
-      }
-      if (greedy) {
-        next = st.at;
-        break;
-      }
-      // The draw, in 64 bits: weights of the row's values in order, summed by
-      // segments of 64 granules; then the segment that holds the point.
-      const bool minus = drafted && has_mass(dst.s);
-      // weights of granule k (the draft's row may be aligned differently: read
-      // value by value)
-      auto weights = [&](int k, bool all, double* wt) {
-        float f[E];
-        row.load(k, f);
-        const int v0 = row.first(k);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int v = v0 + e;
-          wt[e] = v < 0 || v >= V ? 0.0 : prob(f[e], st, inv_t);
-          if (minus && !all && wt[e] > 0.0)
-            wt[e] = fmax(wt[e] - prob(to_f32(drow.x[v]), dst, inv_t), 0.0);
-        }
-        if (!drafted && !all)
-          for (int i = 0; i < nref; ++i)
+  for (int u = 0; u < U; ++u) {
+    if (k + u * stride < end) {
+      raw[u] = r.raw(k + u * stride);
+    } else {  // (the lowest value of every type: 2^-inf below)
+      T t[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (srefused[i] == v0 + e) wt[e] = 0.0;
-      };
-      const int nseg = (row.granules() + 63) / 64;
-      double total = 0.0;
-      bool all = false;
-      for (int pass = 0; pass < 2; ++pass) {
-        for (int g = w; g < nseg; g += VW) {
-          double x = 0.0;
-          const int k = 64 * g + lane;
-          if (k < row.granules()) {
-            double wt[E];
-            weights(k, all, wt);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x += wt[e];
-          }
-#pragma unroll
-          for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-          if (lane == 0) seg[g] = x;
-        }
-        __syncthreads();
-        total = 0.0;
-        for (int g = 0; g < nseg; ++g) total += seg[g];
-        // rounding can leave no mass where all of it was on refused tokens: the
-        // draw is then from the row itself
-        if (total > 0.0 || all) break;
-        all = true;
-        __syncthreads();
-      }
-      if (w == 0) {
-        const double point = (double)su[0] * total;
-        double before = 0.0;
-        int g = 0;
-        for (; g < nseg - 1; ++g) {
-          if (before + seg[g] > point) break;
-          before += seg[g];
-        }
-        const int k = 64 * g + lane;
-        double wt[E], own = 0.0;
-        int last = -1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) wt[e] = 0.0;
-        if (k < row.granules()) {
-          weights(k, all, wt);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            own += wt[e];
-            if (wt[e] > 0.0) last = row.first(k) + e;
-          }
-        }
-        double incl = own;
-        for (int o = 1; o < 64; o <<= 1) {
-          const double y = __shfl_up(incl, o, 64);
-          if (lane >= o) incl += y;
-        }
-        double run = before + (incl - own);
-        int hit = INT_MAX;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          run += wt[e];
-          if (hit == INT_MAX && wt[e] > 0.0 && run > point) hit = row.first(k) + e;
-        }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-          hit = min(hit, __shfl_xor(hit, o, 64));
-          last = max(last, __shfl_xor(last, o, 64));
-        }
-        // (sums of two orders may leave the point behind the segment's last value)
-        if (lane == 0) token = hit != INT_MAX ? hit : last;
-      }
-      __syncthreads();
-      next = token;
-      break;
+      for (int e = 0; e < E; ++e) t[e] = from_f32<T>(-INFINITY);
+      __builtin_memcpy(&raw[u], t, 16);
     }
   }
+}
+template <typename T, bool DP, bool SUM, int U>
+__device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, const u32x4* raw,
+                                          double c, Stat& st) {
+  constexpr int E = Row<T>::E;
+  float m = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float f[E];
+    Row<T>::unpack(raw[u], f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!SUM) nan |= f[e] != f[e];
+      m = fmaxf(m, f[e]);
+    }
+  }
+  if (m > st.m) {
+    if (SUM) {
+      st.s *= weight_of<DP>(st.m, m, c);
+    } else {
+#pragma unroll
+      for (int u = U - 1; u >= 0; --u) {
+        float f[E];
+        Row<T>::unpack(raw[u], f);
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (f[e] == m) st.at = r.first(k + u * stride) + e;
+      }
+    }
+    st.m = m;
+  }
+  if (!SUM) {
+    if (nan) st.s = NAN;
+    return;
+  }
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  const float cf = (float)c, rc = ref * cf;
+  float gs = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float f[E];
+    Row<T>::unpack(raw[u], f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (DP)
+        st.s += exp2_64(((double)f[e] - (double)ref) * c);
+      else
+        gs += __builtin_amdgcn_exp2f(fmaf(f[e], cf, -rc));
+    }
+  }
+  if constexpr (!DP) st.s += (double)gs;
+}
+
+// The workgroup's shares joined, in order; `x` is one Stat per wavefront.
+template <bool DP, int NT>
+__device__ __forceinline__ Stat join_all(Stat st, double c, Stat* x) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    Stat y;
+    y.m = __shfl_xor(st.m, o, 64);
+    y.at = __shfl_xor(st.at, o, 64);
+    y.s = __shfl_xor(st.s, o, 64);
+    join<DP>(st, y, c);
+  }
+  __syncthreads();  // the previous use of x is over
+  if (lane == 0) x[w] = st;
   __syncthreads();
-  if (t < N) a.path[(int64_t)b * N + t] = t < len ? spath[t] : -1;
+  // every wavefront joins the wavefronts' by itself, a lane each
+  st = x[lane % (NT / 64)];
+#pragma unroll
+  for (int o = NT / 128; o >= 1; o >>= 1) {
+    Stat y;
+    y.m = __shfl_xor(st.m, o, 64);
+    y.at = __shfl_xor(st.at, o, 64);
+    y.s = __shfl_xor(st.s, o, 64);
+    join<DP>(st, y, c);
+  }
+  st.s = __shfl(st.s, 0, 64);  // (the lanes' orders differ in the last bit)
+  return st;
+}
+
+constexpr int ST = 256, SU = 4;            // threads, granules of a thread
+constexpr int SLICE = ST * SU;             // granules of a slice
+// slices of a row of V values at any alignment
+__host__ __device__ __forceinline__ int slices_of(int V, int E) {
+  return ((V + 2 * E - 2) / E + SLICE - 1) / SLICE;
+}
+
+// Workgroup (slice, row, sequence): rows 0 .. N - 1 the target's, N .. 2N - 2 the
+// draft's.  Rows of unused nodes are left out.  Bound by HBM: a thread's four
+// granules are in flight before the first is used.
+template <typename T, bool DP, bool SUM>
+__global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a, Stat* __restrict__ out,
+                                                          int* __restrict__ arrived) {
+  __shared__ Stat x[ST / 64];
+  const int b = blockIdx.z, i = blockIdx.y, t = threadIdx.x;
+  const int n = a.counts ? a.counts[b] : a.N;
+  if (t == 0 && i == 0 && blockIdx.x == 0) arrived[b] = 0;
+  const bool draft = i >= a.N;
+  const int at = draft ? i - a.N : i;
+  if (draft ? at + 1 >= n : at >= n) return;
+  const Row<T> r(draft ? (const T*)a.drafts + b * a.drafts_sb + at * a.drafts_sn
+                       : (const T*)a.logits + b * a.logits_sb + at * a.logits_sn,
+                 a.V);
+  const double c = a.inv_t * 1.4426950408889634074;
+  Stat st{-INFINITY, INT_MAX, 0.0};
+  u32x4 raw[SU];
+  const int k = blockIdx.x * SLICE + t;
+  load_batch<T, SU>(r, k, ST, r.granules(), raw);
+  add_batch<T, DP, SUM, SU>(r, k, ST, raw, c, st);
+  st = join_all<DP, ST>(st, c, x);
+  if (t == 0) out[((int64_t)b * gridDim.y + i) * gridDim.x + blockIdx.x] = st;
+}
+
+// What a workgroup knows of its sequence's nodes.
+struct Nodes {
+  int par[MAXN], tok[MAXN];
+  float u[MAXN];
+};
+// Loads the nodes; whether the sequence is refused.
+__device__ __forceinline__ bool load_nodes(const VerifyArgs& a, int b, int n, Nodes& nd) {
+  bool bad = n < 0 || n > a.N;
+  for (int t = threadIdx.x; t < a.N; t += blockDim.x) {
+    int par = t - 1;
+    if (a.parents != nullptr) par = a.parents[(int64_t)b * a.parents_stride + t];
+    const int64_t tok = a.tokens[(int64_t)b * a.N + t];
+    nd.par[t] = par;
+    nd.tok[t] = tok >= 0 && tok < a.V ? (int)tok : -1;
+    nd.u[t] = a.uniforms[(int64_t)b * a.N + t];
+    if (t < n && (t == 0 ? par != -1 : par < 0 || par >= t)) bad = true;
+  }
+  return __syncthreads_or(bad);
+}
+
+// Whether node t is taken once its elder siblings are refused, sp[] holding its
+// and its siblings' probabilities (-1: none, refused).
+__device__ __forceinline__ bool taken(const VerifyArgs& a, const Nodes& nd, const double* sp,
+                                      const double* sq, int t) {
+  const double p = sp[t];
+  if (!(p >= 0.0)) return false;
+  if (a.greedy) return p > 0.0;
+  if (a.drafts != nullptr) return (double)nd.u[t] * sq[t] < p;
+  double left = 1.0;
+  for (int j = nd.par[t] + 1; j < t; ++j)
+    if (nd.par[j] == nd.par[t]) {
+      if (nd.tok[j] == nd.tok[t]) return false;  // refused before
+      left -= fmax(sp[j], 0.0);
+    }
+  // (a repeated token's mass went once: count only the first of equals)
+  for (int j = nd.par[t] + 1; j < t; ++j)
+    if (nd.par[j] == nd.par[t])
+      for (int i = nd.par[t] + 1; i < j; ++i)
+        if (nd.par[i] == nd.par[t] && nd.tok[i] == nd.tok[j]) {
+          left += fmax(sp[j], 0.0);
+          break;
+        }
+  return (double)nd.u[t] * left < p;
+}
+
+constexpr int WT = 1024;
+
+// Row by row down the path, one workgroup per sequence.  A CU forms a row's sums
+// at 64 values a clock at most (about 8 operations each): a row of 131072 takes
+// 8 us, whatever its type.  Leaves the last node and its statistic for the draw;
+// greedy: writes the token too.
+template <typename T>
+__global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __restrict__ last,
+                                                         Stat* __restrict__ out,
+                                                         int* __restrict__ arrived) {
+  __shared__ Nodes nd;
+  __shared__ int path[MAXN];
+  __shared__ double sp[MAXN];
+  __shared__ Stat x[WT / 64];
+  __shared__ int step;
+  const int b = blockIdx.x, t = threadIdx.x;
+  const int n = a.counts ? a.counts[b] : a.N;
+  const bool bad = load_nodes(a, b, n, nd);
+  const double c = a.inv_t * 1.4426950408889634074;
+  int cur = 0, len = 0, end = -1;
+  Stat st{-INFINITY, INT_MAX, 0.0};
+  while (!bad && n > 0) {
+    if (t == 0) {
+      path[len] = cur;
+      step = INT_MAX;
+    }
+    ++len;
+    const Row<T> r((const T*)a.logits + b * a.logits_sb + cur * a.logits_sn, a.V);
+    const int ng = r.granules();
+    st = Stat{-INFINITY, INT_MAX, 0.0};
+    // the next batch's loads run under this one's exponentials
+    constexpr int U = sizeof(T) == 4 ? 4 : 3;  // (registers for 16 wavefronts)
+    u32x4 raw[U], ahead[U];
+    load_batch<T, U>(r, t, WT, ng, raw);
+    for (int k = t; k < ng; k += U * WT) {
+      load_batch<T, U>(r, k + U * WT, WT, ng, ahead);
+      if (a.greedy)
+        add_batch<T, false, false, U>(r, k, WT, raw, c, st);
+      else
+        add_batch<T, false, true, U>(r, k, WT, raw, c, st);
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = ahead[u];
+    }
+    st = join_all<false, WT>(st, c, x);
+    if (a.greedy ? st.s != st.s : !has_mass(st.s)) break;  // no distribution
+    end = cur;
+    const bool child = t > 0 && t < n && nd.par[t] == cur;
+    if (child) {
+      const int tok = nd.tok[t];
+      sp[t] = tok < 0      ? -1.0
+              : a.greedy ? (tok == (st.at == INT_MAX ? 0 : st.at) ? 1.0 : -1.0)
+                         : exp2_64(((double)to_f32(r.x[tok]) - (double)st.m) * c) / st.s;
+    }
+    __syncthreads();
+    if (child && taken(a, nd, sp, nullptr, t)) atomicMin(&step, t);
+    __syncthreads();
+    const int to = step;
+    __syncthreads();  // read by all before it is written again
+    if (to == INT_MAX) break;
+    cur = to;
+    end = -1;
+  }
+  __syncthreads();
+  for (int j = t; j < a.N; j += WT) a.path[(int64_t)b * a.N + j] = j < len ? path[j] : -1;
   if (t == 0) {
     a.kept[b] = len;
-    a.next[b] = next;
+    a.next[b] = a.greedy && end >= 0 ? (st.at == INT_MAX ? 0 : st.at) : -1;
+    last[b] = end;
+    out[b] = st;
+    arrived[b] = 0;
   }
+}
+
+// A slice of the draw: a granule per thread (the weights' 64-bit exponentials,
+// about 20 operations each, are what it spends its time on, so as many CUs as
+// there are); a segment: a wavefront's granules.
+constexpr int DT = 256, DSEG = DT / 64;
+constexpr int MAXSLICES = KF_VERIFY_MAX_VOCAB / (4 * DT) + 2;
+__host__ __device__ __forceinline__ int draw_slices_of(int V, int E) {
+  return ((V + 2 * E - 2) / E + DT - 1) / DT;
+}
+
+// The draw (and, ALL, the walk before it, over the statistics of all rows, by
+// every workgroup of the sequence for itself).  Workgroup (slice, sequence): the
+// weights of a slice's values in 64 bits, summed by segments in order; the last
+// to arrive finds the slice, the segment and the value at which the running sum
+// passes the point.  greedy: one workgroup per sequence, no draw.
+template <typename T, bool ALL, bool DP>
+__global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int* __restrict__ last,
+                                                         const Stat* __restrict__ stats,
+                                                         int nslices, int ndraw, double* sums,
+                                                         int* __restrict__ arrived) {
+  constexpr int E = Row<T>::E;
+  __shared__ Nodes nd;
+  __shared__ Stat row[ALL ? 2 * MAXN : 1];  // nodes 0 .. n - 1, then the draft's
+  __shared__ double sp[MAXN], sq[ALL ? MAXN : 1];
+  __shared__ int pick[MAXN];  // the child taken of each node, then the path
+  __shared__ int refused[MAXN];  // tokens of the last node's children
+  __shared__ double seg[DSEG], all_sums[MAXSLICES];
+  __shared__ int sh[4];
+  const int b = blockIdx.y, slice = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int N = a.N, V = a.V;
+  const int n = a.counts ? a.counts[b] : N;
+  const bool bad = load_nodes(a, b, n, nd);
+  const double c = a.inv_t * 1.4426950408889634074;
+  const T* logits = (const T*)a.logits + b * a.logits_sb;
+  const T* drafts = (const T*)a.drafts + b * a.drafts_sb;
+  const bool drafted = ALL && a.drafts != nullptr;
+  int cur = -1;  // the node drawn after, -1 if its row is no distribution
+  Stat st{}, dst{};
+  if constexpr (ALL) {
+    const int nrows = a.drafts != nullptr ? 2 * N - 1 : N;
+    const bool node = !bad && t < n;
+    static_assert(DT >= MAXN, "a thread per node");
+    float x = 0.f, y = 0.f;
+    if (node && t > 0 && nd.tok[t] >= 0) {
+      x = to_f32(logits[nd.par[t] * a.logits_sn + nd.tok[t]]);
+      if (drafted) y = to_f32(drafts[(t - 1) * a.drafts_sn + nd.tok[t]]);
+    }
+    // the rows' slices joined, 16 lanes a row
+    for (int i = t / 16; i < (bad ? 0 : drafted ? 2 * n - 1 : n); i += DT / 16) {
+      const Stat* p = stats + ((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices;
+      Stat z{-INFINITY, INT_MAX, 0.0};
+      for (int j = t % 16; j < nslices; j += 16) join<DP>(z, p[j], c);
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) {
+        Stat v;
+        v.m = __shfl_xor(z.m, o, 16);
+        v.at = __shfl_xor(z.at, o, 16);
+        v.s = __shfl_xor(z.s, o, 16);
+        join<DP>(z, v, c);
+      }
+      if (t % 16 == 0) row[i] = z;
+    }
+    if (t < N) pick[t] = INT_MAX;
+    __syncthreads();
+    if (node && t > 0) {
+      const Stat& r = row[nd.par[t]];
+      const int tok = nd.tok[t];
+      sp[t] = tok < 0      ? -1.0
+              : a.greedy ? (tok == (r.at == INT_MAX ? 0 : r.at) && r.s == r.s ? 1.0 : -1.0)
+              : has_mass(r.s) ? exp2_64(((double)x - (double)r.m) * c) / r.s
+                              : -1.0;
+      if (drafted) {
+        const Stat& d = row[n + t - 1];
+        sq[t] = exp2_64(((double)y - (double)d.m) * c) / d.s;
+      }
+    }
+    __syncthreads();
+    if (node && t > 0 && taken(a, nd, sp, sq, t)) atomicMin(&pick[nd.par[t]], t);
+    __syncthreads();
+    if (t == 0) {
+      int len = 0, at = 0, lastn = -1;
+      if (!bad && n > 0) {
+        while (true) {
+          const int to = pick[at];
+          pick[len++] = at;  // len <= at: the picks of nodes behind are intact
+          const bool ok = a.greedy ? row[at].s == row[at].s : has_mass(row[at].s);
+          if (ok && to == INT_MAX) lastn = at;
+          if (!ok || to == INT_MAX) break;
+          at = to;
+        }
+      }
+      sh[0] = lastn;
+      sh[1] = len;
+    }
+    __syncthreads();
+    cur = sh[0];
+    if (cur >= 0) st = row[cur];
+    if (slice == 0) {
+      if (t < N) a.path[(int64_t)b * N + t] = t < sh[1] ? pick[t] : -1;
+      if (t == 0) {
+        a.kept[b] = sh[1];
+        if (cur < 0 || a.greedy) a.next[b] = cur < 0 ? -1 : st.at == INT_MAX ? 0 : st.at;
+      }
+    }
+    if (cur >= 0 && drafted && cur + 1 < n) dst = row[n + cur];
+  } else {
+    cur = last[b];
+    if (cur >= 0) st = stats[b];
+  }
+  if (cur < 0 || a.greedy) return;
+  if (t == 0) sh[3] = 0;
+  __syncthreads();
+  if (t > cur && t < n && nd.par[t] == cur) refused[atomicAdd(&sh[3], 1)] = nd.tok[t];
+  __syncthreads();
+  const int nref = sh[3];
+  // weights, times the target's sum (with a draft: probabilities)
+  const bool minus = drafted && cur + 1 < n && has_mass(dst.s);
+  const double rp = minus ? 1.0 / st.s : 1.0, rq = minus ? 1.0 / dst.s : 0.0;
+  const Row<T> r(logits + cur * a.logits_sn, V);
+  const T* dr = drafts + cur * a.drafts_sn;
+  const int ng = r.granules();
+  auto weights = [&](int k, bool all, double* wt) {
+    float f[E];
+    Row<T>::unpack(r.raw(k), f);
+    const int v0 = r.first(k);
+#pragma unroll
+    for (int e = 0; e < E; ++e) wt[e] = exp2_64(((double)f[e] - (double)st.m) * c) * rp;
+    if (all) return;
+    if (minus) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v0 + e >= 0 && v0 + e < V)
+          wt[e] = fmax(wt[e] - exp2_64(((double)to_f32(dr[v0 + e]) - (double)dst.m) * c) * rq, 0.0);
+    } else if (!drafted) {  // (a refused child of probability 0 changes nothing)
+      for (int i = 0; i < nref; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (refused[i] == v0 + e) wt[e] = 0.0;
+    }
+  };
+  // seg[]: the sums of a slice's segments; returns their sum in order
+  auto slice_sum = [&](int sl, bool all) {
+    double x = 0.0;
+    const int k = sl * DT + t;
+    if (k < ng) {
+      double wt[E];
+      weights(k, all, wt);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x += wt[e];
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+    __syncthreads();
+    if (lane == 0) seg[w] = x;
+    __syncthreads();
+    x = 0.0;
+#pragma unroll
+    for (int g = 0; g < DSEG; ++g) x += seg[g];
+    return x;
+  };
+  double* mine = sums + (int64_t)b * ndraw;
+  const double own = slice_sum(slice, false);
+  if (t == 0) {
+    // Device-scope accesses on both sides, past the caches, so the order is all
+    // that is left to see to: the sum has arrived before the count is raised.  (A
+    // release here would write back the XCD's whole L2, an acquire empty it.)
+    __hip_atomic_store(mine + slice, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    sh[2] = __hip_atomic_fetch_add(arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (sh[2] != ndraw - 1) return;
+  // the last of the sequence: every slice's sum is there
+  for (int j = t; j < ndraw; j += DT)
+    all_sums[j] = __hip_atomic_load(mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  // running sums of the slices, a lane's share of them at a time; every wavefront
+  // for itself
+  const int share = (ndraw + 63) / 64, j0 = min(lane * share, ndraw), j1 = min(j0 + share, ndraw);
+  double part, incl, total;
+  auto running = [&]() {
+    part = 0.0;
+    for (int j = j0; j < j1; ++j) part += all_sums[j];
+    incl = part;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    total = __shfl(incl, 63, 64);
+  };
+  running();
+  // rounding can leave no mass where all of it was on refused tokens: the draw is
+  // then from the row itself
+  const bool all = !(total > 0.0);
+  if (all) {
+    for (int j = 0; j < ndraw; ++j) {
+      const double x = slice_sum(j, true);
+      if (t == 0) all_sums[j] = x;
+    }
+    __syncthreads();
+    running();
+  }
+  const double point = (double)nd.u[0] * total;
+  // the first share that passes the point, then its first slice (the last ones,
+  // where sums of two orders leave the point behind them)
+  const uint64_t past = __builtin_amdgcn_ballot_w64(incl > point);
+  const int owner = past ? (int)__builtin_ctzll(past) : (ndraw - 1) / share;
+  double before = __shfl(incl - part, owner, 64);
+  int sl = owner * share;
+  const int end = min(sl + share, ndraw) - 1;
+  for (; sl < end; ++sl) {
+    if (before + all_sums[sl] > point) break;
+    before += all_sums[sl];
+  }
+  slice_sum(sl, all);
+  if (w != 0) return;
+  int g = 0;
+  for (; g < DSEG - 1; ++g) {
+    if (before + seg[g] > point) break;
+    before += seg[g];
+  }
+  const int k = sl * DT + 64 * g + lane;
+  double wt[E], sum = 0.0;
+  int hit = INT_MAX, any = -1;
+#pragma unroll
+  for (int e = 0; e < E; ++e) wt[e] = 0.0;
+  if (k < ng) weights(k, all, wt);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    sum += wt[e];
+    if (wt[e] > 0.0) any = r.first(k) + e;
+  }
+  double run = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(run, o, 64);
+    if (lane >= o) run += y;
+  }
+  run = before + (run - sum);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    run += wt[e];
+    if (hit == INT_MAX && wt[e] > 0.0 && run > point) hit = r.first(k) + e;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    hit = min(hit, __shfl_xor(hit, o, 64));
+    any = max(any, __shfl_xor(any, o, 64));
+  }
+  // (sums of two orders may leave the point behind the segment's last value)
+  if (lane == 0) a.next[b] = hit != INT_MAX ? hit : any;
 }
 
 // ------------------------------------------------------------------ keep
@@ -390,23 +674,81 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(KeepPtrs p, const int32
 
 }  // namespace
 
-int verify_drafts(const VerifyArgs& a) {
-  switch (a.dtype) {
-    case F32:
-      KF_LAUNCH("verify", verify_kernel<float>, dim3(a.B), dim3(VT), 0, a.stream, a);
-      break;
-    case BF16:
-      KF_LAUNCH("verify", verify_kernel<bf16>, dim3(a.B), dim3(VT), 0, a.stream, a);
-      break;
-    case F16:
-      KF_LAUNCH("verify", verify_kernel<_Float16>, dim3(a.B), dim3(VT), 0, a.stream, a);
-      break;
-    default:
-      set_error("unsupported dtype %d", a.dtype);
-      return KF_ERR_UNSUPPORTED;
+namespace {
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct VerifyWs {
+  int* arrived;   // [B]
+  int* last;      // [B]
+  Stat* stats;    // all rows: [B][rows][slices]; walk: [B]
+  double* sums;   // [B][draw]
+  bool all_rows;
+  int rows, slices, draw;
+  size_t bytes;
+};
+VerifyWs verify_carve(const VerifyArgs& a, void* p) {
+  const int el = a.dtype == F32 ? 4 : 2;
+  VerifyWs w;
+  w.slices = slices_of(a.V, 16 / el);
+  w.draw = draw_slices_of(a.V, 16 / el);
+  w.rows = a.drafts != nullptr ? 2 * a.N - 1 : a.N;
+  // All rows cost B N el / 4.5 TB/s per value of the vocabulary, a walk about 65
+  // ps per value and level, some four levels deep.  (A chain's draft rows: their
+  // sums have to hold 64 bits for the draw, which one CU forms too slowly.)
+  w.all_rows = a.drafts != nullptr || (int64_t)a.B * a.N * el <= 1200;
+  char* c = (char*)p;
+  w.arrived = (int*)c;
+  c += up256((size_t)a.B * 4);
+  w.last = (int*)c;
+  c += up256((size_t)a.B * 4);
+  w.stats = (Stat*)c;
+  c += up256((size_t)a.B * (w.all_rows ? (size_t)w.rows * w.slices : 1) * sizeof(Stat));
+  w.sums = (double*)c;
+  c += up256((size_t)a.B * w.draw * sizeof(double));
+  w.bytes = (size_t)(c - (char*)p);
+  return w;
+}
+
+template <typename T>
+int verify_typed(const VerifyArgs& a, void* workspace) {
+  const VerifyWs w = verify_carve(a, workspace);
+  if (w.all_rows) {
+    auto kernel = a.greedy               ? verify_stats_kernel<T, false, false>
+                  : a.drafts != nullptr ? verify_stats_kernel<T, true, true>
+                                        : verify_stats_kernel<T, false, true>;
+    KF_LAUNCH("verify_stats", kernel, dim3(w.slices, w.rows, a.B), dim3(ST), 0, a.stream, a,
+              w.stats, w.arrived);
+    KF_CHECK_LAUNCH();
+    auto draw = a.drafts != nullptr ? verify_draw_kernel<T, true, true>
+                                    : verify_draw_kernel<T, true, false>;
+    KF_LAUNCH("verify_draw", draw, dim3(a.greedy ? 1 : w.draw, a.B), dim3(DT), 0, a.stream, a,
+              w.last, w.stats, w.slices, w.draw, w.sums, w.arrived);
+    KF_CHECK_LAUNCH();
+    return KF_OK;
   }
+  KF_LAUNCH("verify_walk", verify_walk_kernel<T>, dim3(a.B), dim3(WT), 0, a.stream, a, w.last,
+            w.stats, w.arrived);
+  KF_CHECK_LAUNCH();
+  if (a.greedy) return KF_OK;
+  KF_LAUNCH("verify_draw", (verify_draw_kernel<T, false, false>), dim3(w.draw, a.B), dim3(DT), 0,
+            a.stream, a, w.last, w.stats, w.slices, w.draw, w.sums, w.arrived);
   KF_CHECK_LAUNCH();
   return KF_OK;
+}
+
+}  // namespace
+
+size_t verify_workspace(const VerifyArgs& a) { return verify_carve(a, nullptr).bytes; }
+
+int verify_drafts(const VerifyArgs& a, void* workspace) {
+  switch (a.dtype) {
+    case F32: return verify_typed<float>(a, workspace);
+    case BF16: return verify_typed<bf16>(a, workspace);
+    case F16: return verify_typed<_Float16>(a, workspace);
+  }
+  set_error("unsupported dtype %d", a.dtype);
+  return KF_ERR_UNSUPPORTED;
 }
 
 int cache_keep(void* const* k, void* const* v, const int32_t* const* lens,

@@ -172,7 +172,7 @@ _ATTN_KEYS = ("fwd_mfma", "fwd32_kernel", "bwd_dkdv", "dkdv_reduce_kernel", "bwd
               "stats_f32_kernel", "mask_prep_f32_kernel", "dkdv_parts_f32_kernel",
               "widen_kernel", "narrow_kernel", "cache_append", "append_kernel",
               "append_rows_kernel", "tree_prep_kernel", "tree_rows_kernel", "tree_stream_kernel",
-              "tree_merge_kernel", "verify_kernel",
+              "tree_merge_kernel", "verify_stats_kernel", "verify_walk_kernel", "verify_draw_kernel",
               "cache_keep_kernel", "kf::attn", "flash", "fmha", "attention")
 _MATMUL_KEYS = ("gemm", "mm", "matmul", "dot", "bmm", "cublas", "nvjet", "cutlass",
                 "cijk_", "hipblaslt", "rocblas", "ck_tile", "wvsplitk")

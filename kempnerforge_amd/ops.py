@@ -18,7 +18,6 @@ import array
 import contextlib
 import ctypes
 import functools
-import operator
 import weakref
 from typing import Optional
 
@@ -492,7 +491,6 @@ TREE_MAX_NODES = 256  # KF_TREE_MAX_NODES
 
 
 _SAME = contextlib.nullcontext()
-_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def _on_device(index: int):
@@ -665,11 +663,14 @@ def verify_drafts_raw(logits, tokens, uniforms, *, temperature: float = 1.0, par
         path = torch.empty(B, N, dtype=torch.int32, device=logits.device)
         kept = torch.empty(B, dtype=torch.int32, device=logits.device)
         token = torch.empty(B, dtype=torch.int64, device=logits.device)
-        _lib.check(lib.kf_verify_drafts(_ptr(logits), logits.stride(0), logits.stride(1),
-                                        _ptr(tokens), _ptr(parents), stride, _ptr(counts),
-                                        _ptr(draft_logits), dsb, dsn, _ptr(uniforms),
-                                        float(temperature), _ptr(path), _ptr(kept), _ptr(token),
-                                        B, N, V, dt, _stream(logits)),
+        ws = _workspace(_size("kf_verify_drafts_workspace_size", dev, B, N, V,
+                              int(draft_logits is not None), dt), logits.device)
+        _lib.check(lib.kf_verify_drafts(logits.data_ptr(), logits.stride(0), logits.stride(1),
+                                        tokens.data_ptr(), _ptr(parents), stride, _ptr(counts),
+                                        _ptr(draft_logits), dsb, dsn, uniforms.data_ptr(),
+                                        float(temperature), path.data_ptr(), kept.data_ptr(),
+                                        token.data_ptr(), ws.data_ptr(), ws.numel(), B, N, V, dt,
+                                        _stream(logits)),
                    "kf_verify_drafts")
     return path, kept, token
 
@@ -690,38 +691,39 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
     if n == 0 or not n == len(v_caches) == len(lens) == len(lens_out):
         raise ValueError("k_caches, v_caches, lens and lens_out need one tensor per cache "
                          f"(got {n}, {len(v_caches)}, {len(lens)}, {len(lens_out)})")
-    # (a model has tens of layers: one C-level pass over the tensors per property)
-    caches, lengths = k_caches + v_caches, lens + lens_out if lens_out is not lens else lens
-    T = torch.Tensor
-    dev = set(map(T.get_device, caches))
-    dev.update(map(T.get_device, lengths))
-    dev.update((path.get_device(), kept.get_device()))
-    if len(dev) != 1 or -1 in dev:
-        _require_gpu(*caches, *lengths, path, kept)
-        raise RuntimeError(f"the tensors must lie on one device (got {sorted(dev)})")
-    shapes = set(map(T.size, caches))
-    k0 = k_caches[0]
-    if len(shapes) != 1 or k0.dim() != 4 or not all(map(T.is_contiguous, caches)) \
-            or len(set(map(_DTYPE_OF, caches))) != 1:
+    # one host array of the pointers (lengths in and out, keys' and values'
+    # caches), filled by the native checks: one device, dtype and shape a list
+    ptrs = array.array("Q", bytes(32 * n))
+    same = _lib.native().same
+    caches, k0 = k_caches + v_caches, k_caches[0]
+    try:
+        dev = same(caches, ptrs, 2 * n)
+    except ValueError as e:
         raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim], of "
-                         "one shape and one dtype")
+                         f"one device, dtype and shape: {e}") from None
+    try:
+        where = {dev, same(lens, ptrs, 0), same(lens_out, ptrs, n), path.get_device(),
+                 kept.get_device()}
+    except ValueError as e:
+        raise ValueError(f"lens and lens_out must be alike: {e}") from None
+    if where != {dev} or dev < 0:
+        _require_gpu(*caches, *lens, *lens_out, path, kept)
+        raise RuntimeError(f"the tensors must lie on one device (got {sorted(where)})")
+    if k0.dim() != 4:
+        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
     B, Hkv, Smax, D = k0.shape
-    if set(map(T.size, lengths)) != {(B,)} or set(map(_DTYPE_OF, lengths)) != {torch.int32} \
-            or not all(map(T.is_contiguous, lengths)):
-        raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
+    for t in (lens[0], lens_out[0]):
+        if t.dtype != torch.int32 or t.shape != (B,):
+            raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= TREE_MAX_NODES:
         raise ValueError(f"path must be [{B}, N] with N from 1 to {TREE_MAX_NODES} "
                          f"(got {tuple(path.shape)})")
     if kept.shape != (B,) or path.dtype != torch.int32 or kept.dtype != torch.int32:
         raise TypeError(f"path [{B}, N] and kept [{B}] must be int32")
     path, kept = path.contiguous(), kept.contiguous()
-    # one host array of the pointers: keys' caches, values' caches, lengths in and out
-    ptrs = array.array("Q", map(T.data_ptr, caches))
-    ptrs.extend(map(T.data_ptr, lens))
-    ptrs.extend(map(T.data_ptr, lens_out))
     at = ptrs.buffer_info()[0]
-    with _on_device(dev.pop()):
-        _lib.check(_lib.load().kf_kv_cache_keep(at, at + 8 * n, at + 16 * n, at + 24 * n, n,
+    with _on_device(dev):
+        _lib.check(_lib.load().kf_kv_cache_keep(at + 16 * n, at + 24 * n, at, at + 8 * n, n,
                                                 path.data_ptr(), kept.data_ptr(), path.shape[1],
                                                 B, Hkv, Smax, D, _dtype_code(k0), _stream(k0)),
                    "kf_kv_cache_keep")

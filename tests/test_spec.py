@@ -57,14 +57,16 @@ def test_tree_workspace_size():
     (dict(T=-1.0), b"temperature"), (dict(T=float("nan")), b"temperature"),
     (dict(T=float("inf")), b"temperature"), (dict(drafts=P), b"chain"),
     (dict(drafts=P, parents=None, T=0.0), b"chain"), (dict(stride=3), b"parents_stride"),
+    (dict(ws=None), b"workspace"), (dict(ws_bytes=8), b"workspace"), (dict(B=70000), b"65535"),
 ])
 def test_verify_refusals(change, word):
     lib = _library()
-    a = dict(B=2, N=8, V=100, dtype=1, logits=P, T=1.0, drafts=None, parents=P, stride=8) | change
+    a = dict(B=2, N=8, V=100, dtype=1, logits=P, T=1.0, drafts=None, parents=P, stride=8,
+             ws=P, ws_bytes=1 << 30) | change
     rc = lib.kf_verify_drafts(a["logits"], 800, 100, P, a["parents"], a["stride"], P, a["drafts"],
-                              800, 100, P, a["T"], P, P, P, a["B"], a["N"], a["V"], a["dtype"],
-                              None)
-    assert rc == 1 and word in lib.kf_last_error()
+                              800, 100, P, a["T"], P, P, P, a["ws"], a["ws_bytes"], a["B"],
+                              a["N"], a["V"], a["dtype"], None)
+    assert rc == (4 if word == b"workspace" else 1) and word in lib.kf_last_error()
 
 
 @pytest.mark.parametrize("change,word", [
@@ -129,3 +131,22 @@ def test_inputs_exercise_both_answers():
     logits, tokens, u, _ = verify_inputs(torch.float32, 16, 15, 500, 0, par)
     kept = spec_ref.verify(logits, tokens, u, 1.0, par)[1]
     assert min(kept) == 1 and max(kept) >= 3
+
+
+def test_native_checks_of_lists():
+    """The pointers of a list of like tensors, and what it refuses."""
+    import array
+
+    same = _lib.native().same
+    buf = array.array("Q", bytes(8 * 4))
+    ts = [torch.zeros(2, 3) for _ in range(3)]
+    assert same(ts, buf, 1) == -1
+    assert buf.tolist() == [0] + [t.data_ptr() for t in ts]
+    for bad in ([ts[0], torch.zeros(3, 2)], [ts[0], torch.zeros(2, 3, dtype=torch.int32)],
+                [torch.zeros(3, 2).t()], [ts[0], 5], [], ts + ts):
+        with pytest.raises(ValueError):
+            same(bad, buf, 0)
+    with pytest.raises(TypeError):
+        same(tuple(ts), buf, 0)
+    with pytest.raises(ValueError):
+        same(ts, buf, -2)
