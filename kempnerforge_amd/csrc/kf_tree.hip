@@ -7,14 +7,15 @@
 // lens[b] + i, so that the rows of all nodes lie behind the prefix in node order
 // and are read like it, under a mask.
 //
-//  1. prep    the ancestors of every node (as bit masks), the rotated queries,
-//             and the nodes' rows of the caches
-//  2. stream  split-K attention on the matrix cores: a workgroup takes up to 128
+//  1. stream  split-K attention on the matrix cores: a workgroup takes up to 128
 //             (node, query head) rows of a KV head and an equal share of all key
-//             chunks; a row tile that more than one workgroup met leaves float32
-//             partials
-//  3. merge   joins the partials; rows of unused nodes and refused sequences
-// Head sizes other than 64 and 128 run as one wavefront per row (tree_rows).
+//             chunks; it rotates its queries into registers, and the nodes' keys
+//             and values where its chunks hold them (the first row tile's
+//             workgroups write them to the caches); a row tile that more than one
+//             workgroup met leaves float32 partials
+//  2. merge   joins the partials; rows of unused nodes and refused sequences
+// Other head sizes and misaligned buffers: prep (rotated queries, ancestor masks,
+// the nodes' cache rows), then one wavefront per row (rows).
 //
 // Rounding: the norm and the rotation of q and k are formed in 32 bits.  k is
 // rounded once, where it is stored.  q is not rounded to 16 bits: it goes
@@ -68,177 +69,98 @@ struct Piece {
   }
 };
 
-// One workgroup: sequence blockIdx.y, `per` of its N * (Hq + 2 Hkv) rows.  The
-// queries go to `qrot` scaled by D^-1/2 log2(e), as [B][Hkv][node, head of the
-// group][D]: float32, or (SPLIT) hi and, `qlo` elements behind, lo.
+// A sequence's nodes in use and prefix length; -1 nodes where they are out of range.
+__device__ __forceinline__ int2 tree_seq(const TreeArgs& a, int b) {
+  const int n = a.counts ? a.counts[b] : a.N, L = a.lens[b];
+  const bool ok = n >= 0 && n <= a.N && L >= 0 && (int64_t)L + n <= a.max_len;
+  return ok ? make_int2(n, L) : make_int2(-1, 0);
+}
+
+// One sequence's tree in LDS: each node's ancestors (itself among them) as bits,
+// and its depth.
+struct TreeLds {
+  uint32_t mask[MAXN][MAXW + 1];
+  int ptr[MAXN], depth[MAXN];
+};
+
+// Forms the tree of sequence b (s: its nodes and prefix), by a workgroup of 256;
+// returns whether the sequence is refused.  A chain needs no LDS: node i sees
+// nodes 0 .. i and lies at depth i.
 //
-// The ancestor masks come from pointer doubling: after round r, mask[i] holds
-// the 2^r nearest of i and its ancestors and ptr[i] the next one beyond, so 8
-// rounds cover 256 nodes whatever their depth (a walk up a chain of 200 would
-// take 200 dependent reads).  Every workgroup of a sequence forms them again
-// (under a microsecond, no launch of its own); the first one stores them.
-//
-// DV > 0: the head size, rows of 16-byte pieces (G lanes a row, per = 256 / G
-// rows, one per lane group): bound by the latency of three dependent loads (the
-// lengths and parents, the table row, the stores), so a row's own loads are
-// issued before the masks are formed.  DV = 0: any head size, one wavefront a
-// row and element by element.
-template <typename T, bool SPLIT, int DV>
-__global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __restrict__ qrot,
-                                                        int64_t qlo, uint32_t* __restrict__ anc,
-                                                        int2* __restrict__ seq,
-                                                        uint8_t* __restrict__ vbad, int W,
-                                                        int per) {
-  __shared__ uint32_t smask[MAXN][MAXW + 1];
-  __shared__ int sptr[MAXN], sdepth[MAXN];
-  const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int N = a.N, D = DV > 0 ? DV : a.D, half = D / 2;
-  const int heads = a.Hq + 2 * a.Hkv, n_rep = a.Hq / a.Hkv;
-  // the lane group's row: node vi, head vh (queries, keys, values)
-  constexpr int G = DV > 0 ? DV / 2 / Piece<T>::E : 1;
-  const int vr = blockIdx.x * per + t / G;
-  const int vi = vr / heads, vh = vr % heads, vd = t % G * Piece<T>::E;
-  Piece<T> x;
-  if constexpr (DV > 0) {
-    if (vi < N) {
-      const int64_t node = (int64_t)b * N + vi;
-      const T* src = vh < a.Hq            ? (const T*)a.q_new + (node * a.Hq + vh) * D
-                     : vh < a.Hq + a.Hkv ? (const T*)a.k_new + (node * a.Hkv + vh - a.Hq) * D
-                                         : (const T*)a.v_new + (node * a.Hkv + vh - a.Hq - a.Hkv) * D;
-      x.load(src, vd, half);
+// The masks come from pointer doubling: after round r, mask[i] holds the 2^r
+// nearest of i and its ancestors and ptr[i] the next one beyond, so 8 rounds
+// cover 256 nodes whatever their depth (a walk up a chain of 200 would take 200
+// dependent reads).
+__device__ __forceinline__ bool tree_build(const TreeArgs& a, int b, int2 s, int W, TreeLds& lds) {
+  const int64_t low = (int64_t)s.y - a.rope_row_offset;  // table row of depth 0
+  if (a.parents == nullptr)
+    return s.x < 0 || (s.x > 0 && (low < 0 || low + s.x > a.rope_rows));
+  const int t = threadIdx.x, used = max(s.x, 0);
+  bool bad = s.x < 0;
+  int par = -1;
+  if (t < used) {
+    par = a.parents[(int64_t)b * a.parents_stride + t];
+    if (par < -1 || par >= t) {
+      bad = true;
+      par = -1;
     }
   }
-  const int L = a.lens[b], n = a.counts ? a.counts[b] : N;
-  bool bad = n < 0 || n > N || L < 0 || (int64_t)L + n > a.max_len;
-  const int used = bad ? 0 : n;
-  int depth = t;
-  if (a.parents != nullptr) {
-    int par = -1;
-    if (t < used) {
-      par = a.parents[(int64_t)b * a.parents_stride + t];
-      if (par < -1 || par >= t) {
-        bad = true;
-        par = -1;
-      }
+  __syncthreads();  // the previous tree's readers are done
+  for (int k = 0; k < W; ++k) lds.mask[t][k] = k == t >> 5 ? 1u << (t & 31) : 0u;
+  lds.ptr[t] = par;
+  __syncthreads();
+  for (int span = 1; span < used; span <<= 1) {
+    const int p = lds.ptr[t];
+    uint32_t m[MAXW];
+    int next = -1;
+    if (p >= 0) {
+#pragma unroll
+      for (int k = 0; k < MAXW; ++k) m[k] = k < W ? lds.mask[p][k] : 0u;
+      next = lds.ptr[p];
     }
-    for (int k = 0; k < W; ++k) smask[t][k] = 0;
-    smask[t][t >> 5] = 1u << (t & 31);
-    sptr[t] = par;
     __syncthreads();
-    for (int span = 1; span < used; span <<= 1) {
-      const int p = sptr[t];
-      uint32_t m[MAXW];
-      int next = -1;
-      if (p >= 0) {
-        for (int k = 0; k < MAXW; ++k) m[k] = k < W ? smask[p][k] : 0u;
-        next = sptr[p];
-      }
-      __syncthreads();
-      if (p >= 0) {
-        for (int k = 0; k < MAXW; ++k)
-          if (k < W) smask[t][k] |= m[k];
-        sptr[t] = next;
-      }
-      __syncthreads();
+    if (p >= 0) {
+#pragma unroll
+      for (int k = 0; k < MAXW; ++k)
+        if (k < W) lds.mask[t][k] |= m[k];
+      lds.ptr[t] = next;
     }
-    depth = -1;
-    for (int k = 0; k < W; ++k) depth += __popc(smask[t][k]);
-  } else {  // a chain: node i sees nodes 0 .. i
-    for (int k = 0; k < W; ++k) {
-      const int lo = t + 1 - 32 * k;
-      smask[t][k] = lo <= 0 ? 0u : lo >= 32 ? ~0u : (1u << lo) - 1u;
-    }
+    __syncthreads();
   }
-  sdepth[t] = depth;
-  const int64_t trow = (int64_t)L + depth - a.rope_row_offset;
-  if (t < used && (trow < 0 || trow >= a.rope_rows)) bad = true;
-  bad = __syncthreads_or(bad);
+  int depth = -1;
+  for (int k = 0; k < W; ++k) depth += __popc(lds.mask[t][k]);
+  lds.depth[t] = depth;
+  if (t < used && (low + depth < 0 || low + depth >= a.rope_rows)) bad = true;
+  return __syncthreads_or(bad);
+}
+
+// One workgroup: sequence blockIdx.y, `per` of its N * (Hq + 2 Hkv) rows, a
+// wavefront a row.  The queries go to `qrot`, float32 [B][Hkv][node, head of the
+// group][D], scaled by D^-1/2 log2(e).  Every workgroup of a sequence forms its tree
+// (under a microsecond); the first one stores the masks.
+template <typename T>
+__global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, float* __restrict__ qrot,
+                                                        uint32_t* __restrict__ anc,
+                                                        int2* __restrict__ seq, int W, int per) {
+  __shared__ TreeLds tree;
+  const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int N = a.N, D = a.D, half = D / 2;
+  const int heads = a.Hq + 2 * a.Hkv, n_rep = a.Hq / a.Hkv;
+  const int2 s = tree_seq(a, b);
+  const bool bad = tree_build(a, b, s, W, tree);
+  const int n = s.x, L = s.y;
   if (blockIdx.x == 0) {
-    if (t == 0) seq[b] = make_int2(bad ? -1 : n, bad ? 0 : L);
+    if (t == 0) seq[b] = bad ? make_int2(-1, 0) : s;
     if (t < N)
-      for (int k = 0; k < W; ++k) anc[((int64_t)b * N + t) * W + k] = smask[t][k];
+      for (int k = 0; k < W; ++k) {
+        const int lo = t + 1 - 32 * k;  // (chain: nodes 0 .. t)
+        anc[((int64_t)b * N + t) * W + k] = a.parents != nullptr ? tree.mask[t][k]
+                                            : lo <= 0              ? 0u
+                                            : lo >= 32             ? ~0u
+                                                                   : (1u << lo) - 1u;
+      }
   }
   if (bad) return;
-  if constexpr (DV > 0) {
-    constexpr int E = Piece<T>::E;
-    if (vi >= n) return;
-    const int64_t slot = (int64_t)L + vi;
-    float f1[E], f2[E];
-    Piece<T>::unpack(x.a, f1);
-    Piece<T>::unpack(x.b, f2);
-    if (vh >= a.Hq + a.Hkv) {
-      const int g = vh - a.Hq - a.Hkv;
-      T* dst = (T*)a.v_cache + (((int64_t)b * a.Hkv + g) * a.Smax + slot) * D + vd;
-      *(u32x4*)dst = x.a;
-      *(u32x4*)(dst + half) = x.b;
-      bool fin = true;
-#pragma unroll
-      for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
-      const uint64_t m = __builtin_amdgcn_ballot_w64(!fin);
-      const uint64_t mine = ((1ull << G) - 1) << (lane / G * G);
-      if (t % G == 0) vbad[((int64_t)b * a.Hkv + g) * N + vi] = (m & mine) != 0;
-      return;
-    }
-    const bool is_q = vh < a.Hq;
-    const float* nw = is_q ? a.q_norm_w : a.k_norm_w;
-    const int64_t row = ((int64_t)L + sdepth[vi] - a.rope_row_offset) * half + vd;
-    float c[E], sn[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      c[e] = a.cos[row + e];
-      sn[e] = a.sin[row + e];
-    }
-    if (nw != nullptr) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) ss += f1[e] * f1[e] + f2[e] * f2[e];
-#pragma unroll
-      for (int o = 1; o < G; o <<= 1) ss += __shfl_xor(ss, o, 64);
-      const float rs = rsqrtf(ss / (float)D + a.norm_eps);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        f1[e] = f1[e] * rs * nw[vd + e];
-        f2[e] = f2[e] * rs * nw[vd + half + e];
-      }
-    }
-    float y1[E], y2[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      y1[e] = f1[e] * c[e] - f2[e] * sn[e];
-      y2[e] = f2[e] * c[e] + f1[e] * sn[e];
-    }
-    if (!is_q) {
-      const int g = vh - a.Hq;
-      T* dst = (T*)a.k_cache + (((int64_t)b * a.Hkv + g) * a.Smax + slot) * D + vd;
-      *(u32x4*)dst = Piece<T>::pack(y1);
-      *(u32x4*)(dst + half) = Piece<T>::pack(y2);
-      return;
-    }
-    const int g = vh / n_rep;
-    const float sc = a.scale * kLog2e;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      y1[e] *= sc;
-      y2[e] *= sc;
-    }
-    T* dst = (T*)qrot +
-             (((int64_t)b * a.Hkv + g) * N * n_rep + (int64_t)vi * n_rep + vh % n_rep) * D + vd;
-    const u32x4 h1 = Piece<T>::pack(y1), h2 = Piece<T>::pack(y2);
-    *(u32x4*)dst = h1;
-    *(u32x4*)(dst + half) = h2;
-    if constexpr (SPLIT) {
-      Piece<T>::unpack(h1, f1);
-      Piece<T>::unpack(h2, f2);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        y1[e] -= f1[e];
-        y2[e] -= f2[e];
-      }
-      *(u32x4*)(dst + qlo) = Piece<T>::pack(y1);
-      *(u32x4*)(dst + qlo + half) = Piece<T>::pack(y2);
-    }
-    return;
-  }
   const int64_t r1 = min((int64_t)n * heads, (int64_t)(blockIdx.x + 1) * per);
   for (int64_t r = (int64_t)blockIdx.x * per + w; r < r1; r += 4) {
     const int i = (int)(r / heads), h = (int)(r % heads);
@@ -247,14 +169,7 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __rest
       const int g = h - a.Hq - a.Hkv;
       const T* src = (const T*)a.v_new + (node * a.Hkv + g) * D;
       T* dst = (T*)a.v_cache + (((int64_t)b * a.Hkv + g) * a.Smax + L + i) * D;
-      bool fin = true;
-      for (int d = lane; d < D; d += 64) {
-        const T x = src[d];
-        dst[d] = x;
-        fin = fin && finite(x);
-      }
-      const uint64_t all = __builtin_amdgcn_ballot_w64(!fin);
-      if (lane == 0) vbad[((int64_t)b * a.Hkv + g) * N + i] = all != 0;
+      for (int d = lane; d < D; d += 64) dst[d] = src[d];
       continue;
     }
     const bool is_q = h < a.Hq;
@@ -271,28 +186,23 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, void* __rest
       for (int d = lane; d < D; d += 64) ss += to_f32(src[d]) * to_f32(src[d]);
       rs = rsqrtf(wave_sum(ss) / (float)D + a.norm_eps);
     }
-    const int64_t row = ((int64_t)L + sdepth[i] - a.rope_row_offset) * half;
+    const int depth = a.parents != nullptr ? tree.depth[i] : i;
+    const int64_t row = ((int64_t)L + depth - a.rope_row_offset) * half;
     for (int d = lane; d < half; d += 64) {
       float x1 = to_f32(src[d]), x2 = to_f32(src[d + half]);
       if (nw != nullptr) {
         x1 = x1 * rs * nw[d];
         x2 = x2 * rs * nw[d + half];
       }
-      const float c = a.cos[row + d], s = a.sin[row + d];
-      const float y[2] = {x1 * c - x2 * s, x2 * c + x1 * s};
+      const float c = a.cos[row + d], sn = a.sin[row + d];
+      const float y[2] = {x1 * c - x2 * sn, x2 * c + x1 * sn};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int at = d + e * half;
-        if (!is_q) {
+        if (is_q)
+          qrot[qrow + at] = y[e] * (a.scale * kLog2e);
+        else
           kdst[at] = from_f32<T>(y[e]);
-        } else if constexpr (SPLIT) {
-          const float z = y[e] * (a.scale * kLog2e);
-          const T hi = from_f32<T>(z);
-          ((T*)qrot)[qrow + at] = hi;
-          ((T*)qrot)[qlo + qrow + at] = from_f32<T>(z - to_f32(hi));
-        } else {
-          ((float*)qrot)[qrow + at] = y[e] * (a.scale * kLog2e);
-        }
       }
     }
   }
@@ -353,13 +263,13 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const float*
 // (node-major: the heads of a node side by side); every tile meets the nck(b) =
 // ceil((lens[b] + n_b) / KC) key chunks of its pair.
 struct TreeSched {
-  const int2* seq;
-  int B, Hkv, n_rep, rows, kc;
+  const TreeArgs& a;
+  int B, n_rep, rows, kc;
   __device__ __forceinline__ int nck(int2 s) const { return (s.x + s.y + kc - 1) / kc; }
   __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
   __device__ __forceinline__ int chunks(int b) const {
-    const int2 s = seq[b];
-    return s.x > 0 ? Hkv * tiles(s) * nck(s) : 0;
+    const int2 s = tree_seq(a, b);
+    return s.x > 0 ? a.Hkv * tiles(s) * nck(s) : 0;
   }
 };
 
@@ -370,7 +280,7 @@ struct TreeCursor {
   int2 s;
   __device__ __forceinline__ void at(const TreeSched& sched, int b_) {
     b = b_;
-    s = sched.seq[b];
+    s = tree_seq(sched.a, b);
     s.x = __builtin_amdgcn_readfirstlane(s.x);
     s.y = __builtin_amdgcn_readfirstlane(s.y);
     nck = sched.nck(s);
@@ -390,10 +300,10 @@ struct TreeCursor {
     c = 0;
     if (++t < tiles) return;
     t = 0;
-    if (++g < sched.Hkv) return;
+    if (++g < sched.a.Hkv) return;
     g = 0;
     for (int nb = b + 1; nb < sched.B; ++nb) {
-      if (sched.seq[nb].x > 0) {
+      if (tree_seq(sched.a, nb).x > 0) {
         at(sched, nb);
         return;
       }
@@ -497,18 +407,21 @@ struct Shape {
 
 template <typename T, int D, int RW, int BKW>
 __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stream_kernel(
-    TreeArgs a, const T* __restrict__ qrot, int64_t qlo, const uint32_t* __restrict__ anc,
-    const int2* __restrict__ seq, const uint8_t* __restrict__ vbad, int W,
-    float* __restrict__ opart, float* __restrict__ mlpart, int tiles_max) {
+    TreeArgs a, int W, float* __restrict__ opart, float* __restrict__ mlpart,
+    int* __restrict__ refusals, int tiles_max) {
   using namespace mfma;
   using X = Tile<T, D>;
+  using P = Piece<T>;
   using Sh = Shape<T, D, RW, BKW>;
   constexpr int KW = Sh::KW, ROWS = Sh::ROWS, KC = Sh::KC, NB = BKW / 32, DT = D / 32;
+  constexpr int E = P::E, HALF = D / 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ TreeLds tree;
+  __shared__ uint32_t sbad[KC / 32];  // the chunk's V rows with Inf or NaN
   const int w = wave_id(), lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
   const int rw = w % RW, kw = w / RW;
   const int N = a.N, n_rep = a.Hq / a.Hkv;
-  const TreeSched sched{seq, a.B, a.Hkv, n_rep, ROWS, KC};
+  const TreeSched sched{a, a.B, n_rep, ROWS, KC};
   const int C = total_chunks(sched, lane), NW = min((int)gridDim.x, C);
   const int gw = blockIdx.x;
   if (gw >= NW) return;
@@ -525,6 +438,32 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     tile_to_lds<KC, X::R>((const uint16_t*)((const T*)a.v_cache + row * D), D * U,
                           dst + Sh::TILE * U, w, lane, rows);
   };
+  // the table row of node j (kept inside the table: a refused sequence's may not be)
+  auto table_row = [&](int2 s, int j) {
+    const int64_t r = (int64_t)s.y + (a.parents != nullptr ? tree.depth[j] : j) - a.rope_row_offset;
+    return min(max(r, (int64_t)0), a.rope_rows - 1) * HALF;
+  };
+  // E pairs of one row rotated (and normalised by rs with weights nw first), four
+  // at a time: the registers of all their table values would spill others
+  auto rotate = [&](float* f1, float* f2, int64_t trow, int d, const float* nw, float rs) {
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += 4) {
+      const f32x4 c = *(const f32x4*)(a.cos + trow + d + e0);
+      const f32x4 sn = *(const f32x4*)(a.sin + trow + d + e0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = e0 + j;
+        if (nw != nullptr) {
+          f1[e] = f1[e] * rs * nw[d + e];
+          f2[e] = f2[e] * rs * nw[d + HALF + e];
+        }
+        const float y1 = f1[e] * c[j] - f2[e] * sn[j];
+        f2[e] = f2[e] * c[j] + f1[e] * sn[j];
+        f1[e] = y1;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
 
   const typename X::VOff voff = X::v_off(lane);
   u32x4 q[X::QP][X::KS];
@@ -534,22 +473,60 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   cc.seek(sched, c_lo, lane);
   ic = cc;
   issue(ic, c_lo);
-  bool whole = false;  // this workgroup holds all of the row tile's chunks
-  int row = 0, node = 0;
+  bool whole = false;    // this workgroup holds all of the row tile's chunks
+  bool refused = false;  // the sequence's tree or tables are out of range
+  int node = 0, built = -1;
 
   for (int i = c_lo; i < c_hi; ++i) {
-    const bool first = i == c_lo || cc.c == 0;
-    if (first) {
+    if (i == c_lo || cc.c == 0) {
       whole = cc.c == 0;
-      const int nrows = cc.s.x * n_rep;
-      row = min(cc.t * ROWS + 32 * rw + l31, nrows - 1);
+      if (cc.b != built) refused = tree_build(a, cc.b, cc.s, W, tree);
+      built = cc.b;
+      if (whole && cc.g == 0 && cc.t == 0 && threadIdx.x == 0) refusals[cc.b] = refused;
+      // the rotated queries: lane l holds dims of half h, 16-byte pieces 2 ks + h;
+      // a piece's RoPE partner is the lane's own piece KS / 2 further on
+      const int row = min(cc.t * ROWS + 32 * rw + l31, cc.s.x * n_rep - 1);
       node = row / n_rep;
-      const T* qr = qrot + ((((int64_t)cc.b * a.Hkv + cc.g) * N * n_rep + row) * D);
+      const T* qr = (const T*)a.q_new +
+                    (((int64_t)cc.b * N + node) * a.Hq + cc.g * n_rep + row % n_rep) * D;
+      const int64_t trow = table_row(cc.s, node);
+      u32x4 raw[X::KS];
 #pragma unroll
-      for (int p = 0; p < X::QP; ++p)
+      for (int ks = 0; ks < X::KS; ++ks) raw[ks] = *(const u32x4*)(qr + (2 * ks + h) * E);
+      float rs = 1.f;
+      if (a.q_norm_w != nullptr) {
+        float ss = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < X::KS; ++ks)
-          q[p][ks] = *(const u32x4*)(qr + p * qlo + (2 * ks + h) * (16 / (int)sizeof(T)));
+        for (int ks = 0; ks < X::KS; ++ks) {
+          float f[E];
+          P::unpack(raw[ks], f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss += f[e] * f[e];
+        }
+        rs = rsqrtf(pair_sum32(ss) / (float)D + a.norm_eps);
+      }
+      const float sc = a.scale * kLog2e;
+#pragma unroll
+      for (int ks = 0; ks < X::KS / 2; ++ks) {
+        float f[2][E];
+        P::unpack(raw[ks], f[0]);
+        P::unpack(raw[ks + X::KS / 2], f[1]);
+        rotate(f[0], f[1], trow, (2 * ks + h) * E, a.q_norm_w, rs);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = ks + x * (X::KS / 2);
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[x][e] *= sc;
+          q[0][at] = P::pack(f[x]);
+          if constexpr (X::QP == 2) {
+            float hi[E];
+            P::unpack(q[0][at], hi);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[x][e] -= hi[e];
+            q[1][at] = P::pack(f[x]);
+          }
+        }
+      }
       m = -INFINITY;
       lsum = 0.f;
 #pragma unroll
@@ -566,23 +543,83 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     }
     T* kt = stage_k(i);
     T* vt = kt + Sh::TILE;
-    const int L = cc.s.y, keys = L + cc.s.x;
+    const bool tail = cc.c * KC + KC > cc.s.y;  // the chunk holds nodes, or ends behind them
+    if (tail) {
+      // The nodes' rows, from k_new and v_new over what the cache held there;
+      // the first row tile's workgroup writes them to the cache as well.  V rows
+      // behind the last become zero: 0 x NaN must not reach a sum.
+      constexpr int G = HALF / E;  // lanes of a row, a piece of each half a lane
+      const int r0 = cc.c * KC, L = cc.s.y, n = cc.s.x;
+      const int j0 = max(r0 - L, 0), j1 = min(r0 + KC - L, n);
+      const int64_t head = (int64_t)cc.b * a.Hkv + cc.g;
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));  // (nothing of this block is kept across the loop)
+      if (tid < KC / 32) sbad[tid] = 0;
+      __syncthreads();
+      for (int x = tid; x < (j1 - j0) * G; x += 256) {
+        const int j = j0 + x / G, d = x % G * E, lr = L + j - r0, sw = swz<X::R>(lr);
+        const int64_t src = (((int64_t)cc.b * N + j) * a.Hkv + cc.g) * D;
+        const int ca = ((d / E) ^ sw) * E, cb = (((d + HALF) / E) ^ sw) * E;
+        const int64_t dst = (head * a.Smax + L + j) * D + d;
+        const bool store = cc.t == 0 && !refused;
+        P x2;
+        float f1[E], f2[E];
+        x2.load((const T*)a.v_new + src, d, HALF);
+        *(u32x4*)(vt + lr * D + ca) = x2.a;
+        *(u32x4*)(vt + lr * D + cb) = x2.b;
+        if (store) {
+          *(u32x4*)((T*)a.v_cache + dst) = x2.a;
+          *(u32x4*)((T*)a.v_cache + dst + HALF) = x2.b;
+        }
+        P::unpack(x2.a, f1);
+        P::unpack(x2.b, f2);
+        bool fin = true;
+#pragma unroll
+        for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
+        if (!fin) atomicOr(&sbad[lr >> 5], 1u << (lr & 31));
+        __builtin_amdgcn_sched_barrier(0);
+        x2.load((const T*)a.k_new + src, d, HALF);
+        P::unpack(x2.a, f1);
+        P::unpack(x2.b, f2);
+        float rs = 1.f;
+        if (a.k_norm_w != nullptr) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss += f1[e] * f1[e] + f2[e] * f2[e];
+#pragma unroll
+          for (int o = 1; o < G; o <<= 1) ss += __shfl_xor(ss, o, 64);
+          rs = rsqrtf(ss / (float)D + a.norm_eps);
+        }
+        rotate(f1, f2, table_row(cc.s, j), d, a.k_norm_w, rs);
+        x2.a = P::pack(f1);
+        x2.b = P::pack(f2);
+        *(u32x4*)(kt + lr * D + ca) = x2.a;
+        *(u32x4*)(kt + lr * D + cb) = x2.b;
+        if (store) {
+          *(u32x4*)((T*)a.k_cache + dst) = x2.a;
+          *(u32x4*)((T*)a.k_cache + dst + HALF) = x2.b;
+        }
+      }
+      for (int x = (L + j1 - r0) * X::R + tid; x < KC * X::R; x += 256)
+        *(u32x4*)(vt + x * E) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+    const int L = cc.s.y;
     const int k0 = cc.c * KC + kw * BKW;  // the wavefront's first key
-    // Blocks that hold nodes' keys, or places behind the last one (the loads repeat
-    // the last row there): which of the block's 32 keys the lane's row sees, and
-    // which have Inf or NaN in their V row.
-    auto sees = [&](int t0) -> uint32_t {  // t0: node of the block's first key, > -32
-      const uint32_t* words = anc + ((int64_t)cc.b * N + node) * W;
+    // Which of a block's 32 keys the lane's row sees, the first of them node t0 (>
+    // -32; keys before node 0 are the prefix); and which have Inf or NaN in V.
+    auto sees = [&](int t0) -> uint32_t {
+      if (a.parents == nullptr) {  // nodes 0 .. node
+        const int lo = node + 1 - t0;
+        return lo <= 0 ? 0u : lo >= 32 ? ~0u : (1u << lo) - 1u;
+      }
       const int idx = t0 >> 5, sh = t0 & 31;
-      const uint32_t w0 = idx < 0 ? ~0u : idx < W ? words[idx] : 0u;
-      const uint32_t w1 = idx + 1 < W ? words[idx + 1] : 0u;
+      const uint32_t w0 = idx < 0 ? ~0u : idx < W ? tree.mask[node][idx] : 0u;
+      const uint32_t w1 = idx + 1 < W ? tree.mask[node][idx + 1] : 0u;
       return sh ? (w0 >> sh) | (w1 << (32 - sh)) : w0;
     };
-    auto unclean = [&](int t0) -> uint32_t {
-      const uint8_t* flag = vbad + ((int64_t)cc.b * a.Hkv + cc.g) * N;
-      const int kn = t0 + l31;
-      return (uint32_t)__builtin_amdgcn_ballot_w64(
-          kn >= 0 && flag[max(min(kn, cc.s.x - 1), 0)] != 0);
+    auto unclean = [&](int nb) -> uint32_t {
+      return __builtin_amdgcn_readfirstlane(sbad[(kw * BKW + 32 * nb) / 32]);
     };
     f32x16 s[NB];
     bool bad = false;
@@ -598,7 +635,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           s[nb][e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[nb][e] : -INFINITY;
-        bad |= unclean(t0) != 0;
+        bad |= unclean(nb) != 0;
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[nb][e]);
@@ -620,7 +657,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       const int row0 = kw * BKW + 32 * nb;
       const int t0 = k0 + 32 * nb - L;
       if (bad && t0 > -32) {  // 0 x Inf must not reach the rows that do not see the key
-        for (uint32_t x = unclean(t0); x; x &= x - 1) {
+        for (uint32_t x = unclean(nb); x; x &= x - 1) {
           const int r = row0 + __builtin_ctz(x);
           if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
         }
@@ -629,22 +666,25 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       X::values(vt, row0, voff, s[nb], acc, lane);
       if (bad && t0 > -32) {  // those keys one by one, for the rows that see them
         const uint32_t bits = sees(t0);
-        for (uint32_t x = unclean(t0); x; x &= x - 1) {
-          const int kk = __builtin_ctz(x), key = k0 + 32 * nb + kk;
-          if (key >= keys) break;
+        int hh = 4 * h;
+        asm volatile("" : "+v"(hh));  // (as above)
+        for (uint32_t x = unclean(nb); x; x &= x - 1) {
+          const int kk = __builtin_ctz(x);
           float p = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (8 * (e / 4) + 4 * h + e % 4 == kk) p = s[nb][e];
+            if (8 * (e / 4) + hh + e % 4 == kk) p = s[nb][e];
           p = pair_sum32(p);
           if ((bits >> kk) & 1) {
-            const T* vr = (const T*)a.v_cache +
-                          (((int64_t)cc.b * a.Hkv + cc.g) * a.Smax + key) * D + 4 * h;
+            const T* vr = (const T*)a.v_new +
+                          (((int64_t)cc.b * N + t0 + kk) * a.Hkv + cc.g) * D + hh;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
+              for (int e = 0; e < 16; ++e) {
                 acc[dt][e] += p * to_f32(vr[32 * dt + 8 * (e / 4) + e % 4]);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (registers)
+              }
           }
         }
       }
@@ -655,6 +695,10 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       // the stage just computed, then the output, or a partial in slot gw + tile
       whole = whole && last;
       float l = pair_sum32(lsum);
+      if (refused) {
+        m = 0.f;
+        l = NAN;
+      }
       if constexpr (KW > 1) {
         __syncthreads();  // all wavefronts are done with the stage
         float* xo = (float*)kt;                    // [KW - 1][ROWS][D]
@@ -731,20 +775,19 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 // The rows of tile blockIdx.x, 16 bytes of a row per thread and
 // blockIdx.y's share of them: the partials of the workgroups that met the tile
 // rescaled to a common maximum and summed; a tile that one workgroup finished is
-// left alone.  The schedule's divisions are the workgroup's, not each row's:
-// one wavefront per row took 14.5 us where this takes ... (tree_batch's sizes).
+// left alone.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
-    TreeArgs a, const int2* __restrict__ seq, const float* __restrict__ opart,
-    const float* __restrict__ mlpart, int rows, int kc, int NWmax, int tiles_max) {
+    TreeArgs a, const float* __restrict__ opart, const float* __restrict__ mlpart,
+    const int* __restrict__ refusals, int rows, int kc, int NWmax, int tiles_max) {
   constexpr int LPR = D / 4;  // lanes of a row
   const int lane = threadIdx.x & 63, n_rep = a.Hq / a.Hkv;
   const int item = blockIdx.x, t = item % tiles_max, bg = item / tiles_max, b = bg / a.Hkv,
             g = bg % a.Hkv;
   const int r = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
   const int row = t * rows + r, i = row / n_rep, hq = g * n_rep + row % n_rep;
-  const int2 s = seq[b];
-  const TreeSched sched{seq, a.B, a.Hkv, n_rep, rows, kc};
+  const int2 s = tree_seq(a, b);
+  const TreeSched sched{a, a.B, n_rep, rows, kc};
   int tot = 0, pre = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int n = b0 + lane < a.B ? sched.chunks(b0 + lane) : 0;
@@ -755,8 +798,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
   T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + hq) * D + col;
   T y[4];
   if (s.x < 0 || i >= s.x) {  // a refused sequence, or an unused node
+    const bool refused = s.x < 0 || (s.x > 0 && refusals[b]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(s.x < 0 ? NAN : 0.f);
+    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(refused ? NAN : 0.f);
     __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
     return;
   }
@@ -825,44 +869,45 @@ Plan plan_of(const TreeArgs& a) {
   return p;
 }
 
-// workspace: rotated queries (hi and lo, or float32: four bytes an element at
-// the most), ancestor masks, per sequence (nodes in use or -1, prefix length),
-// per (b, KV head, node) whether its V row holds Inf or NaN, the partials
+// workspace: the partials, and whether each sequence's tree or tables are refused
+// (written with its first chunk); or, one wavefront per row, rotated queries, ancestor
+// masks and per sequence (nodes in use or -1, prefix length)
 struct Ws {
-  void* qrot;
+  float *opart, *mlpart;
+  int* refusals;
+  float* qrot;
   uint32_t* anc;
   int2* seq;
-  uint8_t* vbad;
-  float *opart, *mlpart;
   size_t bytes;
 };
-Ws carve(const TreeArgs& a, void* p) {
-  const size_t W = (a.N + 31) / 32;
+Ws carve(const TreeArgs& a, const Plan& pl, void* p) {
   char* c = (char*)p;
-  Ws w;
-  w.qrot = c;
-  c += up256((size_t)a.B * a.N * a.Hq * a.D * 4);
-  w.anc = (uint32_t*)c;
-  c += up256((size_t)a.B * a.N * W * 4);
-  w.seq = (int2*)c;
-  c += up256((size_t)a.B * sizeof(int2));
-  w.vbad = (uint8_t*)c;
-  c += up256((size_t)a.B * a.Hkv * a.N);
-  const Plan pl = plan_of(a);
-  const size_t prow = pl.rw ? ((size_t)pl.grid + (size_t)a.B * a.Hkv * pl.tiles) * pl.rows : 0;
-  w.opart = (float*)c;
-  c += up256(prow * a.D * 4);
-  w.mlpart = (float*)c;
-  c += up256(prow * 2 * 4);
+  Ws w = {};
+  if (pl.rw) {
+    const size_t rows = ((size_t)pl.grid + (size_t)a.B * a.Hkv * pl.tiles) * pl.rows;
+    w.opart = (float*)c;
+    c += up256(rows * a.D * 4);
+    w.mlpart = (float*)c;
+    c += up256(rows * 2 * 4);
+    w.refusals = (int*)c;
+    c += up256((size_t)a.B * 4);
+  } else {
+    w.qrot = (float*)c;
+    c += up256((size_t)a.B * a.N * a.Hq * a.D * 4);
+    w.anc = (uint32_t*)c;
+    c += up256((size_t)a.B * a.N * ((a.N + 31) / 32) * 4);
+    w.seq = (int2*)c;
+    c += up256((size_t)a.B * sizeof(int2));
+  }
   w.bytes = (size_t)(c - (char*)p);
   return w;
 }
 
 template <typename T, int D, int RW, int BKW>
-int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
+int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p) {
   using Sh = Shape<T, D, RW, BKW>;
   auto kernel = tree_stream_kernel<T, D, RW, BKW>;
-  if (Sh::LDS > 64 * 1024) {  // asked for once per device
+  if (Sh::LDS + sizeof(TreeLds) + 1024 > 64 * 1024) {  // asked for once per device
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -878,62 +923,57 @@ int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
     }
   }
   KF_LAUNCH("tree_stream", kernel, dim3(p.grid), dim3(256), Sh::LDS, a.stream, a,
-            (const T*)w.qrot, qlo, w.anc, w.seq, w.vbad, (a.N + 31) / 32, w.opart, w.mlpart,
-            p.tiles);
+            (a.N + 31) / 32, w.opart, w.mlpart, w.refusals, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
 
 template <typename T, int D>
-int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p, int64_t qlo) {
+int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p) {
   int rc;
   if constexpr (std::is_same<T, float>::value)
-    rc = p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p, qlo) : launch_stream<T, D, 4, 32>(a, w, p, qlo);
+    rc = p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p) : launch_stream<T, D, 4, 32>(a, w, p);
   else
-    rc = p.rw == 1   ? launch_stream<T, D, 1, 32>(a, w, p, qlo)
-         : p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p, qlo)
-                     : launch_stream<T, D, 4, 64>(a, w, p, qlo);
+    rc = p.rw == 1   ? launch_stream<T, D, 1, 32>(a, w, p)
+         : p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p)
+                     : launch_stream<T, D, 4, 64>(a, w, p);
   if (rc) return rc;
   const int rpw = 256 / (D / 4);  // rows of a workgroup
   KF_LAUNCH("tree_merge", (tree_merge_kernel<T, D>),
             dim3(a.B * a.Hkv * p.tiles, (p.rows + rpw - 1) / rpw), dim3(256), 0, a.stream, a,
-            w.seq, w.opart, w.mlpart, p.rows, p.kc, p.grid, p.tiles);
+            w.opart, w.mlpart, w.refusals, p.rows, p.kc, p.grid, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
 
 template <typename T>
 int tree_typed(const TreeArgs& a, void* workspace) {
-  const Ws w = carve(a, workspace);
   Plan p = plan_of(a);
-  // (the stream kernel's direct loads and the vector rows need aligned buffers)
+  // (direct loads to LDS and 16-byte rows need aligned buffers)
   if (((uintptr_t)a.q_new | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_cache |
-       (uintptr_t)a.v_cache | (uintptr_t)a.out) % 16 != 0)
+       (uintptr_t)a.v_cache | (uintptr_t)a.out | (uintptr_t)a.cos | (uintptr_t)a.sin) % 16 != 0)
     p = Plan{};
-  const int64_t qlo = (int64_t)a.B * a.N * a.Hq * a.D;
-  constexpr bool SPLIT = !std::is_same<T, float>::value;
-  auto prep = p.rw == 0     ? tree_prep_kernel<T, false, 0>
-              : a.D == 128 ? tree_prep_kernel<T, SPLIT, 128>
-                           : tree_prep_kernel<T, SPLIT, 64>;
-  const int W = (a.N + 31) / 32;
-  const int per = p.rw ? 256 / (a.D / 2 / Piece<T>::E) : 16;
-  const int64_t rows = (int64_t)a.N * (a.Hq + 2 * a.Hkv);
-  KF_LAUNCH("tree_prep", prep, dim3((unsigned)((rows + per - 1) / per), a.B), dim3(256), 0,
-            a.stream, a, w.qrot, qlo, w.anc, w.seq, w.vbad, W, per);
-  KF_CHECK_LAUNCH();
+  const Ws w = carve(a, p, workspace);
   if (p.rw)
-    return a.D == 128 ? stream_and_merge<T, 128>(a, w, p, qlo)
-                      : stream_and_merge<T, 64>(a, w, p, qlo);
+    return a.D == 128 ? stream_and_merge<T, 128>(a, w, p) : stream_and_merge<T, 64>(a, w, p);
+  const int W = (a.N + 31) / 32, per = 16;
+  const int64_t rows = (int64_t)a.N * (a.Hq + 2 * a.Hkv);
+  KF_LAUNCH("tree_prep", tree_prep_kernel<T>, dim3((unsigned)((rows + per - 1) / per), a.B),
+            dim3(256), 0, a.stream, a, w.qrot, w.anc, w.seq, W, per);
+  KF_CHECK_LAUNCH();
   KF_LAUNCH("tree_rows", tree_rows_kernel<T>,
             dim3((unsigned)(((int64_t)a.B * a.N * a.Hq + 3) / 4)), dim3(256), 0, a.stream, a,
-            (const float*)w.qrot, w.anc, w.seq, W);
+            w.qrot, w.anc, w.seq, W);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
 
 }  // namespace
 
-size_t tree_workspace(const TreeArgs& a) { return carve(a, nullptr).bytes; }
+size_t tree_workspace(const TreeArgs& a) {
+  // (which of the two a call takes goes by its buffers' alignment too)
+  return std::max(carve(a, plan_of(a), nullptr).bytes, carve(a, Plan{}, nullptr).bytes);
+}
 
 int tree_attention(const TreeArgs& a, void* workspace) {
   switch (a.dtype) {
