@@ -469,6 +469,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   u32x4 q[X::QP][X::KS];
   f32x16 acc[DT];
   float m = -INFINITY, lsum = 0.f;
+  constexpr float SLACK = 8.f;  // P stays below 2^8, far inside every type
   TreeCursor cc, ic;
   cc.seek(sched, c_lo, lane);
   ic = cc;
@@ -621,50 +622,51 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     auto unclean = [&](int nb) -> uint32_t {
       return __builtin_amdgcn_readfirstlane(sbad[(kw * BKW + 32 * nb) / 32]);
     };
-    f32x16 s[NB];
-    bool bad = false;
-    float tmax = -INFINITY;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[nb][e] = 0.f;
-      X::scores(kt, kw * BKW + 32 * nb, q, s[nb], lane);
+    for (int nb = 0; nb < NB; ++nb) {  // 32 keys at a time
+      const int row0 = kw * BKW + 32 * nb;
       const int t0 = k0 + 32 * nb - L;
+      f32x16 s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+      X::scores(kt, row0, q, s, lane);
+      bool bad = false;
       if (t0 > -32) {  // (uniform)
         const uint32_t bits = sees(t0) >> (4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          s[nb][e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[nb][e] : -INFINITY;
-        bad |= unclean(nb) != 0;
+          s[e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
+        bad = unclean(nb) != 0;
       }
+      float tmax = s[0];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[nb][e]);
-    }
-    const float mnew = fmaxf(m, pair_max32(tmax));
-    const float ref = mnew == -INFINITY ? 0.f : mnew;  // a row that has met no key yet
-    const float alpha = fast_exp2(m - ref);
-    m = mnew;
-    lsum *= alpha;
+      for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, s[e]);
+      // The exponentials are taken against a reference m that need not be the row's
+      // maximum: it moves only when a score is 2^SLACK above it (or none is set
+      // yet), so the sums are hardly ever rescaled.
+      if (__builtin_amdgcn_ballot_w64(tmax > m + SLACK || m == -INFINITY)) {
+        const float mnew = fmaxf(m, pair_max32(tmax));
+        const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
+        m = mnew;
+        lsum *= alpha;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;  // (a row that has met no key yet)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[nb][e] = fast_exp2(s[nb][e] - ref);
-        lsum += s[nb][e];
+        s[e] = fast_exp2(s[e] - ref);
+        lsum += s[e];
       }
-      const int row0 = kw * BKW + 32 * nb;
-      const int t0 = k0 + 32 * nb - L;
-      if (bad && t0 > -32) {  // 0 x Inf must not reach the rows that do not see the key
+      if (bad) {  // 0 x Inf must not reach the rows that do not see the key
         for (uint32_t x = unclean(nb); x; x &= x - 1) {
           const int r = row0 + __builtin_ctz(x);
           if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-      X::values(vt, row0, voff, s[nb], acc, lane);
-      if (bad && t0 > -32) {  // those keys one by one, for the rows that see them
+      X::values(vt, row0, voff, s, acc, lane);
+      if (bad) {  // those keys one by one, for the rows that see them
         const uint32_t bits = sees(t0);
         int hh = 4 * h;
         asm volatile("" : "+v"(hh));  // (as above)
@@ -673,7 +675,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
           float p = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (8 * (e / 4) + hh + e % 4 == kk) p = s[nb][e];
+            if (8 * (e / 4) + hh + e % 4 == kk) p = s[e];
           p = pair_sum32(p);
           if ((bits >> kk) & 1) {
             const T* vr = (const T*)a.v_new +
@@ -695,10 +697,8 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       // the stage just computed, then the output, or a partial in slot gw + tile
       whole = whole && last;
       float l = pair_sum32(lsum);
-      if (refused) {
-        m = 0.f;
-        l = NAN;
-      }
+      if (refused) l = NAN;
+      if (l != l) m = INFINITY;  // (a NaN must not be left out for its weight)
       if constexpr (KW > 1) {
         __syncthreads();  // all wavefronts are done with the stage
         float* xo = (float*)kt;                    // [KW - 1][ROWS][D]
