@@ -423,8 +423,10 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   const int N = a.N, n_rep = a.Hq / a.Hkv;
   const TreeSched sched{a, a.B, n_rep, ROWS, KC};
   const int C = total_chunks(sched, lane), NW = min((int)gridDim.x, C);
-  const int gw = blockIdx.x;
-  if (gw >= NW) return;
+  // block ids go round the 8 XCDs: neighbours in the chunk list, which read the
+  // same keys for other rows, share one XCD's L2
+  if ((int)blockIdx.x >= NW) return;
+  const int xcd = blockIdx.x % 8, gw = xcd * (NW / 8) + min(xcd, NW % 8) + (int)blockIdx.x / 8;
   const int c_lo = range_start(gw, C, NW), c_hi = range_start(gw + 1, C, NW);
 
   auto stage_k = [&](int i) { return (T*)(lds + (i & 1) * Sh::STAGE); };
@@ -443,25 +445,30 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     const int64_t r = (int64_t)s.y + (a.parents != nullptr ? tree.depth[j] : j) - a.rope_row_offset;
     return min(max(r, (int64_t)0), a.rope_rows - 1) * HALF;
   };
-  // E pairs of one row rotated (and normalised by rs with weights nw first), four
-  // at a time: the registers of all their table values would spill others
-  auto rotate = [&](float* f1, float* f2, int64_t trow, int d, const float* nw, float rs) {
+  // E pairs of one row rotated (and normalised by rs with weights nw first)
+  struct Angles {
+    f32x4 c[E / 4], s[E / 4];
+  };
+  auto angles = [&](int64_t trow, int d) {
+    Angles g;
 #pragma unroll
-    for (int e0 = 0; e0 < E; e0 += 4) {
-      const f32x4 c = *(const f32x4*)(a.cos + trow + d + e0);
-      const f32x4 sn = *(const f32x4*)(a.sin + trow + d + e0);
+    for (int x = 0; x < E / 4; ++x) {
+      g.c[x] = *(const f32x4*)(a.cos + trow + d + 4 * x);
+      g.s[x] = *(const f32x4*)(a.sin + trow + d + 4 * x);
+    }
+    return g;
+  };
+  auto rotate = [&](float* f1, float* f2, const Angles& g, int d, const float* nw, float rs) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = e0 + j;
-        if (nw != nullptr) {
-          f1[e] = f1[e] * rs * nw[d + e];
-          f2[e] = f2[e] * rs * nw[d + HALF + e];
-        }
-        const float y1 = f1[e] * c[j] - f2[e] * sn[j];
-        f2[e] = f2[e] * c[j] + f1[e] * sn[j];
-        f1[e] = y1;
+    for (int e = 0; e < E; ++e) {
+      if (nw != nullptr) {
+        f1[e] = f1[e] * rs * nw[d + e];
+        f2[e] = f2[e] * rs * nw[d + HALF + e];
       }
-      __builtin_amdgcn_sched_barrier(0);
+      const float c = g.c[e / 4][e % 4], sn = g.s[e / 4][e % 4];
+      const float y1 = f1[e] * c - f2[e] * sn;
+      f2[e] = f2[e] * c + f1[e] * sn;
+      f1[e] = y1;
     }
   };
 
@@ -494,6 +501,9 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       u32x4 raw[X::KS];
 #pragma unroll
       for (int ks = 0; ks < X::KS; ++ks) raw[ks] = *(const u32x4*)(qr + (2 * ks + h) * E);
+      Angles ang[X::KS / 2];  // (the sums' registers are free here: one round trip for all)
+#pragma unroll
+      for (int ks = 0; ks < X::KS / 2; ++ks) ang[ks] = angles(trow, (2 * ks + h) * E);
       float rs = 1.f;
       if (a.q_norm_w != nullptr) {
         float ss = 0.f;
@@ -512,7 +522,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
         float f[2][E];
         P::unpack(raw[ks], f[0]);
         P::unpack(raw[ks + X::KS / 2], f[1]);
-        rotate(f[0], f[1], trow, (2 * ks + h) * E, a.q_norm_w, rs);
+        rotate(f[0], f[1], ang[ks], (2 * ks + h) * E, a.q_norm_w, rs);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int at = ks + x * (X::KS / 2);
@@ -563,9 +573,11 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
         const int ca = ((d / E) ^ sw) * E, cb = (((d + HALF) / E) ^ sw) * E;
         const int64_t dst = (head * a.Smax + L + j) * D + d;
         const bool store = cc.t == 0 && !refused;
-        P x2;
+        P x2, kx;
         float f1[E], f2[E];
         x2.load((const T*)a.v_new + src, d, HALF);
+        kx.load((const T*)a.k_new + src, d, HALF);
+        const Angles g = angles(table_row(cc.s, j), d);
         *(u32x4*)(vt + lr * D + ca) = x2.a;
         *(u32x4*)(vt + lr * D + cb) = x2.b;
         if (store) {
@@ -578,10 +590,8 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
         for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
         if (!fin) atomicOr(&sbad[lr >> 5], 1u << (lr & 31));
-        __builtin_amdgcn_sched_barrier(0);
-        x2.load((const T*)a.k_new + src, d, HALF);
-        P::unpack(x2.a, f1);
-        P::unpack(x2.b, f2);
+        P::unpack(kx.a, f1);
+        P::unpack(kx.b, f2);
         float rs = 1.f;
         if (a.k_norm_w != nullptr) {
           float ss = 0.f;
@@ -591,7 +601,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
           for (int o = 1; o < G; o <<= 1) ss += __shfl_xor(ss, o, 64);
           rs = rsqrtf(ss / (float)D + a.norm_eps);
         }
-        rotate(f1, f2, table_row(cc.s, j), d, a.k_norm_w, rs);
+        rotate(f1, f2, g, d, a.k_norm_w, rs);
         x2.a = P::pack(f1);
         x2.b = P::pack(f2);
         *(u32x4*)(kt + lr * D + ca) = x2.a;
@@ -622,8 +632,11 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     auto unclean = [&](int nb) -> uint32_t {
       return __builtin_amdgcn_readfirstlane(sbad[(kw * BKW + 32 * nb) / 32]);
     };
+    // (a wavefront of which the tile has no rows leaves the SIMD to the others)
+    const bool active = cc.t * ROWS + 32 * rw < cc.s.x * n_rep;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {  // 32 keys at a time
+      if (!active) break;
       const int row0 = kw * BKW + 32 * nb;
       const int t0 = k0 + 32 * nb - L;
       f32x16 s;
