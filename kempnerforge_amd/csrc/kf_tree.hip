@@ -317,40 +317,58 @@ struct TreeCursor {
 //       of its half h = l / 32 in 16-byte pieces
 //   O^T (dims x rows) += V^T P^T: P^T straight from the S registers (lane l holds
 //       row l % 32, register i key 8 (i / 4) + 4 h + i % 4)
+// Every fragment is read PF steps ahead of its products: left to itself the
+// compiler, short of registers, reads each one right before them and waits out
+// the LDS (42% of the time on the matrix cores instead of ...).
 template <typename T, int D>
 struct Tile {
   static constexpr int R = D / 8;     // 16-byte chunks per cache row
   static constexpr int KS = D / 16;   // pieces of a lane's half row
   static constexpr int QP = 2;        // q as hi and lo
+  static constexpr int PF = 4, NV = D / 16;  // V fragments: 2 of 16 keys for each 32 dims
   typedef mfma::TrOffsets<D> VOff;
+  typedef bf16x8 VFrag[PF];
   static __device__ __forceinline__ VOff v_off(int lane) { return mfma::tr_offsets<D>(lane); }
   static __device__ __forceinline__ void scores(const T* k, int row0, const u32x4 (*q)[KS],
                                                 f32x16& s, int lane) {
     using namespace mfma;
+    bf16x8 f[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i) f[i] = lds_frag<R>(k, row0 + (lane & 31), 2 * i + (lane >> 5));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const bf16x8& a = lds_frag<R>(k, row0 + (lane & 31), 2 * ks + (lane >> 5));
-      s = mfma32<T>(a, as_bf16x8(q[0][ks]), s);
-      s = mfma32<T>(a, as_bf16x8(q[1][ks]), s);
+      s = mfma32<T>(f[ks % PF], as_bf16x8(q[0][ks]), s);
+      s = mfma32<T>(f[ks % PF], as_bf16x8(q[1][ks]), s);
+      if (ks + PF < KS)
+        f[ks % PF] = lds_frag<R>(k, row0 + (lane & 31), 2 * (ks + PF) + (lane >> 5));
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+  static __device__ __forceinline__ void load_v(const T* v, int row0, const VOff& off, VFrag& f,
+                                                int) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) f[i] = mfma::lds_frag_t<D>(v + row0 * D, off, i & 1, i >> 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   static __device__ __forceinline__ void values(const T* v, int row0, const VOff& off,
-                                                const f32x16& p, f32x16* acc, int lane) {
+                                                const f32x16& p, VFrag& f, f32x16* acc, int) {
     using namespace mfma;
     bf16x8 pb[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float f[8];
+      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = p[8 * c + j];
-      pb[c] = as_bf16x8(pack8<T>(f));
+      for (int j = 0; j < 8; ++j) x[j] = p[8 * c + j];
+      pb[c] = as_bf16x8(pack8<T>(x));
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        acc[dt] = mfma32<T>(lds_frag_t<D>(v + row0 * D, off, c, dt), pb[c], acc[dt]);
-    __builtin_amdgcn_sched_barrier(0);  // the next block's reads stay behind these products
+    for (int i = 0; i < NV; ++i) {  // dims 32 (i / 2) .., keys 16 (i % 2) ..
+      acc[i >> 1] = mfma32<T>(f[i % PF], pb[i & 1], acc[i >> 1]);
+      if (i + PF < NV) f[i % PF] = lds_frag_t<D>(v + row0 * D, off, i & 1, (i + PF) >> 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 };
 template <int D>
@@ -358,7 +376,9 @@ struct Tile<float, D> {
   static constexpr int R = D / 4;
   static constexpr int KS = D / 8;
   static constexpr int QP = 1;
+  static constexpr int PF = 2;
   struct VOff {};
+  struct VFrag {};
   static __device__ __forceinline__ VOff v_off(int) { return {}; }
   static __device__ __forceinline__ f32x16 mma(float a, float b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
@@ -366,25 +386,42 @@ struct Tile<float, D> {
   static __device__ __forceinline__ void scores(const float* k, int row0, const u32x4 (*q)[KS],
                                                 f32x16& s, int lane) {
     const int row = row0 + (lane & 31), sw = mfma::swz<R>(row);
+    auto frag = [&](int ks) {
+      return *(const f32x4*)(k + (row * R + ((2 * ks + (lane >> 5)) ^ sw)) * 4);
+    };
+    f32x4 f[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i) f[i] = frag(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const f32x4 a = *(const f32x4*)(k + (row * R + ((2 * ks + (lane >> 5)) ^ sw)) * 4);
       const f32x4 b = __builtin_bit_cast(f32x4, q[0][ks]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = mma(a[e], b[e], s);
+      for (int e = 0; e < 4; ++e) s = mma(f[ks % PF][e], b[e], s);
+      if (ks + PF < KS) f[ks % PF] = frag(ks + PF);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+  static __device__ __forceinline__ void load_v(const float*, int, const VOff&, VFrag&, int) {}
   static __device__ __forceinline__ void values(const float* v, int row0, const VOff&,
-                                                const f32x16& p, f32x16* acc, int lane) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
+                                                const f32x16& p, VFrag&, f32x16* acc, int lane) {
+    constexpr int DT = D / 32;
+    auto frag = [&](int i, float* f) {  // keys 8 (i / 4) + 4 h + i % 4
       const int row = row0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4, sw = mfma::swz<R>(row);
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const int ch = 8 * dt + ((lane & 31) >> 2);
-        acc[dt] = mma(v[(row * R + (ch ^ sw)) * 4 + (lane & 3)], p[i], acc[dt]);
-      }
-      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // later rows' reads stay behind
+      for (int dt = 0; dt < DT; ++dt)
+        f[dt] = v[(row * R + ((8 * dt + ((lane & 31) >> 2)) ^ sw)) * 4 + (lane & 3)];
+    };
+    float f[PF][DT];
+#pragma unroll
+    for (int i = 0; i < PF; ++i) frag(i, f[i]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] = mma(f[i % PF][dt], p[i], acc[dt]);
+      if (i + PF < 16) frag(i + PF, f[i % PF]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -651,6 +688,15 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
           s[e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
         bad = unclean(nb) != 0;
       }
+      if (bad) {  // 0 x Inf must not reach the rows that do not see the key
+        for (uint32_t x = unclean(nb); x; x &= x - 1) {
+          const int r = row0 + __builtin_ctz(x);
+          if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      typename X::VFrag vf;
+      X::load_v(vt, row0, voff, vf, lane);  // (they land under the exponentials)
       float tmax = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, s[e]);
@@ -671,14 +717,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
         s[e] = fast_exp2(s[e] - ref);
         lsum += s[e];
       }
-      if (bad) {  // 0 x Inf must not reach the rows that do not see the key
-        for (uint32_t x = unclean(nb); x; x &= x - 1) {
-          const int r = row0 + __builtin_ctz(x);
-          if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
-      X::values(vt, row0, voff, s, acc, lane);
+      X::values(vt, row0, voff, s, vf, acc, lane);
       if (bad) {  // those keys one by one, for the rows that see them
         const uint32_t bits = sees(t0);
         int hh = 4 * h;
