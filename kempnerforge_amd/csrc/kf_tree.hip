@@ -83,27 +83,29 @@ struct TreeLds {
   int ptr[MAXN], depth[MAXN];
 };
 
-// Forms the tree of sequence b (s: its nodes and prefix), by a workgroup of 256;
-// returns whether the sequence is refused.  A chain needs no LDS: node i sees
+// Forms the tree of a sequence (s: its nodes and prefix; par: thread t's node's
+// parent, from tree_parent), by a workgroup of 256; returns whether the sequence is
+// refused.  A chain needs no LDS: node i sees
 // nodes 0 .. i and lies at depth i.
 //
 // The masks come from pointer doubling: after round r, mask[i] holds the 2^r
 // nearest of i and its ancestors and ptr[i] the next one beyond, so 8 rounds
 // cover 256 nodes whatever their depth (a walk up a chain of 200 would take 200
 // dependent reads).
-__device__ __forceinline__ bool tree_build(const TreeArgs& a, int b, int2 s, int W, TreeLds& lds) {
+__device__ __forceinline__ int tree_parent(const TreeArgs& a, int b, int2 s) {
+  const int t = threadIdx.x;
+  return a.parents != nullptr && t < s.x ? a.parents[(int64_t)b * a.parents_stride + t] : -1;
+}
+__device__ __forceinline__ bool tree_build(const TreeArgs& a, int2 s, int W, TreeLds& lds,
+                                           int par) {
   const int64_t low = (int64_t)s.y - a.rope_row_offset;  // table row of depth 0
   if (a.parents == nullptr)
     return s.x < 0 || (s.x > 0 && (low < 0 || low + s.x > a.rope_rows));
   const int t = threadIdx.x, used = max(s.x, 0);
   bool bad = s.x < 0;
-  int par = -1;
-  if (t < used) {
-    par = a.parents[(int64_t)b * a.parents_stride + t];
-    if (par < -1 || par >= t) {
-      bad = true;
-      par = -1;
-    }
+  if (par < -1 || par >= t) {
+    bad = true;
+    par = -1;
   }
   __syncthreads();  // the previous tree's readers are done
   for (int k = 0; k < W; ++k) lds.mask[t][k] = k == t >> 5 ? 1u << (t & 31) : 0u;
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(256) void tree_prep_kernel(TreeArgs a, float* __res
   const int N = a.N, D = a.D, half = D / 2;
   const int heads = a.Hq + 2 * a.Hkv, n_rep = a.Hq / a.Hkv;
   const int2 s = tree_seq(a, b);
-  const bool bad = tree_build(a, b, s, W, tree);
+  const bool bad = tree_build(a, s, W, tree, tree_parent(a, b, s));
   const int n = s.x, L = s.y;
   if (blockIdx.x == 0) {
     if (t == 0) seq[b] = bad ? make_int2(-1, 0) : s;
@@ -262,21 +264,45 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const float*
 // Row tile t of pair (b, g) holds rows t ROWS .. of the pair's n_b n_rep rows
 // (node-major: the heads of a node side by side); every tile meets the nck(b) =
 // ceil((lens[b] + n_b) / KC) key chunks of its pair.
+//
+// Beginning a row tile costs about as much as OVER chunks (its queries are loaded
+// and rotated, the tree formed), so with several chunks per workgroup each tile
+// has `over` units in front of its chunks in the list that is shared out.
 struct TreeSched {
   const TreeArgs& a;
-  int B, n_rep, rows, kc;
+  int n_rep, rows, kc;
+  int over, C, NW;  // units of the list, workgroups that share it
+  static constexpr int OVER = 2;
+  int B;
+  __device__ __forceinline__ TreeSched(const TreeArgs& a_, int n_rep_, int rows_, int kc_,
+                                       int grid, int lane)
+      : a(a_), n_rep(n_rep_), rows(rows_), kc(kc_), B(a_.B) {
+    int tot = 0, items = 0;
+    for (int b = lane; b < B; b += 64) {
+      const int2 s = tree_seq(a, b);
+      const int i = s.x > 0 ? a.Hkv * tiles(s) : 0;
+      items += i;
+      tot += i > 0 ? i * nck(s) : 0;
+    }
+    tot = wave_sum_int(tot);
+    items = wave_sum_int(items);
+    over = tot >= 4 * grid ? OVER : 0;
+    C = tot + over * items;
+    NW = min(grid, C);
+  }
   __device__ __forceinline__ int nck(int2 s) const { return (s.x + s.y + kc - 1) / kc; }
   __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
+  __device__ __forceinline__ int per(int2 s) const { return nck(s) + over; }
   __device__ __forceinline__ int chunks(int b) const {
     const int2 s = tree_seq(a, b);
-    return s.x > 0 ? a.Hkv * tiles(s) * nck(s) : 0;
+    return s.x > 0 ? a.Hkv * tiles(s) * per(s) : 0;
   }
 };
 
-// Place in the chunk list: sequence b (s: its nodes in use and prefix length),
-// KV head g, row tile t, chunk c of nck.
+// Place in the list: sequence b (s: its nodes in use and prefix length), KV head
+// g, row tile t, chunk c of nck, unit u.
 struct TreeCursor {
-  int b, g, t, c, nck, tiles;
+  int b, g, t, c, u, nck, tiles;
   int2 s;
   __device__ __forceinline__ void at(const TreeSched& sched, int b_) {
     b = b_;
@@ -286,18 +312,22 @@ struct TreeCursor {
     nck = sched.nck(s);
     tiles = sched.tiles(s);
   }
-  __device__ __forceinline__ void seek(const TreeSched& sched, int chunk, int lane) {
+  // the first chunk at or behind a unit
+  __device__ __forceinline__ void seek(const TreeSched& sched, int unit, int lane) {
     int sb, base;
-    locate_chunk(sched, chunk, lane, sb, base);
+    locate_chunk(sched, unit, lane, sb, base);
     at(sched, sb);
-    const int rem = chunk - base;
-    c = rem % nck;
-    t = rem / nck % tiles;
-    g = rem / nck / tiles;
+    const int per = nck + sched.over, item = (unit - base) / per;
+    c = max(unit - base - item * per - sched.over, 0);
+    u = base + item * per + sched.over + c;
+    t = item % tiles;
+    g = item / tiles;
   }
   __device__ __forceinline__ void next(const TreeSched& sched) {
+    ++u;
     if (++c < nck) return;
     c = 0;
+    u += sched.over;
     if (++t < tiles) return;
     t = 0;
     if (++g < sched.a.Hkv) return;
@@ -308,7 +338,7 @@ struct TreeCursor {
         return;
       }
     }
-    b = sched.B;  // behind the last chunk
+    b = sched.B;  // behind the last chunk (u is past every share)
   }
 };
 
@@ -319,16 +349,36 @@ struct TreeCursor {
 //       row l % 32, register i key 8 (i / 4) + 4 h + i % 4)
 // Every fragment is read PF steps ahead of its products: left to itself the
 // compiler, short of registers, reads each one right before them and waits out
-// the LDS (42% of the time on the matrix cores instead of ...).
+// the LDS (512 rows over 16384 keys, 4 x 8 KV heads of 128: 232 us, read ahead 218).
 template <typename T, int D>
 struct Tile {
   static constexpr int R = D / 8;     // 16-byte chunks per cache row
   static constexpr int KS = D / 16;   // pieces of a lane's half row
   static constexpr int QP = 2;        // q as hi and lo
-  static constexpr int PF = 4, NV = D / 16;  // V fragments: 2 of 16 keys for each 32 dims
-  typedef mfma::TrOffsets<D> VOff;
+  static constexpr int PF = D == 128 ? 2 : 4;  // (what the registers hold)
+  static constexpr int NV = D / 16;            // V fragments: 2 of 16 keys for each 32 dims
+  // lds_frag_t's offsets: block dt's are the first block's with bits 6.. flipped by
+  // dt (a swizzled chunk index is 4 dt ^ ...), which saves the registers of the others
+  struct VOff {
+    uint32_t o[2];
+  };
   typedef bf16x8 VFrag[PF];
-  static __device__ __forceinline__ VOff v_off(int lane) { return mfma::tr_offsets<D>(lane); }
+  static __device__ __forceinline__ VOff v_off(int lane) {
+    const mfma::TrOffsets<D> t = mfma::tr_offsets<D>(lane);
+    return VOff{{t.o[0][0], t.o[0][1]}};
+  }
+  static __device__ __forceinline__ bf16x8 v_frag(const T* v, int row0, const VOff& off, int c,
+                                                  int dt) {
+    using namespace mfma;
+    const char* base = (const char*)v + (row0 + c * 16) * D * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4_ptr)(base + (off.o[0] ^ (dt * 64))));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4_ptr)(base + (off.o[1] ^ (dt * 64))));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, x);
+  }
   static __device__ __forceinline__ void scores(const T* k, int row0, const u32x4 (*q)[KS],
                                                 f32x16& s, int lane) {
     using namespace mfma;
@@ -348,7 +398,7 @@ struct Tile {
   static __device__ __forceinline__ void load_v(const T* v, int row0, const VOff& off, VFrag& f,
                                                 int) {
 #pragma unroll
-    for (int i = 0; i < PF; ++i) f[i] = mfma::lds_frag_t<D>(v + row0 * D, off, i & 1, i >> 1);
+    for (int i = 0; i < PF; ++i) f[i] = v_frag(v, row0, off, i & 1, i >> 1);
     __builtin_amdgcn_sched_barrier(0);
   }
   static __device__ __forceinline__ void values(const T* v, int row0, const VOff& off,
@@ -366,7 +416,7 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {  // dims 32 (i / 2) .., keys 16 (i % 2) ..
       acc[i >> 1] = mfma32<T>(f[i % PF], pb[i & 1], acc[i >> 1]);
-      if (i + PF < NV) f[i % PF] = lds_frag_t<D>(v + row0 * D, off, i & 1, (i + PF) >> 1);
+      if (i + PF < NV) f[i % PF] = v_frag(v, row0, off, (i + PF) & 1, (i + PF) >> 1);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -458,13 +508,16 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   const int w = wave_id(), lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
   const int rw = w % RW, kw = w / RW;
   const int N = a.N, n_rep = a.Hq / a.Hkv;
-  const TreeSched sched{a, a.B, n_rep, ROWS, KC};
-  const int C = total_chunks(sched, lane), NW = min((int)gridDim.x, C);
+  const TreeSched sched(a, n_rep, ROWS, KC, gridDim.x, lane);
+  const int C = sched.C, NW = sched.NW;
   // block ids go round the 8 XCDs: neighbours in the chunk list, which read the
   // same keys for other rows, share one XCD's L2
   if ((int)blockIdx.x >= NW) return;
   const int xcd = blockIdx.x % 8, gw = xcd * (NW / 8) + min(xcd, NW % 8) + (int)blockIdx.x / 8;
-  const int c_lo = range_start(gw, C, NW), c_hi = range_start(gw + 1, C, NW);
+  const int u_hi = range_start(gw + 1, C, NW);
+  TreeCursor cc;
+  cc.seek(sched, range_start(gw, C, NW), lane);
+  if (cc.u >= u_hi) return;  // (a share of nothing but a tile's beginning)
 
   auto stage_k = [&](int i) { return (T*)(lds + (i & 1) * Sh::STAGE); };
   auto issue = [&](const TreeCursor& p, int i) {
@@ -472,10 +525,13 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     const int rows = p.s.x + p.s.y - p.c * KC;  // >= 1; rows past the last repeat it
     uint16_t* dst = (uint16_t*)stage_k(i);
     constexpr int U = sizeof(T) / 2;
-    tile_to_lds<KC, X::R>((const uint16_t*)((const T*)a.k_cache + row * D), D * U, dst, w, lane,
-                          rows);
-    tile_to_lds<KC, X::R>((const uint16_t*)((const T*)a.v_cache + row * D), D * U,
-                          dst + Sh::TILE * U, w, lane, rows);
+    // (two row waves: the loads' offsets formed anew each time, for registers; 7%
+    // of the time where the products bound it, nothing where HBM does)
+    constexpr bool FRESH = RW == 2;
+    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)((const T*)a.k_cache + row * D), D * U, dst,
+                                    w, lane, rows);
+    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)((const T*)a.v_cache + row * D), D * U,
+                                    dst + Sh::TILE * U, w, lane, rows);
   };
   // the table row of node j (kept inside the table: a refused sequence's may not be)
   auto table_row = [&](int2 s, int j) {
@@ -514,81 +570,103 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   f32x16 acc[DT];
   float m = -INFINITY, lsum = 0.f;
   constexpr float SLACK = 8.f;  // P stays below 2^8, far inside every type
-  TreeCursor cc, ic;
-  cc.seek(sched, c_lo, lane);
-  ic = cc;
-  issue(ic, c_lo);
   bool whole = false;    // this workgroup holds all of the row tile's chunks
   bool refused = false;  // the sequence's tree or tables are out of range
-  int node = 0, built = -1;
+  int node = 0;
 
-  for (int i = c_lo; i < c_hi; ++i) {
-    if (i == c_lo || cc.c == 0) {
-      whole = cc.c == 0;
-      if (cc.b != built) refused = tree_build(a, cc.b, cc.s, W, tree);
-      built = cc.b;
-      if (whole && cc.g == 0 && cc.t == 0 && threadIdx.x == 0) refusals[cc.b] = refused;
-      // the rotated queries: lane l holds dims of half h, 16-byte pieces 2 ks + h;
-      // a piece's RoPE partner is the lane's own piece KS / 2 further on
-      const int row = min(cc.t * ROWS + 32 * rw + l31, cc.s.x * n_rep - 1);
-      node = row / n_rep;
-      const T* qr = (const T*)a.q_new +
-                    (((int64_t)cc.b * N + node) * a.Hq + cc.g * n_rep + row % n_rep) * D;
-      const int64_t trow = table_row(cc.s, node);
-      u32x4 raw[X::KS];
+  // The beginning of a row tile: lane l's row of the queries, dims of half h,
+  // 16-byte pieces 2 ks + h; a piece's RoPE partner is the lane's own piece KS / 2
+  // further on.
+  auto load_q = [&](u32x4* raw) {
+    const int row = min(cc.t * ROWS + 32 * rw + l31, cc.s.x * n_rep - 1);
+    node = row / n_rep;
+    const T* qr = (const T*)a.q_new +
+                  (((int64_t)cc.b * N + node) * a.Hq + cc.g * n_rep + row % n_rep) * D;
 #pragma unroll
-      for (int ks = 0; ks < X::KS; ++ks) raw[ks] = *(const u32x4*)(qr + (2 * ks + h) * E);
-      Angles ang[X::KS / 2];  // (the sums' registers are free here: one round trip for all)
+    for (int ks = 0; ks < X::KS; ++ks) raw[ks] = *(const u32x4*)(qr + (2 * ks + h) * E);
+  };
+  auto load_angles = [&](Angles* ang) {  // (one round trip for all)
+    const int64_t trow = table_row(cc.s, node);
 #pragma unroll
-      for (int ks = 0; ks < X::KS / 2; ++ks) ang[ks] = angles(trow, (2 * ks + h) * E);
-      float rs = 1.f;
-      if (a.q_norm_w != nullptr) {
-        float ss = 0.f;
+    for (int ks = 0; ks < X::KS / 2; ++ks) ang[ks] = angles(trow, (2 * ks + h) * E);
+  };
+  auto rotate_q = [&](const u32x4* raw, const Angles* ang) {
+    float rs = 1.f;
+    if (a.q_norm_w != nullptr) {
+      float ss = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < X::KS; ++ks) {
-          float f[E];
-          P::unpack(raw[ks], f);
+      for (int ks = 0; ks < X::KS; ++ks) {
+        float f[E];
+        P::unpack(raw[ks], f);
 #pragma unroll
-          for (int e = 0; e < E; ++e) ss += f[e] * f[e];
-        }
-        rs = rsqrtf(pair_sum32(ss) / (float)D + a.norm_eps);
+        for (int e = 0; e < E; ++e) ss += f[e] * f[e];
       }
-      const float sc = a.scale * kLog2e;
-#pragma unroll
-      for (int ks = 0; ks < X::KS / 2; ++ks) {
-        float f[2][E];
-        P::unpack(raw[ks], f[0]);
-        P::unpack(raw[ks + X::KS / 2], f[1]);
-        rotate(f[0], f[1], ang[ks], (2 * ks + h) * E, a.q_norm_w, rs);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int at = ks + x * (X::KS / 2);
-#pragma unroll
-          for (int e = 0; e < E; ++e) f[x][e] *= sc;
-          q[0][at] = P::pack(f[x]);
-          if constexpr (X::QP == 2) {
-            float hi[E];
-            P::unpack(q[0][at], hi);
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[x][e] -= hi[e];
-            q[1][at] = P::pack(f[x]);
-          }
-        }
-      }
-      m = -INFINITY;
-      lsum = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+      rs = rsqrtf(pair_sum32(ss) / (float)D + a.norm_eps);
     }
+    const float sc = a.scale * kLog2e;
+#pragma unroll
+    for (int ks = 0; ks < X::KS / 2; ++ks) {
+      float f[2][E];
+      P::unpack(raw[ks], f[0]);
+      P::unpack(raw[ks + X::KS / 2], f[1]);
+      rotate(f[0], f[1], ang[ks], (2 * ks + h) * E, a.q_norm_w, rs);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int at = ks + x * (X::KS / 2);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[x][e] *= sc;
+        q[0][at] = P::pack(f[x]);
+        if constexpr (X::QP == 2) {
+          float hi[E];
+          P::unpack(q[0][at], hi);
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[x][e] -= hi[e];
+          q[1][at] = P::pack(f[x]);
+        }
+      }
+    }
+    m = -INFINITY;
+    lsum = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+    whole = cc.c == 0;
+    if (whole && cc.g == 0 && cc.t == 0 && threadIdx.x == 0) refusals[cc.b] = refused;
+  };
+  {
+    // Loads return in order, so what the first tile needs is waited for before its
+    // first chunk is asked for, and the rest of its beginning runs under that.
+    u32x4 raw[X::KS];
+    Angles ang[X::KS / 2];
+    int par = tree_parent(a, cc.b, cc.s);
+    load_q(raw);
+    settle(par);
+#pragma unroll
+    for (int ks = 0; ks < X::KS; ++ks) settle(raw[ks]);
+    if (a.parents == nullptr) {
+      load_angles(ang);
+#pragma unroll
+      for (int ks = 0; ks < X::KS / 2; ++ks)
+#pragma unroll
+        for (int x = 0; x < E / 4; ++x) {
+          settle(ang[ks].c[x]);
+          settle(ang[ks].s[x]);
+        }
+    }
+    issue(cc, 0);
+    refused = tree_build(a, cc.s, W, tree, par);
+    if (a.parents != nullptr) load_angles(ang);
+    rotate_q(raw, ang);
+  }
+
+  for (int i = 0;; ++i) {
+    TreeCursor ic = cc;
+    ic.next(sched);
+    const bool more = ic.u < u_hi;
     lds_copy_wait();
     __syncthreads();  // chunk i has landed for all; the other stage is free
-    const bool more = i + 1 < c_hi;
-    if (more) {
-      ic.next(sched);
-      issue(ic, i + 1);
-    }
+    if (more) issue(ic, i + 1);
     T* kt = stage_k(i);
     T* vt = kt + Sh::TILE;
     const bool tail = cc.c * KC + KC > cc.s.y;  // the chunk holds nodes, or ends behind them
@@ -610,23 +688,12 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
         const int ca = ((d / E) ^ sw) * E, cb = (((d + HALF) / E) ^ sw) * E;
         const int64_t dst = (head * a.Smax + L + j) * D + d;
         const bool store = cc.t == 0 && !refused;
-        P x2, kx;
+        P kx, vx;  // all loads first: one round trip
         float f1[E], f2[E];
-        x2.load((const T*)a.v_new + src, d, HALF);
         kx.load((const T*)a.k_new + src, d, HALF);
         const Angles g = angles(table_row(cc.s, j), d);
-        *(u32x4*)(vt + lr * D + ca) = x2.a;
-        *(u32x4*)(vt + lr * D + cb) = x2.b;
-        if (store) {
-          *(u32x4*)((T*)a.v_cache + dst) = x2.a;
-          *(u32x4*)((T*)a.v_cache + dst + HALF) = x2.b;
-        }
-        P::unpack(x2.a, f1);
-        P::unpack(x2.b, f2);
-        bool fin = true;
-#pragma unroll
-        for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
-        if (!fin) atomicOr(&sbad[lr >> 5], 1u << (lr & 31));
+        vx.load((const T*)a.v_new + src, d, HALF);
+        __builtin_amdgcn_sched_barrier(0);
         P::unpack(kx.a, f1);
         P::unpack(kx.b, f2);
         float rs = 1.f;
@@ -639,14 +706,26 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
           rs = rsqrtf(ss / (float)D + a.norm_eps);
         }
         rotate(f1, f2, g, d, a.k_norm_w, rs);
-        x2.a = P::pack(f1);
-        x2.b = P::pack(f2);
-        *(u32x4*)(kt + lr * D + ca) = x2.a;
-        *(u32x4*)(kt + lr * D + cb) = x2.b;
+        kx.a = P::pack(f1);
+        kx.b = P::pack(f2);
+        __builtin_amdgcn_sched_barrier(0);
+        *(u32x4*)(kt + lr * D + ca) = kx.a;
+        *(u32x4*)(kt + lr * D + cb) = kx.b;
+        *(u32x4*)(vt + lr * D + ca) = vx.a;
+        *(u32x4*)(vt + lr * D + cb) = vx.b;
         if (store) {
-          *(u32x4*)((T*)a.k_cache + dst) = x2.a;
-          *(u32x4*)((T*)a.k_cache + dst + HALF) = x2.b;
+          *(u32x4*)((T*)a.k_cache + dst) = kx.a;
+          *(u32x4*)((T*)a.k_cache + dst + HALF) = kx.b;
+          *(u32x4*)((T*)a.v_cache + dst) = vx.a;
+          *(u32x4*)((T*)a.v_cache + dst + HALF) = vx.b;
         }
+        __builtin_amdgcn_sched_barrier(0);
+        P::unpack(vx.a, f1);
+        P::unpack(vx.b, f2);
+        bool fin = true;
+#pragma unroll
+        for (int e = 0; e < E; ++e) fin = fin && finite(f1[e]) && finite(f2[e]);
+        if (!fin) atomicOr(&sbad[lr >> 5], 1u << (lr & 31));
       }
       for (int x = (L + j1 - r0) * X::R + tid; x < KC * X::R; x += 256)
         *(u32x4*)(vt + x * E) = u32x4{0u, 0u, 0u, 0u};
@@ -820,7 +899,17 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
         }
       }
     }
-    cc.next(sched);
+    if (!more) break;
+    const bool new_tree = ic.b != cc.b;
+    cc = ic;
+    if (cc.c == 0) {
+      u32x4 raw[X::KS];
+      Angles ang[X::KS / 2];
+      load_q(raw);
+      if (new_tree) refused = tree_build(a, cc.s, W, tree, tree_parent(a, cc.b, cc.s));
+      load_angles(ang);
+      rotate_q(raw, ang);
+    }
   }
 }
 
@@ -839,13 +928,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
   const int r = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
   const int row = t * rows + r, i = row / n_rep, hq = g * n_rep + row % n_rep;
   const int2 s = tree_seq(a, b);
-  const TreeSched sched{a, a.B, n_rep, rows, kc};
-  int tot = 0, pre = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? sched.chunks(b0 + lane) : 0;
-    tot += wave_sum_int(n);
-    pre += wave_sum_int(b0 + lane < b ? n : 0);
-  }
+  const TreeSched sched(a, n_rep, rows, kc, NWmax, lane);
+  int pre = 0;
+  for (int b0 = lane; b0 < b; b0 += 64) pre += sched.chunks(b0);
+  pre = wave_sum_int(pre);
   if (i >= a.N || r >= rows) return;
   T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + hq) * D + col;
   T y[4];
@@ -856,9 +942,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
     return;
   }
-  const int NW = min(NWmax, tot), nck = sched.nck(s);
-  const int c0 = pre + (g * sched.tiles(s) + t) * nck;
-  const int w0 = chunk_owner(c0, tot, NW), ns = chunk_owner(c0 + nck - 1, tot, NW) - w0 + 1;
+  const int nck = sched.nck(s);
+  const int c0 = pre + (g * sched.tiles(s) + t) * sched.per(s) + sched.over;
+  const int w0 = chunk_owner(c0, sched.C, sched.NW),
+            ns = chunk_owner(c0 + nck - 1, sched.C, sched.NW) - w0 + 1;
   if (ns == 1) return;
   const int64_t first = ((int64_t)w0 + item) * rows + r;
   const float* ob = opart + first * D + col;
@@ -916,7 +1003,7 @@ Plan plan_of(const TreeArgs& a) {
                      (size_t)(4 / p.rw - 1) * p.rows * 8;  // Shape::LDS
   p.per_cu = 2 * lds <= 160 * 1024 && !(a.dtype == F32 && a.D == 128) ? 2 : 1;  // Shape::PER_CU
   const int64_t chunks = (int64_t)a.B * a.Hkv * p.tiles * ((a.max_len + p.kc - 1) / p.kc);
-  if (chunks >= INT_MAX) return Plan{};
+  if (chunks + (int64_t)a.B * a.Hkv * p.tiles * TreeSched::OVER >= INT_MAX) return Plan{};
   p.grid = (int)std::min<int64_t>(p.per_cu * std::min(device_cu_count(), 512), chunks);
   return p;
 }
