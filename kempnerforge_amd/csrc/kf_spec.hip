@@ -274,28 +274,27 @@ __device__ __forceinline__ bool load_nodes(const VerifyArgs& a, int b, int n, No
   return __syncthreads_or(bad);
 }
 
-// Whether node t is taken once its elder siblings are refused, sp[] holding its
-// and its siblings' probabilities (-1: none, refused).
+// Whether an elder sibling of node t has its token: refused again.
+__device__ __forceinline__ bool repeated(const Nodes& nd, int t) {
+  const int par = nd.par[t], tok = nd.tok[t];
+  bool found = false;
+#pragma unroll 8
+  for (int j = par + 1; j < t; ++j) found |= nd.par[j] == par && nd.tok[j] == tok;
+  return found;
+}
+
+// Whether node t is taken once its elder siblings are refused; sp[]: the nodes'
+// probabilities, -1 where refused whatever the rest (none, or repeated).
 __device__ __forceinline__ bool taken(const VerifyArgs& a, const Nodes& nd, const double* sp,
                                       const double* sq, int t) {
   const double p = sp[t];
   if (!(p >= 0.0)) return false;
   if (a.greedy) return p > 0.0;
   if (a.drafts != nullptr) return (double)nd.u[t] * sq[t] < p;
+  const int par = nd.par[t];
   double left = 1.0;
-  for (int j = nd.par[t] + 1; j < t; ++j)
-    if (nd.par[j] == nd.par[t]) {
-      if (nd.tok[j] == nd.tok[t]) return false;  // refused before
-      left -= fmax(sp[j], 0.0);
-    }
-  // (a repeated token's mass went once: count only the first of equals)
-  for (int j = nd.par[t] + 1; j < t; ++j)
-    if (nd.par[j] == nd.par[t])
-      for (int i = nd.par[t] + 1; i < j; ++i)
-        if (nd.par[i] == nd.par[t] && nd.tok[i] == nd.tok[j]) {
-          left += fmax(sp[j], 0.0);
-          break;
-        }
+#pragma unroll 8
+  for (int j = par + 1; j < t; ++j) left -= nd.par[j] == par ? fmax(sp[j], 0.0) : 0.0;
   return (double)nd.u[t] * left < p;
 }
 
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
     const int ng = r.granules();
     st = Stat{-INFINITY, INT_MAX, 0.0};
     // the next batch's loads run under this one's exponentials
-    constexpr int U = sizeof(T) == 4 ? 4 : 3;  // (registers for 16 wavefronts)
+    constexpr int U = sizeof(T) == 4 ? 4 : 2;  // (registers for 16 wavefronts)
     u32x4 raw[U], ahead[U];
     load_batch<T, U>(r, t, WT, ng, raw);
     for (int k = t; k < ng; k += U * WT) {
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
     const bool child = t > 0 && t < n && nd.par[t] == cur;
     if (child) {
       const int tok = nd.tok[t];
-      sp[t] = tok < 0      ? -1.0
+      sp[t] = tok < 0 || repeated(nd, t) ? -1.0
               : a.greedy ? (tok == (st.at == INT_MAX ? 0 : st.at) ? 1.0 : -1.0)
                          : exp2_64(((double)to_f32(r.x[tok]) - (double)st.m) * c) / st.s;
     }
@@ -372,13 +371,14 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
   }
 }
 
-// A slice of the draw: a granule per thread (the weights' 64-bit exponentials,
-// about 20 operations each, are what it spends its time on, so as many CUs as
-// there are); a segment: a wavefront's granules.
-constexpr int DT = 256, DSEG = DT / 64;
-constexpr int MAXSLICES = KF_VERIFY_MAX_VOCAB / (4 * DT) + 2;
-__host__ __device__ __forceinline__ int draw_slices_of(int V, int E) {
-  return ((V + 2 * E - 2) / E + DT - 1) / DT;
+// A slice of the draw: U granules a thread; a segment is the 64 granules that a
+// wavefront takes at a time.  The 64-bit exponentials (about 20 operations each)
+// want many workgroups, the counter they all raise few: U = 1 while that leaves
+// at most 256 (5 nodes, 32000 float32 values: 12.5 us, 16.4 with U = 4), else 4 (16
+// sequences of 131072 values: 23 us with U = 1, 20 with 4).
+constexpr int DT = 256;
+__host__ __device__ __forceinline__ int draw_slices_of(int V, int E, int U) {
+  return ((V + 2 * E - 2) / E + U * DT - 1) / (U * DT);
 }
 
 // The draw (and, ALL, the walk before it, over the statistics of all rows, by
@@ -386,18 +386,18 @@ __host__ __device__ __forceinline__ int draw_slices_of(int V, int E) {
 // weights of a slice's values in 64 bits, summed by segments in order; the last
 // to arrive finds the slice, the segment and the value at which the running sum
 // passes the point.  greedy: one workgroup per sequence, no draw.
-template <typename T, bool ALL, bool DP>
+template <typename T, bool ALL, bool DP, int U>
 __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int* __restrict__ last,
                                                          const Stat* __restrict__ stats,
                                                          int nslices, int ndraw, double* sums,
                                                          int* __restrict__ arrived) {
-  constexpr int E = Row<T>::E;
+  constexpr int E = Row<T>::E, DSEG = U * DT / 64;  // segments of a slice
   __shared__ Nodes nd;
   __shared__ Stat row[ALL ? 2 * MAXN : 1];  // nodes 0 .. n - 1, then the draft's
   __shared__ double sp[MAXN], sq[ALL ? MAXN : 1];
   __shared__ int pick[MAXN];  // the child taken of each node, then the path
   __shared__ int refused[MAXN];  // tokens of the last node's children
-  __shared__ double seg[DSEG], all_sums[MAXSLICES];
+  __shared__ double seg[DSEG], wsum[DT / 64];
   __shared__ int sh[4];
   const int b = blockIdx.y, slice = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
   const int N = a.N, V = a.V;
@@ -418,27 +418,40 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
       x = to_f32(logits[nd.par[t] * a.logits_sn + nd.tok[t]]);
       if (drafted) y = to_f32(drafts[(t - 1) * a.drafts_sn + nd.tok[t]]);
     }
-    // the rows' slices joined, 16 lanes a row
-    for (int i = t / 16; i < (bad ? 0 : drafted ? 2 * n - 1 : n); i += DT / 16) {
-      const Stat* p = stats + ((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices;
-      Stat z{-INFINITY, INT_MAX, 0.0};
-      for (int j = t % 16; j < nslices; j += 16) join<DP>(z, p[j], c);
+    // the rows' slices joined, 16 lanes a row, four rows' loads in flight
+    const int nr = bad ? 0 : drafted ? 2 * n - 1 : n;
+    for (int i0 = t / 16; i0 < nr; i0 += 4 * (DT / 16)) {
+      Stat z[4];
 #pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) {
-        Stat v;
-        v.m = __shfl_xor(z.m, o, 16);
-        v.at = __shfl_xor(z.at, o, 16);
-        v.s = __shfl_xor(z.s, o, 16);
-        join<DP>(z, v, c);
+      for (int x = 0; x < 4; ++x) {
+        const int i = i0 + x * (DT / 16), j = t % 16;
+        z[x] = Stat{-INFINITY, INT_MAX, 0.0};
+        if (i < nr && j < nslices)
+          z[x] = stats[((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices + j];
       }
-      if (t % 16 == 0) row[i] = z;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int i = i0 + x * (DT / 16);
+        if (i >= nr) break;  // (a row's 16 lanes alike)
+        for (int j = t % 16 + 16; j < nslices; j += 16)
+          join<DP>(z[x], stats[((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices + j], c);
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) {
+          Stat v;
+          v.m = __shfl_xor(z[x].m, o, 16);
+          v.at = __shfl_xor(z[x].at, o, 16);
+          v.s = __shfl_xor(z[x].s, o, 16);
+          join<DP>(z[x], v, c);
+        }
+        if (t % 16 == 0) row[i] = z[x];
+      }
     }
     if (t < N) pick[t] = INT_MAX;
     __syncthreads();
     if (node && t > 0) {
       const Stat& r = row[nd.par[t]];
       const int tok = nd.tok[t];
-      sp[t] = tok < 0      ? -1.0
+      sp[t] = tok < 0 || repeated(nd, t) ? -1.0
               : a.greedy ? (tok == (r.at == INT_MAX ? 0 : r.at) && r.s == r.s ? 1.0 : -1.0)
               : has_mass(r.s) ? exp2_64(((double)x - (double)r.m) * c) / r.s
                               : -1.0;
@@ -490,20 +503,27 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
   const bool minus = drafted && cur + 1 < n && has_mass(dst.s);
   const double rp = minus ? 1.0 / st.s : 1.0, rq = minus ? 1.0 / dst.s : 0.0;
   const Row<T> r(logits + cur * a.logits_sn, V);
-  const T* dr = drafts + cur * a.drafts_sn;
+  const Row<T> dr(minus ? drafts + cur * a.drafts_sn : r.x, V);
+  const bool alike = dr.lead == r.lead;  // granules of the two rows hold the same values
   const int ng = r.granules();
-  auto weights = [&](int k, bool all, double* wt) {
+  auto weights = [&](int k, const u32x4& raw, bool all, double* wt) {
     float f[E];
-    Row<T>::unpack(r.raw(k), f);
+    Row<T>::unpack(raw, f);
     const int v0 = r.first(k);
 #pragma unroll
     for (int e = 0; e < E; ++e) wt[e] = exp2_64(((double)f[e] - (double)st.m) * c) * rp;
     if (all) return;
     if (minus) {
+      if (alike) {
+        Row<T>::unpack(dr.raw(k), f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          f[e] = v0 + e >= 0 && v0 + e < V ? to_f32(dr.x[v0 + e]) : -INFINITY;
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (v0 + e >= 0 && v0 + e < V)
-          wt[e] = fmax(wt[e] - exp2_64(((double)to_f32(dr[v0 + e]) - (double)dst.m) * c) * rq, 0.0);
+        wt[e] = fmax(wt[e] - exp2_64(((double)f[e] - (double)dst.m) * c) * rq, 0.0);
     } else if (!drafted) {  // (a refused child of probability 0 changes nothing)
       for (int i = 0; i < nref; ++i)
 #pragma unroll
@@ -511,56 +531,72 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
           if (refused[i] == v0 + e) wt[e] = 0.0;
     }
   };
-  // seg[]: the sums of a slice's segments; returns their sum in order
-  auto slice_sum = [&](int sl, bool all) {
-    double x = 0.0;
-    const int k = sl * DT + t;
-    if (k < ng) {
-      double wt[E];
-      weights(k, all, wt);
+  // the sums of a slice's segments, to seg[0 .. DSEG)
+  auto slice_sums = [&](int sl, bool all, double* seg) {
+    u32x4 raw[U];
+    const int k0 = sl * U * DT + t;
+    load_batch<T, U>(r, k0, DT, ng, raw);
+    double x[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x += wt[e];
+    for (int u = 0; u < U; ++u) {
+      double wt[E];
+      x[u] = 0.0;
+      if (k0 + u * DT < ng) {
+        weights(k0 + u * DT, raw[u], all, wt);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u] += wt[e];
+      }
     }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-    __syncthreads();
-    if (lane == 0) seg[w] = x;
-    __syncthreads();
-    x = 0.0;
+    for (int o = 32; o >= 1; o >>= 1)
 #pragma unroll
-    for (int g = 0; g < DSEG; ++g) x += seg[g];
-    return x;
+      for (int u = 0; u < U; ++u) x[u] += __shfl_xor(x[u], o, 64);
+    if (lane == 0)
+#pragma unroll
+      for (int u = 0; u < U; ++u) seg[u * (DT / 64) + w] = x[u];
+    __syncthreads();
   };
-  double* mine = sums + (int64_t)b * ndraw;
-  const double own = slice_sum(slice, false);
-  if (t == 0) {
+  double* sums_b = sums + (int64_t)b * ndraw * DSEG;
+  slice_sums(slice, false, seg);
+  if (w == 0) {
     // Device-scope accesses on both sides, past the caches, so the order is all
-    // that is left to see to: the sum has arrived before the count is raised.  (A
-    // release here would write back the XCD's whole L2, an acquire empty it.)
-    __hip_atomic_store(mine + slice, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // that is left to see to: the sums have arrived before the count is raised.
+    // (A release here would write back the XCD's whole L2, an acquire empty it.)
+    if (t < DSEG)
+      __hip_atomic_store(sums_b + slice * DSEG + t, seg[t], __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    sh[2] = __hip_atomic_fetch_add(arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (t == 0)
+      sh[2] = __hip_atomic_fetch_add(arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (sh[2] != ndraw - 1) return;
-  // the last of the sequence: every slice's sum is there
-  for (int j = t; j < ndraw; j += DT)
-    all_sums[j] = __hip_atomic_load(mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  // running sums of the slices, a lane's share of them at a time; every wavefront
-  // for itself
-  const int share = (ndraw + 63) / 64, j0 = min(lane * share, ndraw), j1 = min(j0 + share, ndraw);
+  // The last of the sequence: every segment's sum is there.  Thread j's share of
+  // them runs in order, then the shares' sums.
+  const int nseg = ndraw * DSEG, share = (nseg + DT - 1) / DT;
+  const int j0 = min(t * share, nseg), j1 = min(j0 + share, nseg);
   double part, incl, total;
   auto running = [&]() {
     part = 0.0;
-    for (int j = j0; j < j1; ++j) part += all_sums[j];
+    for (int j = j0; j < j1; ++j)
+      part += __hip_atomic_load(sums_b + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     incl = part;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const double y = __shfl_up(incl, o, 64);
       if (lane >= o) incl += y;
     }
-    total = __shfl(incl, 63, 64);
+    __syncthreads();
+    if (lane == 63) wsum[w] = incl;
+    __syncthreads();
+    double below = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int j = 0; j < DT / 64; ++j) {
+      if (j == w) below = total;
+      total += wsum[j];
+    }
+    incl += below;
   };
   running();
   // rounding can leave no mass where all of it was on refused tokens: the draw is
@@ -568,37 +604,44 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
   const bool all = !(total > 0.0);
   if (all) {
     for (int j = 0; j < ndraw; ++j) {
-      const double x = slice_sum(j, true);
-      if (t == 0) all_sums[j] = x;
+      slice_sums(j, true, seg);
+      if (t < DSEG)
+        __hip_atomic_store(sums_b + j * DSEG + t, seg[t], __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
     }
-    __syncthreads();
     running();
   }
   const double point = (double)nd.u[0] * total;
-  // the first share that passes the point, then its first slice (the last ones,
-  // where sums of two orders leave the point behind them)
-  const uint64_t past = __builtin_amdgcn_ballot_w64(incl > point);
-  const int owner = past ? (int)__builtin_ctzll(past) : (ndraw - 1) / share;
-  double before = __shfl(incl - part, owner, 64);
-  int sl = owner * share;
-  const int end = min(sl + share, ndraw) - 1;
-  for (; sl < end; ++sl) {
-    if (before + all_sums[sl] > point) break;
-    before += all_sums[sl];
+  // the first share that passes the point (the last one, where sums of two orders
+  // leave the point behind them), then its first segment
+  if (t == 0) sh[3] = (nseg - 1) / share;
+  __syncthreads();
+  if (incl > point) atomicMin(&sh[3], t);
+  __syncthreads();
+  if (t == sh[3]) {
+    double before = incl - part;
+    sh[0] = j0;
+    for (int g = j0; g < j1; ++g) {  // (a segment of no weight is never picked)
+      const double x = __hip_atomic_load(sums_b + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (x > 0.0) {
+        sh[0] = g;
+        seg[0] = before;
+      }
+      if (before + x > point) break;
+      before += x;
+    }
   }
-  slice_sum(sl, all);
+  __syncthreads();
   if (w != 0) return;
-  int g = 0;
-  for (; g < DSEG - 1; ++g) {
-    if (before + seg[g] > point) break;
-    before += seg[g];
-  }
-  const int k = sl * DT + 64 * g + lane;
+  const int k = 64 * sh[0] + lane;
+  const double before = seg[0];
   double wt[E], sum = 0.0;
   int hit = INT_MAX, any = -1;
 #pragma unroll
   for (int e = 0; e < E; ++e) wt[e] = 0.0;
-  if (k < ng) weights(k, all, wt);
+  if (k < ng) weights(k, r.raw(k), all, wt);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     sum += wt[e];
@@ -682,21 +725,23 @@ struct VerifyWs {
   int* arrived;   // [B]
   int* last;      // [B]
   Stat* stats;    // all rows: [B][rows][slices]; walk: [B]
-  double* sums;   // [B][draw]
+  double* sums;   // [B][segments of the draw]
   bool all_rows;
-  int rows, slices, draw;
+  int rows, slices, draw, unit;  // unit: granules a thread of the draw
   size_t bytes;
 };
 VerifyWs verify_carve(const VerifyArgs& a, void* p) {
   const int el = a.dtype == F32 ? 4 : 2;
   VerifyWs w;
   w.slices = slices_of(a.V, 16 / el);
-  w.draw = draw_slices_of(a.V, 16 / el);
+  w.unit = (int64_t)a.B * draw_slices_of(a.V, 16 / el, 1) <= 256 ? 1 : 4;
+  w.draw = draw_slices_of(a.V, 16 / el, w.unit);
   w.rows = a.drafts != nullptr ? 2 * a.N - 1 : a.N;
-  // All rows cost B N el / 4.5 TB/s per value of the vocabulary, a walk about 65
-  // ps per value and level, some four levels deep.  (A chain's draft rows: their
-  // sums have to hold 64 bits for the draw, which one CU forms too slowly.)
-  w.all_rows = a.drafts != nullptr || (int64_t)a.B * a.N * el <= 1200;
+  // All rows take B N el / 5 TB/s per value of the vocabulary, a walk about 110 ps
+  // per value and level, some four levels deep: equal at 2200 bytes a value.  (A
+  // chain's draft rows: their sums have to hold 64 bits for the draw, which one CU
+  // forms too slowly.)
+  w.all_rows = a.drafts != nullptr || (int64_t)a.B * a.N * el <= 2200;
   char* c = (char*)p;
   w.arrived = (int*)c;
   c += up256((size_t)a.B * 4);
@@ -705,7 +750,7 @@ VerifyWs verify_carve(const VerifyArgs& a, void* p) {
   w.stats = (Stat*)c;
   c += up256((size_t)a.B * (w.all_rows ? (size_t)w.rows * w.slices : 1) * sizeof(Stat));
   w.sums = (double*)c;
-  c += up256((size_t)a.B * w.draw * sizeof(double));
+  c += up256((size_t)a.B * w.draw * w.unit * (DT / 64) * sizeof(double));
   w.bytes = (size_t)(c - (char*)p);
   return w;
 }
@@ -720,8 +765,11 @@ int verify_typed(const VerifyArgs& a, void* workspace) {
     KF_LAUNCH("verify_stats", kernel, dim3(w.slices, w.rows, a.B), dim3(ST), 0, a.stream, a,
               w.stats, w.arrived);
     KF_CHECK_LAUNCH();
-    auto draw = a.drafts != nullptr ? verify_draw_kernel<T, true, true>
-                                    : verify_draw_kernel<T, true, false>;
+    auto draw = a.drafts == nullptr
+                    ? (w.unit == 1 ? verify_draw_kernel<T, true, false, 1>
+                                   : verify_draw_kernel<T, true, false, 4>)
+                    : (w.unit == 1 ? verify_draw_kernel<T, true, true, 1>
+                                   : verify_draw_kernel<T, true, true, 4>);
     KF_LAUNCH("verify_draw", draw, dim3(a.greedy ? 1 : w.draw, a.B), dim3(DT), 0, a.stream, a,
               w.last, w.stats, w.slices, w.draw, w.sums, w.arrived);
     KF_CHECK_LAUNCH();
@@ -731,8 +779,10 @@ int verify_typed(const VerifyArgs& a, void* workspace) {
             w.stats, w.arrived);
   KF_CHECK_LAUNCH();
   if (a.greedy) return KF_OK;
-  KF_LAUNCH("verify_draw", (verify_draw_kernel<T, false, false>), dim3(w.draw, a.B), dim3(DT), 0,
-            a.stream, a, w.last, w.stats, w.slices, w.draw, w.sums, w.arrived);
+  KF_LAUNCH("verify_draw", (w.unit == 1 ? verify_draw_kernel<T, false, false, 1>
+                                        : verify_draw_kernel<T, false, false, 4>),
+            dim3(w.draw, a.B), dim3(DT), 0, a.stream, a, w.last, w.stats, w.slices, w.draw, w.sums,
+            w.arrived);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
