@@ -6,7 +6,7 @@ backward, KV-cache decode, weight capture) runs in hand-written HIP kernels
 behind the C ABI in ``include/kf_attn.h``.
 """
 
-from kempnerforge_amd.attention import Attention, KVCache  # noqa: F401
+from kempnerforge_amd.attention import Attention, KVCache, begin_tree, keep_path  # noqa: F401
 from kempnerforge_amd.mot import MoTAttention  # noqa: F401
 from kempnerforge_amd.norm import RMSNorm  # noqa: F401
 from kempnerforge_amd.position import precompute_rope_frequencies  # noqa: F401

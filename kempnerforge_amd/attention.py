@@ -14,6 +14,9 @@ Paths (reference lines in ``kempnerforge/model/attention.py``):
 * decode, one token with a cache (``:169-175,229-231``): ``kf_attn_decode``;
 * prefill with a cache (``:169-175,229-231``): ``kf_kv_cache_append`` then the
   forward over the cache with the reference's top-left causal alignment;
+* a tree of drafted tokens with a cache (:func:`begin_tree`; no counterpart in the
+  reference): ``kf_attn_tree``, after which :func:`keep_path` makes the accepted
+  tokens the cache's next ones;
 * capture (``:184-189,238-280``): ``kf_attn_capture``;
 * explicit masks without a cache (``:190-227``): ``doc_ids`` (packed
   documents) and ``key_padding_mask`` (padded keys, with the reference's NaN
@@ -60,6 +63,8 @@ class KVCache:
     ragged batch, e.g. right-padded prompts of different lengths), and
     ``use_rope_tables`` hands over the full RoPE tables so that each sequence
     decodes at its own position.  ``seq_len`` is then the longest fill level.
+    ``tree`` (set by :func:`begin_tree`) makes the next forwards score drafted
+    tokens behind the fill level instead of appending.
     """
 
     def __init__(
@@ -79,6 +84,7 @@ class KVCache:
         self._seq_len = 0
         self.rope_tables: tuple[torch.Tensor, torch.Tensor] | None = None
         self.ragged = False
+        self.tree: tuple[torch.Tensor | None, torch.Tensor | None] | None = None
 
     @property
     def max_seq_len(self) -> int:
@@ -153,6 +159,37 @@ class KVCache:
         self.lens.add_(new_len)
 
 
+def begin_tree(caches, parents: torch.Tensor | None = None,
+               counts: torch.Tensor | None = None) -> None:
+    """From here to :func:`keep_path`, a model's forward with these caches (one per
+    layer) scores its tokens as a tree of drafts: token i attends the cached prefix,
+    itself and its ancestors, at the position of its depth, and its key and value go
+    to the cache row ``lens[b] + i`` without advancing the cache.  Several forwards
+    may follow one another (a tree that grows level by level); each overwrites the
+    rows of the last.
+
+    ``parents`` (``[N]`` or ``[B, N]``, integers on the device; None: a chain) and
+    ``counts`` (``[B]``: tokens in use, None: all) as in ``ops.tree_decode_raw``."""
+    for c in caches:
+        c.tree = (parents, counts)
+
+
+def keep_path(caches, path: torch.Tensor, kept: torch.Tensor, lengths=None) -> None:
+    """Ends :func:`begin_tree`: the accepted nodes ``path[b, :kept[b]]`` (what
+    ``ops.verify_drafts_raw`` returns) become the caches' next rows, in all layers
+    in one launch.  ``lengths``: the fill levels after it, a list of ints, where the
+    caller knows them; otherwise they are read back (one host synchronisation)."""
+    ops.cache_keep_raw([c.k for c in caches], [c.v for c in caches], [c.lens for c in caches],
+                       path, kept)
+    if lengths is None:
+        lengths = caches[0].lens.tolist()
+    top, ragged = max(lengths), len(set(lengths)) > 1
+    for c in caches:
+        c.tree = None
+        c._seq_len = top
+        c.ragged = ragged
+
+
 class Attention(nn.Module):
     """Grouped-Query Attention with RoPE on gfx950 HIP kernels."""
 
@@ -208,10 +245,13 @@ class Attention(nn.Module):
         k = self.k_proj(x).view(batch, seq_len, -1, self.head_dim)
         v = self.v_proj(x).view(batch, seq_len, -1, self.head_dim)
         masked = doc_ids is not None or key_padding_mask is not None
+        tree = kv_cache.tree if kv_cache is not None else None
+        if tree is not None and (masked or self.capture_attention_weights):
+            raise ValueError("a tree of drafts takes no doc_ids, no key_padding_mask and no capture")
         decode = (kv_cache is not None and seq_len == 1 and not masked
                   and not self.capture_attention_weights)
         # decode applies the QK-norm inside its kernels (one eps for both)
-        fuse_norm = (decode and self.q_norm is not None
+        fuse_norm = ((decode or tree is not None) and self.q_norm is not None
                      and self.q_norm.eps == self.k_norm.eps)  # type: ignore[union-attr]
         if self.q_norm is not None and not fuse_norm:
             q = self.q_norm(q)
@@ -241,6 +281,16 @@ class Attention(nn.Module):
                                 key_padding_mask=key_padding_mask)
         elif kv_cache is None:
             out = ops.attention(q, k, v, rope_cos, rope_sin, causal=True)
+        elif tree is not None:
+            kv_cache._check_room(seq_len)
+            cos_t, sin_t, row0 = kv_cache._decode_tables(rope_cos, rope_sin)
+            out = ops.tree_decode_raw(
+                q, k, v, kv_cache.k, kv_cache.v, kv_cache.lens, cos_t, sin_t,
+                rope_row_offset=row0, max_len=kv_cache.seq_len + seq_len, parents=tree[0],
+                counts=tree[1],
+                q_norm_weight=self.q_norm.weight if fuse_norm else None,  # type: ignore[union-attr]
+                k_norm_weight=self.k_norm.weight if fuse_norm else None,  # type: ignore[union-attr]
+                norm_eps=self.q_norm.eps if fuse_norm else 1e-5)  # type: ignore[union-attr]
         elif seq_len == 1:
             kv_cache._check_room(1)
             cos_t, sin_t, row0 = kv_cache._decode_tables(rope_cos, rope_sin)

@@ -17,6 +17,10 @@ layer).  Two additions, both off by default:
   step where the last sequence finished, so it is the same as the reference's
   (up to N - 1 decode steps are computed and discarded).
 
+``speculative_generate`` (no counterpart in the reference) emits tokens of the same
+distribution several at a time: a smaller model drafts a chain or a tree of them,
+one forward of the model scores all, and the accepted path is kept.
+
 The model is the reference's ``Transformer`` contract: ``model(tokens,
 kv_caches=...)`` returns logits ``(batch, seq, vocab)``, ``model.config`` has
 ``max_seq_len``, ``n_layers``, ``n_kv_heads``, ``head_dim`` and ``rope_theta``,
@@ -27,7 +31,8 @@ from __future__ import annotations
 
 import torch
 
-from kempnerforge_amd.attention import KVCache
+from kempnerforge_amd import ops
+from kempnerforge_amd.attention import KVCache, begin_tree, keep_path
 from kempnerforge_amd.position import precompute_rope_frequencies
 
 
@@ -38,7 +43,13 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0,
     multinomial draw (``kempnerforge/model/generate.py:15-56``)."""
     if temperature == 0:
         return logits.argmax(dim=-1)
-    logits = logits / temperature
+    logits = _filtered(logits / temperature, top_k, top_p)
+    return torch.multinomial(logits.softmax(dim=-1), num_samples=1).squeeze(-1)
+
+
+def _filtered(logits: torch.Tensor, top_k: int, top_p: float) -> torch.Tensor:
+    """Rows ``(rows, vocab)`` of scaled logits with -inf at the tokens that top-k and
+    nucleus filtering leave out."""
     if top_k > 0:
         top_k = min(top_k, logits.shape[-1])
         threshold = logits.topk(top_k, dim=-1).values[:, -1:]
@@ -50,7 +61,7 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0,
         drop = (probs.cumsum(dim=-1) - probs) >= top_p
         sorted_logits[drop] = float("-inf")
         logits = torch.zeros_like(logits).scatter_(1, sorted_indices, sorted_logits)
-    return torch.multinomial(logits.softmax(dim=-1), num_samples=1).squeeze(-1)
+    return logits
 
 
 def _rope_tables(model, total_len: int, device):
@@ -148,3 +159,212 @@ def generate(
         out[b, :n] = prompt_tokens[b, :n]
         out[b, n:n + gen.shape[1]] = gen[b]
     return out
+
+
+def _tree_levels(tree) -> tuple[list[int], list[int], list[int]]:
+    """A draft tree given as its parents, level by level: (parents, rank of each node
+    among its siblings, first node of each level with the node count at the end)."""
+    parents = [int(p) for p in tree]
+    if not 2 <= len(parents) <= ops.TREE_MAX_NODES:
+        raise ValueError(f"a draft tree has 2 to {ops.TREE_MAX_NODES} nodes (got {len(parents)})")
+    if parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i):
+        raise ValueError("tree must name the parent of each node, before it; node 0 has -1")
+    depth, rank, children = [0], [0], [0] * len(parents)
+    for p in parents[1:]:
+        depth.append(depth[p] + 1)
+        rank.append(children[p])
+        children[p] += 1
+    if depth != sorted(depth):
+        raise ValueError("tree must list its nodes level by level")
+    starts = [i for i, d in enumerate(depth) if i == 0 or d > depth[i - 1]]
+    return parents, rank, starts + [len(parents)]
+
+
+class _Stream:
+    """One model and its caches over the sequences that are being generated."""
+
+    def __init__(self, model, prompt, prompt_lens, rows: int):
+        cfg, device = model.config, prompt.device
+        dtype = next(model.parameters()).dtype
+        self.model = model
+        self.caches = [KVCache(prompt.shape[0], rows, cfg.n_kv_heads, cfg.head_dim, dtype, device)
+                       for _ in range(cfg.n_layers)]
+        logits = model(prompt, kv_caches=self.caches)
+        last = torch.tensor([n - 1 for n in prompt_lens], device=device)
+        self.logits = logits[torch.arange(prompt.shape[0], device=device), last]
+        cos, sin = _rope_tables(model, min(rows, cfg.max_seq_len), device)
+        for c in self.caches:
+            c.set_lengths(prompt_lens)
+            c.use_rope_tables(cos, sin)
+
+    def __call__(self, tokens):
+        return self.model(tokens, kv_caches=self.caches)
+
+    def rewind(self, lens: torch.Tensor, lengths: list[int]) -> None:
+        """Fill levels of another stream over the same sequences."""
+        for c in self.caches:
+            c.lens.copy_(lens)
+            c._seq_len, c.ragged = max(lengths), len(set(lengths)) > 1
+
+
+@torch.no_grad()
+def speculative_generate(
+    model,
+    draft_model,
+    prompt_tokens: torch.Tensor,
+    max_new_tokens: int,
+    *,
+    draft_len: int = 4,
+    tree: list[int] | None = None,
+    temperature: float = 1.0,
+    top_k: int = 0,
+    top_p: float = 1.0,
+    eos_token_id: int | None = None,
+    prompt_lens: list[int] | None = None,
+) -> torch.Tensor:
+    """:func:`generate` with drafts of ``draft_model``: tokens of the same
+    distribution (at temperature 0 the same tokens, up to the rounding of the
+    model's logits), several per forward of ``model``.
+
+    Without ``tree`` the draft model samples a chain of ``draft_len`` tokens.  With
+    it (the parent of each node, level by level, node 0 the last token with -1) the
+    drafts are its most likely tokens after each node, a child per rank.  Each step
+    runs the draft model along the chain (or down the levels), scores all drafts in
+    one forward of ``model`` (``kf_attn_tree``), verifies them
+    (``kf_verify_drafts``) and keeps the accepted path's cache rows
+    (``kf_kv_cache_keep``); it reads the accepted tokens back once.  A sequence near
+    its ``max_new_tokens`` drafts no deeper than it can use.
+
+    Both models share the vocabulary and follow :func:`generate`'s contract.  Returns
+    each prompt followed directly by its tokens, rows padded on the right with
+    ``eos_token_id`` (or 0) to the longest; a row ends with its first
+    ``eos_token_id`` or after ``max_new_tokens``."""
+    device = prompt_tokens.device
+    batch, prompt_len = prompt_tokens.shape
+    if draft_len < 1 or draft_len + 1 > ops.TREE_MAX_NODES:
+        raise ValueError(f"draft_len must lie in [1, {ops.TREE_MAX_NODES - 1}] (got {draft_len})")
+    if tree is None:
+        parents, rank, starts = None, None, list(range(draft_len + 2))
+    else:
+        parents, rank, starts = _tree_levels(tree)
+    nodes = starts[-1]
+    limit = min(model.config.max_seq_len, draft_model.config.max_seq_len)
+    if prompt_len + max_new_tokens > limit:
+        raise ValueError(
+            f"prompt ({prompt_len}) + max_new_tokens ({max_new_tokens}) = "
+            f"{prompt_len + max_new_tokens} exceeds the models' max_seq_len ({limit})"
+        )
+    if prompt_lens is None:
+        prompt_lens = [prompt_len] * batch
+    prompt_lens = [int(n) for n in prompt_lens]
+    if len(prompt_lens) != batch or min(prompt_lens) < 1 or max(prompt_lens) > prompt_len:
+        raise ValueError("prompt_lens needs one length in [1, prompt_len] per sequence")
+    if max_new_tokens < 1:
+        return prompt_tokens.clone()
+    modes = [(m, m.training) for m in (model, draft_model)]
+    for m, _ in modes:
+        m.eval()
+    # The vocabularies before any token of one model reaches the other (token 0 is in both).
+    probe = prompt_tokens.new_zeros(1, 1)
+    vocab, draft_vocab = (m(probe).shape[-1] for m in (model, draft_model))
+    if vocab != draft_vocab:
+        raise ValueError(f"the models' vocabularies differ ({vocab}, {draft_vocab})")
+    # Rows behind the last token for its drafts.  (Positions stay below limit.)
+    rows = prompt_len + max_new_tokens + nodes
+    target = _Stream(model, prompt_tokens, prompt_lens, rows)
+    draft = _Stream(draft_model, prompt_tokens, prompt_lens, rows)
+
+    def dist(logits):
+        """(logits, temperature) of the distribution that is sampled."""
+        if temperature == 0 or (top_k <= 0 and top_p >= 1.0):
+            return logits, temperature
+        flat = _filtered((logits / temperature).reshape(-1, vocab), top_k, top_p)
+        return flat.view(logits.shape), 1.0
+
+    def draw(logits, temp):
+        """A token per row, by a verification of no drafts; -1 for a row that is no
+        distribution."""
+        return ops.verify_drafts_raw(logits[:, None], root, torch.rand(batch, 1, device=device),
+                                     temperature=temp)[2]
+
+    root = prompt_tokens.new_zeros(batch, 1)
+    token = draw(*dist(target.logits))
+    emitted = [[t] for t in token.tolist()]
+    if min(e[0] for e in emitted) < 0:
+        raise RuntimeError("the model's logits are no distribution (NaN, or -inf throughout)")
+    lengths = list(prompt_lens)
+    if tree is not None:
+        parents = torch.tensor(parents, dtype=torch.int32, device=device)
+        rank = torch.tensor(rank, device=device)
+
+    def left(b):
+        """How many more tokens sequence b takes."""
+        row = emitted[b]
+        return 0 if row[-1] == eos_token_id else max_new_tokens - len(row)
+
+    while any(left(b) for b in range(batch)):
+        # levels of drafts that each sequence can use (finished ones: no node at all)
+        deep = [min(left(b), len(starts) - 1) for b in range(batch)]
+        use = [starts[d] for d in deep]
+        n, levels = max(use), max(deep)
+        counts = torch.tensor(use, dtype=torch.int32, device=device)
+        tokens = token.new_zeros(batch, n)
+        tokens[:, 0] = token
+        tree_parents, draft_logits = None, None
+        if tree is None:
+            rowlist = []
+            for j in range(1, n):
+                logits, temp = dist(draft(tokens[:, j - 1:j])[:, -1])
+                rowlist.append(logits)
+                # (a draft that is no distribution ends its path in the verification)
+                tokens[:, j] = draw(logits, temp).clamp_min(0)
+            draft(tokens[:, n - 1:])  # (its key and value, for when all are accepted)
+            if temperature > 0 and n > 1:
+                draft_logits = torch.stack(rowlist, dim=1)
+        else:
+            tree_parents = parents[:n]
+            for d in range(1, levels):
+                lo, hi, end = starts[d - 1], starts[d], starts[d + 1]
+                begin_tree(draft.caches, parents[:hi], counts.clamp_max(hi))
+                logits = draft(tokens[:, :hi])[:, lo:hi]
+                at, want = parents[hi:end].long() - lo, rank[hi:end]
+                # (a rank past the vocabulary repeats its last token: refused again)
+                best = logits.topk(min(vocab, len(tree)), dim=-1).indices
+                tokens[:, hi:end] = best[:, at, want.clamp_max(best.shape[-1] - 1)]
+            begin_tree(draft.caches, tree_parents, counts)
+            draft(tokens)
+        begin_tree(target.caches, tree_parents, counts)
+        logits, temp = dist(target(tokens))
+        path, kept, token = ops.verify_drafts_raw(
+            logits, tokens, torch.rand(batch, n, device=device), temperature=temp,
+            parents=tree_parents, counts=counts, draft_logits=draft_logits)
+        accepted = tokens.gather(1, path.clamp_min(0).long())
+        # the step's one read-back: per sequence, how many, the path's tokens, the next
+        host = torch.cat([kept[:, None].long(), accepted, token[:, None]], dim=1).tolist()
+        for b, (k, *row) in enumerate(host):
+            if use[b] == 0:
+                continue
+            if k == 0 or row[-1] < 0:
+                raise RuntimeError("the model's logits are no distribution (NaN, or -inf "
+                                   "throughout)")
+            lengths[b] += k
+            for t in row[1:k] + row[-1:]:
+                if left(b):
+                    emitted[b].append(t)
+        keep_path(target.caches, path, kept, lengths)
+        if tree is None:
+            draft.rewind(target.caches[0].lens, lengths)
+        else:
+            keep_path(draft.caches, path, kept, lengths)
+        token = token.clamp_min(0)  # (a finished sequence has no next token; any will do)
+
+    for m, was_training in modes:
+        m.train(was_training)
+    pad = eos_token_id if eos_token_id is not None else 0
+    width = max(n + len(e) for n, e in zip(prompt_lens, emitted))
+    out = torch.full((batch, width), pad, dtype=prompt_tokens.dtype)
+    host_prompt = prompt_tokens.cpu()
+    for b, (n, e) in enumerate(zip(prompt_lens, emitted)):
+        out[b, :n] = host_prompt[b, :n]
+        out[b, n:n + len(e)] = torch.tensor(e, dtype=out.dtype)
+    return out.to(device)

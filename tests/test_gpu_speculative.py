@@ -1,0 +1,186 @@
+"""A speculative step through the module and its caches, and generation with
+drafts: the operators together, as a user's program runs them."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gpu_util import DEV, announce, seeded
+from kempnerforge_amd import Attention, KVCache, begin_tree, keep_path
+from kempnerforge_amd.generate import _filtered, generate, speculative_generate
+from kempnerforge_amd.position import precompute_rope_frequencies
+from test_gpu_generate import TinyLM
+
+pytestmark = pytest.mark.gpu
+
+TREE = [-1, 0, 0, 0, 1, 1, 2, 3, 4, 4, 6]
+
+
+def _lm(seed, **kw):
+    torch.manual_seed(seed)
+    return TinyLM(**kw).to(DEV)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("tree", [None, TREE, [-1, 0], [-1] + list(range(7))])
+def test_greedy_equals_generate(tree, qk_norm):
+    """At temperature 0 in float32 the tokens are generate's, whatever the drafts are
+    worth: another model's, or the model's own (all accepted)."""
+    announce(f"speculative greedy {tree} {qk_norm}")
+    model, other = _lm(0, qk_norm=qk_norm), _lm(1, n_layers=1, qk_norm=qk_norm)
+    prompt = torch.randint(0, 97, (3, 11), device=DEV)
+    want = generate(model, prompt, 24, temperature=0)
+    for draft in (other, model):
+        got = speculative_generate(model, draft, prompt, 24, temperature=0, tree=tree, draft_len=5)
+        assert torch.equal(got, want)
+    assert model.training and other.training  # as they were
+
+
+@pytest.mark.parametrize("tree", [None, TREE])
+def test_ragged_prompts_and_eos(tree):
+    announce(f"speculative ragged {tree}")
+    model, draft = _lm(2, vocab=13), _lm(3, vocab=13, n_layers=1)
+    lens = [3, 17, 9, 1]
+    prompt = torch.randint(1, 13, (4, 17), device=DEV)
+    got = speculative_generate(model, draft, prompt, 30, temperature=0, tree=tree,
+                               prompt_lens=lens, eos_token_id=0)
+    for b, n in enumerate(lens):
+        alone = generate(model, prompt[b:b + 1, :n], 30, temperature=0, eos_token_id=0)[0]
+        assert torch.equal(got[b, :alone.numel()], alone), b
+        assert (got[b, alone.numel():] == 0).all()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(tree=[-1, 0, 0, 1]), dict(top_k=4),
+                                dict(top_p=0.7, tree=[-1, 0, 0, 1])], ids=str)
+def test_samples_follow_the_model(kw):
+    """The joint frequencies of the first two emitted tokens over 8192 sequences of one
+    prompt against the model's own distribution, within 5 standard deviations a cell
+    (49 cells: by chance once in 35 000 runs, and the seed is fixed)."""
+    announce(f"speculative distribution {kw}")
+    model, draft = _lm(4, vocab=7), _lm(5, vocab=7, n_layers=1)
+    B, prompt = 4096, torch.randint(0, 7, (1, 5), device=DEV)
+    with torch.no_grad():  # a temperature at which the logits leave a choice
+        T = model(prompt)[0, -1].std().item()
+    torch.manual_seed(7)
+    count = torch.zeros(49, dtype=torch.long, device=DEV)
+    for _ in range(2):
+        out = speculative_generate(model, draft, prompt.expand(B, 5).contiguous(), 3,
+                                   temperature=T, draft_len=2, **kw)
+        count += torch.bincount(out[:, 5] * 7 + out[:, 6], minlength=49)
+
+    def probs(tokens):
+        with torch.no_grad():
+            x = _filtered(model(tokens)[:, -1] / T, kw.get("top_k", 0), kw.get("top_p", 1.0))
+        return torch.softmax(x.double(), -1)
+
+    first = probs(prompt)[0]
+    second = probs(torch.cat([prompt.expand(7, 5), torch.arange(7, device=DEV)[:, None]], 1))
+    p = (first[:, None] * second).reshape(-1)
+    n = count.sum()
+    assert p.max() < 0.7 and (p > 0.01).sum() > 5
+    assert count[p == 0].sum() == 0
+    z = ((count - n * p) / (n * p * (1 - p)).sqrt().clamp_min(1.0)).abs().max().item()
+    print(f"[speculative distribution {kw}] worst z {z:.2f}", flush=True)
+    assert z < 5
+
+
+@pytest.mark.parametrize("tree", [None, TREE])
+def test_bfloat16_steps_emit_their_own_argmax(tree):
+    """head_dim 128 in bfloat16: every emitted token is the most likely one of the
+    logits of the step that scored its predecessor, and those are finite.  (Not
+    compared with a forward over the whole sequence: this model's second layer has
+    scores near 1e5, where bfloat16's half step of a query, 2^-9, is 200 in the
+    exponent, so that any other order of rounding picks other keys.)"""
+    announce(f"speculative bf16 {tree}")
+    torch.manual_seed(8)
+    model = TinyLM(dim=1024, n_heads=8, n_kv=2).to(DEV, torch.bfloat16)
+    prompt = torch.randint(0, 97, (4, 9), device=DEV)
+    seen = []  # per forward of all layers: fill levels, tokens, parents, best tokens
+    draft = TinyLM(dim=1024, n_heads=8, n_kv=2).to(DEV, torch.bfloat16)
+    draft.load_state_dict(model.state_dict())
+
+    def record(module, args, kwargs, out):
+        caches = kwargs.get("kv_caches")
+        if caches is not None and caches[0].tree is not None:
+            assert out.isfinite().all()
+            seen.append((caches[0].lens.tolist(), args[0].tolist(), out.argmax(-1).tolist()))
+
+    model.register_forward_hook(record, with_kwargs=True)
+    out = speculative_generate(model, draft, prompt, 16, temperature=0, tree=tree)
+    checked = 0
+    for lens, tokens, best in seen:
+        n = len(tokens[0])
+        par = list(range(-1, n - 1)) if tree is None else tree[:n]
+        for b in range(4):
+            row, at, pos = out[b].tolist(), 0, lens[b]
+            if pos + 1 >= len(row):
+                continue  # finished
+            assert tokens[b][0] == row[pos]
+            while at is not None and pos + 1 < len(row):
+                assert best[b][at] == row[pos + 1], (b, pos)
+                checked += 1
+                at = next((c for c in range(n) if par[c] == at and tokens[b][c] == row[pos + 1]),
+                          None)
+                pos += 1
+    assert checked == 4 * 15  # all but the first of each sequence, which the prompt gave
+
+
+@pytest.mark.parametrize("dtype,head_dim", [(torch.float32, 64), (torch.bfloat16, 128),
+                                            (torch.float32, 32)])
+def test_one_layer_step_by_step(dtype, head_dim):
+    """A tree step of one Attention layer: each node's output is what a fresh cache
+    gives for the tokens of its own path, and after keep_path the cache decodes on
+    as if the accepted tokens had been fed one by one."""
+    announce(f"module tree step {dtype} {head_dim}")
+    torch.manual_seed(9)
+    Hq, Hkv = 4, 2
+    layer = Attention(Hq * head_dim, Hq, Hkv, head_dim=head_dim, qk_norm=True).to(DEV, dtype)
+    cos, sin = (t.to(DEV) for t in precompute_rope_frequencies(head_dim, 64))
+    B, S, N = 2, 13, len(TREE)
+    x = seeded((B, S + N + 1, Hq * head_dim), 0, dtype).to(DEV)
+    parents = torch.tensor(TREE, device=DEV)
+
+    def cache():
+        return KVCache(B, 40, Hkv, head_dim, dtype, DEV)
+
+    def feed(c, xs, at):
+        return layer(xs, cos[at:at + xs.shape[1]], sin[at:at + xs.shape[1]], kv_cache=c)
+
+    tol = 1e-5 if dtype == torch.float32 else 4e-2
+    with torch.no_grad():
+        c = cache()
+        feed(c, x[:, :S], 0)
+        begin_tree([c], parents)
+        out = feed(c, x[:, S:S + N], S)
+        assert c.seq_len == S and c.lens.tolist() == [S, S]
+        for i in range(N):
+            chain, j = [], i
+            while j >= 0:
+                chain.insert(0, j)
+                j = TREE[j]
+            ref = cache()
+            feed(ref, x[:, :S], 0)
+            for d, j in enumerate(chain):
+                one = feed(ref, x[:, S + j:S + j + 1], S + d)
+            err = (out[:, i:i + 1].float() - one.float()).abs().max().item()
+            assert err <= tol * max(1.0, one.float().abs().max().item()), (i, err)
+        # accept nodes 0, 2, 6 and 10 in row 0, and 0, 1 in row 1
+        path = torch.full((B, N), -1, dtype=torch.int32, device=DEV)
+        path[0, :4] = torch.tensor([0, 2, 6, 10], dtype=torch.int32)
+        path[1, :2] = torch.tensor([0, 1], dtype=torch.int32)
+        kept = torch.tensor([4, 2], dtype=torch.int32, device=DEV)
+        keep_path([c], path, kept)
+        assert c.tree is None and c.seq_len == S + 4 and c.ragged
+        assert c.lens.tolist() == [S + 4, S + 2]
+        c.use_rope_tables(cos, sin)
+        nxt = x[:, S + N:]
+        got = layer(nxt, cos[:1], sin[:1], kv_cache=c)
+        for b, chain in enumerate(([0, 2, 6, 10], [0, 1])):
+            ref = KVCache(1, 40, Hkv, head_dim, dtype, DEV)
+            layer(x[b:b + 1, :S], cos[:S], sin[:S], kv_cache=ref)
+            for d, j in enumerate(chain):
+                feed(ref, x[b:b + 1, S + j:S + j + 1], S + d)
+            one = feed(ref, nxt[b:b + 1], S + len(chain))
+            err = (got[b:b + 1].float() - one.float()).abs().max().item()
+            assert err <= tol * max(1.0, one.float().abs().max().item()), (b, err)
