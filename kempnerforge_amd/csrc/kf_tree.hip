@@ -913,69 +913,102 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   }
 }
 
-// The rows of tile blockIdx.x, 16 bytes of a row per thread and
-// blockIdx.y's share of them: the partials of the workgroups that met the tile
-// rescaled to a common maximum and summed; a tile that one workgroup finished is
-// left alone.
-template <typename T, int D>
+// The rows of tile blockIdx.x, 16 bytes of a row per thread and blockIdx.y's share
+// of them: the partials of the workgroups that met the tile, rescaled to a common
+// maximum and summed; a tile that one workgroup finished is left alone.  JG groups of
+// threads take a row's partials in turn, U at a time, and are joined through LDS:
+// what it costs is the round trips of a thread's loads, one a batch.
+template <typename T, int D, int JG>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
     TreeArgs a, const float* __restrict__ opart, const float* __restrict__ mlpart,
     const int* __restrict__ refusals, int rows, int kc, int NWmax, int tiles_max) {
-  constexpr int LPR = D / 4;  // lanes of a row
+  constexpr int LPR = D / 4, RPW = 256 / (LPR * JG);  // lanes of a row, rows of a workgroup
+  __shared__ f32x4 xo[JG > 1 ? 256 : 1];
+  __shared__ float2 xm[JG > 1 ? 256 : 1];
   const int lane = threadIdx.x & 63, n_rep = a.Hq / a.Hkv;
   const int item = blockIdx.x, t = item % tiles_max, bg = item / tiles_max, b = bg / a.Hkv,
             g = bg % a.Hkv;
-  const int r = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+  const int r = blockIdx.y * RPW + threadIdx.x / (LPR * JG), jg = threadIdx.x / LPR % JG;
+  const int col = threadIdx.x % LPR * 4;
   const int row = t * rows + r, i = row / n_rep, hq = g * n_rep + row % n_rep;
   const int2 s = tree_seq(a, b);
   const TreeSched sched(a, n_rep, rows, kc, NWmax, lane);
   int pre = 0;
   for (int b0 = lane; b0 < b; b0 += 64) pre += sched.chunks(b0);
   pre = wave_sum_int(pre);
-  if (i >= a.N || r >= rows) return;
+  const bool inside = i < a.N && r < rows;
   T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + hq) * D + col;
   T y[4];
-  if (s.x < 0 || i >= s.x) {  // a refused sequence, or an unused node
+  if (inside && jg == 0 && (s.x < 0 || i >= s.x)) {  // a refused sequence, or an unused node
     const bool refused = s.x < 0 || (s.x > 0 && refusals[b]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(refused ? NAN : 0.f);
     __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
-    return;
   }
-  const int nck = sched.nck(s);
-  const int c0 = pre + (g * sched.tiles(s) + t) * sched.per(s) + sched.over;
-  const int w0 = chunk_owner(c0, sched.C, sched.NW),
-            ns = chunk_owner(c0 + nck - 1, sched.C, sched.NW) - w0 + 1;
-  if (ns == 1) return;
-  const int64_t first = ((int64_t)w0 + item) * rows + r;
-  const float* ob = opart + first * D + col;
-  const float2* mb = (const float2*)mlpart + first;
-  // (m, l) of all partials are read twice: for the maximum, then with the sums
-  float M = -INFINITY;
-  constexpr int U = 8;
-  for (int j0 = 0; j0 < ns; j0 += U) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) M = fmaxf(M, mb[(int64_t)min(j0 + u, ns - 1) * rows].x);
+  int ns = 0, w0 = 0;
+  if (inside && i < s.x) {
+    const int nck = sched.nck(s);
+    const int c0 = pre + (g * sched.tiles(s) + t) * sched.per(s) + sched.over;
+    w0 = chunk_owner(c0, sched.C, sched.NW);
+    ns = chunk_owner(c0 + nck - 1, sched.C, sched.NW) - w0 + 1;
   }
-  float l = 0.f;
+  const bool live = ns > 1;
+  float M = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < ns; j0 += U) {
-    f32x4 po[U];
-    float2 ml[U];
+  // joins a partial (of weight 0: left out, whatever it holds)
+  auto add = [&](float f, const float2& ml, const f32x4& po) {
+    const float w = fast_exp2(ml.x - M);
+    l = l * f + (w != 0.f ? w * ml.y : 0.f);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t j = min(j0 + u, ns - 1);
-      ml[u] = mb[j * rows];
-      po[u] = *(const f32x4*)(ob + j * rows * D);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + (w != 0.f ? w * po[e] : 0.f);
+  };
+  if (live) {
+    const int64_t first = ((int64_t)w0 + item) * rows + r;
+    const float* ob = opart + first * D + col;
+    const float2* mb = (const float2*)mlpart + first;
+    constexpr int U = 8;
+    for (int j0 = jg; j0 < ns; j0 += U * JG) {
+      f32x4 po[U];
+      float2 ml[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float w = j0 + u < ns ? fast_exp2(ml[u].x - M) : 0.f;
-      l += w != 0.f ? w * ml[u].y : 0.f;  // (a partial of weight 0 is left out)
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = min(j0 + u * JG, ns - 1);
+        ml[u] = mb[j * rows];
+        po[u] = *(const f32x4*)(ob + j * rows * D);
+      }
+      float mx = M;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += w != 0.f ? w * po[u][e] : 0.f;
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, ml[u].x);
+      // (a chunk's scores can all be -inf: such a partial has no weight)
+      float f = M == -INFINITY ? 0.f : fast_exp2(M - mx);
+      M = mx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j0 + u * JG < ns && ml[u].x != -INFINITY) add(f, ml[u], po[u]), f = 1.f;
+      }
+      if (f != 1.f) l *= f, o *= f;
     }
   }
+  if constexpr (JG > 1) {
+    xo[threadIdx.x] = o;
+    xm[threadIdx.x] = make_float2(M, l);
+    __syncthreads();
+    if (live && jg == 0) {
+      float mx = M;
+#pragma unroll
+      for (int j = 1; j < JG; ++j) mx = fmaxf(mx, xm[threadIdx.x + j * LPR].x);
+      float f = M == -INFINITY ? 0.f : fast_exp2(M - mx);
+      M = mx;
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int j = 1; j < JG; ++j) {
+        const float2 ml = xm[threadIdx.x + j * LPR];
+        if (ml.x != -INFINITY) add(1.f, ml, xo[threadIdx.x + j * LPR]);
+      }
+    }
+  }
+  if (!live || jg != 0) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[e] / l);
   __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
@@ -993,7 +1026,10 @@ Plan plan_of(const TreeArgs& a) {
   Plan p = {};
   const int n_rep = a.Hq / a.Hkv, m = a.N * n_rep;
   if (a.D != 64 && a.D != 128) return p;
-  // enough row waves for the pair's rows; float32 has no LDS for four key waves
+  // Enough row waves for the pair's rows, up to four: finer tiles have fewer rows to
+  // spare, but load the keys more often (800 rows of 4 x 8 heads over 1224 keys: 73 us
+  // with 128 rows a tile, 84 with 64, 125 with 32; 135 rows 36, 39, 38; 36 rows the
+  // other way, 40.9 and 39.5).  float32 has no LDS for four key waves.
   p.rw = m <= 32 && a.dtype != F32 ? 1 : m <= 64 ? 2 : 4;
   p.bkw = p.rw == 4 && a.dtype != F32 ? 64 : 32;
   p.rows = 32 * p.rw;
@@ -1077,10 +1113,19 @@ int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p) {
          : p.rw == 2 ? launch_stream<T, D, 2, 32>(a, w, p)
                      : launch_stream<T, D, 4, 64>(a, w, p);
   if (rc) return rc;
-  const int rpw = 256 / (D / 4);  // rows of a workgroup
-  KF_LAUNCH("tree_merge", (tree_merge_kernel<T, D>),
-            dim3(a.B * a.Hkv * p.tiles, (p.rows + rpw - 1) / rpw), dim3(256), 0, a.stream, a,
-            w.opart, w.mlpart, w.refusals, p.rows, p.kc, p.grid, p.tiles);
+  // About `grid / items` partials a tile; a batch of 8 is one round trip.  63 of them (27
+  // nodes of 5 heads over 4000 keys): the whole call 29.8 us with one group, 26.4 with
+  // two, 23.8 with eight; 16 of them: 29.5 with one, 28.2 with two, 29 with four (each
+  // further group is as many workgroups more).
+  const int items = a.B * a.Hkv * p.tiles;
+  const int jg = p.grid > 32 * items ? 8 : p.grid > 8 * items ? 2 : 1;
+  const int rpw = 256 / (D / 4) / jg;  // rows of a workgroup
+  KF_LAUNCH("tree_merge",
+            (jg == 8   ? tree_merge_kernel<T, D, 8>
+             : jg == 2 ? tree_merge_kernel<T, D, 2>
+                       : tree_merge_kernel<T, D, 1>),
+            dim3(items, (p.rows + rpw - 1) / rpw), dim3(256), 0, a.stream, a, w.opart, w.mlpart,
+            w.refusals, p.rows, p.kc, p.grid, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
