@@ -103,17 +103,14 @@ struct Stat {
 __device__ __forceinline__ bool has_mass(double s) { return s > 0.0 && s < INFINITY; }
 
 // 2^((a - b) c) for two maxima, 1 where both are -inf
-template <bool DP>
 __device__ __forceinline__ double weight_of(float a, float b, double c) {
-  if (a == b) return 1.0;
-  return DP ? exp2_64(((double)a - (double)b) * c) : (double)exp2f((float)((a - b) * (float)c));
+  return a == b ? 1.0 : (double)exp2f((a - b) * (float)c);
 }
 
 // Joins a statistic of other values of the row.  Equal maxima: the lower place.
-template <bool DP>
 __device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
   const float m = fmaxf(x.m, y.m);
-  x.s = x.s * weight_of<DP>(x.m, m, c) + y.s * weight_of<DP>(y.m, m, c);
+  x.s = x.s * weight_of(x.m, m, c) + y.s * weight_of(y.m, m, c);
   x.at = x.m > y.m ? x.at : y.m > x.m ? y.at : min(x.at, y.at);
   x.m = m;
 }
@@ -121,8 +118,10 @@ __device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
 // Adds granules k, k + stride, ... (U of them, below `end`) to a thread's share:
 // the maximum of the batch first, then (SUM) one exponential a value; without SUM
 // the place of the maximum.  s becomes NaN where a value is NaN or (SUM) +inf.
-// DP: exponentials in 64 bits; else one float32 instruction each (relative error
-// 2^-22 and that of its argument), summed in 64 bits a batch at a time.
+// The exponentials are one float32 instruction each (relative error 2^-22 and that of
+// its argument; in 64 bits a chain of 16 nodes with the draft's rows, 16 sequences of
+// 131072 values, takes 108 us instead of 51), summed in 64 bits a batch at a time: a
+// probability is off by some 2^-22 of itself, and so is the chance of a token.
 template <typename T, int U>
 __device__ __forceinline__ void load_batch(const Row<T>& r, int k, int stride, int end,
                                            u32x4* raw) {
@@ -139,7 +138,7 @@ __device__ __forceinline__ void load_batch(const Row<T>& r, int k, int stride, i
     }
   }
 }
-template <typename T, bool DP, bool SUM, int U>
+template <typename T, bool SUM, int U>
 __device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, const u32x4* raw,
                                           double c, Stat& st) {
   constexpr int E = Row<T>::E;
@@ -157,7 +156,7 @@ __device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, co
   }
   if (m > st.m) {
     if (SUM) {
-      st.s *= weight_of<DP>(st.m, m, c);
+      st.s *= weight_of(st.m, m, c);
     } else {
 #pragma unroll
       for (int u = U - 1; u >= 0; --u) {
@@ -183,17 +182,14 @@ __device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, co
     Row<T>::unpack(raw[u], f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if constexpr (DP)
-        st.s += exp2_64(((double)f[e] - (double)ref) * c);
-      else
-        gs += __builtin_amdgcn_exp2f(fmaf(f[e], cf, -rc));
+      gs += __builtin_amdgcn_exp2f(fmaf(f[e], cf, -rc));
     }
   }
-  if constexpr (!DP) st.s += (double)gs;
+  st.s += (double)gs;
 }
 
 // The workgroup's shares joined, in order; `x` is one Stat per wavefront.
-template <bool DP, int NT>
+template <int NT>
 __device__ __forceinline__ Stat join_all(Stat st, double c, Stat* x) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -202,7 +198,7 @@ __device__ __forceinline__ Stat join_all(Stat st, double c, Stat* x) {
     y.m = __shfl_xor(st.m, o, 64);
     y.at = __shfl_xor(st.at, o, 64);
     y.s = __shfl_xor(st.s, o, 64);
-    join<DP>(st, y, c);
+    join(st, y, c);
   }
   __syncthreads();  // the previous use of x is over
   if (lane == 0) x[w] = st;
@@ -215,7 +211,7 @@ __device__ __forceinline__ Stat join_all(Stat st, double c, Stat* x) {
     y.m = __shfl_xor(st.m, o, 64);
     y.at = __shfl_xor(st.at, o, 64);
     y.s = __shfl_xor(st.s, o, 64);
-    join<DP>(st, y, c);
+    join(st, y, c);
   }
   st.s = __shfl(st.s, 0, 64);  // (the lanes' orders differ in the last bit)
   return st;
@@ -231,7 +227,7 @@ __host__ __device__ __forceinline__ int slices_of(int V, int E) {
 // Workgroup (slice, row, sequence): rows 0 .. N - 1 the target's, N .. 2N - 2 the
 // draft's.  Rows of unused nodes are left out.  Bound by HBM: a thread's four
 // granules are in flight before the first is used.
-template <typename T, bool DP, bool SUM>
+template <typename T, bool SUM>
 __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a, Stat* __restrict__ out,
                                                           int* __restrict__ arrived) {
   __shared__ Stat x[ST / 64];
@@ -249,8 +245,8 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a, Stat* __
   u32x4 raw[SU];
   const int k = blockIdx.x * SLICE + t;
   load_batch<T, SU>(r, k, ST, r.granules(), raw);
-  add_batch<T, DP, SUM, SU>(r, k, ST, raw, c, st);
-  st = join_all<DP, ST>(st, c, x);
+  add_batch<T, SUM, SU>(r, k, ST, raw, c, st);
+  st = join_all<ST>(st, c, x);
   if (t == 0) out[((int64_t)b * gridDim.y + i) * gridDim.x + blockIdx.x] = st;
 }
 
@@ -350,13 +346,13 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
     for (int k = t; k < ng; k += U * WT) {
       load_batch<T, U>(r, k + U * WT, WT, ng, ahead);
       if (a.greedy)
-        add_batch<T, false, false, U>(r, k, WT, raw, c, st);
+        add_batch<T, false, U>(r, k, WT, raw, c, st);
       else
-        add_batch<T, false, true, U>(r, k, WT, raw, c, st);
+        add_batch<T, true, U>(r, k, WT, raw, c, st);
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = ahead[u];
     }
-    st = join_all<false, WT>(st, c, x);
+    st = join_all<WT>(st, c, x);
     if (a.greedy ? st.s != st.s : !has_mass(st.s)) break;  // no distribution
     end = cur;
     const bool child = t > 0 && t < n && nd.par[t] == cur;
@@ -401,7 +397,7 @@ __host__ __device__ __forceinline__ int draw_slices_of(int V, int E, int U) {
 // weights of a slice's values in 64 bits, summed by segments in order; the last
 // to arrive finds the slice, the segment and the value at which the running sum
 // passes the point.  greedy: one workgroup per sequence, no draw.
-template <typename T, bool ALL, bool DP, int U>
+template <typename T, bool ALL, int U>
 __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int* __restrict__ last,
                                                          const Stat* __restrict__ stats,
                                                          int nslices, int ndraw, double* sums,
@@ -449,14 +445,14 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
         const int i = i0 + x * (DT / 16);
         if (i >= nr) break;  // (a row's 16 lanes alike)
         for (int j = t % 16 + 16; j < nslices; j += 16)
-          join<DP>(z[x], stats[((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices + j], c);
+          join(z[x], stats[((int64_t)b * nrows + (i < n ? i : N + i - n)) * nslices + j], c);
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) {
           Stat v;
           v.m = __shfl_xor(z[x].m, o, 16);
           v.at = __shfl_xor(z[x].at, o, 16);
           v.s = __shfl_xor(z[x].s, o, 16);
-          join<DP>(z[x], v, c);
+          join(z[x], v, c);
         }
         if (t % 16 == 0) row[i] = z[x];
       }
@@ -772,8 +768,7 @@ VerifyWs verify_carve(const VerifyArgs& a, void* p) {
   w.rows = a.drafts != nullptr ? 2 * a.N - 1 : a.N;
   // All rows take B N el / 5 TB/s per value of the vocabulary, a walk about 110 ps
   // per value and level, some four levels deep: equal at 2200 bytes a value.  (A
-  // chain's draft rows: their sums have to hold 64 bits for the draw, which one CU
-  // forms too slowly.)
+  // draft's rows are read by the first way only.)
   w.all_rows = a.drafts != nullptr || (int64_t)a.B * a.N * el <= 2200;
   char* c = (char*)p;
   w.arrived = (int*)c;
@@ -792,17 +787,11 @@ template <typename T>
 int verify_typed(const VerifyArgs& a, void* workspace) {
   const VerifyWs w = verify_carve(a, workspace);
   if (w.all_rows) {
-    auto kernel = a.greedy               ? verify_stats_kernel<T, false, false>
-                  : a.drafts != nullptr ? verify_stats_kernel<T, true, true>
-                                        : verify_stats_kernel<T, false, true>;
+    auto kernel = a.greedy ? verify_stats_kernel<T, false> : verify_stats_kernel<T, true>;
     KF_LAUNCH("verify_stats", kernel, dim3(w.slices, w.rows, a.B), dim3(ST), 0, a.stream, a,
               w.stats, w.arrived);
     KF_CHECK_LAUNCH();
-    auto draw = a.drafts == nullptr
-                    ? (w.unit == 1 ? verify_draw_kernel<T, true, false, 1>
-                                   : verify_draw_kernel<T, true, false, 4>)
-                    : (w.unit == 1 ? verify_draw_kernel<T, true, true, 1>
-                                   : verify_draw_kernel<T, true, true, 4>);
+    auto draw = w.unit == 1 ? verify_draw_kernel<T, true, 1> : verify_draw_kernel<T, true, 4>;
     KF_LAUNCH("verify_draw", draw, dim3(a.greedy ? 1 : w.draw, a.B), dim3(DT), 0, a.stream, a,
               w.last, w.stats, w.slices, w.draw, w.sums, w.arrived);
     KF_CHECK_LAUNCH();
@@ -812,8 +801,8 @@ int verify_typed(const VerifyArgs& a, void* workspace) {
             w.stats, w.arrived);
   KF_CHECK_LAUNCH();
   if (a.greedy) return KF_OK;
-  KF_LAUNCH("verify_draw", (w.unit == 1 ? verify_draw_kernel<T, false, false, 1>
-                                        : verify_draw_kernel<T, false, false, 4>),
+  KF_LAUNCH("verify_draw", (w.unit == 1 ? verify_draw_kernel<T, false, 1>
+                                        : verify_draw_kernel<T, false, 4>),
             dim3(w.draw, a.B), dim3(DT), 0, a.stream, a, w.last, w.stats, w.slices, w.draw, w.sums,
             w.arrived);
   KF_CHECK_LAUNCH();
