@@ -312,9 +312,9 @@ __device__ __forceinline__ bool taken(const VerifyArgs& a, const Nodes& nd, cons
 constexpr int WT = 1024;
 
 // Row by row down the path, one workgroup per sequence.  A CU forms a row's sums
-// at 64 values a clock at most (about 8 operations each): a row of 131072 takes
-// 8 us, whatever its type.  Leaves the last node and its statistic for the draw;
-// greedy: writes the token too.
+// at 64 values a clock at most (about 8 operations each): a row of 131072 takes 14 us,
+// whatever its type.  Leaves the last node and its statistic for the draw; greedy:
+// writes the token too.
 template <typename T>
 __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __restrict__ last,
                                                          Stat* __restrict__ out,
@@ -767,9 +767,11 @@ VerifyWs verify_carve(const VerifyArgs& a, void* p) {
   w.draw = draw_slices_of(a.V, 16 / el, w.unit);
   w.rows = a.drafts != nullptr ? 2 * a.N - 1 : a.N;
   // All rows take B N el / 5 TB/s per value of the vocabulary, a walk about 110 ps
-  // per value and level, some four levels deep: equal at 2200 bytes a value.  (A
-  // draft's rows are read by the first way only.)
-  w.all_rows = a.drafts != nullptr || (int64_t)a.B * a.N * el <= 2200;
+  // per value and level of the longest path: equal at 2200 bytes a value for trees,
+  // whose paths have some four levels (64 trees of 64 nodes, 131072 16-bit values: walk
+  // 73 us, all rows 260; 16 of them 67 and 46).  A chain's can be as long as the chain
+  // (64 of 18 nodes: walk 202 us, all rows 91), and a draft's rows come with chains.
+  w.all_rows = a.parents == nullptr || (int64_t)a.B * a.N * el <= 2200;
   char* c = (char*)p;
   w.arrived = (int*)c;
   c += up256((size_t)a.B * 4);

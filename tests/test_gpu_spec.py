@@ -38,6 +38,9 @@ CASES = [
     (FH, 6, 12, 7, "star", 2.0, False, None),            # repeated tokens among siblings
     (F32, 4, 64, 131072, "random", 1.0, False, None),
     (F32, 3, 256, 300, "random", 1.0, False, None),
+    (BF, 24, 48, 1001, "random", 1.0, False, [48, 0, 30] * 8),  # many nodes: row by row
+    (FH, 24, 60, 515, "binary", 0.0, False, None),
+    (F32, 70, 33, 333, "chain", 1.0, False, None),       # a long chain: all rows
     (BF, 8, 20, 1001, "random", 0.0, False, None),       # greedy
     (FH, 8, 6, 50001, "chain", 0.0, False, [6, 6, 0, 2, 1, 6, 6, 6]),
     (F32, 4, 3, 200000, "chain", 0.0, False, None),

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from gpu_util import DEV, announce, seeded
-from kempnerforge_amd import Attention, KVCache, begin_tree, keep_path
+from kempnerforge_amd import Attention, KVCache, begin_tree, keep_path, ops
 from kempnerforge_amd.generate import _filtered, generate, speculative_generate
 from kempnerforge_amd.position import precompute_rope_frequencies
 from test_gpu_generate import TinyLM
@@ -184,3 +184,106 @@ def test_one_layer_step_by_step(dtype, head_dim):
             one = feed(ref, nxt[b:b + 1], S + len(chain))
             err = (got[b:b + 1].float() - one.float()).abs().max().item()
             assert err <= tol * max(1.0, one.float().abs().max().item()), (b, err)
+
+
+class _Step:
+    """The three operators over a model's caches, as a serving loop runs them: two
+    layers' attention, the verification, the move."""
+
+    def __init__(self, seed, B, N, V, tree, layers=2, dtype=torch.bfloat16):
+        Hq, Hkv, D, S = 8, 2, 128, 400
+        dev = lambda t: t.to(DEV)  # noqa: E731
+        self.q = [dev(seeded((B, N, Hq, D), seed + i, dtype)) for i in range(layers)]
+        self.k = [dev(seeded((B, N, Hkv, D), seed + 10 + i, dtype)) for i in range(layers)]
+        self.kc = [dev(seeded((B, Hkv, S, D), seed + 20 + i, dtype)) for i in range(layers)]
+        self.vc = [dev(seeded((B, Hkv, S, D), seed + 30 + i, dtype)) for i in range(layers)]
+        self.lens = [dev(torch.tensor([37 * (b + 1) for b in range(B)], dtype=torch.int32))
+                     for _ in range(layers)]
+        self.parents = None if tree is None else dev(torch.tensor(tree, dtype=torch.int32))
+        self.head = dev(seeded((Hq * D, V), seed + 40, dtype))
+        self.tokens = dev(torch.randint(0, V, (B, N), generator=torch.Generator().manual_seed(seed)))
+        self.u = dev(torch.rand(B, N, generator=torch.Generator().manual_seed(seed + 1)))
+        self.cos, self.sin = (dev(t) for t in precompute_rope_frequencies(D, S))
+
+    def state(self):
+        return self.kc + self.vc + self.lens
+
+    def __call__(self):
+        x = 0
+        for i in range(len(self.q)):
+            x = x + ops.tree_decode_raw(self.q[i], self.k[i], self.k[i], self.kc[i], self.vc[i],
+                                        self.lens[i], self.cos, self.sin, rope_row_offset=0,
+                                        max_len=400, parents=self.parents)
+        logits = x.flatten(2) @ self.head
+        path, kept, token = ops.verify_drafts_raw(logits, self.tokens, self.u, temperature=40.0,
+                                                  parents=self.parents)
+        ops.cache_keep_raw(self.kc, self.vc, self.lens, path, kept)
+        return path, kept, token
+
+
+STEPS = [(0, 3, 11, 4, TREE), (100, 2, 5, 3, None)]  # (few tokens, so that drafts are accepted)
+
+
+def _eager(runs):
+    """Outputs of `runs` steps one after the other, and the state they leave."""
+    steps = [_Step(*cfg) for cfg in STEPS]
+    outs = [[[t.clone() for t in s()] for _ in range(runs)] for s in steps]
+    torch.cuda.synchronize()
+    return steps, outs
+
+
+def test_whole_steps_captured_and_replayed():
+    """Each step's graph replayed in turn with the other's and with eager calls between:
+    tokens, caches and lengths as from eager steps."""
+    announce("speculative step graphs")
+    runs = 4
+    want_steps, want = _eager(runs)
+    assert any(k > 1 for outs in want for o in outs for k in o[1].tolist())
+    steps = [_Step(*cfg) for cfg in STEPS]
+    other = _Step(7, 4, 20, 100, None)
+    graphs, outs = [], []
+    for s in steps:
+        saved = [t.clone() for t in s.state()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        for t, x in zip(s.state(), saved):
+            t.copy_(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s())
+        graphs.append(g)
+    for r in range(runs):
+        for i, g in enumerate(graphs):
+            g.replay()
+            if r % 2:
+                other()
+            torch.cuda.synchronize()
+            for a, b in zip(outs[i], want[i][r]):
+                assert torch.equal(a, b), (r, i)
+    for s, w in zip(steps, want_steps):
+        for a, b in zip(s.state(), w.state()):
+            assert torch.equal(a, b)
+
+
+def test_steps_on_two_streams_at_once():
+    announce("speculative steps on two streams")
+    runs = 6
+    want_steps, want = _eager(runs)
+    steps = [_Step(*cfg) for cfg in STEPS]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    got = [[] for _ in steps]
+    for _ in range(runs):
+        for i, (s, st) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(st):
+                got[i].append([t.clone() for t in s()])
+    torch.cuda.synchronize()
+    for i in range(len(steps)):
+        for a, b in zip(got[i], want[i]):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+        for a, b in zip(steps[i].state(), want_steps[i].state()):
+            assert torch.equal(a, b)
