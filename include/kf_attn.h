@@ -336,7 +336,8 @@ int kf_verify_drafts_workspace_size(int B, int N, int V, int with_drafts, int dt
  * uniforms[b][0] times their total.
  * counts[b] = 0, a count outside 0 .. N or a parent out of range: kept 0, next
  * -1.  A row on the path that is no distribution (NaN, +inf, or -inf
- * throughout) ends the path, and next is -1. */
+ * throughout) ends the path, and next is -1; a draft's row that is none has its
+ * token refused, and next is drawn from p. */
 int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_n,
                      const int64_t* tokens, const int32_t* parents, int64_t parents_stride,
                      const int32_t* counts, const void* draft_logits, int64_t draft_stride_b,

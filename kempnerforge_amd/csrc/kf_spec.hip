@@ -38,6 +38,11 @@ constexpr int MAXN = KF_TREE_MAX_NODES;
 // at one CU's; verify_drafts says which is taken.  The draw's weights are formed by
 // all workgroups of a sequence, a slice of the row each, and the last one to
 // arrive picks the token.
+//
+// Measured: a chain of 5 with drafts over 32000 float32 values 18 us (4 of sums, 12 of
+// ten dependent round trips); 16 trees of 64 nodes over 131072 16-bit values 42 to 50
+// us (268 MB of logits: 5.4 TB/s and more where they lie in the last-level cache, then
+// 19 us of walk and draw).
 
 // 16 bytes of a row as floats: granule k of the row's aligned granules, the
 // row's first element at place `lead` of granule 0.  Places outside the row are
@@ -701,7 +706,8 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
 // Row L + path[j] to row L + j for j < kept, in every cache.  path rises, so
 // path[j] >= j: a row is overwritten only after the only move that reads it (an
 // earlier j).  A thread moves the same 16 bytes of every row, in order of j, so
-// its own program order is all the ordering that needs.
+// its own program order is all the ordering that needs.  Bound by its launch: 32
+// layers of 16 sequences 3.8 us.
 struct KeepPtrs {
   char *k[KEEP_CACHES], *v[KEEP_CACHES];
   const int32_t* lens[KEEP_CACHES];
