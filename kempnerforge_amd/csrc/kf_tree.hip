@@ -503,7 +503,7 @@ struct Shape {
 template <typename T, int D, int RW, int BKW>
 __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stream_kernel(
     TreeArgs a, int W, float* __restrict__ opart, float* __restrict__ mlpart,
-    int* __restrict__ refusals, int tiles_max) {
+    int* __restrict__ refusals, int2* __restrict__ shares, int tiles_max) {
   using namespace mfma;
   using X = Tile<T, D>;
   using P = Piece<T>;
@@ -640,7 +640,10 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
     whole = cc.c == 0;
-    if (whole && cc.g == 0 && cc.t == 0 && threadIdx.x == 0) refusals[cc.b] = refused;
+    if (whole && threadIdx.x == 0) {
+      shares[(cc.b * a.Hkv + cc.g) * tiles_max + cc.t].x = gw;
+      if (cc.g == 0 && cc.t == 0) refusals[cc.b] = refused;
+    }
   };
   {
     // Loads return in order, so what the first tile needs is waited for before its
@@ -835,6 +838,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       // the row tile's part of this workgroup ends: the key waves' sums joined in
       // the stage just computed, then the output, or a partial in slot gw + tile
       whole = whole && last;
+      if (last && threadIdx.x == 0) shares[(cc.b * a.Hkv + cc.g) * tiles_max + cc.t].y = gw;
       float l = pair_sum32(lsum);
       if (refused) l = NAN;
       if (l != l) m = INFINITY;  // (a NaN must not be left out for its weight)
@@ -929,21 +933,17 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 template <typename T, int D, int JG>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
     TreeArgs a, const float* __restrict__ opart, const float* __restrict__ mlpart,
-    const int* __restrict__ refusals, int rows, int kc, int NWmax, int tiles_max) {
+    const int* __restrict__ refusals, const int2* __restrict__ shares, int rows, int tiles_max) {
   constexpr int LPR = D / 4, RPW = 256 / (LPR * JG);  // lanes of a row, rows of a workgroup
   __shared__ f32x4 xo[JG > 1 ? 256 : 1];
   __shared__ float2 xm[JG > 1 ? 256 : 1];
-  const int lane = threadIdx.x & 63, n_rep = a.Hq / a.Hkv;
+  const int n_rep = a.Hq / a.Hkv;
   const int item = blockIdx.x, t = item % tiles_max, bg = item / tiles_max, b = bg / a.Hkv,
             g = bg % a.Hkv;
   const int r = blockIdx.y * RPW + threadIdx.x / (LPR * JG), jg = threadIdx.x / LPR % JG;
   const int col = threadIdx.x % LPR * 4;
   const int row = t * rows + r, i = row / n_rep, hq = g * n_rep + row % n_rep;
   const int2 s = tree_seq(a, b);
-  const TreeSched sched(a, n_rep, rows, kc, NWmax, lane);
-  int pre = 0;
-  for (int b0 = lane; b0 < b; b0 += 64) pre += sched.chunks(b0);
-  pre = wave_sum_int(pre);
   const bool inside = i < a.N && r < rows;
   T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + hq) * D + col;
   T y[4];
@@ -953,13 +953,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(refused ? NAN : 0.f);
     __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
   }
-  int ns = 0, w0 = 0;
-  if (inside && i < s.x) {
-    const int nck = sched.nck(s);
-    const int c0 = pre + (g * sched.tiles(s) + t) * sched.per(s) + sched.over;
-    w0 = chunk_owner(c0, sched.C, sched.NW);
-    ns = chunk_owner(c0 + nck - 1, sched.C, sched.NW) - w0 + 1;
-  }
+  const int2 share = shares[item];  // (of a tile without rows: whatever was there)
+  const int w0 = share.x, ns = inside && i < s.x ? share.y - w0 + 1 : 0;
   const bool live = ns > 1;
   float M = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -1052,12 +1047,14 @@ Plan plan_of(const TreeArgs& a) {
   return p;
 }
 
-// workspace: the partials, and whether each sequence's tree or tables are refused
-// (written with its first chunk); or, one wavefront per row, rotated queries, ancestor
+// workspace: the partials, per row tile the first and last of the workgroups that met it
+// (each writes itself; formed again from the lengths by every workgroup of the merge
+// it cost that 3 us), whether each sequence's tree or tables are refused; or, one wavefront per row, rotated queries, ancestor
 // masks and per sequence (nodes in use or -1, prefix length)
 struct Ws {
   float *opart, *mlpart;
   int* refusals;
+  int2* shares;
   float* qrot;
   uint32_t* anc;
   int2* seq;
@@ -1074,6 +1071,8 @@ Ws carve(const TreeArgs& a, const Plan& pl, void* p) {
     c += up256(rows * 2 * 4);
     w.refusals = (int*)c;
     c += up256((size_t)a.B * 4);
+    w.shares = (int2*)c;
+    c += up256((size_t)a.B * a.Hkv * pl.tiles * sizeof(int2));
   } else {
     w.qrot = (float*)c;
     c += up256((size_t)a.B * a.N * a.Hq * a.D * 4);
@@ -1106,7 +1105,7 @@ int launch_stream(const TreeArgs& a, const Ws& w, const Plan& p) {
     }
   }
   KF_LAUNCH("tree_stream", kernel, dim3(p.grid), dim3(256), Sh::LDS, a.stream, a,
-            (a.N + 31) / 32, w.opart, w.mlpart, w.refusals, p.tiles);
+            (a.N + 31) / 32, w.opart, w.mlpart, w.refusals, w.shares, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
@@ -1133,7 +1132,7 @@ int stream_and_merge(const TreeArgs& a, const Ws& w, const Plan& p) {
              : jg == 2 ? tree_merge_kernel<T, D, 2>
                        : tree_merge_kernel<T, D, 1>),
             dim3(items, (p.rows + rpw - 1) / rpw), dim3(256), 0, a.stream, a, w.opart, w.mlpart,
-            w.refusals, p.rows, p.kc, p.grid, p.tiles);
+            w.refusals, w.shares, p.rows, p.tiles);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }
