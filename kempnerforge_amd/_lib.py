@@ -109,6 +109,10 @@ def native():
         spec = importlib.util.spec_from_file_location("kf_torch", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        lib = load()
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "kf_attn_tree_workspace_size", "kf_attn_tree", "kf_verify_drafts_workspace_size",
+            "kf_verify_drafts", "kf_kv_cache_keep")))
         _native = module
     return _native
 

@@ -498,6 +498,15 @@ def _on_device(index: int):
     return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
+def _here(t: torch.Tensor) -> tuple[int, int] | None:
+    """The current device and its stream for a call in its plain form (``csrc/kf_torch.cpp``);
+    None for a tensor that is not on a GPU."""
+    if not t.is_cuda:
+        return None
+    device = torch._C._cuda_getDevice()
+    return device, torch._C._cuda_getCurrentRawStream(device)
+
+
 def _one_device(*ts) -> int:
     """The one GPU that all tensors (None: absent) lie on."""
     dev = {t.get_device() for t in ts if t is not None}
@@ -550,6 +559,15 @@ def tree_decode_raw(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, *,
     As in :func:`decode_raw`, what lies on the device is checked there: a
     sequence whose length, count, parents or RoPE rows are out of range gets NaN
     outputs and no cache write."""
+    here = _here(q_new)
+    if here is not None:
+        out = _lib.native().tree(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, parents,
+                                 counts, q_norm_weight, k_norm_weight, norm_eps, rope_row_offset,
+                                 max_len, *here)
+        if isinstance(out, torch.Tensor):
+            return out
+        if out is not None:
+            _lib.check(out, "kf_attn_tree")
     lib = _lib.load()
     qs, ks, cs, dtype = q_new.shape, k_new.shape, k_cache.shape, q_new.dtype
     if len(qs) != 4 or len(ks) != 4 or len(cs) != 4:
@@ -625,6 +643,14 @@ def verify_drafts_raw(logits, tokens, uniforms, *, temperature: float = 1.0, par
     Unused sequences (``counts[b]`` 0) and counts or parents out of range give kept
     0 and next -1; a row on the path that is no distribution (NaN, +inf, all -inf)
     ends the path with next -1."""
+    here = _here(logits)
+    if here is not None:
+        out = _lib.native().verify(logits, tokens, uniforms, parents, counts, draft_logits,
+                                   temperature, *here)
+        if isinstance(out, tuple):
+            return out
+        if out is not None:
+            _lib.check(out, "kf_verify_drafts")
     lib = _lib.load()
     ls = logits.shape
     if len(ls) != 3 or (logits.stride(2) != 1 and ls[2] != 1):
@@ -688,6 +714,11 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
     k_caches, v_caches, lens = list(k_caches), list(v_caches), list(lens)
     lens_out = lens if lens_out is None else list(lens_out)
     n = len(k_caches)
+    here = _here(path)
+    if here is not None:
+        rc = _lib.native().keep(k_caches, v_caches, lens, lens_out, path, kept, *here)
+        if rc is not None:
+            return _lib.check(rc, "kf_kv_cache_keep")
     if n == 0 or not n == len(v_caches) == len(lens) == len(lens_out):
         raise ValueError("k_caches, v_caches, lens and lens_out need one tensor per cache "
                          f"(got {n}, {len(v_caches)}, {len(lens)}, {len(lens_out)})")

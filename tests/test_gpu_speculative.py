@@ -287,3 +287,84 @@ def test_steps_on_two_streams_at_once():
             assert all(torch.equal(x, y) for x, y in zip(a, b))
         for a, b in zip(steps[i].state(), want_steps[i].state()):
             assert torch.equal(a, b)
+
+
+def test_plain_and_other_forms_of_a_call_agree():
+    """Arguments that Python converts (other integer types, strided views, a tensor's
+    subclass, numbers as tensors) give the bits of the plain form."""
+    announce("speculative call forms")
+    s = _Step(3, 3, 11, 7, TREE, layers=1)
+    s2 = _Step(3, 3, 11, 7, TREE, layers=1)
+
+    class Sub(torch.Tensor):
+        pass
+
+    wide = torch.empty(3, 11, 8, 200, dtype=torch.bfloat16, device=DEV)
+    wide[..., :128] = s2.q[0]
+    kw = dict(rope_row_offset=0, max_len=400)
+    counts = torch.tensor([11, 4, 0], dtype=torch.int32, device=DEV)
+    a = ops.tree_decode_raw(s.q[0], s.k[0], s.k[0], s.kc[0], s.vc[0], s.lens[0], s.cos, s.sin,
+                            parents=s.parents, counts=counts, **kw)
+    b = ops.tree_decode_raw(wide[..., :128], s2.k[0].as_subclass(Sub), s2.k[0], s2.kc[0], s2.vc[0],
+                            s2.lens[0], s2.cos.double(), s2.sin, parents=s2.parents.long(),
+                            counts=counts.long(), rope_row_offset=0,
+                            max_len=torch.tensor(400))
+    assert torch.equal(a, b) and torch.equal(s.kc[0], s2.kc[0]) and torch.equal(s.vc[0], s2.vc[0])
+    logits = (a.flatten(2) @ s.head).float()
+    a = ops.verify_drafts_raw(logits, s.tokens, s.u, temperature=1.0, parents=s.parents,
+                              counts=counts)
+    b = ops.verify_drafts_raw(logits, s.tokens.int(), s.u.t().contiguous().t(), temperature=True,
+                              parents=s.parents.expand(3, 11), counts=counts.long())
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    lens = [torch.zeros(3, dtype=torch.int32, device=DEV) for _ in range(2)]
+    ops.cache_keep_raw(s.kc, s.vc, s.lens, a[0], a[1], lens_out=lens[:1])
+    ops.cache_keep_raw(tuple(s2.kc), s2.vc, s2.lens, a[0].t().contiguous().t(), a[1],
+                       lens_out=lens[1:])
+    assert torch.equal(*lens) and torch.equal(s.kc[0], s2.kc[0])
+
+
+def test_refusals_keep_their_errors_on_the_device():
+    """What the host's checks refuse (all before any launch), with tensors on the GPU."""
+    announce("speculative host refusals")
+    s = _Step(3, 3, 11, 7, None, layers=1)
+    args = [s.q[0], s.k[0], s.k[0], s.kc[0], s.vc[0], s.lens[0], s.cos, s.sin]
+    before = [t.clone() for t in s.state()]
+    for kw, kind in ((dict(max_len=401), RuntimeError), (dict(max_len=0), RuntimeError),
+                     (dict(max_len=400, parents=s.tokens), ValueError),
+                     (dict(max_len=400, counts=s.u[0]), TypeError),
+                     (dict(max_len=400, parents=torch.zeros(11).int()), RuntimeError),
+                     (dict(max_len=400, q_norm_weight=torch.ones(128, device=DEV)), ValueError)):
+        if "parents" in kw and kw["parents"] is s.tokens:
+            kw["parents"] = s.tokens[:, :5]
+        with pytest.raises(kind):
+            ops.tree_decode_raw(*args, rope_row_offset=0, **kw)
+    logits = torch.zeros(3, 11, 7, device=DEV)
+    for kw, kind in ((dict(temperature=-1.0), RuntimeError),
+                     (dict(temperature=float("nan")), RuntimeError),
+                     (dict(draft_logits=logits), ValueError),
+                     (dict(draft_logits=logits[:, 1:], temperature=0), ValueError)):
+        with pytest.raises(kind):
+            ops.verify_drafts_raw(logits, s.tokens, s.u, **kw)
+    path, kept = torch.zeros(3, 11, device=DEV).int(), torch.zeros(3, device=DEV).int()
+    for a in (([s.kc[0]], [s.kc[0]], s.lens, path, kept), (s.kc, s.vc, s.lens, path, kept.long()),
+              (s.kc * 2, s.vc * 2, s.lens * 2, path, kept), (s.kc, s.vc, [s.lens[0][:2]], path, kept)):
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            ops.cache_keep_raw(*a)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(s.state(), before))
+
+
+def test_a_draft_row_without_a_distribution_is_refused():
+    """Its token is refused and the next one drawn from the target's row."""
+    announce("verify bad draft rows")
+    B, N, V = 3, 4, 50
+    g = torch.Generator().manual_seed(0)
+    logits, u = torch.randn(B, N, V, generator=g), torch.rand(B, N, generator=g)
+    tokens = torch.randint(0, V, (B, N), generator=g)
+    drafts = torch.randn(B, N - 1, V, generator=g)
+    drafts[0, 0], drafts[1, 0], drafts[2, 0] = float("nan"), -float("inf"), float("inf")
+    dev = [t.to(DEV) for t in (logits, tokens, u)]
+    path, kept, token = ops.verify_drafts_raw(*dev, draft_logits=drafts.to(DEV))
+    one = ops.verify_drafts_raw(dev[0][:, :1], dev[1][:, :1].contiguous(),
+                                dev[2][:, :1].contiguous())
+    assert kept.tolist() == [1, 1, 1] and torch.equal(token, one[2])

@@ -10,7 +10,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from kempnerforge_amd import Attention, KVCache, begin_tree, keep_path, ops
+from kempnerforge_amd import Attention, KVCache, _lib, begin_tree, keep_path, ops
 from kempnerforge_amd.generate import generate, speculative_generate
 from oracle import spec_ref
 
@@ -212,3 +212,23 @@ def test_keep_path_without_the_lengths(oracle):
     keep_path(caches, z(2, 3).int(), torch.tensor([3, 1]))
     for c in caches:
         assert c.lens.tolist() == [7, 5] and c.seq_len == 7 and c.ragged and c.tree is None
+
+
+def test_native_calls_answer_only_their_plain_form():
+    """Tensors off the GPU, other objects and argument lists of another length are
+    left to Python; nothing is read from them."""
+    native = _lib.native()
+    tree = [Q, KV, KV, C, C, LENS, TAB, TAB, None, None, None, None, 1e-5, 0, 8, 0, 0]
+    verify = [LOG, TOK, U, None, None, None, 1.0, 0, 0]
+    keep = [[C], [C], [LENS], [LENS], PATH, KEPT, 0, 0]
+    for f, args in ((native.tree, tree), (native.verify, verify), (native.keep, keep)):
+        assert f(*args) is None and f() is None and f(*args, 0) is None
+        for i in range(len(args)):
+            for bad in (None, 3, 1 << 70, "x", [], [None], float("nan")):
+                assert f(*args[:i], bad, *args[i + 1:]) is None
+    with pytest.raises(TypeError):
+        native.bind(1)
+    with pytest.raises(ValueError):
+        native.bind(0, 0, 0, 0, 0)
+    with pytest.raises(TypeError):
+        native.bind("x", 0, 0, 0, 0)
