@@ -759,11 +759,15 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
     auto unclean = [&](int nb) -> uint32_t {
       return __builtin_amdgcn_readfirstlane(sbad[(kw * BKW + 32 * nb) / 32]);
     };
-    // (a wavefront of which the tile has no rows leaves the SIMD to the others)
-    const bool active = cc.t * ROWS + 32 * rw < cc.s.x * n_rep;
+    // The blocks of 32 keys that the wavefront's last row sees (no node sees one behind
+    // it; a chain of 200 for 4 sequences: 58.3 us with all of them, 57.1 without); a
+    // wavefront of which the tile has no rows leaves the SIMD to the others.
+    const int blocks = cc.t * ROWS + 32 * rw < cc.s.x * n_rep
+                           ? (__builtin_amdgcn_readlane(node, 31) + L - k0 + 32) >> 5
+                           : 0;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {  // 32 keys at a time
-      if (!active) break;
+      if (nb >= blocks) break;
       const int row0 = kw * BKW + 32 * nb;
       const int t0 = k0 + 32 * nb - L;
       f32x16 s;
