@@ -282,6 +282,7 @@ struct TreeSched {
   int over, C, NW;  // units of the list, workgroups that share it
   static constexpr int OVER = 2;
   int B;
+  int2 own{-1, 0};  // sequence `lane`'s tree_seq, all there are up to 64 of them
   __device__ __forceinline__ TreeSched(const TreeArgs& a_, int n_rep_, int rows_, int kc_,
                                        int grid, int lane)
       : a(a_), n_rep(n_rep_), rows(rows_), kc(kc_), B(a_.B) {
@@ -291,6 +292,7 @@ struct TreeSched {
       const int i = s.x > 0 ? a.Hkv * tiles(s) : 0;
       items += i;
       tot += i > 0 ? i * nck(s) : 0;
+      own = s;
     }
     tot = wave_sum_int(tot);
     items = wave_sum_int(items);
@@ -301,8 +303,9 @@ struct TreeSched {
   __device__ __forceinline__ int nck(int2 s) const { return (s.x + s.y + kc - 1) / kc; }
   __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
   __device__ __forceinline__ int per(int2 s) const { return nck(s) + over; }
+  // (locate_chunk asks lane by lane: up to 64 sequences without another load)
   __device__ __forceinline__ int chunks(int b) const {
-    const int2 s = tree_seq(a, b);
+    const int2 s = B <= 64 ? own : tree_seq(a, b);
     return s.x > 0 ? a.Hkv * tiles(s) * per(s) : 0;
   }
 };
@@ -312,9 +315,9 @@ struct TreeSched {
 struct TreeCursor {
   int b, g, t, c, u, nck, tiles;
   int2 s;
-  __device__ __forceinline__ void at(const TreeSched& sched, int b_) {
+  __device__ __forceinline__ void at(const TreeSched& sched, int b_, int2 s_) {
     b = b_;
-    s = tree_seq(sched.a, b);
+    s = s_;
     s.x = __builtin_amdgcn_readfirstlane(s.x);
     s.y = __builtin_amdgcn_readfirstlane(s.y);
     nck = sched.nck(s);
@@ -324,7 +327,8 @@ struct TreeCursor {
   __device__ __forceinline__ void seek(const TreeSched& sched, int unit, int lane) {
     int sb, base;
     locate_chunk(sched, unit, lane, sb, base);
-    at(sched, sb);
+    at(sched, sb, sched.B <= 64 ? make_int2(__shfl(sched.own.x, sb, 64), __shfl(sched.own.y, sb, 64))
+                                : tree_seq(sched.a, sb));
     const int per = nck + sched.over, item = (unit - base) / per;
     c = max(unit - base - item * per - sched.over, 0);
     u = base + item * per + sched.over + c;
@@ -341,8 +345,9 @@ struct TreeCursor {
     if (++g < sched.a.Hkv) return;
     g = 0;
     for (int nb = b + 1; nb < sched.B; ++nb) {
-      if (tree_seq(sched.a, nb).x > 0) {
-        at(sched, nb);
+      const int2 sn = tree_seq(sched.a, nb);
+      if (sn.x > 0) {
+        at(sched, nb, sn);
         return;
       }
     }
@@ -493,7 +498,7 @@ struct Shape {
   static constexpr int KW = 4 / RW, ROWS = 32 * RW, KC = BKW * KW;
   static constexpr int TILE = KC * D;                  // elements of a K (or V) tile
   static constexpr size_t STAGE = 2 * TILE * sizeof(T);
-  static constexpr size_t LDS = 2 * STAGE + (KW - 1) * ROWS * 2 * sizeof(float);
+  static constexpr size_t LDS = 2 * STAGE + (KW > 1 ? KW : 0) * ROWS * 2 * sizeof(float);
   // (float32 rows of 128: q, the sums and a block's scores leave no room for two
   // wavefronts per SIMD)
   static constexpr int PER_CU = LDS * 2 <= 160 * 1024 && D * sizeof(T) <= 256 ? 2 : 1;
@@ -846,47 +851,63 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
       float l = pair_sum32(lsum);
       if (refused) l = NAN;
       if (l != l) m = INFINITY;  // (a NaN must not be left out for its weight)
+      // The key waves share the join out by blocks of 32 dims: block dt is wave
+      // owner(dt)'s, the others leave theirs in LDS (one wave joining all of them: 5
+      // nodes over 1000 keys 15.8 us, shared out 14.6).
+      auto owner = [](int dt) { return dt * KW / DT; };
       if constexpr (KW > 1) {
         __syncthreads();  // all wavefronts are done with the stage
         float* xo = (float*)kt;                    // [KW - 1][ROWS][D]
-        float* xm = (float*)(lds + 2 * Sh::STAGE);  // [KW - 1][ROWS][2]
+        float* xm = (float*)(lds + 2 * Sh::STAGE);  // [KW][ROWS][2]
         const int r = 32 * rw + l31;
-        if (kw > 0) {
-          float* o = xo + ((kw - 1) * ROWS + r) * D + 4 * h;
+        // place of a piece of wave j's block dt (a lane's pieces rotated by its row: the
+        // rows lie D floats apart)
+        auto piece = [&](int j, int dt, int e) {
+          const int slot = j < owner(dt) ? j : j - 1;
+          return (f32x4*)(xo + (slot * ROWS + r) * D + 4 * h +
+                          (((8 * dt + 2 * (e / 4)) ^ (2 * (r & 3))) * 4));
+        };
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
+          if (owner(dt) != kw)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              // (a lane's pieces rotated by its row: the rows lie D floats apart)
-              const int ch = ((8 * dt + 2 * (e / 4)) ^ (2 * (r & 3))) * 4;
-              *(f32x4*)(o + ch) = f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
-            }
-          if (h == 0) *(float2*)(xm + ((kw - 1) * ROWS + r) * 2) = make_float2(m, l);
-        }
+            for (int e = 0; e < 16; e += 4)
+              *piece(kw, dt, e) = f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
+        if (h == 0) *(float2*)(xm + (kw * ROWS + r) * 2) = make_float2(m, l);
         __syncthreads();
-        if (kw == 0) {
+        float2 ml[KW];
+        float mj = -INFINITY;
 #pragma unroll
-          for (int x = 0; x < KW - 1; ++x) {
-            const float2 ml = *(const float2*)(xm + (x * ROWS + r) * 2);
-            const float mj = fmaxf(m, ml.x), rj = mj == -INFINITY ? 0.f : mj;
-            const float f0 = fast_exp2(m - rj), f1 = fast_exp2(ml.x - rj);
-            m = mj;
-            l = l * f0 + ml.y * f1;
-            const float* o = xo + (x * ROWS + r) * D + 4 * h;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-              for (int e = 0; e < 16; e += 4) {
-                const int ch = ((8 * dt + 2 * (e / 4)) ^ (2 * (r & 3))) * 4;
-                const f32x4 y = *(const f32x4*)(o + ch);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[dt][e + j] = acc[dt][e + j] * f0 + y[j] * f1;
-              }
-          }
+        for (int j = 0; j < KW; ++j) {
+          ml[j] = *(const float2*)(xm + (j * ROWS + r) * 2);
+          mj = fmaxf(mj, ml[j].x);
         }
+        const float rj = mj == -INFINITY ? 0.f : mj;
+        const float own = fast_exp2(m - rj);
+        m = mj;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+          ml[j].x = fast_exp2(ml[j].x - rj);
+          l += ml[j].y * ml[j].x;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          if (owner(dt) == kw) {
+            acc[dt] *= own;
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+              if (j != owner(dt))
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                  const f32x4 y = *piece(j, dt, e);
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) acc[dt][e + x] += y[x] * ml[j].x;
+                }
+          }
       }
       const int r = cc.t * ROWS + 32 * rw + l31;
-      if (kw == 0 && r < cc.s.x * n_rep) {
+      if (r < cc.s.x * n_rep) {
         if (whole) {
           const float inv = 1.f / l;
           T* o = (T*)a.out + (((int64_t)cc.b * N + r / n_rep) * a.Hq + cc.g * n_rep + r % n_rep) * D +
@@ -894,7 +915,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
+            for (int e = 0; e < 16 && owner(dt) == kw; e += 4) {
               T y[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) y[j] = from_f32<T>(acc[dt][e + j] * inv);
@@ -907,10 +928,10 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
+            for (int e = 0; e < 16 && owner(dt) == kw; e += 4)
               *(f32x4*)(o + 32 * dt + 2 * e) =
                   f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
-          if (h == 0)
+          if (h == 0 && kw == 0)
             *(float2*)(mlpart + (slot * ROWS + 32 * rw + l31) * 2) = make_float2(m, l);
         }
       }
@@ -1043,7 +1064,7 @@ Plan plan_of(const TreeArgs& a) {
   p.kc = p.bkw * 4 / p.rw;
   p.tiles = (m + p.rows - 1) / p.rows;
   const size_t lds = (size_t)4 * p.kc * a.D * (a.dtype == F32 ? 4 : 2) +
-                     (size_t)(4 / p.rw - 1) * p.rows * 8;  // Shape::LDS
+                     (p.rw < 4 ? (size_t)(4 / p.rw) * p.rows * 8 : 0);  // Shape::LDS
   p.per_cu = 2 * lds <= 160 * 1024 && !(a.dtype == F32 && a.D == 128) ? 2 : 1;  // Shape::PER_CU
   const int64_t chunks = (int64_t)a.B * a.Hkv * p.tiles * ((a.max_len + p.kc - 1) / p.kc);
   if (chunks + (int64_t)a.B * a.Hkv * p.tiles * TreeSched::OVER >= INT_MAX) return Plan{};
