@@ -276,6 +276,19 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const float*
 // Beginning a row tile costs about as much as OVER chunks (its queries are loaded
 // and rotated, the tree formed), so with several chunks per workgroup each tile
 // has `over` units in front of its chunks in the list that is shared out.
+// Inclusive prefix sums over the wavefront, by data parallel primitives (a shuffle
+// goes through the LDS, six of them cost 0.3 us): within rows of 16 lanes, then lane
+// 15 of rows 0 and 2 into the next row, then lane 31 into rows 2 and 3.
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
 struct TreeSched {
   const TreeArgs& a;
   int n_rep, rows, kc;
@@ -294,20 +307,24 @@ struct TreeSched {
       tot += i > 0 ? i * nck(s) : 0;
       own = s;
     }
-    tot = wave_sum_int(tot);
-    items = wave_sum_int(items);
+    tot = __builtin_amdgcn_readlane(wave_prefix(tot), 63);
+    items = __builtin_amdgcn_readlane(wave_prefix(items), 63);
     over = tot >= 4 * grid ? OVER : 0;
     C = tot + over * items;
     NW = min(grid, C);
   }
+  // the first unit of workgroup w's share, floor(w C / NW) (w and NW are far below 2^16)
+  __device__ __forceinline__ int start(int w) const {
+    const unsigned n = max(NW, 1), q = (unsigned)C / n, r = (unsigned)C % n;
+    return (int)(w * q + (unsigned)w * r / n);
+  }
   __device__ __forceinline__ int nck(int2 s) const { return (s.x + s.y + kc - 1) / kc; }
   __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
   __device__ __forceinline__ int per(int2 s) const { return nck(s) + over; }
-  // (locate_chunk asks lane by lane: up to 64 sequences without another load)
-  __device__ __forceinline__ int chunks(int b) const {
-    const int2 s = B <= 64 ? own : tree_seq(a, b);
+  __device__ __forceinline__ int units(int2 s) const {
     return s.x > 0 ? a.Hkv * tiles(s) * per(s) : 0;
   }
+  __device__ __forceinline__ int chunks(int b) const { return units(tree_seq(a, b)); }
 };
 
 // Place in the list: sequence b (s: its nodes in use and prefix length), KV head
@@ -326,9 +343,16 @@ struct TreeCursor {
   // the first chunk at or behind a unit
   __device__ __forceinline__ void seek(const TreeSched& sched, int unit, int lane) {
     int sb, base;
-    locate_chunk(sched, unit, lane, sb, base);
-    at(sched, sb, sched.B <= 64 ? make_int2(__shfl(sched.own.x, sb, 64), __shfl(sched.own.y, sb, 64))
-                                : tree_seq(sched.a, sb));
+    if (sched.B <= 64) {  // a lane a sequence, without another load
+      const int n = sched.units(sched.own), end = wave_prefix(n);
+      sb = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end - n <= unit && unit < end) | 1ull << 63);
+      base = __builtin_amdgcn_readlane(end - n, sb);
+      at(sched, sb, make_int2(__builtin_amdgcn_readlane(sched.own.x, sb),
+                              __builtin_amdgcn_readlane(sched.own.y, sb)));
+    } else {
+      locate_chunk(sched, unit, lane, sb, base);
+      at(sched, sb, tree_seq(sched.a, sb));
+    }
     const int per = nck + sched.over, item = (unit - base) / per;
     c = max(unit - base - item * per - sched.over, 0);
     u = base + item * per + sched.over + c;
@@ -522,14 +546,14 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   const int rw = w % RW, kw = w / RW;
   const int N = a.N, n_rep = a.Hq / a.Hkv;
   const TreeSched sched(a, n_rep, ROWS, KC, gridDim.x, lane);
-  const int C = sched.C, NW = sched.NW;
+  const int NW = sched.NW;
   // block ids go round the 8 XCDs: neighbours in the chunk list, which read the
   // same keys for other rows, share one XCD's L2
   if ((int)blockIdx.x >= NW) return;
   const int xcd = blockIdx.x % 8, gw = xcd * (NW / 8) + min(xcd, NW % 8) + (int)blockIdx.x / 8;
-  const int u_hi = range_start(gw + 1, C, NW);
+  const int u_hi = sched.start(gw + 1);
   TreeCursor cc;
-  cc.seek(sched, range_start(gw, C, NW), lane);
+  cc.seek(sched, sched.start(gw), lane);
   if (cc.u >= u_hi) return;  // (a share of nothing but a tile's beginning)
 
   auto stage_k = [&](int i) { return (T*)(lds + (i & 1) * Sh::STAGE); };
