@@ -91,17 +91,19 @@ struct TreeLds {
   int ptr[MAXN], depth[MAXN];
 };
 
-// Forms the tree of a sequence (s: its nodes and prefix; par: thread t's node's
-// parent, from tree_parent), by a workgroup of 256; returns whether the sequence is
+// Forms the tree of a sequence (s: its nodes and prefix; par: the parent of the node that
+// tree_parent gives the thread), by a workgroup of 256; returns whether the sequence is
 // refused.  A chain needs no LDS: node i sees
 // nodes 0 .. i and lies at depth i.
 //
 // The masks come from pointer doubling: after round r, mask[i] holds the 2^r
 // nearest of i and its ancestors and ptr[i] the next one beyond, so 8 rounds
 // cover 256 nodes whatever their depth (a walk up a chain of 200 would take 200
-// dependent reads).
+// dependent reads).  Up to 64 nodes every wavefront forms them all by itself, a lane a
+// node, by shuffles and as many rounds as the depth needs (27 nodes: 1.3 us where the rounds
+// with barriers take 2.7).
 __device__ __forceinline__ int tree_parent(const TreeArgs& a, int b, int2 s) {
-  const int t = threadIdx.x;
+  const int t = a.N <= 64 ? threadIdx.x & 63 : threadIdx.x;
   return a.parents != nullptr && t < s.x ? a.parents[(int64_t)b * a.parents_stride + t] : -1;
 }
 __device__ __forceinline__ bool tree_build(const TreeArgs& a, int2 s, int W, TreeLds& lds,
@@ -111,6 +113,33 @@ __device__ __forceinline__ bool tree_build(const TreeArgs& a, int2 s, int W, Tre
     return s.x < 0 || (s.x > 0 && (low < 0 || low + s.x > a.rope_rows));
   const int t = threadIdx.x, used = max(s.x, 0);
   bool bad = s.x < 0;
+  if (a.N <= 64) {
+    const int lane = t & 63;
+    if (par < -1 || par >= lane) {
+      bad = true;
+      par = -1;
+    }
+    uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+    while (__builtin_amdgcn_ballot_w64(par >= 0)) {  // (parents come first: it ends)
+      const int from = max(par, 0), next = __shfl(par, from, 64);
+      const uint32_t l = __shfl(lo, from, 64), h = __shfl(hi, from, 64);
+      if (par >= 0) {
+        lo |= l;
+        hi |= h;
+        par = next;
+      }
+    }
+    const int depth = __popc(lo) + __popc(hi) - 1;
+    bad |= lane < used && (low + depth < 0 || low + depth >= a.rope_rows);
+    __syncthreads();  // the previous tree's readers are done
+    if (t < 64) {
+      lds.mask[t][0] = lo;
+      lds.mask[t][1] = hi;
+      lds.depth[t] = depth;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
+  }
   if (par < -1 || par >= t) {
     bad = true;
     par = -1;
