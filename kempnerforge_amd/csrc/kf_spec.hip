@@ -39,8 +39,8 @@ constexpr int MAXN = KF_TREE_MAX_NODES;
 // all workgroups of a sequence, a slice of the row each, and the last one to
 // arrive picks the token.
 //
-// Measured: a chain of 5 with drafts over 32000 float32 values 18 us (4 of sums, 12 of
-// ten dependent round trips); 16 trees of 64 nodes over 131072 16-bit values 42 to 50
+// Measured: a chain of 5 with drafts over 32000 float32 values 15 us (4 of sums, 11 of
+// ten dependent round trips); 16 trees of 64 nodes over 131072 16-bit values 41 to 54
 // us (268 MB of logits: 5.4 TB/s and more where they lie in the last-level cache, then
 // 19 us of walk and draw).
 

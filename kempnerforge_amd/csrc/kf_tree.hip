@@ -24,13 +24,13 @@
 // half as many more products.  P is rounded to the input type before it
 // multiplies V; the sums, the row maxima and the row sums stay in 32 bits.  Against
 // 64 bits that is an error of 1.4 times what rounding the outputs costs; with q
-// rounded to 16 bits it would be 1.7 times (and 163 us instead of 214 below).
+// rounded to 16 bits it would be 1.7 times (and 163 us instead of 213 below).
 //
 // What bounds it, in bfloat16 with heads of 128: the matrix instructions for wide
-// trees (4 sequences, 64 nodes, 16384 keys, 64 / 8 heads: 214 us, 966 TFLOP/s with
+// trees (4 sequences, 64 nodes, 16384 keys, 64 / 8 heads: 213 us, 970 TFLOP/s with
 // the lo products), HBM for narrow ones (32 sequences of up to 8192 keys, 16 nodes,
-// 32 / 8 heads: 145 us, 4.9 TB/s), dependent loads for single ones (5 nodes, 1000
-// keys: 17 us in two launches, 20 with a launch for the rotation in front).
+// 32 / 8 heads: 135 us, 5.3 TB/s), dependent loads for single ones (5 nodes, 1000
+// keys: 13.7 us in two launches; a launch for the rotation in front costs 2.8 more).
 #include "kf_common.h"
 #include "kf_internal.h"
 #include "kf_mfma.h"
