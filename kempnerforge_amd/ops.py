@@ -598,7 +598,8 @@ def tree_decode_raw(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, *,
     if (q_norm_weight is None) != (k_norm_weight is None):
         raise ValueError("QK-norm needs both q_norm_weight and k_norm_weight")
     qnw = knw = None
-    dt, max_len = _dtype_code(q_new), int(max_len)
+    # (a C int: what is out of its range must not come back into the cache's)
+    dt, max_len = _dtype_code(q_new), max(min(int(max_len), Smax + 1), 0)
     with _on_device(dev):
         if q_norm_weight is not None:
             qnw, knw = (_norm_weight(w, D, q_new.device) for w in (q_norm_weight, k_norm_weight))

@@ -330,6 +330,8 @@ def test_refusals_keep_their_errors_on_the_device():
     args = [s.q[0], s.k[0], s.k[0], s.kc[0], s.vc[0], s.lens[0], s.cos, s.sin]
     before = [t.clone() for t in s.state()]
     for kw, kind in ((dict(max_len=401), RuntimeError), (dict(max_len=0), RuntimeError),
+                     (dict(max_len=(1 << 32) + 8), RuntimeError),
+                     (dict(max_len=8 - (1 << 32)), RuntimeError),
                      (dict(max_len=400, parents=s.tokens), ValueError),
                      (dict(max_len=400, counts=s.u[0]), TypeError),
                      (dict(max_len=400, parents=torch.zeros(11).int()), RuntimeError),
