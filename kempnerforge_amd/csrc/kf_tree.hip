@@ -1110,8 +1110,12 @@ Plan plan_of(const TreeArgs& a) {
   // Enough row waves for the pair's rows, up to four: finer tiles have fewer rows to
   // spare, but load the keys more often (800 rows of 4 x 8 heads over 1224 keys: 73 us
   // with 128 rows a tile, 84 with 64, 125 with 32; 135 rows 36, 39, 38; 36 rows the
-  // other way, 40.9 and 39.5).  float32 has no LDS for four key waves.
-  p.rw = m <= 32 && a.dtype != F32 ? 1 : m <= 64 ? 2 : 4;
+  // other way, 40.9 and 39.5).  float32, which has no LDS for four key waves, is bound
+  // by its products: two row waves where they need five sixths of four's row waves or
+  // fewer (30 x 2 heads, 2121 keys, 145 rows, 6 to 8: 157 us with two, 170 with four; 4 x
+  // 8 heads, 1224 keys, 400 rows, 14 to 16: 133 and 126).
+  const int two = 2 * ((m + 63) / 64), four = 4 * ((m + 127) / 128);
+  p.rw = a.dtype == F32 ? (6 * two <= 5 * four ? 2 : 4) : m <= 32 ? 1 : m <= 64 ? 2 : 4;
   p.bkw = p.rw == 4 && a.dtype != F32 ? 64 : 32;
   p.rows = 32 * p.rw;
   p.kc = p.bkw * 4 / p.rw;

@@ -77,6 +77,9 @@ CASES = [
     (F32, (2, 9, 4, 2, 64), [250, 31], "binary", None),
     (F32, (2, 20, 8, 2, 128), [128, 300], "random", [20, 3]),
     (F32, (1, 70, 8, 1, 128), [65], "random", None),
+    (F32, (2, 29, 10, 2, 128), [210, 64], "binary", [29, 5]),  # 145 rows: three tiles of 64
+    (F32, (2, 33, 8, 2, 64), [99, 1], "random", None),         # 132 rows
+    (F32, (1, 100, 8, 2, 128), [33], "random", None),          # 400 rows: tiles of 128
     (BF, (2, 6, 32, 1, 128), [70, 9], "binary", None),       # 32 heads a group
     (BF, (2, 6, 6, 2, 96), [70, 9], "binary", None),         # other head sizes
     (FH, (1, 11, 4, 4, 80), [90], "random", None),
