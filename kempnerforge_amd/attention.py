@@ -179,6 +179,8 @@ def keep_path(caches, path: torch.Tensor, kept: torch.Tensor, lengths=None) -> N
     ``ops.verify_drafts_raw`` returns) become the caches' next rows, in all layers
     in one launch.  ``lengths``: the fill levels after it, a list of ints, where the
     caller knows them; otherwise they are read back (one host synchronisation)."""
+    if lengths is not None and len(lengths) != path.shape[0]:
+        raise ValueError(f"need {path.shape[0]} lengths (got {len(lengths)})")
     ops.cache_keep_raw([c.k for c in caches], [c.v for c in caches], [c.lens for c in caches],
                        path, kept)
     if lengths is None:
@@ -245,7 +247,7 @@ class Attention(nn.Module):
         k = self.k_proj(x).view(batch, seq_len, -1, self.head_dim)
         v = self.v_proj(x).view(batch, seq_len, -1, self.head_dim)
         masked = doc_ids is not None or key_padding_mask is not None
-        tree = kv_cache.tree if kv_cache is not None else None
+        tree = getattr(kv_cache, "tree", None)  # (no cache, or a caller's own kind: none)
         if tree is not None and (masked or self.capture_attention_weights):
             raise ValueError("a tree of drafts takes no doc_ids, no key_padding_mask and no capture")
         decode = (kv_cache is not None and seq_len == 1 and not masked

@@ -212,6 +212,8 @@ def test_keep_path_without_the_lengths(oracle):
     keep_path(caches, z(2, 3).int(), torch.tensor([3, 1]))
     for c in caches:
         assert c.lens.tolist() == [7, 5] and c.seq_len == 7 and c.ragged and c.tree is None
+    with pytest.raises(ValueError, match="lengths"):
+        keep_path(caches, z(2, 3).int(), torch.tensor([3, 1]), [7])
 
 
 def test_native_calls_answer_only_their_plain_form():
