@@ -297,14 +297,6 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeArgs a, const float*
     if (lane + 64 * e < D) out[lane + 64 * e] = from_f32<T>(acc[e] / l);
 }
 
-// ---- split-K attention on the matrix cores -------------------------------------
-// Row tile t of pair (b, g) holds rows t ROWS .. of the pair's n_b n_rep rows
-// (node-major: the heads of a node side by side); every tile meets the nck(b) =
-// ceil((lens[b] + n_b) / KC) key chunks of its pair.
-//
-// Beginning a row tile costs about as much as OVER chunks (its queries are loaded
-// and rotated, the tree formed), so with several chunks per workgroup each tile
-// has `over` units in front of its chunks in the list that is shared out.
 // Inclusive prefix sums over the wavefront, by data parallel primitives (a shuffle
 // goes through the LDS, six of them cost 0.3 us): within rows of 16 lanes, then lane
 // 15 of rows 0 and 2 into the next row, then lane 31 into rows 2 and 3.
@@ -318,6 +310,17 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return x;
 }
 
+// ---- split-K attention on the matrix cores -------------------------------------
+// Row tile t of pair (b, g) holds rows t ROWS .. of the pair's n_b n_rep rows
+// (node-major: the heads of a node side by side); every tile meets the nck(b) =
+// ceil((lens[b] + n_b) / KC) key chunks of its pair.
+//
+// Beginning a row tile costs about as much as OVER chunks (its queries are loaded
+// and rotated, the tree formed), so with several chunks per workgroup each tile
+// has `over` units in front of its chunks in the list that is shared out: OVER, or
+// one where that spares the largest share a unit (8 x 8 heads, 4000 keys, 80 rows: 8
+// units for 9, 43.3 -> 40.6 us; 4 x 8 heads, 1224 keys, 800 rows, 11 units with two or
+// one: 61 and 64).
 struct TreeSched {
   const TreeArgs& a;
   int n_rep, rows, kc;
@@ -339,6 +342,9 @@ struct TreeSched {
     tot = __builtin_amdgcn_readlane(wave_prefix(tot), 63);
     items = __builtin_amdgcn_readlane(wave_prefix(items), 63);
     over = tot >= 4 * grid ? OVER : 0;
+    const unsigned one = (unsigned)(tot + items + grid - 1) / (unsigned)grid,
+                   two = (unsigned)(tot + OVER * items + grid - 1) / (unsigned)grid;
+    if (over && one < two) over = 1;
     C = tot + over * items;
     NW = min(grid, C);
   }
