@@ -342,8 +342,8 @@ struct TreeSched {
     tot = __builtin_amdgcn_readlane(wave_prefix(tot), 63);
     items = __builtin_amdgcn_readlane(wave_prefix(items), 63);
     over = tot >= 4 * grid ? OVER : 0;
-    const unsigned one = (unsigned)(tot + items + grid - 1) / (unsigned)grid,
-                   two = (unsigned)(tot + OVER * items + grid - 1) / (unsigned)grid;
+    const unsigned n = grid, chunks = tot, one = (chunks + items + n - 1) / n,
+                   two = (chunks + OVER * items + n - 1) / n;
     if (over && one < two) over = 1;
     C = tot + over * items;
     NW = min(grid, C);
