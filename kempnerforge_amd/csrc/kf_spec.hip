@@ -541,10 +541,14 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
       for (int e = 0; e < E; ++e)
         wt[e] = fmax(wt[e] - exp2_64(((double)f[e] - (double)dst.m) * c) * rq, 0.0);
     } else if (!drafted) {  // (a refused child of probability 0 changes nothing)
-      for (int i = 0; i < nref; ++i)
+      for (int i = 0; i < nref; ++i) {
+        const int at = refused[i] - v0;  // (hardly ever in the granule)
+        if (at >= 0 && at < E) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (refused[i] == v0 + e) wt[e] = 0.0;
+          for (int e = 0; e < E; ++e)
+            if (at == e) wt[e] = 0.0;
+        }
+      }
     }
   };
   // the sums of a slice's segments, to seg[0 .. DSEG)
