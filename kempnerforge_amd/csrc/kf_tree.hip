@@ -18,19 +18,20 @@
 // the nodes' cache rows), then one wavefront per row (rows).
 //
 // Rounding: the norm and the rotation of q and k are formed in 32 bits.  k is
-// rounded once, where it is stored.  q is not rounded to 16 bits: it goes
-// through the 16-bit matrix instructions as the sum of two numbers of the input
-// type (hi = q rounded, lo = q - hi rounded), which keeps 16 of its bits for
-// half as many more products.  P is rounded to the input type before it
-// multiplies V; the sums, the row maxima and the row sums stay in 32 bits.  Against
-// 64 bits that is an error of 1.4 times what rounding the outputs costs; with q
-// rounded to 16 bits it would be 1.7 times (and 163 us instead of 213 below).
+// rounded once, where it is stored.  What goes through the 16-bit matrix
+// instructions is not rounded to 16 bits: q and P enter as sums of two numbers of the
+// input type (hi = x rounded, lo = x - hi rounded: 16 bits in bfloat16, 22 in float16),
+// for twice the products; the sums, the row maxima and the row sums stay in 32 bits.
+// Against 64 bits that leaves the error of rounding the outputs and no more.  With P
+// alone rounded to the type it would be 1.2 to 1.4 times (and 220 us instead of 266
+// below), with q too 1.7 times (and 163 us).
 //
 // What bounds it, in bfloat16 with heads of 128: the matrix instructions for wide
-// trees (4 sequences, 64 nodes, 16384 keys, 64 / 8 heads: 213 us, 970 TFLOP/s with
+// trees (4 sequences, 64 nodes, 16384 keys, 64 / 8 heads: 266 us, 1030 TFLOP/s with
 // the lo products), HBM for narrow ones (32 sequences of up to 8192 keys, 16 nodes,
-// 32 / 8 heads: 135 us, 5.3 TB/s), dependent loads for single ones (5 nodes, 1000
-// keys: 13.7 us in two launches; a launch for the rotation in front costs 2.8 more).
+// 32 / 8 heads: 133 to 141 us, 5.0 to 5.3 TB/s), dependent loads for single ones (5
+// nodes, 1000 keys: 13.7 us in two launches; a launch for the rotation in front costs
+// 2.8 more).
 #include "kf_common.h"
 #include "kf_internal.h"
 #include "kf_mfma.h"
@@ -418,7 +419,9 @@ struct TreeCursor {
 //   S^T (keys x rows) += K q^T: lane l supplies row l % 32 of both operands, dims
 //       of its half h = l / 32 in 16-byte pieces
 //   O^T (dims x rows) += V^T P^T: P^T straight from the S registers (lane l holds
-//       row l % 32, register i key 8 (i / 4) + 4 h + i % 4)
+//       row l % 32, register i key 8 (i / 4) + 4 h + i % 4), hi and lo one after the
+//       other on each V fragment: 16 keys at a time, so that those of the other 16 hold
+//       no registers
 // Every fragment is read PF steps ahead of its products: left to itself the
 // compiler, short of registers, reads each one right before them and waits out
 // the LDS (512 rows over 16384 keys, 4 x 8 KV heads of 128: 232 us, read ahead 218).
@@ -428,7 +431,7 @@ struct Tile {
   static constexpr int KS = D / 16;   // pieces of a lane's half row
   static constexpr int QP = 2;        // q as hi and lo
   static constexpr int PF = D == 128 ? 2 : 4;  // (what the registers hold)
-  static constexpr int NV = D / 16;            // V fragments: 2 of 16 keys for each 32 dims
+  static constexpr int DT = D / 32, NV = 2 * DT;  // V fragments: 16 keys of 32 dims
   // lds_frag_t's offsets: block dt's are the first block's with bits 6.. flipped by
   // dt (a swizzled chunk index is 4 dt ^ ...), which saves the registers of the others
   struct VOff {
@@ -470,25 +473,35 @@ struct Tile {
   static __device__ __forceinline__ void load_v(const T* v, int row0, const VOff& off, VFrag& f,
                                                 int) {
 #pragma unroll
-    for (int i = 0; i < PF; ++i) f[i] = v_frag(v, row0, off, i & 1, i >> 1);
+    for (int i = 0; i < PF; ++i) f[i] = v_frag(v, row0, off, i / DT, i % DT);
     __builtin_amdgcn_sched_barrier(0);
+  }
+  // x and y as sums hi + lo of two numbers of the type
+  static __device__ __forceinline__ uint2 split2(float x, float y) {
+    const uint32_t hi = pack2<T>(x, y);
+    float a, b;
+    unpack2<T>(hi, a, b);
+    return make_uint2(hi, pack2<T>(x - a, y - b));
   }
   static __device__ __forceinline__ void values(const T* v, int row0, const VOff& off,
                                                 const f32x16& p, VFrag& f, f32x16* acc, int) {
     using namespace mfma;
-    bf16x8 pb[2];
+    u32x4 hi, lo;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x[8];
+    for (int i = 0; i < NV; ++i) {  // keys 16 (i / DT) .., dims 32 (i % DT) ..
+      if (i % DT == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = p[8 * c + j];
-      pb[c] = as_bf16x8(pack8<T>(x));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {  // dims 32 (i / 2) .., keys 16 (i % 2) ..
-      acc[i >> 1] = mfma32<T>(f[i % PF], pb[i & 1], acc[i >> 1]);
-      if (i + PF < NV) f[i % PF] = v_frag(v, row0, off, (i + PF) & 1, (i + PF) >> 1);
+        for (int j = 0; j < 4; ++j) {
+          const int e = 8 * (i / DT) + 2 * j;
+          const uint2 u = split2(p[e], p[e + 1]);
+          hi[j] = u.x;
+          lo[j] = u.y;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      acc[i % DT] = mfma32<T>(f[i % PF], as_bf16x8(hi), acc[i % DT]);
+      acc[i % DT] = mfma32<T>(f[i % PF], as_bf16x8(lo), acc[i % DT]);
+      if (i + PF < NV) f[i % PF] = v_frag(v, row0, off, (i + PF) / DT, (i + PF) % DT);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
