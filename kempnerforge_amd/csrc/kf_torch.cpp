@@ -22,6 +22,8 @@ namespace {
 // no tensor, differs from the first in device, dtype or shape, or is not
 // contiguous.  The data pointers go to out[at], out[at + 1], ...
 PyObject* same(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  // (fake and symbolic tensors throw where they are asked for sizes or an address)
+  HANDLE_TH_ERRORS
   if (nargs != 3 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "same(list, buffer, first)");
     return nullptr;
@@ -29,11 +31,18 @@ PyObject* same(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
   const Py_ssize_t at = PyLong_AsSsize_t(args[2]);
   if (at == -1 && PyErr_Occurred()) return nullptr;
-  Py_buffer buf;
-  if (PyObject_GetBuffer(args[1], &buf, PyBUF_WRITABLE) != 0) return nullptr;
+  struct Buffer {
+    Py_buffer b;
+    bool held;
+    ~Buffer() {
+      if (held) PyBuffer_Release(&b);
+    }
+  } buf = {};
+  buf.held = PyObject_GetBuffer(args[1], &buf.b, PyBUF_WRITABLE) == 0;
+  if (!buf.held) return nullptr;
   const char* wrong = nullptr;
   long device = -1;
-  if (at < 0 || n < 1 || (at + n) * 8 > buf.len) wrong = "no room for the pointers";
+  if (at < 0 || n < 1 || (at + n) * 8 > buf.b.len) wrong = "no room for the pointers";
   const at::Tensor* first = nullptr;
   for (Py_ssize_t i = 0; !wrong && i < n; ++i) {
     PyObject* o = PyList_GET_ITEM(args[0], i);
@@ -57,14 +66,14 @@ PyObject* same(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       device = t.is_cuda() ? (long)t.get_device() : -1;
     }
     const uint64_t p = wrong ? 0 : (uint64_t)(uintptr_t)t.data_ptr();
-    std::memcpy((char*)buf.buf + (at + i) * 8, &p, 8);
+    std::memcpy((char*)buf.b.buf + (at + i) * 8, &p, 8);
   }
-  PyBuffer_Release(&buf);
   if (wrong) {
     PyErr_SetString(PyExc_ValueError, wrong);
     return nullptr;
   }
   return PyLong_FromLong(device);
+  END_HANDLE_TH_ERRORS
 }
 
 // The library's entry points, by bind() (the library is opened by Python).
