@@ -123,10 +123,15 @@ __device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
 // Adds granules k, k + stride, ... (U of them, below `end`) to a thread's share:
 // the maximum of the batch first, then (SUM) one exponential a value; without SUM
 // the place of the maximum.  s becomes NaN where a value is NaN or (SUM) +inf.
-// The exponentials are one float32 instruction each (relative error 2^-22 and that of
-// its argument; in 64 bits a chain of 16 nodes with the draft's rows, 16 sequences of
-// 131072 values, takes 108 us instead of 51), summed in 64 bits a batch at a time: a
-// probability is off by some 2^-22 of itself, and so is the chance of a token.
+// The exponentials are one float32 instruction each (in 64 bits a chain of 16 nodes
+// with the draft's rows, 16 sequences of 131072 values, takes 108 us instead of 51) of
+// the difference to the maximum: the maximum's own is 1 and a constant added to the
+// row, or a low temperature, moves no other.  An argument x is off by 2^-23 of itself,
+// its exponential by that times |x| ln 2 and by 2^-22, a batch's sum (16 or 32 values)
+// by some 2^-22 more; the batches are summed in 64 bits.  The mean of |x| over a
+// distribution of V values is below log2 V, so a row's sum, and with it every
+// probability, is off by less than 2^-18.5 of itself at V = 2^20, by some 2^-22 where a few
+// tokens hold most of it, and so is the chance of a token.
 template <typename T, int U>
 __device__ __forceinline__ void load_batch(const Row<T>& r, int k, int stride, int end,
                                            u32x4* raw) {
@@ -179,7 +184,7 @@ __device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, co
     return;
   }
   const float ref = st.m == -INFINITY ? 0.f : st.m;
-  const float cf = (float)c, rc = ref * cf;
+  const float cf = (float)c;
   float gs = 0.f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -187,7 +192,7 @@ __device__ __forceinline__ void add_batch(const Row<T>& r, int k, int stride, co
     Row<T>::unpack(raw[u], f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      gs += __builtin_amdgcn_exp2f(fmaf(f[e], cf, -rc));
+      gs += __builtin_amdgcn_exp2f((f[e] - ref) * cf);
     }
   }
   st.s += (double)gs;
