@@ -324,6 +324,7 @@ int kf_verify_drafts_workspace_size(int B, int N, int V, int with_drafts, int dt
  *       next
  *   temperature  0: a node is accepted if its token is its parent's most likely
  *       (the lowest of equals), next is the last node's most likely token
+ *       Below 2^-126 it counts as 2^-126, above 2^126 as 2^126
  *   path  [B, N] int32: the accepted nodes in order, node 0 first, -1 behind
  *   kept  [B] int32: how many they are
  *   next  [B] int64: the token after the path

@@ -577,7 +577,9 @@ int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits
   a.drafts_sb = draft_stride_b; a.drafts_sn = draft_stride_n;
   a.uniforms = uniforms;
   a.greedy = !(temperature > 0.0);
-  a.inv_t = a.greedy ? 1.0 : 1.0 / temperature;
+  // (a normal float32 times log2 e, and its exponents' differences no 0 times Inf: past these
+  // bounds the distribution is that of the most likely tokens, or uniform, anyway)
+  a.inv_t = a.greedy ? 1.0 : fmin(fmax(1.0 / temperature, 0x1p-126), 0x1p126);
   a.path = path; a.kept = kept; a.next = next;
   a.B = B; a.N = N; a.V = V; a.dtype = dtype; a.stream = (hipStream_t)stream;
   const size_t need = verify_workspace(a);

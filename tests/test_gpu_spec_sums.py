@@ -84,3 +84,30 @@ def test_equal_top_logits_share_the_mass():
     tokens = torch.zeros(B, 1, dtype=torch.long, device=DEV)
     got = ops.verify_drafts_raw(logits, tokens, u, temperature=1e-6)[2].tolist()
     assert got == [17] * (B // 2) + [900] * (B // 2)
+
+
+@pytest.mark.parametrize("way", ["all", "walk", "drafts"])
+@pytest.mark.parametrize("T", [5e-324, 1e-300, 1e-40, 1e-38, 1e39, 1e46, 1e308])
+def test_temperatures_at_the_ends_of_their_range(T, way):
+    """The most likely tokens share the mass, or all tokens that are possible do."""
+    announce(f"verify temperature {T} {way}")
+    B, N, V = (160, 4, 600) if way == "walk" else (8, 2, 600)
+    logits = torch.randn(B, N, V, generator=torch.Generator().manual_seed(0)).to(DEV)
+    logits[:, :, 200:] = float("-inf")
+    logits[:, :, [7, 150]] = 9.0
+    share = 0.5 if T < 1 else 1 / 200
+    tokens = torch.full((B, N), 7, device=DEV)
+    u = torch.full((B, N), share * 0.999, device=DEV)
+    u[B // 2:, 1] = share * 1.001
+    draft = parents = None
+    if way == "walk":
+        tokens[:, 2:] = 300  # impossible
+        parents = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device=DEV)
+    if way == "drafts":  # certain of the token
+        draft = torch.full((B, 1, V), float("-inf"), device=DEV)
+        draft[:, :, 7] = 0.0
+    u[:, 0] = 0.9999
+    _, kept, token = ops.verify_drafts_raw(logits, tokens, u, temperature=T, parents=parents,
+                                           draft_logits=draft)
+    assert kept.tolist() == [2] * (B // 2) + [1] * (B - B // 2)
+    assert token.tolist() == [150 if T < 1 else 199] * B
