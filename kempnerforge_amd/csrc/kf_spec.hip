@@ -106,6 +106,11 @@ struct Stat {
   double s;  // sum of 2^((x - m) c); not positive and finite: no distribution
 };
 __device__ __forceinline__ bool has_mass(double s) { return s > 0.0 && s < INFINITY; }
+// Whether the row is a distribution.  greedy: only NaN shows in s, so the maximum has to
+// be finite (+inf, or -inf throughout).
+__device__ __forceinline__ bool is_distribution(const Stat& st, bool greedy) {
+  return greedy ? st.s == st.s && fabsf(st.m) < INFINITY : has_mass(st.s);
+}
 
 // 2^((a - b) c) for two maxima, 1 where both are -inf
 __device__ __forceinline__ double weight_of(float a, float b, double c) {
@@ -363,13 +368,13 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
       for (int u = 0; u < U; ++u) raw[u] = ahead[u];
     }
     st = join_all<WT>(st, c, x);
-    if (a.greedy ? st.s != st.s : !has_mass(st.s)) break;  // no distribution
+    if (!is_distribution(st, a.greedy)) break;
     end = cur;
     const bool child = t > 0 && t < n && nd.par[t] == cur;
     if (child) {
       const int tok = nd.tok[t];
       sp[t] = tok < 0 || repeated(nd, t) ? -1.0
-              : a.greedy ? (tok == (st.at == INT_MAX ? 0 : st.at) ? 1.0 : -1.0)
+              : a.greedy ? (tok == st.at ? 1.0 : -1.0)
                          : exp2_64(((double)to_f32(r.x[tok]) - (double)st.m) * c) / st.s;
     }
     __syncthreads();
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(WT) void verify_walk_kernel(VerifyArgs a, int* __re
   for (int j = t; j < a.N; j += WT) a.path[(int64_t)b * a.N + j] = j < len ? path[j] : -1;
   if (t == 0) {
     a.kept[b] = len;
-    a.next[b] = a.greedy && end >= 0 ? (st.at == INT_MAX ? 0 : st.at) : -1;
+    a.next[b] = a.greedy && end >= 0 ? st.at : -1;
     last[b] = end;
     out[b] = st;
     arrived[b] = 0;
@@ -473,9 +478,9 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
       const Stat& r = row[nd.par[t]];
       const int tok = nd.tok[t];
       sp[t] = tok < 0 || repeated(nd, t) ? -1.0
-              : a.greedy ? (tok == (r.at == INT_MAX ? 0 : r.at) && r.s == r.s ? 1.0 : -1.0)
-              : has_mass(r.s) ? exp2_64(((double)x - (double)r.m) * c) / r.s
-                              : -1.0;
+              : !is_distribution(r, a.greedy) ? -1.0
+              : a.greedy ? (tok == r.at ? 1.0 : -1.0)
+                         : exp2_64(((double)x - (double)r.m) * c) / r.s;
       if (drafted) {
         const Stat& d = row[n + t - 1];
         sq[t] = exp2_64(((double)y - (double)d.m) * c) / d.s;
@@ -490,7 +495,7 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
         while (true) {
           const int to = pick[at];
           pick[len++] = at;  // len <= at: the picks of nodes behind are intact
-          const bool ok = a.greedy ? row[at].s == row[at].s : has_mass(row[at].s);
+          const bool ok = is_distribution(row[at], a.greedy);
           if (ok && to == INT_MAX) lastn = at;
           if (!ok || to == INT_MAX) break;
           at = to;
@@ -506,7 +511,7 @@ __global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyArgs a, const int
       if (t < N) a.path[(int64_t)b * N + t] = t < sh[1] ? pick[t] : -1;
       if (t == 0) {
         a.kept[b] = sh[1];
-        if (cur < 0 || a.greedy) a.next[b] = cur < 0 ? -1 : st.at == INT_MAX ? 0 : st.at;
+        if (cur < 0 || a.greedy) a.next[b] = cur < 0 ? -1 : st.at;
       }
     }
     if (cur >= 0 && drafted && cur + 1 < n) dst = row[n + cur];

@@ -84,8 +84,8 @@ def verify(logits, tokens, uniforms, temperature, parents, counts=None, draft_lo
                 path.append(cur)
                 row = logits[b, cur]
                 if temperature == 0:
-                    if torch.isnan(row).any():
-                        w = None
+                    if not torch.isfinite(row.max()):  # (NaN is the maximum of any row)
+                        best = -1
                         break
                     best = int((row == row.max()).nonzero()[0])
                 else:
@@ -118,7 +118,7 @@ def verify(logits, tokens, uniforms, temperature, parents, counts=None, draft_lo
                     break
                 cur = step
             if temperature == 0:
-                nxt = -1 if torch.isnan(logits[b, cur]).any() else best
+                nxt = best
             elif w is not None:
                 cum = w.cumsum(0)
                 nxt = min(V - 1, int((cum <= float(uniforms[b, 0]) * cum[-1]).sum()))

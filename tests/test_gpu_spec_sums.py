@@ -9,6 +9,7 @@ import torch
 
 from gpu_util import DEV, announce
 from kempnerforge_amd import ops
+from oracle import spec_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +112,38 @@ def test_temperatures_at_the_ends_of_their_range(T, way):
                                            draft_logits=draft)
     assert kept.tolist() == [2] * (B // 2) + [1] * (B - B // 2)
     assert token.tolist() == [150 if T < 1 else 199] * B
+
+
+@pytest.mark.parametrize("way", ["all", "walk"])
+@pytest.mark.parametrize("dtype", [F32, FH])
+def test_greedy_rows_without_a_distribution(dtype, way):
+    """At temperature 0 too a row with +inf, or of -inf throughout, ends the path with no
+    token: of node 0, and of a node further down."""
+    announce(f"verify greedy bad rows {dtype} {way}")
+    B, N, V = (400, 4, 700) if way == "walk" else (40, 4, 700)
+    inf = float("inf")
+    logits = torch.randn(B, N, V, generator=torch.Generator().manual_seed(0)).to(dtype)
+    logits[:, :, 5] = 20.0
+    for at in range(8):
+        bad = logits[at::10, at % 2]
+        if at < 2:
+            bad[:, 333] = inf
+        elif at < 4:
+            bad[:] = -inf
+        elif at < 6:
+            bad[:, 699] = float("nan")
+        else:
+            bad[:, 6:] = -inf  # (a distribution)
+    tokens = torch.full((B, N), 5)
+    tokens[:, 3] = 0  # (what a row of -inf must not take)
+    parents = None
+    par = [[-1, 0, 1, 0]] * B if way == "walk" else [[-1, 0, 1, 2]] * B
+    if way == "walk":
+        parents = torch.tensor(par, dtype=torch.int32, device=DEV)
+    got = ops.verify_drafts_raw(logits.to(DEV), tokens.to(DEV), torch.zeros(B, N, device=DEV),
+                                temperature=0.0, parents=parents)
+    path, kept, token = (t.tolist() for t in got)
+    want = spec_ref.verify(logits, tokens, torch.zeros(B, N), 0.0, par)
+    wrong = [b for b in range(B) if (path[b], kept[b], token[b]) != tuple(x[b] for x in want)]
+    assert not wrong, wrong[:10]
+    assert kept[:10] == [1, 2, 1, 2, 1, 2, 3, 3, 3, 3] and token[:10] == [-1] * 6 + [5] * 4
