@@ -235,7 +235,8 @@ def speculative_generate(
     (``kf_kv_cache_keep``); it reads the accepted tokens back once.  A sequence near
     its ``max_new_tokens`` drafts no deeper than it can use.
 
-    Both models share the vocabulary and follow :func:`generate`'s contract.  Returns
+    Both models share the vocabulary and follow :func:`generate`'s contract; their dtypes
+    may differ (a chain is then drawn and verified in the type that holds both).  Returns
     each prompt followed directly by its tokens, rows padded on the right with
     ``eos_token_id`` (or 0) to the longest; a row ends with its first
     ``eos_token_id`` or after ``max_new_tokens``."""
@@ -274,8 +275,15 @@ def speculative_generate(
     target = _Stream(model, prompt_tokens, prompt_lens, rows)
     draft = _Stream(draft_model, prompt_tokens, prompt_lens, rows)
 
+    # A sampled chain's drafts are drawn from the rows that they are verified against, in a
+    # type that holds both models' logits.
+    dtype = target.logits.dtype
+    if tree is None:
+        dtype = torch.promote_types(dtype, draft.logits.dtype)
+
     def dist(logits):
         """(logits, temperature) of the distribution that is sampled."""
+        logits = logits.to(dtype)
         if temperature == 0 or (top_k <= 0 and top_p >= 1.0):
             return logits, temperature
         flat = _filtered((logits / temperature).reshape(-1, vocab), top_k, top_p)
