@@ -29,6 +29,8 @@ and the attention layers are ``kempnerforge_amd.Attention``.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from kempnerforge_amd import ops
@@ -207,6 +209,19 @@ class _Stream:
             c._seq_len, c.ragged = max(lengths), len(set(lengths)) > 1
 
 
+@contextlib.contextmanager
+def _evaluating(*models):
+    """The models in eval mode; as they were afterwards, however that comes."""
+    modes = [(m, m.training) for m in models]
+    for m in models:
+        m.eval()
+    try:
+        yield
+    finally:
+        for m, was_training in modes:
+            m.train(was_training)
+
+
 @torch.no_grad()
 def speculative_generate(
     model,
@@ -240,7 +255,6 @@ def speculative_generate(
     each prompt followed directly by its tokens, rows padded on the right with
     ``eos_token_id`` (or 0) to the longest; a row ends with its first
     ``eos_token_id`` or after ``max_new_tokens``."""
-    device = prompt_tokens.device
     batch, prompt_len = prompt_tokens.shape
     if draft_len < 1 or draft_len + 1 > ops.TREE_MAX_NODES:
         raise ValueError(f"draft_len must lie in [1, {ops.TREE_MAX_NODES - 1}] (got {draft_len})")
@@ -248,7 +262,6 @@ def speculative_generate(
         parents, rank, starts = None, None, list(range(draft_len + 2))
     else:
         parents, rank, starts = _tree_levels(tree)
-    nodes = starts[-1]
     limit = min(model.config.max_seq_len, draft_model.config.max_seq_len)
     if prompt_len + max_new_tokens > limit:
         raise ValueError(
@@ -262,23 +275,40 @@ def speculative_generate(
         raise ValueError("prompt_lens needs one length in [1, prompt_len] per sequence")
     if max_new_tokens < 1:
         return prompt_tokens.clone()
-    modes = [(m, m.training) for m in (model, draft_model)]
-    for m, _ in modes:
-        m.eval()
+    with _evaluating(model, draft_model):
+        emitted = _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parents, rank,
+                        starts, temperature, top_k, top_p, eos_token_id)
+    pad = eos_token_id if eos_token_id is not None else 0
+    width = max(n + len(e) for n, e in zip(prompt_lens, emitted))
+    out = torch.full((batch, width), pad, dtype=prompt_tokens.dtype)
+    host_prompt = prompt_tokens.cpu()
+    for b, (n, e) in enumerate(zip(prompt_lens, emitted)):
+        out[b, :n] = host_prompt[b, :n]
+        out[b, n:n + len(e)] = torch.tensor(e, dtype=out.dtype)
+    return out.to(prompt_tokens.device)
+
+
+def _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parents, rank, starts,
+          temperature, top_k, top_p, eos_token_id) -> list[list[int]]:
+    """The tokens of :func:`speculative_generate`, a list per sequence; the drafts' tree as
+    :func:`_tree_levels` gives it (a chain: no parents)."""
+    device = prompt_tokens.device
+    batch, prompt_len = prompt_tokens.shape
+    chain = parents is None
     # The vocabularies before any token of one model reaches the other (token 0 is in both).
     probe = prompt_tokens.new_zeros(1, 1)
     vocab, draft_vocab = (m(probe).shape[-1] for m in (model, draft_model))
     if vocab != draft_vocab:
         raise ValueError(f"the models' vocabularies differ ({vocab}, {draft_vocab})")
     # Rows behind the last token for its drafts.  (Positions stay below limit.)
-    rows = prompt_len + max_new_tokens + nodes
+    rows = prompt_len + max_new_tokens + starts[-1]
     target = _Stream(model, prompt_tokens, prompt_lens, rows)
     draft = _Stream(draft_model, prompt_tokens, prompt_lens, rows)
 
     # A sampled chain's drafts are drawn from the rows that they are verified against, in a
     # type that holds both models' logits.
     dtype = target.logits.dtype
-    if tree is None:
+    if chain:
         dtype = torch.promote_types(dtype, draft.logits.dtype)
 
     def dist(logits):
@@ -301,7 +331,7 @@ def speculative_generate(
     if min(e[0] for e in emitted) < 0:
         raise RuntimeError("the model's logits are no distribution (NaN, or -inf throughout)")
     lengths = list(prompt_lens)
-    if tree is not None:
+    if not chain:
         parents = torch.tensor(parents, dtype=torch.int32, device=device)
         rank = torch.tensor(rank, device=device)
 
@@ -319,7 +349,7 @@ def speculative_generate(
         tokens = token.new_zeros(batch, n)
         tokens[:, 0] = token
         tree_parents, draft_logits = None, None
-        if tree is None:
+        if chain:
             rowlist = []
             for j in range(1, n):
                 logits, temp = dist(draft(tokens[:, j - 1:j])[:, -1])
@@ -337,7 +367,7 @@ def speculative_generate(
                 logits = draft(tokens[:, :hi])[:, lo:hi]
                 at, want = parents[hi:end].long() - lo, rank[hi:end]
                 # (a rank past the vocabulary repeats its last token: refused again)
-                best = logits.topk(min(vocab, len(tree)), dim=-1).indices
+                best = logits.topk(min(vocab, len(rank)), dim=-1).indices
                 tokens[:, hi:end] = best[:, at, want.clamp_max(best.shape[-1] - 1)]
             begin_tree(draft.caches, tree_parents, counts)
             draft(tokens)
@@ -360,19 +390,10 @@ def speculative_generate(
                 if left(b):
                     emitted[b].append(t)
         keep_path(target.caches, path, kept, lengths)
-        if tree is None:
+        if chain:
             draft.rewind(target.caches[0].lens, lengths)
         else:
             keep_path(draft.caches, path, kept, lengths)
         token = token.clamp_min(0)  # (a finished sequence has no next token; any will do)
 
-    for m, was_training in modes:
-        m.train(was_training)
-    pad = eos_token_id if eos_token_id is not None else 0
-    width = max(n + len(e) for n, e in zip(prompt_lens, emitted))
-    out = torch.full((batch, width), pad, dtype=prompt_tokens.dtype)
-    host_prompt = prompt_tokens.cpu()
-    for b, (n, e) in enumerate(zip(prompt_lens, emitted)):
-        out[b, :n] = host_prompt[b, :n]
-        out[b, n:n + len(e)] = torch.tensor(e, dtype=out.dtype)
-    return out.to(device)
+    return emitted

@@ -37,3 +37,31 @@ def test_models_of_different_dtypes(oracle, monkeypatch, dtypes, common, kw):  #
     assert bool(seen) == (kw["temperature"] > 0 and "tree" not in kw)
     if kw["temperature"] == 0:
         assert torch.equal(out, generate(model, prompt, 9, temperature=0))
+
+
+@pytest.mark.parametrize("training", [(True, True), (False, True), (True, False)], ids=str)
+def test_the_models_modes_come_back(oracle, training):  # noqa: F811
+    """After the result, and after a refusal: vocabularies that differ, a model without a
+    distribution at once, or at a later step, an argument that the verification refuses."""
+    def check(model, draft, kind=None, **kw):
+        for m, on in zip((model, draft), training):
+            m.train(on)
+        if kind is None:
+            speculative_generate(model, draft, torch.tensor([[1, 2]]), 6, temperature=0, **kw)
+        else:
+            with pytest.raises(kind):
+                speculative_generate(model, draft, torch.tensor([[1, 2]]), 6, temperature=0, **kw)
+        assert (model.training, draft.training) == training
+
+    bad, late = Bigram(5, 0), Bigram(5, 0)
+    with torch.no_grad():
+        bad.table[:] = float("nan")
+        late.table[:] = 0.0
+        late.table[2, 3] = 1.0  # 2 is followed by 3, and 3 by nothing
+        late.table[3] = float("nan")
+    check(Bigram(5, 0), Bigram(5, 1))
+    check(Bigram(5, 0), Bigram(5, 1), tree=[-1, 0, 0])
+    check(Bigram(5, 0), Bigram(9, 1), ValueError)
+    check(bad, Bigram(5, 1), RuntimeError)
+    check(late, Bigram(5, 1), RuntimeError)
+    check(late, Bigram(5, 1), RuntimeError, tree=[-1, 0, 0])
