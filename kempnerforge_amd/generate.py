@@ -273,11 +273,11 @@ def speculative_generate(
     prompt_lens = [int(n) for n in prompt_lens]
     if len(prompt_lens) != batch or min(prompt_lens) < 1 or max(prompt_lens) > prompt_len:
         raise ValueError("prompt_lens needs one length in [1, prompt_len] per sequence")
-    if max_new_tokens < 1:
-        return prompt_tokens.clone()
-    with _evaluating(model, draft_model):
-        emitted = _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parents, rank,
-                        starts, temperature, top_k, top_p, eos_token_id)
+    emitted: list[list[int]] = [[] for _ in range(batch)]
+    if max_new_tokens > 0:
+        with _evaluating(model, draft_model):
+            emitted = _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parents,
+                            rank, starts, temperature, top_k, top_p, eos_token_id)
     pad = eos_token_id if eos_token_id is not None else 0
     width = max(n + len(e) for n, e in zip(prompt_lens, emitted))
     out = torch.full((batch, width), pad, dtype=prompt_tokens.dtype)

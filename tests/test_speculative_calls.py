@@ -65,3 +65,12 @@ def test_the_models_modes_come_back(oracle, training):  # noqa: F811
     check(bad, Bigram(5, 1), RuntimeError)
     check(late, Bigram(5, 1), RuntimeError)
     check(late, Bigram(5, 1), RuntimeError, tree=[-1, 0, 0])
+
+
+@pytest.mark.parametrize("lens", [None, [2, 1, 3]])
+def test_no_new_tokens(oracle, lens):  # noqa: F811
+    """generate's result: the prompts, padded on the right to the longest."""
+    model, prompt = Bigram(5, 0), torch.tensor([[1, 2, 3, 4], [4, 3, 2, 1], [1, 1, 1, 1]])
+    want = generate(model, prompt, 0, prompt_lens=lens, eos_token_id=0)
+    got = speculative_generate(model, Bigram(5, 1), prompt, 0, prompt_lens=lens, eos_token_id=0)
+    assert torch.equal(got, want)
