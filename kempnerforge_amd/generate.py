@@ -295,14 +295,15 @@ def _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parent
     device = prompt_tokens.device
     batch, prompt_len = prompt_tokens.shape
     chain = parents is None
-    # The vocabularies before any token of one model reaches the other (token 0 is in both).
-    probe = prompt_tokens.new_zeros(1, 1)
-    vocab, draft_vocab = (m(probe).shape[-1] for m in (model, draft_model))
-    if vocab != draft_vocab:
-        raise ValueError(f"the models' vocabularies differ ({vocab}, {draft_vocab})")
     # Rows behind the last token for its drafts.  (Positions stay below limit.)
     rows = prompt_len + max_new_tokens + starts[-1]
     target = _Stream(model, prompt_tokens, prompt_lens, rows)
+    vocab = target.logits.shape[-1]
+    # The draft model's vocabulary before any token of the other's reaches it (token 0 is in
+    # both): what lies past its embedding would be read out of range.
+    draft_vocab = draft_model(prompt_tokens.new_zeros(1, 1)).shape[-1]
+    if vocab != draft_vocab:
+        raise ValueError(f"the models' vocabularies differ ({vocab}, {draft_vocab})")
     draft = _Stream(draft_model, prompt_tokens, prompt_lens, rows)
 
     # A sampled chain's drafts are drawn from the rows that they are verified against, in a

@@ -74,3 +74,33 @@ def test_no_new_tokens(oracle, lens):  # noqa: F811
     want = generate(model, prompt, 0, prompt_lens=lens, eos_token_id=0)
     got = speculative_generate(model, Bigram(5, 1), prompt, 0, prompt_lens=lens, eos_token_id=0)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tree,forwards", [(None, (6, 14)), ([-1, 0, 0], (6, 11))], ids=str)
+def test_forwards_of_a_call(oracle, tree, forwards):  # noqa: F811
+    """The model runs for the prompts and once a step, and for nothing else (here every
+    draft is refused, so that five steps follow the prompts' token).  The draft model runs
+    for its vocabulary, the prompts, and in a step once a level of drafts and once more:
+    chains of 2, 2, 2, 2 and then no drafts but the last token, 3 + 3 + 3 + 2 + 1, levels
+    of one 2 + 2 + 2 + 2 + 1."""
+    model, draft, calls = Bigram(5, 0), Bigram(5, 1), [0, 0]
+    with torch.no_grad():
+        model.table[:] = torch.eye(5)[[1, 2, 3, 4, 0]]  # counts up
+        draft.table[:] = torch.eye(5)  # repeats
+        if tree is not None:
+            draft.table[:, [0, 1]] = 9.0  # of the next tokens 3, 4, 0, 1, 2 it has 0 and 1
+            draft.table[:, 2] = 8.0
+            model.table[:] = torch.eye(5)[[3, 3, 3, 4, 3]]  # 3, 4, 3, 4, ..
+
+    def count(i):
+        def hook(*_):
+            calls[i] += 1
+        return hook
+
+    for i, m in enumerate((model, draft)):
+        m.register_forward_hook(count(i))
+    out = speculative_generate(model, draft, torch.tensor([[2]]), 6, temperature=0, tree=tree,
+                               draft_len=2)
+    want = [2, 3, 4, 0, 1, 2, 3] if tree is None else [2, 3, 4, 3, 4, 3, 4]
+    assert out.tolist() == [want]
+    assert tuple(calls) == forwards
