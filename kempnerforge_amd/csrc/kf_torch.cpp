@@ -179,7 +179,8 @@ PyObject* tree(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                    *cos = tensor(args[6], device), *parents, *counts, *qnw, *knw;
   if (dt < 0 || !k || !v || !vc || !lens || !cos || cos->dim() != 2 ||
       !tensor(args[3], device, type, {B, Hkv, Smax, D}) ||
-      !tensor(args[6], device, at::kFloat, {cos->size(0), D / 2}) || !fits(B) || !fits(Smax))
+      !tensor(args[6], device, at::kFloat, {cos->size(0), D / 2}) || !fits(B) || !fits(N) ||
+      !fits(Hq) || !fits(Hkv) || !fits(Smax) || !fits(D))
     Py_RETURN_NONE;
   const at::Tensor* sin = tensor(args[7], device, at::kFloat, cos->sizes());
   if (!sin || !tree_shape(args[8], args[9], device, B, N, &parents, &stride, &counts) ||
@@ -277,8 +278,9 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor* kept = tensor(args[5], device, at::kInt, {B});
   std::vector<void*> p;
   p.reserve(4 * n);
-  if (dt < 0 || !kept || !tensor(args[4], device, at::kInt, {B, N}) || !fits(N) ||
-      !fits(k0->size(2)) || !pointers(args[0], n, device, type, k0->sizes(), p) ||
+  if (dt < 0 || !kept || !tensor(args[4], device, at::kInt, {B, N}) || !fits(B) || !fits(N) ||
+      !fits(k0->size(1)) || !fits(k0->size(2)) || !fits(k0->size(3)) ||
+      !pointers(args[0], n, device, type, k0->sizes(), p) ||
       !pointers(args[1], n, device, type, k0->sizes(), p) ||
       !pointers(args[2], n, device, at::kInt, {B}, p) ||
       !pointers(args[3], n, device, at::kInt, {B}, p))

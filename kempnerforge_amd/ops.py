@@ -516,6 +516,13 @@ def _one_device(*ts) -> int:
     return dev.pop()
 
 
+def _c_ints(**sizes) -> None:
+    """Sizes that do not fit the library's ints (they would come back as others)."""
+    for name, n in sizes.items():
+        if n > 0x7FFFFFFF:
+            raise ValueError(f"{name} is at most 2^31 - 1 (got {n})")
+
+
 _INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
@@ -574,6 +581,7 @@ def tree_decode_raw(q_new, k_new, v_new, k_cache, v_cache, lens, cos, sin, *,
         raise ValueError("q_new, k_new, v_new and the caches must have four dimensions")
     B, N, Hq, D = qs
     Hkv, Smax = cs[1], cs[2]
+    _c_ints(batch=B, n_heads=Hq, n_kv_heads=Hkv, max_seq_len=Smax, head_dim=D)
     if ks != (B, N, Hkv, D) or v_new.shape != ks:
         raise ValueError(f"k_new and v_new must be [{B}, {N}, {Hkv}, {D}] "
                          f"(got {tuple(ks)}, {tuple(v_new.shape)})")
@@ -658,6 +666,7 @@ def verify_drafts_raw(logits, tokens, uniforms, *, temperature: float = 1.0, par
         raise ValueError("logits must be [B, N, V] with contiguous values "
                          f"(got {tuple(ls)}, strides {logits.stride()})")
     B, N, V = ls
+    _c_ints(batch=B, vocabulary=V)
     if not 1 <= N <= TREE_MAX_NODES:
         raise ValueError(f"1 to {TREE_MAX_NODES} nodes per sequence (got {N})")
     if tokens.shape != (B, N) or uniforms.shape != (B, N):
@@ -733,6 +742,10 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
     except ValueError as e:
         raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim], of "
                          f"one device, dtype and shape: {e}") from None
+    if k0.dim() != 4:
+        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
+    B, Hkv, Smax, D = k0.shape
+    _c_ints(batch=B, n_kv_heads=Hkv, max_seq_len=Smax, head_dim=D)
     try:
         where = {dev, same(lens, ptrs, 0), same(lens_out, ptrs, n), path.get_device(),
                  kept.get_device()}
@@ -741,9 +754,6 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
     if where != {dev} or dev < 0:
         _require_gpu(*caches, *lens, *lens_out, path, kept)
         raise RuntimeError(f"the tensors must lie on one device (got {sorted(where)})")
-    if k0.dim() != 4:
-        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
-    B, Hkv, Smax, D = k0.shape
     for t in (lens[0], lens_out[0]):
         if t.dtype != torch.int32 or t.shape != (B,):
             raise TypeError(f"lens and lens_out must be contiguous int32 tensors [{B}]")
