@@ -353,6 +353,7 @@ int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits
  *       [B, Hkv, Smax, D] contiguous
  *   lens, lens_out  host arrays of n_caches device pointers to [B] int32;
  *       lens_out[c] may be lens[c] where no other cache reads it
+ *       (otherwise nothing that is written may overlap anything else given here)
  *   path [B, N], kept [B]  what kf_verify_drafts returned
  * Other rows stay as they are.  A sequence with kept[b] outside 0 .. N, or a
  * path that does not rise or leaves the nodes or the cache, is left alone

@@ -7,8 +7,11 @@
 #include "kf_common.h"
 #include "kf_internal.h"
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
+#include <memory>
+#include <new>
 
 namespace kf {
 
@@ -590,6 +593,41 @@ int kf_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits
   return verify_drafts(a, workspace);
 }
 
+}  // extern "C"
+
+namespace {
+// Whether two of n buffers of `size` bytes meet; sorts them.
+bool meet(uintptr_t* p, int n, size_t size) {
+  std::sort(p, p + n);
+  for (int i = 1; i < n; ++i)
+    if (p[i] - p[i - 1] < size) return true;
+  return false;
+}
+// The workgroups of one cache know nothing of the others': none may write what another
+// reads or writes.  Whether any does: K and V tensors of `bytes`, lens and lens_out of
+// `lens_bytes` each; lens_out[c] may be lens[c].  at: room for 3 n addresses.
+bool keep_overlap(void* const* k, void* const* v, const int32_t* const* lens,
+                  int32_t* const* lens_out, int n, size_t bytes, size_t lens_bytes,
+                  uintptr_t* at) {
+  uintptr_t *rows = at, *out = at + 2 * (size_t)n;
+  for (int c = 0; c < n; ++c) {
+    rows[2 * c] = (uintptr_t)k[c];
+    rows[2 * c + 1] = (uintptr_t)v[c];
+    out[c] = (uintptr_t)lens_out[c];
+  }
+  if (meet(rows, 2 * n, bytes) || meet(out, n, lens_bytes)) return true;
+  for (int c = 0; c < n; ++c) {
+    const uintptr_t p = (uintptr_t)lens[c];
+    if (lens[c] == lens_out[c]) continue;  // (the others' lie apart from it)
+    const uintptr_t* x = std::lower_bound(out, out + n, p);
+    if ((x != out + n && *x - p < lens_bytes) || (x != out && p - x[-1] < lens_bytes)) return true;
+  }
+  return false;
+}
+}  // namespace
+
+extern "C" {
+
 int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t* const* lens,
                      int32_t* const* lens_out, int n_caches, const int32_t* path,
                      const int32_t* kept, int N, int B, int Hkv, int Smax, int D, int dtype,
@@ -598,16 +636,25 @@ int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t
   if (rc) return rc;
   KF_CHECK_ARG(n_caches > 0, "n_caches must be positive (got %d)", n_caches);
   KF_CHECK_ARG(k_caches && v_caches && lens && lens_out && path && kept, "null tensor pointer");
-  for (int c = 0; c < n_caches; ++c) {
+  for (int c = 0; c < n_caches; ++c)
     KF_CHECK_ARG(k_caches[c] && v_caches[c] && lens[c] && lens_out[c],
                  "null tensor pointer (cache %d)", c);
-    // the workgroups of one cache know nothing of the others': none may write
-    // what another reads or writes
-    KF_CHECK_ARG(k_caches[c] != v_caches[c], "cache %d has one tensor for K and V", c);
-    for (int d = 0; d < n_caches; ++d)
-      KF_CHECK_ARG(d == c || (lens_out[c] != lens[d] && k_caches[c] != k_caches[d] &&
-                              v_caches[c] != v_caches[d] && k_caches[c] != v_caches[d]),
-                   "caches %d and %d share a tensor that one of them writes", c, d);
+  constexpr int FEW = 256;  // (a model's layers: no allocation)
+  uintptr_t few[3 * FEW];
+  std::unique_ptr<uintptr_t[]> many(n_caches > FEW ? new (std::nothrow) uintptr_t[3 * (size_t)n_caches]
+                                                   : nullptr);
+  KF_CHECK_ARG(n_caches <= FEW || many, "no host memory to check %d caches", n_caches);
+  if (keep_overlap(k_caches, v_caches, lens, lens_out, n_caches,
+                   (size_t)B * Hkv * Smax * D * (dtype == F32 ? 4 : 2), (size_t)B * 4,
+                   n_caches > FEW ? many.get() : few)) {
+    for (int c = 0; c < n_caches; ++c) {
+      KF_CHECK_ARG(k_caches[c] != v_caches[c], "cache %d has one tensor for K and V", c);
+      for (int d = 0; d < n_caches; ++d)
+        KF_CHECK_ARG(d == c || (lens_out[c] != lens[d] && k_caches[c] != k_caches[d] &&
+                                v_caches[c] != v_caches[d] && k_caches[c] != v_caches[d]),
+                     "caches %d and %d share a tensor that one of them writes", c, d);
+    }
+    KF_CHECK_ARG(false, "the caches (or their lengths) overlap: they share memory that one writes");
   }
   return cache_keep(k_caches, v_caches, lens, lens_out, n_caches, path, kept, N, B, Hkv, Smax, D,
                     dtype, (hipStream_t)stream);

@@ -3,10 +3,13 @@
 
 from __future__ import annotations
 
+import ctypes
+import os
+
 import pytest
 import torch
 
-from kempnerforge_amd import ops
+from kempnerforge_amd import _lib, ops
 from test_speculative import no_device  # noqa: F401
 
 BIG = (1 << 32) + 8  # 8 in a C int
@@ -48,3 +51,46 @@ def test_logits_past_a_c_int(no_device, B, V, what):  # noqa: F811
     with pytest.raises(ValueError, match=f"{what} is at most"):
         ops.verify_drafts_raw(_meta(B, 3, V), _meta(B, 3, dtype=torch.int64),
                               _meta(B, 3, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("n", [2, 300])
+@pytest.mark.parametrize("what", ["k", "v", "k and v", "own k and v", "lens_out", "lens", "own lens",
+                                  "lens shared"])
+def test_views_that_overlap(what, n):
+    """Not the same tensors, but memory that one cache's workgroups write and another's
+    read: views a row, or a sequence's length, apart.  (The addresses are never read.)"""
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    B, H, S, D = 2, 2, 64, 64
+    size, row = B * H * S * D * 2, D * 2
+    base = 1 << 40
+    k = [base + 2 * c * size for c in range(n)]
+    v = [base + (2 * c + 1) * size for c in range(n)]
+    lens = [(1 << 50) + 8 * c for c in range(n)]
+    out = list(lens)
+    if what == "k":
+        k[-1] = k[0] + row
+    elif what == "v":
+        v[0] = v[-1] + size - row
+    elif what == "k and v":
+        k[-1] = v[0] - row
+    elif what == "own k and v":
+        v[-1] = k[-1] + row
+    elif what == "lens_out":
+        out[-1] = lens[-1] = out[0] + 4
+    elif what == "lens":
+        lens[-1] = out[0] - 4
+    elif what == "own lens":
+        lens[-1] = out[-1] + 4
+    else:  # several caches may read one tensor that none writes, but not lens_out
+        lens = [1 << 49] * n
+        out[1] = lens[1]
+    arr = ctypes.c_void_p * n
+    p = ctypes.c_void_p(1 << 20)
+
+    def call(B=B):
+        return lib.kf_kv_cache_keep(arr(*k), arr(*v), arr(*lens), arr(*out), n, p, p, 8, B, H, S, D,
+                                    1, None)
+
+    assert call() == 1 and b"share" in lib.kf_last_error()
