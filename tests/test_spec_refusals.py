@@ -94,3 +94,44 @@ def test_views_that_overlap(what, n):
                                     1, None)
 
     assert call() == 1 and b"share" in lib.kf_last_error()
+
+
+z = torch.zeros
+CACHE, LENS = z(1, 2, 8, 64), z(1).int()
+PATH, KEPT = z(1, 3).int(), z(1).int()
+
+
+@pytest.mark.parametrize("change,kind,word", [
+    (dict(k=[]), ValueError, "one tensor per cache"), (dict(v=[]), ValueError, "one tensor per cache"),
+    (dict(lens=[LENS, LENS]), ValueError, "one tensor per cache"),
+    (dict(lens=[LENS.long()]), TypeError, "int32"), (dict(lens=[z(2).int()]), TypeError, "int32"),
+    (dict(out=[LENS.long()]), TypeError, "int32"), (dict(lens=[z(1, 1).int()]), TypeError, "int32"),
+    (dict(path=PATH.long()), TypeError, "must be int32"), (dict(kept=KEPT.long()), TypeError, "must be int32"),
+    (dict(kept=z(2).int()), TypeError, "must be int32"), (dict(path=z(2, 3).int()), ValueError, "path must be"),
+    (dict(path=z(3).int()), ValueError, "path must be"), (dict(path=z(1, 0).int()), ValueError, "path must be"),
+    (dict(path=z(1, 257).int()), ValueError, "path must be"),
+    (dict(v=[CACHE.half()]), ValueError, "share a dtype"), (dict(v=[z(1, 2, 9, 64)]), ValueError, "share a shape"),
+    (dict(v=[z(1, 8, 2, 64).transpose(1, 2)]), ValueError, "contiguous tensors"),
+    (dict(k=[CACHE[0]], v=[CACHE[0].clone()]), ValueError, r"must be \[B, n_kv_heads"),
+    (dict(k=[5]), ValueError, "tensors are needed"), (dict(lens=["x"]), ValueError, "must be alike"),
+    (dict(), AssertionError, "nothing was refused"),
+], ids=lambda x: "-".join(x) if isinstance(x, dict) else x if isinstance(x, str) else x.__name__)
+def test_keep_arguments(no_device, monkeypatch, change, kind, word):  # noqa: F811
+    """With the tensors taken for ones on the device."""
+    class Native:
+        keep = staticmethod(lambda *a: None)
+
+        @staticmethod
+        def same(*a, same=_lib.native().same):
+            same(*a)
+            return 0
+
+    class OnDevice(torch.Tensor):
+        def get_device(self):
+            return 0
+
+    monkeypatch.setattr(_lib, "native", lambda: Native)
+    a = dict(k=[CACHE], v=[CACHE.clone()], lens=[LENS], out=None, path=PATH, kept=KEPT) | change
+    path, kept = (t.as_subclass(OnDevice) for t in (a["path"], a["kept"]))
+    with pytest.raises(kind, match=word):
+        ops.cache_keep_raw(a["k"], a["v"], a["lens"], path, kept, lens_out=a["out"])
