@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+import re
 import threading
 
 # In-tree build; KF_ATTN_LIB may name another build of the same library (an
@@ -109,6 +110,12 @@ def native():
         spec = importlib.util.spec_from_file_location("kf_torch", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        import torch
+
+        if re.match(r"[0-9.]*[0-9]", torch.__version__)[0] != module.torch_version:
+            raise RuntimeError(f"kempnerforge_amd: {path} was built for torch "
+                               f"{module.torch_version}, this is {torch.__version__}; build it again "
+                               "with `python -c 'import __graft_entry__ as g; g.build()'`")
         lib = load()
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "kf_attn_tree_workspace_size", "kf_attn_tree", "kf_verify_drafts_workspace_size",

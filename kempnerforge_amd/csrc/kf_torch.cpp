@@ -8,6 +8,7 @@
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <climits>
 #include <cstring>
@@ -306,4 +307,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "kf_torch", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_kf_torch(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_kf_torch(void) {
+  PyObject* m = PyModule_Create(&module);
+  // what it was built for, by the headers
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
