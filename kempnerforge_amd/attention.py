@@ -166,7 +166,8 @@ def begin_tree(caches, parents: torch.Tensor | None = None,
     itself and its ancestors, at the position of its depth, and its key and value go
     to the cache row ``lens[b] + i`` without advancing the cache.  Several forwards
     may follow one another (a tree that grows level by level); each overwrites the
-    rows of the last.
+    rows of the last.  (``tree = None`` on each cache leaves it as it was before: the
+    drafts' rows lie behind the fill level.)
 
     ``parents`` (``[N]`` or ``[B, N]``, integers on the device; None: a chain) and
     ``counts`` (``[B]``: tokens in use, None: all) as in ``ops.tree_decode_raw``."""
