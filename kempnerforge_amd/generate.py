@@ -320,11 +320,14 @@ def _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parent
         flat = _filtered((logits / temperature).reshape(-1, vocab), top_k, top_p)
         return flat.view(logits.shape), 1.0
 
+    def uniforms(n):
+        """Random numbers for n nodes a sequence, whatever torch's default dtype."""
+        return torch.rand(batch, n, device=device, dtype=torch.float32)
+
     def draw(logits, temp):
         """A token per row, by a verification of no drafts; -1 for a row that is no
         distribution."""
-        return ops.verify_drafts_raw(logits[:, None], root, torch.rand(batch, 1, device=device),
-                                     temperature=temp)[2]
+        return ops.verify_drafts_raw(logits[:, None], root, uniforms(1), temperature=temp)[2]
 
     root = prompt_tokens.new_zeros(batch, 1)
     token = draw(*dist(target.logits))
@@ -375,8 +378,8 @@ def _emit(model, draft_model, prompt_tokens, prompt_lens, max_new_tokens, parent
         begin_tree(target.caches, tree_parents, counts)
         logits, temp = dist(target(tokens))
         path, kept, token = ops.verify_drafts_raw(
-            logits, tokens, torch.rand(batch, n, device=device), temperature=temp,
-            parents=tree_parents, counts=counts, draft_logits=draft_logits)
+            logits, tokens, uniforms(n), temperature=temp, parents=tree_parents, counts=counts,
+            draft_logits=draft_logits)
         accepted = tokens.gather(1, path.clamp_min(0).long())
         # the step's one read-back: per sequence, how many, the path's tokens, the next
         host = torch.cat([kept[:, None].long(), accepted, token[:, None]], dim=1).tolist()

@@ -104,3 +104,22 @@ def test_forwards_of_a_call(oracle, tree, forwards):  # noqa: F811
     want = [2, 3, 4, 0, 1, 2, 3] if tree is None else [2, 3, 4, 3, 4, 3, 4]
     assert out.tolist() == [want]
     assert tuple(calls) == forwards
+
+
+@pytest.mark.parametrize("default", [BF, FH, torch.float64])
+def test_whatever_the_default_dtype(oracle, monkeypatch, default):  # noqa: F811
+    """The random numbers are float32, as the verification asks it."""
+    verify = ops.verify_drafts_raw
+
+    def check(logits, tokens, uniforms, **more):
+        assert uniforms.dtype == F32
+        return verify(logits, tokens, uniforms, **more)
+
+    monkeypatch.setattr(ops, "verify_drafts_raw", check)
+    torch.set_default_dtype(default)
+    try:
+        for kw in (dict(), dict(tree=[-1, 0, 0])):
+            out = speculative_generate(Bigram(5, 0), Bigram(5, 1), torch.tensor([[1, 2]]), 6, **kw)
+            assert out.shape == (1, 8)
+    finally:
+        torch.set_default_dtype(F32)
