@@ -40,6 +40,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 namespace kf {
 
@@ -654,7 +655,14 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
   u32x4 q[X::QP][X::KS];
   f32x16 acc[DT];
   float m = -INFINITY, lsum = 0.f;
-  constexpr float SLACK = 8.f;  // P stays below 2^8, far inside every type
+  // P = 2^(s - m + LIFT) stays below 2^(SLACK + LIFT).  float16 has no numbers below 2^-24:
+  // thousands of keys at 2^-25 of one key's probability (a first token that takes most of
+  // the mass and has no value) would all round to 0, so its P fills the range up to 2^15
+  // and the reference moves more often; the other types have float32's range.  (tree of 64
+  // nodes, 16384 keys, as above: 282 us in float16, of which 10 for the conversions of P's
+  // split and this.)
+  constexpr bool HALF_P = std::is_same<T, _Float16>::value;
+  constexpr float SLACK = HALF_P ? 2.f : 8.f, LIFT = HALF_P ? 13.f : 0.f;
   bool whole = false;    // this workgroup holds all of the row tile's chunks
   bool refused = false;  // the sequence's tree or tables are out of range
   int node = 0;
@@ -882,7 +890,7 @@ __global__ __launch_bounds__(256, (Shape<T, D, RW, BKW>::PER_CU)) void tree_stre
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
       }
-      const float ref = m == -INFINITY ? 0.f : m;  // (a row that has met no key yet)
+      const float ref = (m == -INFINITY ? 0.f : m) - LIFT;  // (-inf: has met no key yet)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] = fast_exp2(s[e] - ref);

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from gpu_util import announce
-from spec_util import tree_inputs, trees
-from test_gpu_tree import BF, FH, _reference, _step
+from spec_util import P_STEP, tree_bound, tree_inputs, trees
+from test_gpu_tree import BF, F32, FH, _reference, _step
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,30 @@ def test_the_error_is_that_of_rounding_the_outputs(cfg):
     ratio = rms(out.cpu().double() - want) / rms(want.to(dtype).double() - want)
     print(f"[{dtype} {cfg[1]}] error / rounding {ratio:.3f}", flush=True)
     assert ratio <= 1.05
+
+
+@pytest.mark.parametrize("dtype,D", [(FH, 128), (FH, 64), (BF, 128), (F32, 64), (FH, 96)])
+@pytest.mark.parametrize("X", [12.0, 14.0, 16.0, 17.2])
+@pytest.mark.parametrize("first", [True, False])
+def test_a_key_that_takes_the_mass_and_gives_nothing(dtype, D, X, first):
+    """One key's score stands X above thousands of equal others and its value is zero (as
+    the first token's of many models does), so the outputs are made of probabilities e^-X
+    of the largest: all rounded alike, by the same error, if they are rounded."""
+    announce(f"tree sink {dtype} {D} {X} {first}")
+    B, N, Hq, Hkv, L = 1, 9, 4, 2, 7000
+    q, k, v, kc, vc, cos, sin = tree_inputs(dtype, B, N, Hq, Hkv, D, L + N, seed=5)
+    cos, sin = torch.ones_like(cos), torch.zeros_like(sin)
+    q[:] = 1.0
+    k[:], kc[:] = 0.0, 0.0
+    sink = 3 if first else L - 5
+    kc[:, :, sink, 0] = X * D ** 0.5
+    vc[:], v[:] = vc.abs() + 0.5, v.abs() + 0.5
+    vc[:, :, sink] = 0.0
+    out, kcd, vcd = _step(q, k, v, kc, vc, [L], cos, sin, L + N)
+    want, mag = _reference(q, k, v, kc, vc, kcd, vcd, [L], cos, sin, trees("chain", B, N))
+    # (scores of X or 0; P is not what is rounded, so nothing is allowed for it)
+    got = out.cpu().double()
+    bound = tree_bound(want, mag, dtype, D, L + N, dot=X) - P_STEP[dtype] * mag
+    ratio = ((got - want).abs() / bound).max().item()
+    print(f"[sink {dtype} {D} {X} {first}] worst error / bound {ratio:.3f}", flush=True)
+    assert ratio <= 1.0
