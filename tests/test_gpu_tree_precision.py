@@ -37,7 +37,7 @@ def test_the_error_is_that_of_rounding_the_outputs(cfg):
     probability by some 2^-17; P to 2^-17 (2^-22 and an absolute 2^-25); float32 sums and
     exponentials by some 2^-21 with the spread of their arguments.  Together below 3e-5
     (5e-6) of a value, a thirtieth of the rounding's, which adds its square: 0.1%.
-    P in a single number of the type makes it 1.2 to 1.4 times."""
+    P in a single number of the type makes it 1.2 to 1.4 times, q 1.3 to 1.5."""
     dtype, (B, N, Hq, Hkv, D), lens, tree = cfg
     announce(f"tree precision {cfg}")
     q, k, v, kc, vc, cos, sin = tree_inputs(dtype, B, N, Hq, Hkv, D, max(lens) + N, seed=3)
