@@ -363,6 +363,86 @@ int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t
                      const int32_t* kept, int N, int B, int Hkv, int Smax, int D, int dtype,
                      void* stream);
 
+/* ---- Several continuations of one prompt: beam search, several samples of a
+ * prompt, a batch behind one system prompt.  The prompt's keys and values are
+ * kept and read once for all its sequences.  No counterpart in the reference
+ * (a batch there holds a copy of the prompt per sequence).  A step of a beam
+ * search is kf_attn_branch in every layer, kf_beam_select on the logits,
+ * kf_kv_cache_reorder on the caches. */
+
+/* Workspace bytes kf_attn_branch needs. */
+int kf_attn_branch_workspace_size(int G, int B, int N, int Hq, int Hkv, int D, int max_prefix,
+                                  int max_len, int dtype, size_t* bytes);
+
+/* Appends N new tokens to each sequence's own cache and attends each to the
+ * prefix of the sequence's group, to the sequence's own cached tokens, to itself
+ * and to the new tokens before it.
+ *   q_new [B, N, Hq, D], k_new, v_new [B, N, Hkv, D] contiguous, before RoPE;
+ *       sequence b belongs to group b / (B / G) (B is a multiple of G)
+ *   k_prefix, v_prefix [G, Hkv, Pmax, D] contiguous, prefix_lens [G] int32 on the
+ *       device: the groups' prefixes, rotated at positions 0 .. prefix_lens[g] - 1
+ *   k_cache, v_cache [B, Hkv, Smax, D] contiguous, lens [B] int32 on the device:
+ *       the sequences' own tokens; on return rows lens[b] + i of sequence b hold
+ *       new token i's rotated key and its value (i < counts[b])
+ *   counts  [B] int32 on the device, new tokens in use per sequence, 0 .. N, or
+ *       NULL for N: the others' rows of out are zero, their cache rows stay
+ *   rope_cos/sin [rope_rows, D/2]: new token i is at position prefix_lens[g] +
+ *       lens[b] + i and uses that row less rope_row_offset
+ *   out  [B, N, Hq, D]
+ *   max_prefix, max_len  upper bounds on prefix_lens[g] (<= Pmax, 0 allowed) and
+ *       on lens[b] + counts[b] (<= Smax)
+ *   q_norm_weight, k_norm_weight, norm_eps  as for kf_attn_decode
+ * The prefixes may not overlap the caches.  lens is not modified.  Inf and NaN in
+ * rows a token does not see do not reach its output.  prefix_lens, lens and counts live on the device, so they cannot be
+ * validated before the launch: a sequence with prefix_lens[g] outside 0 ..
+ * max_prefix, a count outside 0 .. N, lens[b] + counts[b] beyond max_len, or a
+ * table row outside [0, rope_rows) gets NaN outputs and no cache write. */
+int kf_attn_branch(const void* q_new, const void* k_new, const void* v_new, const void* k_prefix,
+                   const void* v_prefix, const int32_t* prefix_lens, void* k_cache, void* v_cache,
+                   const int32_t* lens, const int32_t* counts, const float* rope_cos,
+                   const float* rope_sin, int64_t rope_row_offset, int64_t rope_rows, void* out,
+                   void* workspace, size_t workspace_bytes, int G, int B, int N, int Pmax, int Smax,
+                   int Hq, int Hkv, int D, int max_prefix, int max_len, const float* q_norm_weight,
+                   const float* k_norm_weight, float norm_eps, int dtype, void* stream);
+
+/* Most beams of a group, and most candidates kf_beam_select picks. */
+#define KF_BEAM_MAX 64
+#define KF_BEAM_MAX_SELECT 128
+
+/* Workspace bytes kf_beam_select needs. */
+int kf_beam_select_workspace_size(int G, int W, int V, int K, int dtype, size_t* bytes);
+
+/* The K best continuations of each group of W beams.
+ *   logits  [G, W, V], row (g, w) at g * logits_stride_g + w * logits_stride_w
+ *   scores  [G, W] float32: the beams' summed log-probabilities so far
+ *   out_scores [G, K] float32, parents [G, K] int32, tokens [G, K] int64: the K
+ *       largest of scores[g][w] + log softmax(logits[g][w])[v], in 64 bits, largest
+ *       first, equals by the lowest w, then v; rounded to out_scores; parents are the w
+ * A score of -inf is a beam that is not in use; one that is not finite otherwise,
+ * and a row that is no distribution (NaN, +inf, or -inf throughout), count as
+ * such (a largest logit of 2^127 or more counts as +inf).  -inf is a token of no
+ * probability: never picked.  Behind the last candidate: score -inf, parent and token -1.  V <= KF_VERIFY_MAX_VOCAB. */
+int kf_beam_select(const void* logits, int64_t logits_stride_g, int64_t logits_stride_w,
+                   const float* scores, float* out_scores, int32_t* parents, int64_t* tokens,
+                   void* workspace, size_t workspace_bytes, int G, int W, int V, int K, int dtype,
+                   void* stream);
+
+/* Gives sequences the cache rows of the sequences they continue, in place, in
+ * n_caches KV caches (the layers of a model).  The B sequences form groups of W,
+ * one after the other; sequence b takes rows 0 .. lens[p] - 1 of sequence p =
+ * (b / W) * W + parents[b].
+ *   k_caches, v_caches  host arrays of n_caches device pointers to caches
+ *       [B, Hkv, Smax, D] contiguous; no two of them may overlap
+ *   lens  [B] int32 on the device: tokens of each sequence, in every cache; not
+ *       modified
+ *   parents  [B] int32 on the device, 0 .. W - 1 (a sequence may be continued by
+ *       several, and by none)
+ * Other rows stay as they are.  A sequence whose parent is out of range (-1: no
+ * beam), or whose parent's length is outside 0 .. Smax, is left alone. */
+int kf_kv_cache_reorder(void* const* k_caches, void* const* v_caches, int n_caches,
+                        const int32_t* lens, const int32_t* parents, int W, int B, int Hkv,
+                        int Smax, int D, int dtype, void* stream);
+
 /* Workspace bytes kf_attn_capture needs. */
 int kf_attn_capture_workspace_size(int B, int Sq, int Sk, int Hq, int Hkv, int D, int dtype,
                                    size_t* bytes);

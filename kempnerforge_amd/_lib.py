@@ -55,6 +55,13 @@ SIGNATURES = {
                           ctypes.c_double, _vp, _vp, _vp, _vp, _c_sz] + [_c_int] * 4 + [_vp], _c_int),
     "kf_verify_drafts_workspace_size": ([_c_int] * 5 + [_szp], _c_int),
     "kf_kv_cache_keep": ([_vp] * 4 + [_c_int] + [_vp] * 2 + [_c_int] * 6 + [_vp], _c_int),
+    "kf_attn_branch_workspace_size": ([_c_int] * 9 + [_szp], _c_int),
+    "kf_attn_branch": ([_vp] * 10 + [_fp, _fp, _c_i64, _c_i64, _vp, _vp, _c_sz] + [_c_int] * 10
+                       + [_fp, _fp, ctypes.c_float, _c_int, _vp], _c_int),
+    "kf_beam_select_workspace_size": ([_c_int] * 5 + [_szp], _c_int),
+    "kf_beam_select": ([_vp, _c_i64, _c_i64, _fp, _fp, _vp, _vp, _vp, _c_sz] + [_c_int] * 5 + [_vp],
+                       _c_int),
+    "kf_kv_cache_reorder": ([_vp, _vp, _c_int, _vp, _vp] + [_c_int] * 6 + [_vp], _c_int),
     "kf_attn_capture_workspace_size": ([_c_int] * 7 + [_szp], _c_int),
     "kf_attn_capture": ([_vp, _vp, _vp, _fp, _fp, _fp, _vp, _fp, _vp, _c_sz] + [_c_int] * 6
                         + [_c_i64] * 6 + [_c_int] * 2 + [_vp, _vp, _c_int, _vp], _c_int),

@@ -660,6 +660,162 @@ int kf_kv_cache_keep(void* const* k_caches, void* const* v_caches, const int32_t
                     dtype, (hipStream_t)stream);
 }
 
+}  // extern "C"
+
+namespace {
+int check_branch(int G, int B, int N, int Hq, int Hkv, int D, int max_prefix, int max_len,
+                 int dtype) {
+  int rc = check_common(B, N, max_len, Hq, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(G > 0 && B % G == 0, "the batch (%d) must be a positive multiple of the groups (%d)",
+               B, G);
+  KF_CHECK_ARG(max_prefix >= 0, "max_prefix must not be negative (got %d)", max_prefix);
+  KF_CHECK_ARG(B <= 65535, "at most 65535 sequences (got %d)", B);
+  // (a workgroup of 256 threads per four rows, fewer than 2^32 threads a launch)
+  KF_CHECK_ARG((int64_t)B * N * Hq < 1 << 26, "B * N * n_heads must be below 2^26 (%d, %d, %d)", B,
+               N, Hq);
+  KF_CHECK_ARG((int64_t)max_prefix + max_len <= INT_MAX,
+               "max_prefix + max_len exceeds 2^31 (%d, %d)", max_prefix, max_len);
+  return KF_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int kf_attn_branch_workspace_size(int G, int B, int N, int Hq, int Hkv, int D, int max_prefix,
+                                  int max_len, int dtype, size_t* bytes) {
+  int rc = check_branch(G, B, N, Hq, Hkv, D, max_prefix, max_len, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(bytes != nullptr, "bytes is null");
+  BranchArgs a = {};
+  a.G = G; a.B = B; a.N = N; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  a.max_prefix = max_prefix; a.max_len = max_len; a.dtype = dtype;
+  *bytes = branch_workspace(a);
+  return KF_OK;
+}
+
+int kf_attn_branch(const void* q_new, const void* k_new, const void* v_new, const void* k_prefix,
+                   const void* v_prefix, const int32_t* prefix_lens, void* k_cache, void* v_cache,
+                   const int32_t* lens, const int32_t* counts, const float* rope_cos,
+                   const float* rope_sin, int64_t rope_row_offset, int64_t rope_rows, void* out,
+                   void* workspace, size_t workspace_bytes, int G, int B, int N, int Pmax, int Smax,
+                   int Hq, int Hkv, int D, int max_prefix, int max_len, const float* q_norm_weight,
+                   const float* k_norm_weight, float norm_eps, int dtype, void* stream) {
+  int rc = check_branch(G, B, N, Hq, Hkv, D, max_prefix, max_len, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(q_new && k_new && v_new && prefix_lens && k_cache && v_cache && lens && rope_cos &&
+                   rope_sin && out && (max_prefix == 0 || (k_prefix && v_prefix)),
+               "null tensor pointer");
+  KF_CHECK_ARG(!q_norm_weight == !k_norm_weight,
+               "QK-norm needs both q_norm_weight and k_norm_weight (or neither)");
+  KF_CHECK_ARG(max_prefix <= Pmax, "max_prefix (%d) exceeds the prefix caches' length (%d)",
+               max_prefix, Pmax);
+  KF_CHECK_ARG(max_len <= Smax, "max_len (%d) exceeds the cache length (%d)", max_len, Smax);
+  KF_CHECK_ARG(rope_rows > 0, "rope tables must have at least one row");
+  const size_t el = dtype == F32 ? 4 : 2, row = (size_t)Hkv * D * el;
+  const uintptr_t pre[] = {(uintptr_t)k_prefix, (uintptr_t)v_prefix},
+                  own[] = {(uintptr_t)k_cache, (uintptr_t)v_cache};
+  for (uintptr_t p : pre)
+    for (uintptr_t c : own)
+      KF_CHECK_ARG(max_prefix == 0 || p + (size_t)G * Pmax * row <= c ||
+                       c + (size_t)B * Smax * row <= p,
+                   "a prefix overlaps a cache that is written");
+  BranchArgs a;
+  a.q_new = q_new; a.k_new = k_new; a.v_new = v_new;
+  a.k_prefix = k_prefix; a.v_prefix = v_prefix; a.prefix_lens = prefix_lens;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.lens = lens; a.counts = counts;
+  a.cos = rope_cos; a.sin = rope_sin; a.rope_row_offset = rope_row_offset;
+  a.rope_rows = rope_rows; a.out = out;
+  a.G = G; a.B = B; a.N = N; a.Pmax = Pmax; a.Smax = Smax; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  a.max_prefix = max_prefix; a.max_len = max_len;
+  a.q_norm_w = q_norm_weight; a.k_norm_w = k_norm_weight; a.norm_eps = norm_eps;
+  a.dtype = dtype; a.scale = 1.0f / sqrtf((float)D); a.stream = (hipStream_t)stream;
+  const size_t need = branch_workspace(a);
+  if (workspace_bytes < need || !workspace) {
+    set_error("workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return KF_ERR_WORKSPACE;
+  }
+  return branch_attention(a, workspace);
+}
+
+}  // extern "C"
+
+namespace {
+int check_select(int G, int W, int V, int K, int dtype) {
+  KF_CHECK_ARG(G > 0 && W > 0 && V > 0 && K > 0, "G, W, V, K must be positive (got %d, %d, %d, %d)",
+               G, W, V, K);
+  KF_CHECK_ARG(G <= 65535, "at most 65535 groups (got %d)", G);
+  KF_CHECK_ARG(W <= KF_BEAM_MAX, "at most %d beams of a group (got %d)", KF_BEAM_MAX, W);
+  KF_CHECK_ARG(K <= KF_BEAM_MAX_SELECT, "at most %d candidates are picked (got %d)",
+               KF_BEAM_MAX_SELECT, K);
+  KF_CHECK_ARG(V <= KF_VERIFY_MAX_VOCAB, "at most %d tokens in the vocabulary (got %d)",
+               KF_VERIFY_MAX_VOCAB, V);
+  KF_CHECK_ARG(dtype == F32 || dtype == BF16 || dtype == F16, "unsupported dtype code %d", dtype);
+  return KF_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int kf_beam_select_workspace_size(int G, int W, int V, int K, int dtype, size_t* bytes) {
+  int rc = check_select(G, W, V, K, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(bytes != nullptr, "bytes is null");
+  SelectArgs a = {};
+  a.G = G; a.W = W; a.V = V; a.K = K; a.dtype = dtype;
+  *bytes = select_workspace(a);
+  return KF_OK;
+}
+
+int kf_beam_select(const void* logits, int64_t logits_stride_g, int64_t logits_stride_w,
+                   const float* scores, float* out_scores, int32_t* parents, int64_t* tokens,
+                   void* workspace, size_t workspace_bytes, int G, int W, int V, int K, int dtype,
+                   void* stream) {
+  int rc = check_select(G, W, V, K, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(logits && scores && out_scores && parents && tokens, "null tensor pointer");
+  SelectArgs a;
+  a.logits = logits; a.logits_sg = logits_stride_g; a.logits_sw = logits_stride_w;
+  a.scores = scores; a.out_scores = out_scores; a.parents = parents; a.tokens = tokens;
+  a.G = G; a.W = W; a.V = V; a.K = K; a.dtype = dtype; a.stream = (hipStream_t)stream;
+  const size_t need = select_workspace(a);
+  if (workspace_bytes < need || !workspace) {
+    set_error("workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return KF_ERR_WORKSPACE;
+  }
+  return beam_select(a, workspace);
+}
+
+int kf_kv_cache_reorder(void* const* k_caches, void* const* v_caches, int n_caches,
+                        const int32_t* lens, const int32_t* parents, int W, int B, int Hkv,
+                        int Smax, int D, int dtype, void* stream) {
+  int rc = check_common(B, 1, Smax, Hkv, Hkv, D, dtype);
+  if (rc) return rc;
+  KF_CHECK_ARG(n_caches > 0, "n_caches must be positive (got %d)", n_caches);
+  KF_CHECK_ARG(W > 0 && B % W == 0, "the batch (%d) must be a positive multiple of the beams (%d)",
+               B, W);
+  KF_CHECK_ARG(W <= KF_BEAM_MAX, "at most %d beams of a group (got %d)", KF_BEAM_MAX, W);
+  KF_CHECK_ARG(B <= 65535, "at most 65535 sequences (got %d)", B);
+  KF_CHECK_ARG((int64_t)B * Hkv < 1 << 24, "B * n_kv_heads must be below 2^24 (%d, %d)", B, Hkv);
+  KF_CHECK_ARG(k_caches && v_caches && lens && parents, "null tensor pointer");
+  for (int c = 0; c < n_caches; ++c)
+    KF_CHECK_ARG(k_caches[c] && v_caches[c], "null tensor pointer (cache %d)", c);
+  constexpr int FEW = 256;  // (a model's layers: no allocation)
+  uintptr_t few[2 * FEW];
+  std::unique_ptr<uintptr_t[]> many(n_caches > FEW ? new (std::nothrow) uintptr_t[2 * (size_t)n_caches]
+                                                   : nullptr);
+  KF_CHECK_ARG(n_caches <= FEW || many, "no host memory to check %d caches", n_caches);
+  uintptr_t* at = n_caches > FEW ? many.get() : few;
+  for (int c = 0; c < n_caches; ++c) {
+    at[2 * c] = (uintptr_t)k_caches[c];
+    at[2 * c + 1] = (uintptr_t)v_caches[c];
+  }
+  KF_CHECK_ARG(!meet(at, 2 * n_caches, (size_t)B * Hkv * Smax * D * (dtype == F32 ? 4 : 2)),
+               "the caches overlap: they share memory that one writes");
+  return cache_reorder(k_caches, v_caches, n_caches, lens, parents, W, B, Hkv, Smax, D, dtype,
+                       (hipStream_t)stream);
+}
+
 int kf_attn_capture_workspace_size(int B, int Sq, int Sk, int Hq, int Hkv, int D, int dtype,
                                    size_t* bytes) {
   return kf_attn_fwd_workspace_size(B, Sq, Sk, Hq, Hkv, D, dtype, bytes);

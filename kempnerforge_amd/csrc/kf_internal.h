@@ -229,4 +229,44 @@ int cache_keep(void* const* k, void* const* v, const int32_t* const* lens,
                int32_t* const* lens_out, int n_caches, const int32_t* path, const int32_t* kept,
                int N, int B, int Hkv, int Smax, int D, int dtype, hipStream_t stream);
 
+// attention behind shared prefixes (kf_branch.hip)
+struct BranchArgs {
+  const void *q_new, *k_new, *v_new;  // [B, N, Hq, D], [B, N, Hkv, D] contiguous, pre-RoPE
+  const void *k_prefix, *v_prefix;    // [G, Hkv, Pmax, D] contiguous
+  const int32_t* prefix_lens;         // [G]
+  void *k_cache, *v_cache;            // [B, Hkv, Smax, D] contiguous, B a multiple of G
+  const int32_t* lens;                // [B] tokens of each sequence's own cache
+  const int32_t* counts;              // [B] new tokens in use, null: N
+  const float *cos, *sin;             // table; row = position - rope_row_offset
+  int64_t rope_row_offset, rope_rows;
+  void* out;                          // [B, N, Hq, D]
+  int G, B, N, Pmax, Smax, Hq, Hkv, D, max_prefix, max_len;
+  const float *q_norm_w, *k_norm_w;
+  float norm_eps;
+  int dtype;
+  float scale;
+  hipStream_t stream;
+};
+size_t branch_workspace(const BranchArgs& a);
+int branch_attention(const BranchArgs& a, void* workspace);
+
+// beam search: the selection over beams and vocabulary, and the caches of the beams
+// that go on (kf_beam.hip)
+struct SelectArgs {
+  const void* logits;  // row (g, w) at g * logits_sg + w * logits_sw, V contiguous values
+  int64_t logits_sg, logits_sw;
+  const float* scores;     // [G, W]
+  float* out_scores;       // [G, K]
+  int32_t* parents;        // [G, K]
+  int64_t* tokens;         // [G, K]
+  int G, W, V, K;
+  int dtype;
+  hipStream_t stream;
+};
+size_t select_workspace(const SelectArgs& a);
+int beam_select(const SelectArgs& a, void* workspace);
+int cache_reorder(void* const* k, void* const* v, int n_caches, const int32_t* lens,
+                  const int32_t* parents, int W, int B, int Hkv, int Smax, int D, int dtype,
+                  hipStream_t stream);
+
 }  // namespace kf

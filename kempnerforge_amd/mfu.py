@@ -173,7 +173,9 @@ _ATTN_KEYS = ("fwd_mfma", "fwd32_kernel", "bwd_dkdv", "dkdv_reduce_kernel", "bwd
               "widen_kernel", "narrow_kernel", "cache_append", "append_kernel",
               "append_rows_kernel", "tree_prep_kernel", "tree_rows_kernel", "tree_stream_kernel",
               "tree_merge_kernel", "verify_stats_kernel", "verify_walk_kernel", "verify_draw_kernel",
-              "cache_keep_kernel", "kf::attn", "flash", "fmha", "attention")
+              "cache_keep_kernel", "branch_prep_kernel", "branch_rows_kernel",
+              "branch_stream_kernel", "branch_merge_kernel", "select_rows_kernel",
+              "select_pick_kernel", "cache_reorder_kernel", "kf::attn", "flash", "fmha", "attention")
 _MATMUL_KEYS = ("gemm", "mm", "matmul", "dot", "bmm", "cublas", "nvjet", "cutlass",
                 "cijk_", "hipblaslt", "rocblas", "ck_tile", "wvsplitk")
 _COMM_KEYS = ("nccl", "rccl", "allreduce", "allgather", "reduce_scatter", "alltoall")

@@ -771,6 +771,177 @@ def cache_keep_raw(k_caches, v_caches, lens, path, kept, *, lens_out=None) -> No
                    "kf_kv_cache_keep")
 
 
+# --------------------------------------------------------------------------- continuations of one prompt
+BEAM_MAX, BEAM_MAX_SELECT = 64, 128  # KF_BEAM_MAX, KF_BEAM_MAX_SELECT
+
+
+def branch_decode_raw(q_new, k_new, v_new, k_prefix, v_prefix, prefix_lens, k_cache, v_cache, lens,
+                      cos, sin, *, rope_row_offset: int, max_prefix: int, max_len: int, counts=None,
+                      q_norm_weight=None, k_norm_weight=None, norm_eps: float = 1e-5):
+    """Attention of new tokens to the prefix that their group shares and to their own
+    sequence (``kf_attn_branch``); returns out ``[B,N,Hq,D]``.
+
+    ``k_prefix``, ``v_prefix`` ``[G,Hkv,Pmax,D]`` hold G prompts' rotated keys and
+    values, ``prefix_lens [G]`` int32 their lengths; B is a multiple of G, and sequence
+    b follows prompt ``b // (B // G)``.  ``q_new [B,N,Hq,D]``, ``k_new`` and ``v_new``
+    ``[B,N,Hkv,D]`` are N new tokens of each sequence before RoPE, ``counts [B]``
+    (integers, None: all) those in use; the others give zeros.  Token i is rotated at
+    position ``prefix_lens[g] + lens[b] + i``, written to row ``lens[b] + i`` of the
+    sequence's own cache (``[B,Hkv,Smax,D]``), and attends the prefix, the sequence's
+    own rows, itself and the new tokens before it.  ``max_prefix`` and ``max_len`` bound
+    ``prefix_lens[g]`` and ``lens[b] + counts[b]``.  ``lens`` is not modified.
+
+    As in :func:`decode_raw`, what lies on the device is checked there: a sequence whose
+    lengths, count or RoPE rows are out of range gets NaN outputs and no cache write."""
+    lib = _lib.load()
+    qs, ks, cs, ps, dtype = q_new.shape, k_new.shape, k_cache.shape, k_prefix.shape, q_new.dtype
+    if not len(qs) == len(ks) == len(cs) == len(ps) == 4:
+        raise ValueError("q_new, k_new, v_new, the prefixes and the caches must have four "
+                         "dimensions")
+    B, N, Hq, D = qs
+    G, Hkv, Pmax, Smax = ps[0], cs[1], ps[2], cs[2]
+    _c_ints(batch=B, new_tokens=N, n_heads=Hq, n_kv_heads=Hkv, max_seq_len=Smax, head_dim=D,
+            prefix_length=Pmax)
+    if ks != (B, N, Hkv, D) or v_new.shape != ks:
+        raise ValueError(f"k_new and v_new must be [{B}, {N}, {Hkv}, {D}] "
+                         f"(got {tuple(ks)}, {tuple(v_new.shape)})")
+    if cs[0] != B or cs[3] != D or v_cache.shape != cs:
+        raise ValueError(f"the KV caches must be [{B}, n_kv_heads, max_seq_len, {D}] "
+                         f"(got {tuple(cs)}, {tuple(v_cache.shape)})")
+    if G < 1 or B % G or ps[1] != Hkv or ps[3] != D or v_prefix.shape != ps:
+        raise ValueError(f"the prefixes must be [groups, {Hkv}, length, {D}] with groups dividing "
+                         f"{B} (got {tuple(ps)}, {tuple(v_prefix.shape)})")
+    if not (dtype == k_new.dtype == v_new.dtype == k_cache.dtype == v_cache.dtype
+            == k_prefix.dtype == v_prefix.dtype):
+        raise TypeError("q_new, k_new, v_new, the prefixes and the caches must share a dtype")
+    if not all(t.is_contiguous() for t in (k_cache, v_cache, k_prefix, v_prefix)):
+        raise ValueError("KV caches and prefixes must be contiguous [.., n_kv_heads, length, "
+                         "head_dim]")
+    for name, t, n in (("lens", lens, B), ("prefix_lens", prefix_lens, G)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != (n,):
+            raise TypeError(f"{name} must be a contiguous int32 tensor [{n}]")
+    dev = _one_device(q_new, k_new, v_new, k_prefix, v_prefix, prefix_lens, k_cache, v_cache, lens,
+                      cos, sin, counts)
+    q_new, k_new, v_new = q_new.contiguous(), k_new.contiguous(), v_new.contiguous()
+    cos = _rope_table(cos, 1, D // 2, "rope_cos")
+    sin = _rope_table(sin, 1, D // 2, "rope_sin")
+    if cos.shape != sin.shape:
+        raise ValueError("rope_cos and rope_sin must have the same shape")
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("QK-norm needs both q_norm_weight and k_norm_weight")
+    qnw = knw = None
+    # (C ints: what is out of their range must not come back into the caches')
+    dt, max_len = _dtype_code(q_new), max(min(int(max_len), Smax + 1), 0)
+    max_prefix = max(min(int(max_prefix), Pmax + 1), -1)
+    with _on_device(dev):
+        _, _, counts = _tree_args(None, counts, B, N)
+        if q_norm_weight is not None:
+            qnw, knw = (_norm_weight(w, D, q_new.device) for w in (q_norm_weight, k_norm_weight))
+        out = torch.empty_like(q_new)
+        # (max_len grows from step to step: asked per step, not kept)
+        nbytes = _lib.size_out()
+        rc = lib.kf_attn_branch_workspace_size(G, B, N, Hq, Hkv, D, max_prefix, max_len, dt,
+                                               ctypes.byref(nbytes))
+        if rc == 0:
+            ws = _workspace(nbytes.value, q_new.device)
+            rc = lib.kf_attn_branch(
+                q_new.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_prefix.data_ptr(),
+                v_prefix.data_ptr(), prefix_lens.data_ptr(), k_cache.data_ptr(),
+                v_cache.data_ptr(), lens.data_ptr(), _ptr(counts), cos.data_ptr(), sin.data_ptr(),
+                int(rope_row_offset), cos.shape[0], out.data_ptr(), ws.data_ptr(), ws.numel(), G, B,
+                N, Pmax, Smax, Hq, Hkv, D, max_prefix, max_len, _ptr(qnw), _ptr(knw),
+                float(norm_eps), dt, _stream(q_new))
+        _lib.check(rc, "kf_attn_branch")
+    return out
+
+
+def beam_select_raw(logits, scores, *, select: int):
+    """The ``select`` best continuations of each group of beams (``kf_beam_select``);
+    returns scores ``[G,select]`` float32, parents ``[G,select]`` int32 and tokens
+    ``[G,select]`` int64, all on the device.
+
+    ``logits [G,W,V]`` (contiguous values; any strides between rows) are the W beams' of
+    each group, ``scores [G,W]`` float32 their summed log-probabilities.  Candidate (w,
+    v) has ``scores[g,w] + log softmax(logits[g,w])[v]``; the largest come first, equals
+    by the lowest beam, then token.  A score of -inf (or none: NaN, +inf) is a beam that
+    is not in use, a logit of -inf a token that cannot be picked, and a row that is no
+    distribution (NaN, +inf, -inf throughout) has no candidates.  Behind the last
+    candidate: score -inf, parent and token -1."""
+    lib = _lib.load()
+    ls = logits.shape
+    if len(ls) != 3 or (logits.stride(2) != 1 and ls[2] != 1):
+        raise ValueError("logits must be [G, W, V] with contiguous values "
+                         f"(got {tuple(ls)}, strides {logits.stride()})")
+    G, W, V = ls
+    _c_ints(groups=G, vocabulary=V)
+    if not 1 <= W <= BEAM_MAX:
+        raise ValueError(f"1 to {BEAM_MAX} beams of a group (got {W})")
+    if not 1 <= select <= BEAM_MAX_SELECT:
+        raise ValueError(f"select must lie in [1, {BEAM_MAX_SELECT}] (got {select})")
+    if scores.shape != (G, W) or scores.dtype != torch.float32:
+        raise ValueError(f"scores must be float32 [{G}, {W}] "
+                         f"(got {scores.dtype} {tuple(scores.shape)})")
+    dev = _one_device(logits, scores)
+    dt, scores, K = _dtype_code(logits), scores.contiguous(), int(select)
+    with _on_device(dev):
+        best = torch.empty(G, K, dtype=torch.float32, device=logits.device)
+        parents = torch.empty(G, K, dtype=torch.int32, device=logits.device)
+        tokens = torch.empty(G, K, dtype=torch.int64, device=logits.device)
+        ws = _workspace(_size("kf_beam_select_workspace_size", dev, G, W, V, K, dt), logits.device)
+        _lib.check(lib.kf_beam_select(logits.data_ptr(), logits.stride(0), logits.stride(1),
+                                      scores.data_ptr(), best.data_ptr(), parents.data_ptr(),
+                                      tokens.data_ptr(), ws.data_ptr(), ws.numel(), G, W, V, K, dt,
+                                      _stream(logits)),
+                   "kf_beam_select")
+    return best, parents, tokens
+
+
+def cache_reorder_raw(k_caches, v_caches, lens, parents) -> None:
+    """Gives sequences the cache rows of those they continue, in the KV caches of all
+    layers, in place (``kf_kv_cache_reorder``): with ``parents [G,W]`` int32, sequence
+    ``g W + w`` takes rows ``0 .. lens[p] - 1`` of sequence ``p = g W + parents[g,w]``.
+    ``k_caches`` and ``v_caches`` are lists with one tensor per layer (``[G W,
+    n_kv_heads, max_seq_len, head_dim]`` contiguous), ``lens [G W]`` int32 the sequences'
+    lengths in all of them (not modified).  Other rows stay as they are.  A sequence
+    whose parent is out of range (-1: no beam) is left alone."""
+    k_caches, v_caches = list(k_caches), list(v_caches)
+    n = len(k_caches)
+    if n == 0 or n != len(v_caches):
+        raise ValueError(f"k_caches and v_caches need one tensor per cache (got {n}, "
+                         f"{len(v_caches)})")
+    ptrs = array.array("Q", bytes(16 * n))
+    caches, k0 = k_caches + v_caches, k_caches[0]
+    try:
+        dev = _lib.native().same(caches, ptrs, 0)
+    except ValueError as e:
+        raise ValueError("KV caches must be contiguous [B, n_kv_heads, max_seq_len, head_dim], of "
+                         f"one device, dtype and shape: {e}") from None
+    if k0.dim() != 4:
+        raise ValueError("KV caches must be [B, n_kv_heads, max_seq_len, head_dim]")
+    B, Hkv, Smax, D = k0.shape
+    _c_ints(batch=B, n_kv_heads=Hkv, max_seq_len=Smax, head_dim=D)
+    if parents.dim() != 2 or parents.shape[0] * parents.shape[1] != B:
+        raise ValueError(f"parents must be [groups, beams] for {B} sequences "
+                         f"(got {tuple(parents.shape)})")
+    W = parents.shape[1]
+    if W > BEAM_MAX:
+        raise ValueError(f"at most {BEAM_MAX} beams of a group (got {W})")
+    if parents.dtype != torch.int32 or lens.dtype != torch.int32 or lens.shape != (B,):
+        raise TypeError(f"parents and lens [{B}] must be int32 "
+                        f"(got {parents.dtype}, {lens.dtype} {tuple(lens.shape)})")
+    where = {dev, lens.get_device(), parents.get_device()}
+    if where != {dev} or dev < 0:
+        _require_gpu(*caches, lens, parents)
+        raise RuntimeError(f"the tensors must lie on one device (got {sorted(where)})")
+    lens, parents = lens.contiguous(), parents.contiguous()
+    at = ptrs.buffer_info()[0]
+    with _on_device(dev):
+        _lib.check(_lib.load().kf_kv_cache_reorder(at, at + 8 * n, n, lens.data_ptr(),
+                                                   parents.data_ptr(), W, B, Hkv, Smax, D,
+                                                   _dtype_code(k0), _stream(k0)),
+                   "kf_kv_cache_reorder")
+
+
 def capture_raw(q, k, v, cos, sin, *, causal: bool, k_rotated: bool, k_layout: str = "bshd",
                 doc_ids=None, key_padding_mask=None):
     """out, probs, lse with probs the float32 softmax matrix ``[B,Hq,Sq,Sk]``

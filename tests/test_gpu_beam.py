@@ -1,0 +1,300 @@
+"""GPU parity of the beams' selection (kf_beam_select) and the caches' reordering
+(kf_kv_cache_reorder) with the 64-bit restatement."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gpu_util import DEV, announce, half_ulp
+from kempnerforge_amd import ops
+from oracle import branch_ref
+
+pytestmark = pytest.mark.gpu
+
+BF, FH, F32 = torch.bfloat16, torch.float16, torch.float32
+INF = float("inf")
+
+# How far a row's log of its sum may be off.  A term 2^t is off by |t| 2^-24 (its
+# argument's rounding) and |t| 2^-25 (log2 e in 32 bits) times ln 2, and by 2^-22 (the
+# instruction); the mean of |t| over a distribution of V <= 2^17 values is at most 17 +
+# log2 e; a thread's values are 128 at most, in sums of 8 and 16: 24 steps of 2^-24.
+LSE = 18.5 * 1.5 * 2.0 ** -24 * 0.7 + 2.0 ** -22 + 24 * 2.0 ** -24
+
+
+def inputs(dtype, G, W, V, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = 2.5 * torch.randn(G, W, V, generator=g)
+    if V > 16:
+        top = torch.randint(V, (G, W, 6), generator=g)
+        x.scatter_(2, top, 6.0 + 2.0 * torch.randn(G, W, 6, generator=g))
+    return x.to(dtype), -9.0 * torch.rand(G, W, generator=g)
+
+
+def call(x, s, K):
+    out = ops.beam_select_raw(x.to(DEV) if not x.is_cuda else x, s.to(DEV), select=K)
+    torch.cuda.synchronize()
+    return out
+
+
+def check(x, s, K, got):
+    """The scores at every place, to their error; the candidates the same where the
+    64-bit values tell them apart by more than that, and in the order of places where
+    they are equal."""
+    G, W, V = x.shape
+    best, parents, tokens = (t.cpu() for t in got)
+    want, wp, wt = branch_ref.select(x, s, K)
+    assert best.dtype == F32 and parents.dtype == torch.int32 and tokens.dtype == torch.int64
+    none = torch.isinf(want)
+    assert torch.equal(torch.isinf(best), none) and (best[none] == -INF).all()
+    assert (parents[none] == -1).all() and (tokens[none] == -1).all()
+    ok = ~none
+    err = (best.double() - want)[ok].abs()
+    assert (err <= LSE + half_ulp(want[ok], F32)).all(), err.max()
+    total = branch_ref.totals(x, s).view(G, W * V)
+    at = parents.long() * V + tokens
+    for g in range(G):
+        n = int(ok[g].sum())
+        assert len(set(at[g, :n].tolist())) == n
+        mine = total[g, at[g, :n]]
+        assert ((mine - want[g, :n]).abs() <= 2 * LSE).all(), g
+        # equal values of one beam: lowest token first
+        for i in range(1, n):
+            if mine[i] == mine[i - 1] and parents[g, i] == parents[g, i - 1]:
+                assert tokens[g, i] > tokens[g, i - 1]
+        apart = torch.ones(n, dtype=torch.bool)
+        nxt = total[g].topk(min(n + 1, W * V)).values
+        gap = (nxt[:-1] - nxt[1:])
+        gap[gap == 0] = INF  # (equals have an order of their own)
+        for i in range(n):
+            near = [gap[j] for j in (i - 1, i) if 0 <= j < len(gap)]
+            apart[i] = not near or min(near) > 2 * LSE
+        assert torch.equal(parents[g, :n][apart], wp[g, :n][apart])
+        assert torch.equal(tokens[g, :n][apart], wt[g, :n][apart])
+
+
+@pytest.mark.parametrize("dtype,G,W,V,K", [
+    (F32, 1, 1, 1, 1), (F32, 1, 4, 1, 8), (BF, 1, 1, 7, 7), (BF, 2, 3, 5, 9), (FH, 3, 1, 300, 2),
+    (F32, 1, 4, 32000, 8), (BF, 3, 5, 50001, 10), (FH, 2, 4, 50001, 5), (BF, 5, 8, 8192, 16),
+    (F32, 2, 3, 4097, 6), (BF, 1, 64, 1000, 128), (F32, 2, 16, 3001, 32), (FH, 1, 33, 2048, 47),
+    (BF, 2, 2, 33000, 48), (BF, 2, 7, 1234, 49), (BF, 16, 8, 131072, 16), (F32, 64, 8, 40003, 16),
+    (BF, 9, 64, 9000, 128),
+])
+def test_against_64_bits(dtype, G, W, V, K):
+    announce(f"select {dtype} {G} {W} {V} {K}")
+    x, s = inputs(dtype, G, W, V, seed=V + K)
+    check(x, s, K, call(x, s, K))
+
+
+@pytest.mark.parametrize("dtype,fill", [(BF, 0.0), (F32, -3.5), (FH, 2.0)])
+@pytest.mark.parametrize("K", [4, 64])
+def test_equal_values(dtype, fill, K):
+    """Rows of one value, and of two: the lowest beams and tokens."""
+    announce(f"select equals {dtype} {K}")
+    x = torch.full((2, 3, 5003), fill, dtype=dtype)
+    x[1, :, ::2] += 1
+    s = torch.zeros(2, 3)
+    best, parents, tokens = (t.cpu() for t in call(x, s, K))
+    assert (parents == 0).all()
+    assert torch.equal(tokens[0], torch.arange(K)) and torch.equal(tokens[1], 2 * torch.arange(K))
+    check(x, s, K, (best, parents, tokens))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("K,hot", [(16, 10), (48, 40), (100, 40), (3, 2)])
+@pytest.mark.parametrize("lead", [0, 3])
+def test_values_ordered_against_the_threads(dtype, K, hot, lead):
+    """All of the large values lie with few threads: more of them pass the bound on the
+    K-th largest than are gathered at once."""
+    announce(f"select hot lanes {dtype} {K} {hot} {lead}")
+    V, e = 40000, 16 // torch.empty((), dtype=dtype).element_size()
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(1, 2, V, generator=g)
+    lane = (torch.arange(V) + lead) // e % 64
+    x = torch.where(lane < hot, x.abs() + 8, x).to(dtype)
+    s = torch.tensor([[-0.3, 0.0]])
+    buf = torch.zeros(2 * V + lead + e, dtype=dtype, device=DEV)
+    view = buf[lead:lead + 2 * V].view(1, 2, V)
+    view.copy_(x)
+    check(x, s, K, call(view, s, K))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_beams_without_candidates(dtype):
+    """Beams that are not in use, rows that are no distribution, tokens of no
+    probability."""
+    announce(f"select none {dtype}")
+    G, W, V, K = 4, 5, 3000, 10
+    x, s = inputs(dtype, G, W, V)
+    s[0, 1], s[0, 3], s[1, 2] = -INF, float("nan"), INF
+    x[1, 0, 2999], x[1, 1, 5], x[1, 3] = float("nan"), INF, -INF
+    x[2, :, 4:] = -INF              # twenty candidates
+    x[3, :, 1:] = -INF              # five
+    out = call(x, s, K)
+    check(x, s, K, out)
+    best, parents, tokens = (t.cpu() for t in out)
+    assert set(parents[0].tolist()) <= {0, 2, 4} and (parents[1] == 4).all()
+    assert (tokens[3, :5] == 0).all() and (tokens[3, 5:] == -1).all() and (best[3, 5:] == -INF).all()
+    # nothing at all
+    best, parents, tokens = call(x, torch.full((G, W), -INF), K)
+    assert (best == -INF).all() and (parents == -1).all() and (tokens == -1).all()
+
+
+@pytest.mark.parametrize("shift", [0.0, 1000.0, -3e4])
+def test_a_constant_moves_nothing(shift):
+    """Rows of whole numbers, so that the constant is exact."""
+    announce(f"select shift {shift}")
+    g = torch.Generator().manual_seed(1)
+    x = torch.randint(-20, 20, (2, 4, 9001), generator=g).float()
+    s = -torch.rand(2, 4, generator=g)
+    a, b = call(x, s, 8), call(x + shift, s, 8)
+    assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+    assert (a[0] - b[0]).abs().max().item() <= 2 * LSE + 2.0 ** -20
+
+
+def test_scores_far_apart():
+    """A beam that lies far behind is not picked, and one far down picks among its own."""
+    announce("select far scores")
+    x, s = inputs(F32, 2, 3, 5000)
+    s[0], s[1] = torch.tensor([0.0, -1e4, -2e30]), torch.tensor([-1e4, -1e4 - 50, -3e4])
+    check(x[:1], s[:1], 6, call(x[:1], s[:1], 6))
+    _, parents, tokens = (t.cpu() for t in call(x[1:], s[1:], 6))
+    assert (parents == 0).all()
+    assert torch.equal(tokens[0], x[1, 0].sort(descending=True, stable=True).indices[:6])
+
+
+def test_strided_logits():
+    """The last token's logits of every sequence: rows apart, off 16-byte boundaries."""
+    announce("select strides")
+    B, T, V, W = 6, 3, 4001, 3
+    x, _ = inputs(BF, B, T, V)
+    s = -torch.rand(2, W, generator=torch.Generator().manual_seed(0))
+    last = x.to(DEV)[:, -1].view(2, W, V)
+    assert not last.is_contiguous()
+    check(x[:, -1].reshape(2, W, V), s, 6, call(last, s, 6))
+
+
+def test_graph_replays():
+    announce("select graph")
+    x, s = inputs(BF, 3, 4, 20000)
+    x, s = x.to(DEV), s.to(DEV)
+    ops.beam_select_raw(x, s, select=8)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.beam_select_raw(x, s, select=8)
+    for rep in range(4):
+        a, b = inputs(BF, 3, 4, 20000, seed=10 + rep)
+        if rep == 2:
+            b[1, 1:] = -INF
+        x.copy_(a)
+        s.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = ops.beam_select_raw(x, s, select=8)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), rep
+
+
+# ------------------------------------------------------------------ reorder
+def _caches(dtype, n, B, H, S, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(B, H, S, D, generator=g).to(dtype) for _ in range(2 * n)]
+
+
+def _reorder(caches, lens, parents, to=lambda t: t.to(DEV)):
+    n = len(caches) // 2
+    dev = [to(t) for t in caches]
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ops.cache_reorder_raw(dev[:n], dev[n:], lens_d,
+                          torch.tensor(parents, dtype=torch.int32, device=DEV))
+    torch.cuda.synchronize()
+    assert lens_d.tolist() == list(lens)
+    return dev
+
+
+@pytest.mark.parametrize("dtype,n,parents,H,S,D,lens", [
+    (BF, 2, [[0]], 2, 9, 64, [5]),
+    (BF, 3, [[1, 0]], 2, 9, 64, [5, 5]),                      # a swap
+    (BF, 2, [[0, 0, 1, 3], [3, 2, 1, 0]], 8, 70, 128, [64, 64, 64, 64, 1, 33, 70, 0]),
+    (FH, 1, [[2, 2, 2, 2, 2]], 1, 40, 128, [40, 3, 17, 9, 0]),
+    (F32, 2, [[1, 2, 0], [2, 0, 2]], 2, 33, 64, [33, 12, 7, 1, 2, 3]),  # a cycle
+    (BF, 2, [[(5 * w + 3) % 9 for w in range(9)]], 2, 300, 64, list(range(9, 18))),
+    (BF, 1, [[(7 * w) % 16 for w in range(16)]] * 2, 2, 129, 128, [128 - w for w in range(32)]),
+    (BF, 1, [[(3 * w + 1) % 17 // 2 for w in range(17)]], 1, 50, 128, [50] * 17),
+    (F32, 1, [[(11 * w + 5) % 64 for w in range(64)]], 1, 20, 128, [20 - w % 5 for w in range(64)]),
+    (BF, 2, [[1, 0, 0]], 3, 21, 6, [21, 20, 0]),              # rows of 12 bytes
+    (FH, 1, [[2, 0, 1]], 2, 11, 81 * 2, [11, 4, 9]),
+    (BF, 70, [[1, 1]], 1, 5, 64, [5, 4]),                     # more caches than one launch takes
+    (BF, 2, [[-1, 0, 9, 1]], 2, 12, 64, [12, 3, 5, 6]),       # parents out of range
+    (BF, 2, [[1, 0, 3, 2]], 2, 12, 64, [12, 13, -1, 6]),      # lengths out of range
+])
+def test_reorder(dtype, n, parents, H, S, D, lens):
+    announce(f"reorder {dtype} {parents} {S} {D}")
+    caches = _caches(dtype, n, len(lens), H, S, D)
+    got = _reorder(caches, lens, parents)
+    for c, (x, y) in enumerate(zip(caches, got)):
+        assert torch.equal(y.cpu(), branch_ref.reorder(x, lens, parents)), c
+
+
+def test_reorder_misaligned():
+    announce("reorder misaligned")
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        o = buf[1:].view(t.shape)
+        o.copy_(t)
+        return o
+
+    lens, parents = [30, 7, 30], [[2, 2, 0]]
+    caches = _caches(BF, 2, 3, 2, 31, 128)
+    for x, y in zip(caches, _reorder(caches, lens, parents, off)):
+        assert torch.equal(y.cpu(), branch_ref.reorder(x, lens, parents))
+
+
+def test_reorder_leaves_nan_rows_alone():
+    announce("reorder NaN")
+    caches = _caches(BF, 1, 4, 2, 20, 64)
+    for t in caches:
+        t[:, :, 9:] = float("nan")
+        t[2, :, 3] = INF
+    parents = [[2, 0, 1, 2]]
+    for x, y in zip(caches, _reorder(caches, [9] * 4, parents)):
+        want = branch_ref.reorder(x, [9] * 4, parents)
+        assert torch.equal(y.cpu().view(torch.int16), want.view(torch.int16))
+
+
+def test_reorder_captured():
+    """Replayed with other parents and lengths."""
+    announce("reorder graph")
+    caches = [t.to(DEV) for t in _caches(BF, 2, 4, 2, 50, 64)]
+    lens = torch.tensor([3, 4, 5, 6], dtype=torch.int32, device=DEV)
+    par = torch.tensor([[1, 0, 3, 2]], dtype=torch.int32, device=DEV)
+    ops.cache_reorder_raw(caches[:2], caches[2:], lens, par)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.cache_reorder_raw(caches[:2], caches[2:], lens, par)
+    for rep in range(4):
+        par.copy_(torch.tensor([[rep, 3, 0, (rep + 1) % 4]], dtype=torch.int32))
+        lens.copy_(torch.tensor([50 - rep, 7, 20 * rep % 51, 33], dtype=torch.int32))
+        before = [t.cpu() for t in caches]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(before, caches):
+            assert torch.equal(y.cpu(), branch_ref.reorder(x, lens.tolist(), par.tolist())), rep
+
+
+def test_reorder_past_32_bit_offsets():
+    announce("reorder long caches")
+    k = torch.zeros(4, 2, 1 << 22, 128, dtype=BF, device=DEV)  # 8.6 GB
+    v = torch.zeros(4, 2, 1 << 22, 128, dtype=BF, device=DEV)
+    rows = torch.randn(2, 4, 2, 40, 128, generator=torch.Generator().manual_seed(0)).bfloat16()
+    at = (1 << 22) - 40
+    for t, r in zip((k, v), rows):
+        t[:, :, at:] = r.to(DEV)
+    parents = [[3, 0, 0, 1]]
+    lens = torch.tensor([(1 << 22)] * 4, dtype=torch.int32, device=DEV)
+    ops.cache_reorder_raw([k], [v], lens, torch.tensor(parents, dtype=torch.int32, device=DEV))
+    for t, r in zip((k, v), rows):
+        assert torch.equal(t[:, :, at:].cpu(), branch_ref.reorder(r, [40] * 4, parents))
