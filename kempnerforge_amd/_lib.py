@@ -124,9 +124,13 @@ def native():
                                f"{module.torch_version}, this is {torch.__version__}; build it again "
                                "with `python -c 'import __graft_entry__ as g; g.build()'`")
         lib = load()
-        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "kf_attn_tree_workspace_size", "kf_attn_tree", "kf_verify_drafts_workspace_size",
-            "kf_verify_drafts", "kf_kv_cache_keep")))
+        for bind, names in ((module.bind, (
+                "kf_attn_tree_workspace_size", "kf_attn_tree", "kf_verify_drafts_workspace_size",
+                "kf_verify_drafts", "kf_kv_cache_keep")),
+                            (module.bind_branches, (
+                "kf_attn_branch_workspace_size", "kf_attn_branch", "kf_beam_select_workspace_size",
+                "kf_beam_select", "kf_kv_cache_reorder"))):
+            bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names))
         _native = module
     return _native
 

@@ -13,6 +13,7 @@
 // launches the smallest calls.
 #include "kf_common.h"
 #include "kf_internal.h"
+#include "kf_mfma.h"
 #include "kf_row.h"
 
 #include <algorithm>
@@ -38,7 +39,14 @@ struct TopLds {
   V val[CAP];
   int idx[CAP];
   int count, best;
-  V red[NT / 64];
+  V edge, red[NT / 64];
+  __device__ __forceinline__ void add(V x, int i) {
+    const int at = atomicAdd(&count, 1);
+    if (at < CAP) {
+      val[at] = x;
+      idx[at] = i;
+    }
+  }
 };
 
 __device__ __forceinline__ float lane_of(float x, int j) {
@@ -51,28 +59,23 @@ __device__ __forceinline__ double lane_of(double x, int j) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// own: the thread's largest value (-inf: none).  some(T, f): f(value, index) for the
-// thread's values >= T above -inf.  out(place, value, index), place < K; returns how many
-// places there are values for.
-template <typename V, typename Some, typename Out>
-__device__ __forceinline__ int top_k(int K, V own, Some some, Out out, TopLds<V>& lds) {
-  const int t = threadIdx.x, lane = t & 63;
-  lds.top[t] = own;
-  if (t == 0) lds.count = 0;
-  __syncthreads();
-  V edge = INFINITY;
+// A value that K of the workgroup's values reach, if there are as many above -inf, given
+// each thread's largest in lds.top: by one wavefront, each lane gets it.
+template <typename V>
+__device__ __forceinline__ V top_bound(int K, const TopLds<V>& lds) {
+  const int lane = threadIdx.x & 63;
+  V g[NT / 64], edge = INFINITY;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) g[i] = lds.top[lane + 64 * i];
   if (K <= 48) {
-    V g = lds.top[lane];
 #pragma unroll
-    for (int i = 1; i < NT / 64; ++i) g = fmax(g, lds.top[lane + 64 * i]);
+    for (int i = 1; i < NT / 64; ++i) g[0] = fmax(g[0], g[i]);
     int above = 0;
-    for (int j = 0; j < 64; ++j) above += lane_of(g, j) > g;
-    if (above < K) edge = g;
-  } else {
-    V g[NT / 64];
-    int above[NT / 64] = {};
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) g[i] = lds.top[lane + 64 * i];
+    for (int j = 0; j < 64; ++j) above += lane_of(g[0], j) > g[0];
+    if (above < K) edge = g[0];
+  } else {
+    int above[NT / 64] = {};
     for (int j = 0; j < NT; ++j) {
       const V x = lds.top[j];
 #pragma unroll
@@ -84,43 +87,47 @@ __device__ __forceinline__ int top_k(int K, V own, Some some, Out out, TopLds<V>
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) edge = fmin(edge, __shfl_xor(edge, o, 64));
-  if (own >= edge)
-    some(edge, [&](V x, int i) {
-      const int at = atomicAdd(&lds.count, 1);
-      if (at < CAP) {
-        lds.val[at] = x;
-        lds.idx[at] = i;
-      }
-    });
-  __syncthreads();
-  const int n = lds.count;
-  if (n <= CAP) {
-    for (int a = t; a < n; a += NT) {
-      const V x = lds.val[a];
-      const int i = lds.idx[a];
-      int place = 0;
-      for (int b = 0; b < n; ++b) place += lds.val[b] > x || (lds.val[b] == x && lds.idx[b] < i);
-      if (place < K) out(place, x, i);
+  return edge;
+}
+
+// The K first of the n <= CAP gathered values, by out(place, value, index).
+template <typename V, typename Out>
+__device__ __forceinline__ void top_order(int K, int n, Out out, const TopLds<V>& lds) {
+  for (int a = threadIdx.x; a < n; a += NT) {
+    const V x = lds.val[a];
+    const int i = lds.idx[a];
+    int place = 0;
+#pragma unroll 4
+    for (int b = 0; b < n; ++b) {
+      const V y = lds.val[b];
+      place += (y > x) | ((y == x) & (lds.idx[b] < i));
     }
-    return min(n, K);
+    if (place < K) out(place, x, i);
   }
+}
+
+// The same, one at a time: each(f) gives f(value, index) for the thread's values; there are
+// K of them.
+template <typename V, typename Each, typename Out>
+__device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds<V>& lds) {
+  const int t = threadIdx.x;
   V last = INFINITY;
   int after = -1;
   for (int place = 0; place < K; ++place) {
     // the largest value behind (last, after), then the lowest index that has it
     V x = -INFINITY;
-    some(edge, [&](V v, int i) {
+    each([&](V v, int i) {
       if (v < last || (v == last && i > after)) x = fmax(x, v);
     });
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) x = fmax(x, __shfl_xor(x, o, 64));
     __syncthreads();
-    if (lane == 0) lds.red[t >> 6] = x;
+    if ((t & 63) == 0) lds.red[t >> 6] = x;
     if (t == 0) lds.best = INT_MAX;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) x = fmax(x, lds.red[w]);
-    some(edge, [&](V v, int i) {
+    each([&](V v, int i) {
       if (v == x && (v < last || i > after)) atomicMin(&lds.best, i);
     });
     __syncthreads();
@@ -128,7 +135,6 @@ __device__ __forceinline__ int top_k(int K, V own, Some some, Out out, TopLds<V>
     last = x;
     after = lds.best;
   }
-  return K;
 }
 
 // ------------------------------------------------------------------ rows
@@ -144,151 +150,256 @@ struct Candidate {
 // Slices of a row of V values, U granules of E a thread.
 int slices_of(int V, int E, int U) { return ((V + E - 1) / E + NT * U - 1) / (NT * U); }
 
+// A granule of -inf, and one without its first k values.
+template <typename T>
+__device__ __forceinline__ u32x4 none_of() {
+  const uint32_t n = sizeof(T) == 4                ? 0xff800000u
+                     : std::is_same<T, bf16>::value ? 0xff80ff80u
+                                                    : 0xfc00fc00u;
+  return u32x4{n, n, n, n};
+}
+template <typename T>
+__device__ __forceinline__ void drop_first(u32x4& x, int k) {
+  constexpr int P = 4 / sizeof(T);  // values of a dword
+  const u32x4 none = none_of<T>();
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    x[d] = k >= P * (d + 1)                ? none[d]
+           : P == 2 && k == P * d + 1      ? (x[d] & 0xffff0000u) | (none[d] & 0xffffu)
+                                           : x[d];
+}
+
+// Granules that hold a value of the bound or more, put aside to be looked through by all
+// threads: eight tests and appends in each thread's own code would cost as much as the
+// sums.
+constexpr int GRANULES = 256;
+
 // Workgroup (row, slice).  Exponentials are float32 instructions of the difference to the
-// thread's maximum, x log2 e - m log2 e in one rounding (2^-24 of it, so a term of weight
-// p is off by 2^-24 |ln p|), sums of a thread's values in 32 bits, of the threads' in 64;
-// what m log2 e was rounded by is taken back in 64 bits.  A thread's granules are counted
-// from the row's first value, whatever its alignment (the loads may be unaligned): rows of
-// equal values have equal sums, to the last bit, and their beams' candidates are equals.
+// thread's maximum so far, x log2 e - m log2 e in one rounding (2^-24 of it, so a term of
+// weight p is off by 2^-24 |ln p|), sums of a thread's values in 32 bits, of the threads' in
+// 64; what m log2 e was rounded by is taken back in 64 bits.  A thread's granules are
+// counted from the row's first value, whatever its alignment (the loads may be unaligned):
+// rows of equal values have equal sums, to the last bit, and their beams' candidates are
+// equals.
 template <typename T, int U>
-__global__ __launch_bounds__(NT) void select_rows_kernel(SelectArgs a, SliceSum* __restrict__ sums,
-                                                         Candidate* __restrict__ best) {
+__global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
+                                                            SliceSum* __restrict__ sums,
+                                                            Candidate* __restrict__ best) {
   __shared__ TopLds<float> lds;
-  __shared__ float sm[NT / 64];
-  __shared__ double ss[NT / 64];
-  constexpr int E = Row<T>::E;
+  __shared__ u32x4 hot[GRANULES];
+  __shared__ int hot_at[GRANULES], hots;
+  __shared__ float2 parts[NT];
+  constexpr int E = Row<T>::E, BATCH = 4;  // granules whose maximum is taken at once
   const int g = blockIdx.x / a.W, w = blockIdx.x % a.W, t = threadIdx.x, lane = t & 63;
   if (!(fabsf(a.scores[blockIdx.x]) < INFINITY)) return;  // a beam that is not in use
   const T* row = (const T*)a.logits + g * a.logits_sg + w * a.logits_sw;
   const int v0 = (blockIdx.y * (NT * U) + t) * E;  // the thread's first value
-  u32x4 raw[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
+  // A granule that would pass the row's end begins E values before it, and leaves out those
+  // that are another's.
+  auto first = [&](int u) {
     const int v = v0 + u * NT * E;
-    if (v + E <= a.V) {
-      __builtin_memcpy(&raw[u], row + v, 16);
-    } else {
-      T x[E];
+    return a.V >= E ? min(v, a.V - E) : v;
+  };
+  u32x4 raw[U];
+  if (a.V >= E) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = v + e < a.V ? row[v + e] : from_f32<T>(-INFINITY);
-      __builtin_memcpy(&raw[u], x, 16);
+    for (int u = 0; u < U; ++u) __builtin_memcpy(&raw[u], row + first(u), 16);
+  } else {
+    T x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      x[e] = t == 0 && e < a.V ? row[min(e, a.V - 1)] : from_f32<T>(-INFINITY);
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = none_of<T>();
+    __builtin_memcpy(&raw[0], x, 16);
+  }
+  if ((blockIdx.y + 1) * (NT * U * E) > a.V && a.V >= E) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) drop_first<T>(raw[u], v0 + u * NT * E - first(u));
+  }
+  float gm[U], m = -INFINITY, ml = 0.f, part = 0.f;
+#pragma unroll
+  for (int b = 0; b < U; b += BATCH) {
+    const float old = m;
+#pragma unroll
+    for (int u = b; u < b + BATCH; ++u) {
+      float f[E];
+      Row<T>::unpack(raw[u], f);
+      gm[u] = f[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) gm[u] = fmaxf(gm[u], f[e]);
+      m = fmaxf(m, gm[u]);
+      mfma::settle(raw[u]);  // (kept as they are: unpacked they would take twice the registers)
     }
+    const float was = ml;
+    ml = m == -INFINITY ? 0.f : m * kLog2e;
+    // (moved by the difference of the rounded references, which the terms were taken
+    // against)
+    if (old != -INFINITY && m > old) part *= fast_exp2(was - ml);
+#pragma unroll
+    for (int u = b; u < b + BATCH; ++u) {
+      float f[E], x = 0.f;
+      Row<T>::unpack(raw[u], f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x += fast_exp2(__builtin_fmaf(f[e], kLog2e, -ml));
+      part += x;
+      mfma::settle(raw[u]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
-  float gm[U], m = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float f[E];
-    Row<T>::unpack(raw[u], f);
-    gm[u] = f[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) gm[u] = fmaxf(gm[u], f[e]);
-    m = fmaxf(m, gm[u]);
-  }
-  const float ref = m == -INFINITY ? 0.f : m, ml = ref * kLog2e;
-  float part = 0.f;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float f[E], x = 0.f;
-    Row<T>::unpack(raw[u], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x += fast_exp2(__builtin_fmaf(f[e], kLog2e, -ml));
-    part += x;
-  }
-  constexpr double L = 1.4426950408889634074;
-  float M = m;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  if (lane == 0) sm[t >> 6] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) M = fmaxf(M, sm[i]);
-  double s = m == -INFINITY ? (double)(part != part ? part : 0.f)
-                            : (double)part * exp2_64(((double)m - (double)M) * L +
-                                                     (ml - (double)m * (double)kLog2e));
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) ss[t >> 6] = s;
+  // One wavefront finds the bound, another the sum: all four would spend on them what they
+  // spend on the values.
+  lds.top[t] = m;
+  parts[t] = make_float2(part, ml);
+  if (t == 0) lds.count = hots = 0;
   __syncthreads();
   const int64_t at = (int64_t)blockIdx.x * gridDim.y + blockIdx.y;
-  if (t == 0) {
-    s = 0.0;
-    for (int i = 0; i < NT / 64; ++i) s += ss[i];
-    sums[at] = SliceSum{M, s};
+  if (t >> 6 == 0) {
+    const float x = top_bound(a.K, lds);
+    if (lane == 0) lds.edge = x;
+  } else if (t >> 6 == 1) {
+    constexpr double L = 1.4426950408889634074;
+    float M = -INFINITY;
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) M = fmaxf(M, lds.top[lane + 64 * i]);
+    M = wave_max(M);
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+      const double x = lds.top[lane + 64 * i];
+      const float2 p = parts[lane + 64 * i];
+      if (x == -INFINITY)
+        s += p.x != p.x ? p.x : 0.f;
+      else
+        s += (double)p.x * exp2_64((x - (double)M) * L + ((double)p.y - x * (double)kLog2e));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) sums[at] = SliceSum{M, s};
   }
+  __syncthreads();
+  const float edge = lds.edge;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (gm[u] >= edge && gm[u] > -INFINITY) {
+      const int x = atomicAdd(&hots, 1);
+      if (x < GRANULES) {
+        hot[x] = raw[u];
+        hot_at[x] = first(u);
+      }
+    }
+  __syncthreads();
   Candidate* out = best + at * a.K;
-  const int n = top_k(
-      a.K, m,
-      [&](float edge, auto f) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (gm[u] >= edge) {
-            float x[E];
-            Row<T>::unpack(raw[u], x);
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (x[e] >= edge && x[e] > -INFINITY) f(x[e], v0 + u * NT * E + e);
-          }
-      },
-      [&](int place, float x, int v) { out[place] = Candidate{x, v}; }, lds);
-  for (int i = n + t; i < a.K; i += NT) out[i] = Candidate{-INFINITY, -1};
+  auto put = [&](int place, float x, int v) { out[place] = Candidate{x, v}; };
+  const int nh = hots;
+  for (int x = t; x < min(nh, GRANULES) * E; x += NT) {
+    const float f = to_f32(((const T*)hot)[x]);
+    if (f >= edge && f > -INFINITY) lds.add(f, hot_at[x / E] + x % E);
+  }
+  __syncthreads();
+  int n = lds.count;
+  if (nh <= GRANULES && n <= CAP) {
+    top_order(a.K, n, put, lds);
+  } else {
+    top_one_by_one(
+        a.K,
+        [&](auto f) {
+#pragma unroll 1
+          for (int u = 0; u < U; ++u)
+#pragma unroll 1
+            for (int e = 0; e < E; ++e) {
+              const int v = v0 + u * NT * E + e;
+              const float x = v < a.V ? to_f32(row[v]) : -INFINITY;
+              if (x > -INFINITY) f(x, v);
+            }
+        },
+        put, lds);
+    n = a.K;
+  }
+  for (int i = n + t; i < a.K; i += NT) put(i, -INFINITY, -1);
 }
 
 // ------------------------------------------------------------------ pick
+// The candidates are asked for before anything is waited for: each round trip to what
+// other compute units wrote costs as much as the rest.
 __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
                                                          const SliceSum* __restrict__ sums,
                                                          const Candidate* __restrict__ best,
                                                          int slices) {
   __shared__ TopLds<double> lds;
   __shared__ double score[KF_BEAM_MAX], lse[KF_BEAM_MAX];
-  const int g = blockIdx.x, t = threadIdx.x, lane = t & 63, W = a.W;
+  const int g = blockIdx.x, t = threadIdx.x, W = a.W;
   constexpr double L = 1.4426950408889634074;
-  for (int w = t >> 6; w < W; w += NT / 64) {
+  constexpr int R = 4;  // candidates of a thread in registers
+  const int per = slices * a.K, n = W * per;
+  const Candidate* c = best + (int64_t)g * n;
+  Candidate mine[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) mine[r] = c[min(t + r * NT, n - 1)];
+  // a row per group of lanes, all rows at once
+  const int lanes = W <= 4 ? 64 : W <= 8 ? 32 : W <= 16 ? 16 : W <= 32 ? 8 : 4;
+  {
+    const int w = min(t / lanes, W - 1), x = t % lanes;
+    const SliceSum* row = sums + ((int64_t)g * W + w) * slices;
     const float sc = a.scores[(int64_t)g * W + w];
-    bool ok = fabsf(sc) < INFINITY;
+    SliceSum y = row[min(x, slices - 1)];
+    const bool live = fabsf(sc) < INFINITY;  // (else what the slices hold was not written)
     double s = 0.0;
     float M = -INFINITY;
-    if (ok) {
-      const SliceSum* row = sums + ((int64_t)g * W + w) * slices;
-      for (int i = lane; i < slices; i += 64) M = fmaxf(M, row[i].m);
-      M = wave_max(M);
-      for (int i = lane; i < slices; i += 64)
-        s += row[i].m == M ? row[i].s : row[i].s * exp2_64(((double)row[i].m - (double)M) * L);
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-      ok = s > 0.0 && s < INFINITY;
+    if (live) {
+      M = x < slices ? y.m : -INFINITY;
+      for (int i = x + lanes; i < slices; i += lanes) M = fmaxf(M, row[i].m);
     }
-    if (lane == 0) {
+    for (int o = lanes / 2; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if (live)
+      for (int i = x; i < slices; i += lanes) {
+        if (i != x) y = row[i];
+        s += y.m == M ? y.s : y.s * exp2_64(((double)y.m - (double)M) * L);
+      }
+    for (int o = lanes / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    const bool ok = live && s > 0.0 && s < INFINITY;
+    if (x == 0 && t / lanes < W) {
       score[w] = ok ? (double)sc : -INFINITY;
       lse[w] = ok ? (double)M + log(s) : 0.0;
     }
   }
   __syncthreads();
-  const int per = slices * a.K, n = W * per;
-  const Candidate* c = best + (int64_t)g * n;
   auto each = [&](auto f) {
-    for (int i = t; i < n; i += NT) {
-      const int w = i / per;
-      if (score[w] == -INFINITY) continue;  // (what its slices hold was not written)
-      const Candidate x = c[i];
-      if (x.v >= 0) f(score[w] + ((double)x.x - lse[w]), w * a.V + x.v);
-    }
+    auto one = [&](int i, const Candidate& x) {
+      const int w = (int)((unsigned)i / (unsigned)per);
+      const double sc = score[w];
+      if (sc != -INFINITY && x.v >= 0) f(sc + ((double)x.x - lse[w]), w * a.V + x.v);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (t + r * NT < n) one(t + r * NT, mine[r]);
+    for (int i = t + R * NT; i < n; i += NT) one(i, c[i]);
   };
   double own = -INFINITY;
   each([&](double x, int) { own = fmax(own, x); });
+  lds.top[t] = own;
+  if (t == 0) lds.count = 0;
+  __syncthreads();
+  const double edge = top_bound(a.K, lds);  // (each wavefront by itself: no other barrier)
+  if (own >= edge)
+    each([&](double x, int i) {
+      if (x >= edge) lds.add(x, i);
+    });
+  __syncthreads();
   const int64_t at = (int64_t)g * a.K;
-  const int m = top_k(
-      a.K, own,
-      [&](double edge, auto f) {
-        each([&](double x, int i) {
-          if (x >= edge) f(x, i);
-        });
-      },
-      [&](int place, double x, int i) {
-        a.out_scores[at + place] = (float)x;
-        a.parents[at + place] = i / a.V;
-        a.tokens[at + place] = i % a.V;
-      },
-      lds);
+  auto put = [&](int place, double x, int i) {
+    const int w = (int)((unsigned)i / (unsigned)a.V);
+    a.out_scores[at + place] = (float)x;
+    a.parents[at + place] = w;
+    a.tokens[at + place] = i - w * a.V;
+  };
+  int m = lds.count;
+  if (m <= CAP) {
+    top_order(a.K, m, put, lds);
+  } else {
+    top_one_by_one(a.K, each, put, lds);
+    m = a.K;
+  }
   for (int i = m + t; i < a.K; i += NT) {
     a.out_scores[at + i] = -INFINITY;
     a.parents[at + i] = -1;
@@ -354,7 +465,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Granules a thread of the rows kernel: few where many would leave compute units without a
 // workgroup.
 int unit_of(const SelectArgs& a) {
-  return (int64_t)a.G * a.W * slices_of(a.V, a.dtype == F32 ? 4 : 8, 16) >= 512 ? 16 : 4;
+  return (int64_t)a.G * a.W * slices_of(a.V, a.dtype == F32 ? 4 : 8, 8) >= 512 ? 8 : 4;
 }
 int slices_of(const SelectArgs& a) { return slices_of(a.V, a.dtype == F32 ? 4 : 8, unit_of(a)); }
 
@@ -364,7 +475,7 @@ int select_typed(const SelectArgs& a, void* workspace) {
   SliceSum* sums = (SliceSum*)workspace;
   Candidate* best =
       (Candidate*)((char*)workspace + up256((size_t)a.G * a.W * slices * sizeof(SliceSum)));
-  KF_LAUNCH("select_rows", (unit == 16 ? select_rows_kernel<T, 16> : select_rows_kernel<T, 4>),
+  KF_LAUNCH("select_rows", (unit == 8 ? select_rows_kernel<T, 8> : select_rows_kernel<T, 4>),
             dim3(a.G * a.W, slices), dim3(NT), 0, a.stream, a, sums, best);
   KF_CHECK_LAUNCH();
   KF_LAUNCH("select_pick", select_pick_kernel, dim3(a.G), dim3(NT), 0, a.stream, a, sums, best,

@@ -1,5 +1,6 @@
 // The host's side of calls that are shorter than Python's checks of their arguments: a
-// layer's tree attention, the verification, the move in a model's caches (128 tensors).
+// layer's tree or branch attention, the verification, the beams' selection, the moves in a
+// model's caches (128 tensors).
 // Python reads a tensor's device, dtype, shape, contiguity and address in about 0.3 us
 // each, and ctypes a call of 30 arguments in 4.  Here a call in its plain form (every
 // tensor of the type and layout that the kernels read, on the current device) is checked
@@ -85,8 +86,16 @@ struct Entries {
   decltype(&kf_verify_drafts) verify;
   decltype(&kf_kv_cache_keep) keep;
 } lib = {};
+// Those of several continuations of one prompt, by bind_branches().
+struct BranchEntries {
+  decltype(&kf_attn_branch_workspace_size) branch_size;
+  decltype(&kf_attn_branch) branch;
+  decltype(&kf_beam_select_workspace_size) select_size;
+  decltype(&kf_beam_select) select;
+  decltype(&kf_kv_cache_reorder) reorder;
+} branches = {};
 
-PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+PyObject* bind_to(void* entries, PyObject* const* args, Py_ssize_t nargs) {
   void* p[5];
   if (nargs != 5) {
     PyErr_SetString(PyExc_TypeError, "bind(five addresses)");
@@ -97,8 +106,16 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
       return nullptr;
     }
-  std::memcpy(&lib, p, sizeof(p));
+  std::memcpy(entries, p, sizeof(p));
   Py_RETURN_NONE;
+}
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  static_assert(sizeof(lib) == 5 * sizeof(void*), "an address each");
+  return bind_to(&lib, args, nargs);
+}
+PyObject* bind_branches(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  static_assert(sizeof(branches) == 5 * sizeof(void*), "an address each");
+  return bind_to(&branches, args, nargs);
 }
 
 // An argument's tensor if it is one of the plain type on the device, else null.
@@ -294,13 +311,135 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// branch(q, k, v, k_prefix, v_prefix, prefix_lens, k_cache, v_cache, lens, cos, sin, counts,
+//        q_norm_weight, k_norm_weight, norm_eps, rope_row_offset, max_prefix, max_len,
+//        device, stream) -> out, an error code, or None
+PyObject* branch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t offset, max_prefix, max_len, device, stream;
+  double eps;
+  if (nargs != 20 || !branches.branch || !number(args[14], &eps) || !integer(args[15], &offset) ||
+      !integer(args[16], &max_prefix) || !fits(max_prefix) || !integer(args[17], &max_len) ||
+      !fits(max_len) || !integer(args[18], &device) || !integer(args[19], &stream))
+    Py_RETURN_NONE;
+  const at::Tensor *q = tensor(args[0], device), *kp = tensor(args[3], device),
+                   *kc = tensor(args[6], device);
+  if (!q || !kp || !kc || q->dim() != 4 || kp->dim() != 4 || kc->dim() != 4 ||
+      !q->is_contiguous())
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), N = q->size(1), Hq = q->size(2), D = q->size(3);
+  const int64_t G = kp->size(0), Pmax = kp->size(2), Hkv = kc->size(1), Smax = kc->size(2);
+  const auto type = q->scalar_type();
+  const int dt = dtype_of(*q);
+  const at::Tensor *k = tensor(args[1], device, type, {B, N, Hkv, D}),
+                   *v = tensor(args[2], device, type, {B, N, Hkv, D}),
+                   *vp = tensor(args[4], device, type, {G, Hkv, Pmax, D}),
+                   *plens = tensor(args[5], device, at::kInt, {G}),
+                   *vc = tensor(args[7], device, type, {B, Hkv, Smax, D}),
+                   *lens = tensor(args[8], device, at::kInt, {B}),
+                   *cos = tensor(args[9], device), *counts, *qnw, *knw;
+  if (dt < 0 || !k || !v || !vp || !plens || !vc || !lens || !cos || cos->dim() != 2 ||
+      !tensor(args[3], device, type, {G, Hkv, Pmax, D}) ||
+      !tensor(args[6], device, type, {B, Hkv, Smax, D}) ||
+      !tensor(args[9], device, at::kFloat, {cos->size(0), D / 2}) || G < 1 || B % G || !fits(B) ||
+      !fits(N) || !fits(Hq) || !fits(Hkv) || !fits(Pmax) || !fits(Smax) || !fits(D))
+    Py_RETURN_NONE;
+  const at::Tensor* sin = tensor(args[10], device, at::kFloat, cos->sizes());
+  if (!sin || !optional(args[11], device, at::kInt, {B}, &counts) ||
+      !optional(args[12], device, at::kFloat, {D}, &qnw) ||
+      !optional(args[13], device, at::kFloat, {D}, &knw) || !qnw != !knw)
+    Py_RETURN_NONE;
+  size_t need = 0;
+  int rc = branches.branch_size((int)G, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)max_prefix,
+                           (int)max_len, dt, &need);
+  if (rc) return PyLong_FromLong(rc);
+  at::Tensor out = at::empty(q->sizes(), q->options()), ws = bytes(need, *q);
+  rc = branches.branch(q->data_ptr(), k->data_ptr(), v->data_ptr(), kp->data_ptr(), vp->data_ptr(),
+                  data<int32_t>(plens), kc->data_ptr(), vc->data_ptr(), data<int32_t>(lens),
+                  data<int32_t>(counts), data<float>(cos), data<float>(sin), offset, cos->size(0),
+                  out.data_ptr(), ws.data_ptr(), ws.numel(), (int)G, (int)B, (int)N, (int)Pmax,
+                  (int)Smax, (int)Hq, (int)Hkv, (int)D, (int)max_prefix, (int)max_len,
+                  data<float>(qnw), data<float>(knw), (float)eps, dt, (void*)stream);
+  return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// select(logits, scores, K, device, stream) -> (scores, parents, tokens), an error code, or None
+PyObject* select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t K, device, stream;
+  if (nargs != 5 || !branches.select || !integer(args[2], &K) || !fits(K) ||
+      !integer(args[3], &device) || !integer(args[4], &stream))
+    Py_RETURN_NONE;
+  const at::Tensor* x = tensor(args[0], device);
+  if (!x || x->dim() != 3 || x->stride(2) != 1) Py_RETURN_NONE;
+  const int64_t G = x->size(0), W = x->size(1), V = x->size(2);
+  const int dt = dtype_of(*x);
+  const at::Tensor* scores = tensor(args[1], device, at::kFloat, {G, W});
+  if (dt < 0 || !scores || !fits(G) || !fits(W) || !fits(V)) Py_RETURN_NONE;
+  size_t need = 0;
+  int rc = branches.select_size((int)G, (int)W, (int)V, (int)K, dt, &need);
+  if (rc) return PyLong_FromLong(rc);
+  const auto options = x->options();
+  at::Tensor best = at::empty({G, K}, options.dtype(at::kFloat)),
+             parents = at::empty({G, K}, options.dtype(at::kInt)),
+             tokens = at::empty({G, K}, options.dtype(at::kLong)), ws = bytes(need, *x);
+  rc = branches.select(x->data_ptr(), x->stride(0), x->stride(1), data<float>(scores),
+                  data<float>(&best), data<int32_t>(&parents), data<int64_t>(&tokens),
+                  ws.data_ptr(), ws.numel(), (int)G, (int)W, (int)V, (int)K, dt, (void*)stream);
+  if (rc) return PyLong_FromLong(rc);
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(best));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(parents));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(tokens));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// reorder(k_caches, v_caches, lens, parents, device, stream) -> error code or None
+PyObject* reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t device, stream;
+  if (nargs != 6 || !branches.reorder || !integer(args[4], &device) || !integer(args[5], &stream) ||
+      !PyList_CheckExact(args[0]) || PyList_GET_SIZE(args[0]) < 1)
+    Py_RETURN_NONE;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  const at::Tensor *k0 = tensor(PyList_GET_ITEM(args[0], 0), device),
+                   *parents = tensor(args[3], device);
+  if (!k0 || k0->dim() != 4 || !parents || parents->dim() != 2 || !fits(n)) Py_RETURN_NONE;
+  const int64_t B = k0->size(0), G = parents->size(0), W = parents->size(1);
+  const int dt = dtype_of(*k0);
+  const auto type = k0->scalar_type();
+  const at::Tensor* lens = tensor(args[2], device, at::kInt, {B});
+  std::vector<void*> p;
+  p.reserve(2 * n);
+  if (dt < 0 || !lens || !tensor(args[3], device, at::kInt, {G, W}) || !fits(B) || !fits(G) ||
+      !fits(W) || G * W != B || !fits(k0->size(1)) || !fits(k0->size(2)) || !fits(k0->size(3)) ||
+      !pointers(args[0], n, device, type, k0->sizes(), p) ||
+      !pointers(args[1], n, device, type, k0->sizes(), p))
+    Py_RETURN_NONE;
+  return PyLong_FromLong(branches.reorder(p.data(), p.data() + n, (int)n, data<int32_t>(lens),
+                                     data<int32_t>(parents), (int)W, (int)B, (int)k0->size(1),
+                                     (int)k0->size(2), (int)k0->size(3), dt, (void*)stream));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"same", (PyCFunction)(void (*)())same, METH_FASTCALL,
      "same(list, buffer, first) -> device index (-1: not on a GPU)"},
     {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, "bind(addresses of the entry points)"},
+    {"bind_branches", (PyCFunction)(void (*)())bind_branches, METH_FASTCALL,
+     "bind_branches(addresses of the entry points)"},
     {"tree", (PyCFunction)(void (*)())tree, METH_FASTCALL, "tree attention, if in plain form"},
     {"verify", (PyCFunction)(void (*)())verify, METH_FASTCALL, "verification, if in plain form"},
     {"keep", (PyCFunction)(void (*)())keep, METH_FASTCALL, "the caches' move, if in plain form"},
+    {"branch", (PyCFunction)(void (*)())branch, METH_FASTCALL,
+     "attention behind shared prefixes, if in plain form"},
+    {"select", (PyCFunction)(void (*)())select, METH_FASTCALL,
+     "the beams' selection, if in plain form"},
+    {"reorder", (PyCFunction)(void (*)())reorder, METH_FASTCALL,
+     "the caches' reordering, if in plain form"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kf_torch", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -793,6 +793,15 @@ def branch_decode_raw(q_new, k_new, v_new, k_prefix, v_prefix, prefix_lens, k_ca
 
     As in :func:`decode_raw`, what lies on the device is checked there: a sequence whose
     lengths, count or RoPE rows are out of range gets NaN outputs and no cache write."""
+    here = _here(q_new)
+    if here is not None:
+        out = _lib.native().branch(q_new, k_new, v_new, k_prefix, v_prefix, prefix_lens, k_cache,
+                                   v_cache, lens, cos, sin, counts, q_norm_weight, k_norm_weight,
+                                   norm_eps, rope_row_offset, max_prefix, max_len, *here)
+        if isinstance(out, torch.Tensor):
+            return out
+        if out is not None:
+            _lib.check(out, "kf_attn_branch")
     lib = _lib.load()
     qs, ks, cs, ps, dtype = q_new.shape, k_new.shape, k_cache.shape, k_prefix.shape, q_new.dtype
     if not len(qs) == len(ks) == len(cs) == len(ps) == 4:
@@ -867,6 +876,13 @@ def beam_select_raw(logits, scores, *, select: int):
     is not in use, a logit of -inf a token that cannot be picked, and a row that is no
     distribution (NaN, +inf, -inf throughout) has no candidates.  Behind the last
     candidate: score -inf, parent and token -1."""
+    here = _here(logits)
+    if here is not None:
+        out = _lib.native().select(logits, scores, select, *here)
+        if isinstance(out, tuple):
+            return out
+        if out is not None:
+            _lib.check(out, "kf_beam_select")
     lib = _lib.load()
     ls = logits.shape
     if len(ls) != 3 or (logits.stride(2) != 1 and ls[2] != 1):
@@ -906,6 +922,11 @@ def cache_reorder_raw(k_caches, v_caches, lens, parents) -> None:
     whose parent is out of range (-1: no beam) is left alone."""
     k_caches, v_caches = list(k_caches), list(v_caches)
     n = len(k_caches)
+    here = _here(parents)
+    if here is not None:
+        rc = _lib.native().reorder(k_caches, v_caches, lens, parents, *here)
+        if rc is not None:
+            return _lib.check(rc, "kf_kv_cache_reorder")
     if n == 0 or n != len(v_caches):
         raise ValueError(f"k_caches and v_caches need one tensor per cache (got {n}, "
                          f"{len(v_caches)})")
