@@ -130,7 +130,8 @@ def native():
                             (module.bind_branches, (
                 "kf_attn_branch_workspace_size", "kf_attn_branch", "kf_beam_select_workspace_size",
                 "kf_beam_select", "kf_kv_cache_reorder"))):
-            bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names))
+            if all(hasattr(lib, name) for name in names):  # (as above)
+                bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names))
         _native = module
     return _native
 

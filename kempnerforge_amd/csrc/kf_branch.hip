@@ -184,21 +184,41 @@ constexpr int WK = 32;  // keys of a chunk
 template <bool ALL>
 struct WaveSched {
   const BranchArgs& a;
-  int G0, B;  // groups in front, entities
-  __device__ __forceinline__ WaveSched(const BranchArgs& a_)
-      : a(a_), G0(ALL ? a_.G : 0), B(G0 + a_.B) {}
-  // (cached keys, new tokens)
-  __device__ __forceinline__ int2 keys(int e) const {
-    if (ALL && e < G0) return make_int2(prefix_keys(a, e), 0);
-    const Seq s = branch_seq(a, e - G0);
-    return s.n > 0 ? make_int2(s.L, s.n) : make_int2(0, 0);
-  }
-  static __device__ __forceinline__ int nck(int2 k) { return (k.x + WK - 1) / WK + (k.y > 0); }
-  __device__ __forceinline__ int chunks(int e) const { return nck(keys(e)) * a.Hkv; }
-  __device__ __forceinline__ int total(int lane) const {
+  int G0, B, C;  // groups in front, entities, chunks
+  // entity `lane`'s, all there are up to 64 of them: cached keys, new tokens (0: a prefix),
+  // keys of the prefix
+  int3 own{0, 0, 0};
+  __device__ __forceinline__ WaveSched(const BranchArgs& a_, int lane)
+      : a(a_), G0(ALL ? a_.G : 0), B(G0 + a_.B) {
     int n = 0;
-    for (int e = lane; e < B; e += 64) n += chunks(e);
-    return __builtin_amdgcn_readlane(wave_prefix(n), 63);
+    for (int e = lane; e < B; e += 64) {
+      own = keys(e);
+      n += nck(own) * a.Hkv;
+    }
+    C = __builtin_amdgcn_readlane(wave_prefix(n), 63);
+  }
+  __device__ __forceinline__ int3 keys(int e) const {
+    if (ALL && e < G0) return make_int3(prefix_keys(a, e), 0, 0);
+    const Seq s = branch_seq(a, e - G0);
+    return s.n > 0 ? make_int3(s.L, s.n, s.P) : make_int3(0, 0, 0);
+  }
+  __device__ __forceinline__ int3 keys_of(int e) const {  // (uniform e)
+    const int3 x = B <= 64 ? own : keys(e);
+    const int at = B <= 64 ? e : 0;
+    return make_int3(__builtin_amdgcn_readlane(x.x, at), __builtin_amdgcn_readlane(x.y, at),
+                     __builtin_amdgcn_readlane(x.z, at));
+  }
+  static __device__ __forceinline__ int nck(int3 k) { return (k.x + WK - 1) / WK + (k.y > 0); }
+  __device__ __forceinline__ int chunks(int e) const { return nck(keys(e)) * a.Hkv; }
+  // the entity that holds a chunk, and its first one
+  __device__ __forceinline__ void locate(int c, int lane, int& e, int& base) const {
+    if (B > 64) {
+      locate_chunk(*this, c, lane, e, base);
+      return;
+    }
+    const int n = nck(own) * a.Hkv, end = wave_prefix(n);
+    e = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end - n <= c && c < end) | 1ull << 63);
+    base = __builtin_amdgcn_readlane(end - n, e);
   }
 };
 
@@ -208,29 +228,29 @@ struct WaveLds {
 };
 
 template <typename T, int D, bool ALL>
-__device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, char* lds, int gw,
-                                          int NW, int C) {
+__device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, char* lds,
+                                          const WaveSched<ALL>& sched, int gw, int NW) {
   using namespace mfma;
   constexpr int KT = D / 32, DB = D / 16, KR = D / 8, HALF = D / 2;
   constexpr int VL = WK * KR / 64;
-  constexpr float LIFT = std::is_same<T, _Float16>::value ? 13.f : 0.f;  // (as in the tiles below)
+  // P = 2^(s - m + LIFT), m moved only when a score is 2^SLACK above it (as in the tiles below):
+  // chunk after chunk nothing crosses lanes
+  constexpr bool HALF_P = std::is_same<T, _Float16>::value;
+  constexpr float SLACK = HALF_P ? 2.f : 8.f, LIFT = HALF_P ? 13.f : 0.f;
   if (gw >= NW) return;
   gw = __builtin_amdgcn_readfirstlane(gw);
   const int w = wave_id(), lane = threadIdx.x & 63, q4 = lane >> 4, c16 = lane & 15;
   T* lv = ((WaveLds<T, D>*)lds)[w].v;
   const int n_rep = a.Hq / a.Hkv, W = a.B / a.G, N = a.N;
-  const WaveSched<ALL> sched(a);
-  const int c_lo = range_start(gw, C, NW), c_hi = range_start(gw + 1, C, NW);
+  const int c_lo = range_start(gw, sched.C, NW), c_hi = range_start(gw + 1, sched.C, NW);
 
   struct Cursor {
     int e, g, lc, nck;
-    int2 k;  // cached keys, new tokens (0: a prefix)
+    int3 k;  // cached keys, new tokens (0: a prefix), keys of the prefix
   };
   auto enter = [&](Cursor& c, int e) {
     c.e = e;
-    c.k = sched.keys(e);
-    c.k.x = __builtin_amdgcn_readfirstlane(c.k.x);
-    c.k.y = __builtin_amdgcn_readfirstlane(c.k.y);
+    c.k = sched.keys_of(e);
     c.nck = sched.nck(c.k);
   };
   auto next = [&](Cursor& c) {
@@ -289,13 +309,19 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     }
   };
   // Pieces of a row (dims d ..) and of its other half, rotated, after the norm if there is one.
-  auto rotate = [&](float* f1, float* f2, int64_t trow, int d, const float* nw, float rs) {
-    float c[8], sn[8];
+  struct Angles {
+    float c[8], s[8];
+  };
+  auto angles = [&](int64_t trow, int d) {
+    Angles g;
 #pragma unroll
     for (int x = 0; x < 8; x += 4) {
-      *(f32x4*)(c + x) = *(const f32x4*)(a.cos + trow + d + x);
-      *(f32x4*)(sn + x) = *(const f32x4*)(a.sin + trow + d + x);
+      *(f32x4*)(g.c + x) = *(const f32x4*)(a.cos + trow + d + x);
+      *(f32x4*)(g.s + x) = *(const f32x4*)(a.sin + trow + d + x);
     }
+    return g;
+  };
+  auto rotate = [&](float* f1, float* f2, const Angles& g, int d, const float* nw, float rs) {
     if (nw != nullptr) {
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
@@ -305,8 +331,8 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const float y1 = f1[x] * c[x] - f2[x] * sn[x];
-      f2[x] = f2[x] * c[x] + f1[x] * sn[x];
+      const float y1 = f1[x] * g.c[x] - f2[x] * g.s[x];
+      f2[x] = f2[x] * g.c[x] + f1[x] * g.s[x];
       f1[x] = y1;
     }
   };
@@ -339,54 +365,84 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
   Cursor cc;
   {
     int e, base;
-    locate_chunk(sched, c_lo, lane, e, base);
+    sched.locate(c_lo, lane, e, base);
     enter(cc, e);
     cc.g = __builtin_amdgcn_readfirstlane((c_lo - base) / max(cc.nck, 1));
     cc.lc = c_lo - base - cc.g * cc.nck;
   }
-  load_k(cc);
-  load_v(cc);
+  // A pair's queries: the lane's row of them and of the tables, then rotated.
+  auto pair_rows = [&](const Cursor& c) { return (is_prefix(c) ? W * N : c.k.y) * n_rep; };
+  auto load_q = [&](const Cursor& c, u32x4* raw, Angles* ang) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (nothing of this is kept across the loop)
+    const int q4 = ln >> 4, c16 = ln & 15;
+    const bool pre = is_prefix(c);
+    const int r = min(c16, pair_rows(c) - 1), tok = r / n_rep;
+    const int at = pre ? tok / N : 0;
+    const int64_t b = pre ? c.e * W + at : c.e - sched.G0;
+    token = pre ? tok - at * N : tok;
+    const T* qr =
+        (const T*)a.q_new + ((b * N + token) * a.Hq + (int64_t)c.g * n_rep + r % n_rep) * D + 8 * q4;
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) raw[ks] = *(const u32x4*)(qr + 32 * ks);
+    int64_t pos = (int64_t)c.k.z + c.k.x + token;
+    if (pre)
+      pos = (int64_t)c.k.x + token +
+            (sched.B <= 64 ? __shfl(sched.own.x, (int)b + sched.G0, 64) : a.lens[b]);
+    const int64_t trow = table_row(a, pos);
+#pragma unroll
+    for (int ks = 0; ks < KT / 2; ++ks) ang[ks] = angles(trow, 32 * ks + 8 * q4);
+  };
+  auto rotate_q = [&](const u32x4* raw, const Angles* ang) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int q4 = ln >> 4;
+    const float rs = a.q_norm_w != nullptr ? row_norm(raw) : 1.f;
+    const float sc = a.scale * kLog2e;
+#pragma unroll
+    for (int ks = 0; ks < KT / 2; ++ks) {
+      float f[2][8];
+      unpack8<T>(raw[ks], f[0]);
+      unpack8<T>(raw[ks + KT / 2], f[1]);
+      rotate(f[0], f[1], ang[ks], 32 * ks + 8 * q4, a.q_norm_w, rs);
+      __builtin_amdgcn_sched_barrier(0);  // (registers)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float hi[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) f[x][y] *= sc;
+        qh[ks + x * (KT / 2)] = pack8<T>(f[x]);
+        unpack8<T>(qh[ks + x * (KT / 2)], hi);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) f[x][y] -= hi[y];
+        ql[ks + x * (KT / 2)] = pack8<T>(f[x]);
+      }
+    }
+    m = -INFINITY;
+    lsum = 0.f;
+#pragma unroll
+    for (int blk = 0; blk < DB; ++blk) acc[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  {
+    // (the queries first: loads return in order)
+    u32x4 raw[KT];
+    Angles ang[KT / 2];
+    load_q(cc, raw, ang);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(cc);
+    load_v(cc);
+    __builtin_amdgcn_sched_barrier(0);
+    rotate_q(raw, ang);
+  }
   for (int i = c_lo; i < c_hi; ++i) {
     const bool pre = is_prefix(cc), fresh = is_new(cc), more = i + 1 < c_hi;
-    const int rows = (pre ? W * N : cc.k.y) * n_rep, keys = chunk_rows(cc);
+    const int keys = chunk_rows(cc);
     const int64_t b0 = cc.e - sched.G0;  // (own) the sequence
-    if (i == c_lo || cc.lc == 0) {       // a pair begins: its queries
-      int ln = lane;
-      asm volatile("" : "+v"(ln));  // (as below)
-      const int q4 = ln >> 4, c16 = ln & 15;
-      const int r = min(c16, rows - 1), tok = r / n_rep;
-      const int64_t b = pre ? cc.e * W + tok / N : b0;
-      token = pre ? tok % N : tok;
-      const T* qr = (const T*)a.q_new +
-                    ((b * N + token) * a.Hq + (int64_t)cc.g * n_rep + r % n_rep) * D + 8 * q4;
+    if (i > c_lo && cc.lc == 0) {        // a pair begins
       u32x4 raw[KT];
-#pragma unroll
-      for (int ks = 0; ks < KT; ++ks) raw[ks] = *(const u32x4*)(qr + 32 * ks);
-      const int64_t trow = table_row(a, (int64_t)a.prefix_lens[b / W] + a.lens[b] + token);
-      const float rs = a.q_norm_w != nullptr ? row_norm(raw) : 1.f;
-      const float sc = a.scale * kLog2e;
-#pragma unroll
-      for (int ks = 0; ks < KT / 2; ++ks) {
-        float f[2][8];
-        unpack8<T>(raw[ks], f[0]);
-        unpack8<T>(raw[ks + KT / 2], f[1]);
-        rotate(f[0], f[1], trow, 32 * ks + 8 * q4, a.q_norm_w, rs);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float hi[8];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) f[x][y] *= sc;
-          qh[ks + x * (KT / 2)] = pack8<T>(f[x]);
-          unpack8<T>(qh[ks + x * (KT / 2)], hi);
-#pragma unroll
-          for (int y = 0; y < 8; ++y) f[x][y] -= hi[y];
-          ql[ks + x * (KT / 2)] = pack8<T>(f[x]);
-        }
-      }
-      m = -INFINITY;
-      lsum = 0.f;
-#pragma unroll
-      for (int blk = 0; blk < DB; ++blk) acc[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+      Angles ang[KT / 2];
+      load_q(cc, raw, ang);
+      rotate_q(raw, ang);
     }
     uint32_t bad = 0;  // V rows with Inf or NaN that not all rows see
     if (fresh) {       // (16 keys at most: kb = 0)
@@ -396,15 +452,14 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
       const int64_t at = (b0 * a.Hkv + cc.g) * a.Smax + cc.k.x;  // the first new row
       const float rs = a.k_norm_w != nullptr ? row_norm(kreg[0]) : 1.f;
       if (c16 < keys) {
-        const int64_t trow =
-            table_row(a, (int64_t)a.prefix_lens[b0 / W] + cc.k.x + c16);
+        const int64_t trow = table_row(a, (int64_t)cc.k.z + cc.k.x + c16);
         T* dst = (T*)a.k_cache + (at + c16) * D + 8 * q4;
 #pragma unroll
         for (int ks = 0; ks < KT / 2; ++ks) {
           float f[2][8];
           unpack8<T>(kreg[0][ks], f[0]);
           unpack8<T>(kreg[0][ks + KT / 2], f[1]);
-          rotate(f[0], f[1], trow, 32 * ks + 8 * q4, a.k_norm_w, rs);
+          rotate(f[0], f[1], angles(trow, 32 * ks + 8 * q4), 32 * ks + 8 * q4, a.k_norm_w, rs);
           __builtin_amdgcn_sched_barrier(0);  // (registers)
           kreg[0][ks] = pack8<T>(f[0]);
           kreg[0][ks + KT / 2] = pack8<T>(f[1]);
@@ -432,37 +487,46 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     }
     Cursor ic = cc;
     if (more) next(ic);
-    f32x4 sc[2];
-    float tmax = -INFINITY;
-    const int limit = fresh ? token + 1 : keys;
+    f32x4 sc[2], sl[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      sc[kb] = sl[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KT; ++ks) {
         sc[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(qh[ks]), sc[kb]);
-        sc[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(ql[ks]), sc[kb]);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        sc[kb][t] = 16 * kb + 4 * q4 + t < limit ? sc[kb][t] : -INFINITY;
-        tmax = fmaxf(tmax, sc[kb][t]);
+        sl[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(ql[ks]), sl[kb]);
       }
     }
     if (more) load_k(ic);
-    tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-    tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-    const float mnew = fmaxf(m, tmax);
-    const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
-    const float ref = (mnew == -INFINITY ? 0.f : mnew) - LIFT;  // (-inf: no key yet)
-    m = mnew;
-    float p[8], psum = 0.f;
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) sc[kb] += sl[kb];
+    if (keys < WK) {  // (a new token sees those before it and itself)
+      const int limit = fresh ? token + 1 : keys;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        sc[t / 4][t % 4] =
+            16 * (t / 4) + 4 * q4 + t % 4 < limit ? sc[t / 4][t % 4] : -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) tmax = fmaxf(tmax, sc[t / 4][t % 4]);
+    if (__builtin_amdgcn_ballot_w64(tmax > m + SLACK || m == -INFINITY)) {
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      const float mnew = fmaxf(m, tmax);
+      const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
+      m = mnew;
+      lsum *= alpha;
+#pragma unroll
+      for (int blk = 0; blk < DB; ++blk) acc[blk] *= alpha;
+    }
+    const float ref = (m == -INFINITY ? 0.f : m) - LIFT;  // (-inf: no key yet)
+    float p[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       p[t] = fast_exp2(sc[t / 4][t % 4] - ref);
-      psum += p[t];
+      lsum += p[t];
     }
-    lsum = lsum * alpha + psum;
     u32x4 ph, pl;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -480,7 +544,6 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     if (more) load_v(ic);
 #pragma unroll
     for (int blk = 0; blk < DB; ++blk) {
-      acc[blk] *= alpha;
       const char* base = (const char*)lv + tr_base + (uint32_t)((blk ^ tr_hs) * 32);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)base);
       const s16x4 hi =
@@ -518,7 +581,7 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
       const int q4 = ln >> 4, c16 = ln & 15;
       float l = lsum + __shfl_xor(lsum, 16, 64);
       l += __shfl_xor(l, 32, 64);
-      if (c16 < rows) {
+      if (c16 < pair_rows(cc)) {
         const int64_t at = ((int64_t)gw + item) * ls.rows_b + c16;
         float* o = ls.ob + at * D + 4 * q4;
 #pragma unroll
@@ -532,36 +595,76 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
 }
 
 // ---- a workgroup a share: row tiles of 32 RW rows
-// Entities: the groups (rows: the tokens of their sequences, key chunks of the prefix) or
-// (OWN) the sequences.  Row r of an entity is query head r % n_rep of the KV head's of its
-// token r / n_rep.
-template <bool OWN>
+// Entities: the groups (PREFIX: the tokens of their sequences over the prefix), the sequences
+// (OWN: their tokens over their own rows), or the sequences over both (BOTH: where a
+// sequence's tokens fill tiles of their own, so that nothing has to be joined).  Row r of an
+// entity is query head r % n_rep of the KV head's of its token r / n_rep.  A tile meets the
+// chunks of the prefix, then those of the own rows up to its last token's.
+//
+// Beginning a row tile and leaving its partial cost about as much as OVER chunks, so with
+// several chunks per workgroup each tile has OVER units in front of its chunks in the list
+// that is shared out.  (Without them the own rows' tiles of one chunk count for so little
+// that a few workgroups get them all: 4 sequences of 64 new tokens behind 16384 keys, 64 / 8
+// heads: 681 us.)
+enum Role : int { PREFIX, OWN, BOTH };
+constexpr int OVER = 2;
+// tokens, own keys (the new tokens' among them), keys of the prefix
+struct Entity {
+  int n, y, p;
+};
+template <int ROLE>
 struct TileSched {
   const BranchArgs& a;
-  int n_rep, rows, kc, E, C;
+  int n_rep, rows, kc, E, C, items, over = 0;  // C: units; items: tiles
   bool compact;
-  int2 own{0, 0};  // entity `lane`'s (tokens, keys), all there are up to 64 of them
+  Entity own{0, 0, 0};  // entity `lane`'s, all there are up to 64 of them
   __device__ __forceinline__ TileSched(const BranchArgs& a_, int rows_, int kc_, bool compact_,
                                        int lane)
-      : a(a_), n_rep(a_.Hq / a_.Hkv), rows(rows_), kc(kc_), E(OWN ? a_.B : a_.G),
+      : a(a_), n_rep(a_.Hq / a_.Hkv), rows(rows_), kc(kc_), E(ROLE == PREFIX ? a_.G : a_.B),
         compact(compact_) {
-    int tot = 0;
+    int tot = 0, n = 0;
     for (int e = lane; e < E; e += 64) {
       own = entity(e);
       tot += units(own);
+      n += own.y + own.p > 0 ? a.Hkv * tiles(own) : 0;
     }
     C = __builtin_amdgcn_readlane(wave_prefix(tot), 63);
+    items = __builtin_amdgcn_readlane(wave_prefix(n), 63);
   }
-  __device__ __forceinline__ int2 entity(int e) const {
-    if (OWN) {
-      const Seq s = branch_seq(a, e);
-      return s.n > 0 ? make_int2(s.n, s.L + s.n) : make_int2(0, 0);
-    }
-    return make_int2(group_tokens(a, e, compact), prefix_keys(a, e));
+  __device__ __forceinline__ void count_beginnings() {
+    over = OVER;
+    C += OVER * items;
   }
-  __device__ __forceinline__ int nck(int2 s) const { return (s.y + kc - 1) / kc; }
-  __device__ __forceinline__ int tiles(int2 s) const { return (s.x * n_rep + rows - 1) / rows; }
-  __device__ __forceinline__ int units(int2 s) const { return a.Hkv * tiles(s) * nck(s); }
+  __device__ __forceinline__ Entity entity(int e) const {
+    if (ROLE == PREFIX) return Entity{group_tokens(a, e, compact), 0, prefix_keys(a, e)};
+    const Seq s = branch_seq(a, e);
+    return s.n > 0 ? Entity{s.n, s.L + s.n, ROLE == BOTH ? s.P : 0} : Entity{0, 0, 0};
+  }
+  __device__ __forceinline__ Entity entity_of(int e) const {  // (uniform e)
+    Entity x = E <= 64 ? own : entity(e);
+    const int at = E <= 64 ? e : 0;
+    return Entity{__builtin_amdgcn_readlane(x.n, at), __builtin_amdgcn_readlane(x.y, at),
+                  __builtin_amdgcn_readlane(x.p, at)};
+  }
+  __device__ __forceinline__ int tiles(Entity s) const { return (s.n * n_rep + rows - 1) / rows; }
+  __device__ __forceinline__ int prefix_chunks(Entity s) const { return (s.p + kc - 1) / kc; }
+  // the last key of its own that a tile of the sequence sees, and one
+  __device__ __forceinline__ int reach(Entity s, int t) const {
+    return s.y - s.n + min(((t + 1) * rows - 1) / n_rep + 1, s.n);
+  }
+  __device__ __forceinline__ int nck(Entity s, int t) const {
+    return prefix_chunks(s) + (ROLE == PREFIX ? 0 : (reach(s, t) + kc - 1) / kc);
+  }
+  // of one KV head
+  __device__ __forceinline__ int head_units(Entity s) const {
+    if (s.y + s.p == 0) return 0;
+    const int n = tiles(s);
+    if (ROLE == PREFIX) return n * (prefix_chunks(s) + over);
+    int u = 0;
+    for (int t = 0; t < n; ++t) u += nck(s, t) + over;
+    return u;
+  }
+  __device__ __forceinline__ int units(Entity s) const { return a.Hkv * head_units(s); }
   // the first unit of worker w's share of n, floor(w C / n) (w and n are far below 2^16)
   __device__ __forceinline__ int start(int w, int n) const {
     const unsigned q = (unsigned)C / n, r = (unsigned)C % n;
@@ -572,18 +675,17 @@ struct TileSched {
   __device__ __forceinline__ int chunks(int e) const { return units(entity(e)); }
 };
 
-// Place in the list: entity e (tokens s.x, keys s.y), KV head g, row tile t, chunk c of nck,
-// unit u.
-template <typename S>
+// Place in the list: entity e, KV head g, row tile t, chunk c of nck, unit u.
+template <int ROLE>
 struct TileCursor {
-  int e, g, t, c, u, nck, tiles;
-  int2 s;
-  __device__ __forceinline__ void at(const S& sched, int e_, int2 s_) {
+  using S = TileSched<ROLE>;
+  int e, g, t, c, u, nck, tiles, pck;  // pck: chunks of the prefix
+  Entity s;
+  __device__ __forceinline__ void at(const S& sched, int e_) {
     e = e_;
-    s.x = __builtin_amdgcn_readfirstlane(s_.x);
-    s.y = __builtin_amdgcn_readfirstlane(s_.y);
-    nck = sched.nck(s);
+    s = sched.entity_of(e);
     tiles = sched.tiles(s);
+    pck = sched.prefix_chunks(s);
   }
   __device__ __forceinline__ void seek(const S& sched, int unit, int lane) {
     int se, base;
@@ -591,45 +693,62 @@ struct TileCursor {
       const int n = sched.units(sched.own), end = wave_prefix(n);
       se = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end - n <= unit && unit < end) | 1ull << 63);
       base = __builtin_amdgcn_readlane(end - n, se);
-      at(sched, se, make_int2(__builtin_amdgcn_readlane(sched.own.x, se),
-                              __builtin_amdgcn_readlane(sched.own.y, se)));
     } else {
       locate_chunk(sched, unit, lane, se, base);
-      at(sched, se, sched.entity(se));
     }
-    const int item = (unit - base) / nck;
-    c = unit - base - item * nck;
-    u = unit;
-    t = item % tiles;
-    g = item / tiles;
+    at(sched, se);
+    const int per = sched.head_units(s);
+    int off = unit - base;
+    g = off / per;
+    off -= g * per;
+    u = unit - off;
+    if (ROLE == PREFIX) {
+      t = off / (pck + sched.over);
+      u += t * (pck + sched.over);
+      off -= t * (pck + sched.over);
+      nck = pck;
+    } else {
+      for (t = 0;; ++t) {
+        nck = sched.nck(s, t);
+        if (off < nck + sched.over || t == tiles - 1) break;
+        off -= nck + sched.over;
+        u += nck + sched.over;
+      }
+    }
+    c = max(off - sched.over, 0);
+    u += sched.over + c;
   }
   __device__ __forceinline__ void next(const S& sched) {
     ++u;
     if (++c < nck) return;
     c = 0;
-    if (++t < tiles) return;
-    t = 0;
-    if (++g < sched.a.Hkv) return;
-    g = 0;
-    for (int ne = e + 1; ne < sched.E; ++ne) {
-      const int2 sn = sched.E <= 64
-                          ? make_int2(__builtin_amdgcn_readlane(sched.own.x, ne),
-                                      __builtin_amdgcn_readlane(sched.own.y, ne))
-                          : sched.entity(ne);
-      if (sched.units(sn) > 0) {
-        at(sched, ne, sn);
-        return;
+    u += sched.over;
+    if (++t >= tiles) {
+      t = 0;
+      if (++g >= sched.a.Hkv) {
+        g = 0;
+        do {
+          if (++e >= sched.E) return;  // behind the last chunk (u is past every share)
+          at(sched, e);
+        } while (s.y + s.p == 0 || tiles == 0);
       }
     }
-    e = sched.E;  // behind the last chunk (u is past every share)
+    nck = sched.nck(s, t);
   }
 };
 
+// (a value that is the same for all lanes, in scalar registers)
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x),
+                 hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 constexpr int MAX_COMPACT = 1024;  // sequences of a group whose rows are counted
 
-template <typename T, int D, int RW, int BKW, bool OWN>
+template <typename T, int D, int RW, int BKW, int ROLE>
 __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, char* lds, int* pre,
-                                          uint32_t* sbad, const TileSched<OWN>& sched, int blk,
+                                          uint32_t* sbad, const TileSched<ROLE>& sched, int blk,
                                           int nblk) {
   using namespace mfma;
   using X = Tile<T, D>;
@@ -646,22 +765,34 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
   if (blk >= NW) return;
   const int xcd = blk % 8, gw = xcd * (NW / 8) + min(xcd, NW % 8) + blk / 8;
   const int u_hi = sched.start(gw + 1, NW);
-  TileCursor<TileSched<OWN>> cc;
+  TileCursor<ROLE> cc;
   cc.seek(sched, sched.start(gw, NW), lane);
+  if (cc.u >= u_hi) return;  // (a share of nothing but a tile's beginning)
 
-  const T* kbase = (const T*)(OWN ? a.k_cache : a.k_prefix);
-  const T* vbase = (const T*)(OWN ? a.v_cache : a.v_prefix);
-  const int stride = OWN ? a.Smax : a.Pmax;
+  // A chunk is KC keys of the prefix or of the own rows, from key `key0` of keys `keys`.
+  auto of_prefix = [&](const TileCursor<ROLE>& p) {
+    return ROLE == PREFIX || (ROLE == BOTH && p.c < p.pck);
+  };
   auto stage_k = [&](int i) { return (T*)(lds + (i & 1) * Sh::STAGE); };
-  auto issue = [&](const TileCursor<TileSched<OWN>>& p, int i) {
-    const int64_t row = ((int64_t)p.e * a.Hkv + p.g) * stride + (int64_t)p.c * KC;
-    const int rows = p.s.y - p.c * KC;  // >= 1; rows past the last repeat it
+  auto issue = [&](const TileCursor<ROLE>& p, int i) {
+    const bool pre = of_prefix(p);
+    const int key0 = (pre ? p.c : p.c - p.pck) * KC;
+    const int64_t b = ROLE == BOTH && pre ? p.e / W : p.e;
+    // (the tensors by their distance from one of them, as in the wavefronts' list)
+    int64_t at = ((b * a.Hkv + p.g) * (pre ? a.Pmax : a.Smax) + key0) * (D * (int)sizeof(T));
+    int64_t vt = at;
+    if (ROLE == BOTH && pre) {
+      at += (const char*)a.k_prefix - (const char*)a.k_cache;
+      vt += (const char*)a.v_prefix - (const char*)a.v_cache;
+    }
+    const char* kb = (const char*)(ROLE == PREFIX ? a.k_prefix : a.k_cache) + uniform(at);
+    const char* vb = (const char*)(ROLE == PREFIX ? a.v_prefix : a.v_cache) + uniform(vt);
+    const int rows = (pre ? p.s.p : p.s.y) - key0;  // >= 1; rows past the last repeat it
     uint16_t* dst = (uint16_t*)stage_k(i);
     constexpr int U = sizeof(T) / 2;
     constexpr bool FRESH = RW == 2;  // (registers)
-    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)(kbase + row * D), D * U, dst, w, lane, rows);
-    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)(vbase + row * D), D * U, dst + Sh::TILE * U, w,
-                                    lane, rows);
+    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)kb, D * U, dst, w, lane, rows);
+    tile_to_lds<KC, X::R, 4, FRESH>((const uint16_t*)vb, D * U, dst + Sh::TILE * U, w, lane, rows);
   };
   // E pairs of one row rotated (and normalised by rs with weights nw first)
   struct Angles {
@@ -698,7 +829,8 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
   // it has no numbers below 2^-24.
   constexpr bool HALF_P = std::is_same<T, _Float16>::value;
   constexpr float SLACK = HALF_P ? 2.f : 8.f, LIFT = HALF_P ? 13.f : 0.f;
-  int limit = 0;  // keys that the lane's row sees
+  int limit = 0;  // own keys that the lane's row sees
+  bool whole = false;  // (BOTH) this workgroup holds all of the row tile's chunks
 
   // the first compact token of each of a group's sequences (exclusive sums)
   auto count_group = [&](int grp) {
@@ -718,10 +850,10 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
   // The beginning of a row tile: lane l's row of the queries, dims of half h, 16-byte pieces
   // 2 ks + h; a piece's RoPE partner is the lane's own piece KS / 2 further on.
   auto load_q = [&](u32x4* raw, int64_t& trow) {
-    const int row = min(cc.t * ROWS + 32 * rw + l31, cc.s.x * n_rep - 1);
+    const int row = min(cc.t * ROWS + 32 * rw + l31, cc.s.n * n_rep - 1);
     const int tok = row / n_rep;
     int b = cc.e, i = tok;
-    if (!OWN) {
+    if (ROLE == PREFIX) {
       int at;
       if (sched.compact) {
         int lo = 0, hi = W;  // the last sequence that begins at or before the token
@@ -745,8 +877,8 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
 #pragma unroll
     for (int ks = 0; ks < X::KS; ++ks) raw[ks] = *(const u32x4*)(qr + (2 * ks + h) * E);
     const int L = a.lens[b];
-    trow = table_row(a, (OWN ? (int64_t)a.prefix_lens[b / W] : (int64_t)cc.s.y) + L + i);
-    limit = OWN ? L + i + 1 : cc.s.y;
+    trow = table_row(a, (int64_t)a.prefix_lens[b / W] + L + i);
+    limit = L + i + 1;
   };
   auto load_angles = [&](Angles* ang, int64_t trow) {  // (one round trip for all)
 #pragma unroll
@@ -789,6 +921,7 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
     }
     m = -INFINITY;
     lsum = 0.f;
+    whole = ROLE == BOTH && cc.c == 0;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -817,7 +950,7 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
   }
 
   for (int i = 0;; ++i) {
-    TileCursor<TileSched<OWN>> ic = cc;
+    TileCursor<ROLE> ic = cc;
     ic.next(sched);
     const bool more = ic.u < u_hi;
     lds_copy_wait();
@@ -825,17 +958,19 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
     if (more) issue(ic, i + 1);
     T* kt = stage_k(i);
     T* vt = kt + Sh::TILE;
-    const int r0 = cc.c * KC;
-    const int old = cc.s.y - (OWN ? cc.s.x : 0);  // keys that every row sees, but for the new
+    const bool pre = of_prefix(cc);
+    const int r0 = (pre ? cc.c : cc.c - cc.pck) * KC;  // the chunk's first key
+    const int keys = pre ? cc.s.p : cc.s.y;
+    const int old = pre ? keys : cc.s.y - cc.s.n;  // keys that every row sees, but for the new
     if (r0 + KC > old) {
-      // (OWN) the new tokens' rows, from k_new and v_new over what the cache held there;
-      // the first row tile's workgroup writes them to the cache as well.  V rows behind the
-      // last become zero: 0 x NaN must not reach a sum.
+      // The new tokens' rows, from k_new and v_new over what the cache held there; the
+      // workgroup whose row tile a token begins in writes them to the cache as well.  V
+      // rows behind the last become zero: 0 x NaN must not reach a sum.
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));  // (nothing of this block is kept across the loop)
-      if constexpr (OWN) {
+      if (!pre) {
         constexpr int G = HALF / E;  // lanes of a row, a piece of each half a lane
-        const int j0 = max(r0 - old, 0), j1 = min(r0 + KC - old, cc.s.x);
+        const int j0 = max(r0 - old, 0), j1 = min(r0 + KC - old, cc.s.n);
         const int64_t head = (int64_t)cc.e * a.Hkv + cc.g;
         if (tid < KC / 32) sbad[tid] = 0;
         __syncthreads();
@@ -870,7 +1005,7 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
           *(u32x4*)(kt + lr * D + cb) = kx.b;
           *(u32x4*)(vt + lr * D + ca) = vx.a;
           *(u32x4*)(vt + lr * D + cb) = vx.b;
-          if (cc.t == 0) {
+          if (j * n_rep / ROWS == cc.t) {
             *(u32x4*)((T*)a.k_cache + dst) = kx.a;
             *(u32x4*)((T*)a.k_cache + dst + HALF) = kx.b;
             *(u32x4*)((T*)a.v_cache + dst) = vx.a;
@@ -885,13 +1020,13 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
           if (!fin) atomicOr(&sbad[lr >> 5], 1u << (lr & 31));
         }
       }
-      for (int x = max(cc.s.y - r0, 0) * X::R + tid; x < KC * X::R; x += 256)
+      for (int x = max(keys - r0, 0) * X::R + tid; x < KC * X::R; x += 256)
         *(u32x4*)(vt + x * E) = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
     }
     const int k0 = r0 + kw * BKW;  // the wavefront's first key
     auto sees = [&](int key) -> uint32_t {  // which of 32 keys the lane's row sees
-      const int lo = limit - key;
+      const int lo = (pre ? keys : limit) - key;
       return lo <= 0 ? 0u : lo >= 32 ? ~0u : (1u << lo) - 1u;
     };
     auto unclean = [&](int nb) -> uint32_t {
@@ -899,9 +1034,10 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
     };
     // The blocks of 32 keys that the wavefront's last row sees; a wavefront of which the
     // tile has no rows leaves the SIMD to the others.
-    const int blocks = cc.t * ROWS + 32 * rw < cc.s.x * n_rep
-                           ? (__builtin_amdgcn_readlane(limit, 31) - k0 + 31) >> 5
-                           : 0;
+    const int blocks =
+        cc.t * ROWS + 32 * rw < cc.s.n * n_rep
+            ? ((pre ? keys : __builtin_amdgcn_readlane(limit, 31)) - k0 + 31) >> 5
+            : 0;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {  // 32 keys at a time
       if (nb >= blocks) break;
@@ -916,9 +1052,9 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           s[e] = (bits >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
-        if constexpr (OWN) bad = unclean(nb) != 0;
+        if (ROLE != PREFIX && !pre) bad = unclean(nb) != 0;
       }
-      if (OWN && bad) {  // 0 x Inf must not reach the rows that do not see the key
+      if (ROLE != PREFIX && bad) {  // 0 x Inf must not reach the rows that do not see the key
         for (uint32_t x = unclean(nb); x; x &= x - 1) {
           const int r = row0 + __builtin_ctz(x);
           if (lane < X::R) *(u32x4*)(vt + (r * X::R + lane) * (16 / (int)sizeof(T))) = u32x4{0, 0, 0, 0};
@@ -948,7 +1084,7 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
         lsum += s[e];
       }
       X::values(vt, row0, voff, s, vf, acc, lane);
-      if (OWN && bad) {  // those keys one by one, for the rows that see them
+      if (ROLE != PREFIX && bad) {  // those keys one by one, for the rows that see them
         const uint32_t bits = sees(key0);
         int hh = 4 * h;
         asm volatile("" : "+v"(hh));  // (as above)
@@ -974,8 +1110,8 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
       }
     }
     const bool last = cc.c == cc.nck - 1;
-    const int item = (cc.e * a.Hkv + cc.g) * (OWN ? ls.tiles_b : ls.tiles_a) + cc.t;
-    int2* sh = (OWN ? ls.shb : ls.sha) + item;
+    const int item = (cc.e * a.Hkv + cc.g) * (ROLE == PREFIX ? ls.tiles_a : ls.tiles_b) + cc.t;
+    int2* sh = (ROLE == PREFIX ? ls.sha : ls.shb) + item;
     if (threadIdx.x == 0) {
       if (cc.c == 0) sh->x = gw;
       if (last) sh->y = gw;
@@ -1039,17 +1175,34 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
                 }
           }
       }
-      if (cc.t * ROWS + 32 * rw + l31 < cc.s.x * n_rep) {
-        const int64_t at = ((int64_t)gw + item) * ROWS + 32 * rw + l31;
-        float* o = (OWN ? ls.ob : ls.oa) + at * D + 4 * h;
+      const int r = cc.t * ROWS + 32 * rw + l31;
+      if (r < cc.s.n * n_rep) {
+        if (whole && last) {
+          const float inv = 1.f / l;
+          T* o = (T*)a.out +
+                 (((int64_t)cc.e * N + r / n_rep) * a.Hq + cc.g * n_rep + r % n_rep) * D + 4 * h;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int e = 0; e < 16 && owner(dt) == kw; e += 4)
-            *(f32x4*)(o + 32 * dt + 2 * e) =
-                f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
-        if (h == 0 && kw == 0)
-          *(float2*)((OWN ? ls.mlb : ls.mla) + at * 2) = make_float2(m, l);
+            for (int e = 0; e < 16 && owner(dt) == kw; e += 4) {
+              T y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] = from_f32<T>(acc[dt][e + j] * inv);
+              __builtin_memcpy(__builtin_assume_aligned(o + 32 * dt + 2 * e, 4 * sizeof(T)), y,
+                               sizeof(y));
+            }
+        } else {
+          const int64_t at = ((int64_t)gw + item) * ROWS + 32 * rw + l31;
+          float* o = (ROLE == PREFIX ? ls.oa : ls.ob) + at * D + 4 * h;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16 && owner(dt) == kw; e += 4)
+              *(f32x4*)(o + 32 * dt + 2 * e) =
+                  f32x4{acc[dt][e], acc[dt][e + 1], acc[dt][e + 2], acc[dt][e + 3]};
+          if (h == 0 && kw == 0)
+            *(float2*)((ROLE == PREFIX ? ls.mla : ls.mlb) + at * 2) = make_float2(m, l);
+        }
       }
     }
     if (!more) break;
@@ -1067,18 +1220,20 @@ __device__ __forceinline__ void tile_role(const BranchArgs& a, const Lists& ls, 
   }
 }
 
-// Row waves of the prefixes' and the own rows' tiles (0: one wavefront a share).
+// Row waves of the prefixes' and the own rows' tiles (0: one wavefront a share; prefixes -1:
+// one list of the sequences over both).
 template <typename T>
 constexpr int bkw_of(int rw) {
   return rw == 4 && sizeof(T) == 2 ? 64 : 32;
 }
 template <typename T, int D, int RWA, int RWB>
 struct Variant {
-  static constexpr int RW = RWA > 0 ? RWA : 4;
+  static constexpr int RW = RWA > 0 ? RWA : RWB > 0 ? RWB : 4;
   using Sh = Shape<T, D, RW, bkw_of<T>(RW)>;
   static constexpr size_t LDS =
-      RWA == 0 ? 4 * sizeof(WaveLds<T, D>)
-               : (Sh::LDS > 4 * sizeof(WaveLds<T, D>) ? Sh::LDS : 4 * sizeof(WaveLds<T, D>));
+      RWA == 0  ? 4 * sizeof(WaveLds<T, D>)
+      : RWA < 0 ? Sh::LDS
+                : (Sh::LDS > 4 * sizeof(WaveLds<T, D>) ? Sh::LDS : 4 * sizeof(WaveLds<T, D>));
   static constexpr int PER_CU = sizeof(T) == 2 || D == 64 ? 2 : 1;
 };
 
@@ -1088,38 +1243,48 @@ __global__ __launch_bounds__(256, (Variant<T, D, RWA, RWB>::PER_CU)) void branch
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, grid = gridDim.x, blk = blockIdx.x;
   if constexpr (RWA == 0) {  // one list for both
-    const WaveSched<true> sched(a);
-    const int C = sched.total(lane);
-    wave_role<T, D, true>(a, ls, lds, blk * 4 + mfma::wave_id(), min(4 * grid, C), C);
+    const WaveSched<true> sched(a, lane);
+    wave_role<T, D, true>(a, ls, lds, sched, blk * 4 + mfma::wave_id(), min(4 * grid, sched.C));
+  } else if constexpr (RWA < 0) {
+    constexpr int BKW = bkw_of<T>(RWB);
+    using Sh = Shape<T, D, RWB, BKW>;
+    __shared__ uint32_t sbad[Sh::KC / 32];
+    TileSched<BOTH> s(a, Sh::ROWS, Sh::KC, false, lane);
+    if (s.C >= 4 * grid) s.count_beginnings();
+    tile_role<T, D, RWB, BKW, BOTH>(a, ls, lds, nullptr, sbad, s, blk, grid);
   } else {
     constexpr int BKW = bkw_of<T>(RWA);
     using Sh = Shape<T, D, RWA, BKW>;
     __shared__ int pre[MAX_COMPACT];
     __shared__ uint32_t sbad[Sh::KC / 32];
-    const TileSched<false> sa(a, Sh::ROWS, Sh::KC, ls.compact, lane);
+    TileSched<PREFIX> sa(a, Sh::ROWS, Sh::KC, ls.compact, lane);
     // The workgroups are shared out by the bytes of the two lists.
     auto split = [&](int most_b, float cost_b) {
       if (sa.C == 0 || most_b == 0) return sa.C == 0 ? 0 : grid;
       if (sa.C + most_b <= grid) return sa.C;
-      const int n = (int)((float)grid * (float)sa.C / ((float)sa.C + cost_b) + 0.5f);
+      const int n = (int)((float)grid * (float)sa.C / ((float)sa.C + cost_b) + 1.f);
       return min(max(n, 1), grid - 1);
     };
     if constexpr (RWB == 0) {
-      const WaveSched<false> sb(a);
-      const int C = sb.total(lane);
-      const int na = split((C + 3) / 4, (float)C * WK / Sh::KC);
+      const WaveSched<false> sb(a, lane);
+      if (sa.C + sb.C >= 4 * grid) sa.count_beginnings();
+      const int na = split((sb.C + 3) / 4, (float)sb.C * WK / Sh::KC);
       if (blk < na)
-        tile_role<T, D, RWA, BKW, false>(a, ls, lds, pre, sbad, sa, blk, na);
+        tile_role<T, D, RWA, BKW, PREFIX>(a, ls, lds, pre, sbad, sa, blk, na);
       else
-        wave_role<T, D, false>(a, ls, lds, (blk - na) * 4 + mfma::wave_id(),
-                               min(4 * (grid - na), C), C);
+        wave_role<T, D, false>(a, ls, lds, sb, (blk - na) * 4 + mfma::wave_id(),
+                               min(4 * (grid - na), sb.C));
     } else {
-      const TileSched<true> sb(a, Sh::ROWS, Sh::KC, false, lane);
+      TileSched<OWN> sb(a, Sh::ROWS, Sh::KC, false, lane);
+      if (sa.C + sb.C >= 4 * grid) {
+        sa.count_beginnings();
+        sb.count_beginnings();
+      }
       const int na = split(sb.C, (float)sb.C);
       if (blk < na)
-        tile_role<T, D, RWA, BKW, false>(a, ls, lds, pre, sbad, sa, blk, na);
+        tile_role<T, D, RWA, BKW, PREFIX>(a, ls, lds, pre, sbad, sa, blk, na);
       else
-        tile_role<T, D, RWA, BKW, true>(a, ls, lds, pre, sbad, sb, blk - na, grid - na);
+        tile_role<T, D, RWA, BKW, OWN>(a, ls, lds, pre, sbad, sb, blk - na, grid - na);
     }
   }
 }
@@ -1157,14 +1322,14 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
     __syncthreads();
     first = before;
   }
-  const bool live = inside && i < s.n;
+  bool live = inside && i < s.n;
   const int ra = (first + i) * n_rep + r % n_rep;
-  const int ia = (grp * a.Hkv + g) * ls.tiles_a + ra / ls.rows_a;
+  const int ia = (grp * a.Hkv + g) * ls.tiles_a + ra / max(ls.rows_a, 1);
   const int ib = (b * a.Hkv + g) * ls.tiles_b + r / ls.rows_b;
   int na = 0, nb = 0;
   int64_t at = 0, bt = 0;
   if (live) {
-    if (s.P > 0) {
+    if (s.P > 0 && ls.tiles_a > 0) {
       const int2 sh = ls.sha[ia];
       na = sh.y - sh.x + 1;
       at = ((int64_t)sh.x + ia) * ls.rows_a + ra % ls.rows_a;
@@ -1174,6 +1339,8 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
     bt = ((int64_t)sh.x + ib + ls.item_b) * ls.rows_b + r % ls.rows_b;
   }
   const int ns = na + nb;
+  // (one list for both and one worker: it wrote the outputs)
+  if (ls.tiles_a == 0 && ns == 1) live = false;
   float M = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   // joins a partial (of weight 0: left out, whatever it holds)
@@ -1184,7 +1351,7 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f + (w != 0.f ? w * po[e] : 0.f);
   };
   constexpr int U = 8;
-  for (int j0 = jg; j0 < ns; j0 += U * JG) {
+  for (int j0 = jg; live && j0 < ns; j0 += U * JG) {
     f32x4 po[U];
     float2 ml[U];
 #pragma unroll
@@ -1237,6 +1404,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // The stream kernel's shape for a call: row waves of the prefixes' tiles and of the own
 // rows' (0: one wavefront a share), or (none) one wavefront a row.
+constexpr int BOTH_ROWS = 96;
 struct Plan {
   bool none;
   int rwa, rwb, rows_a, rows_b, tiles_a, tiles_b, grid, workers_a, workers_b;
@@ -1247,20 +1415,26 @@ Plan plan_of(const BranchArgs& a) {
   const int n_rep = a.Hq / a.Hkv, W = a.B / a.G;
   if (a.D != 64 && a.D != 128) return p;
   const int64_t ma = (int64_t)W * a.N * n_rep, mb = (int64_t)a.N * n_rep;
+  // One list where the sequences' rows fill tiles of their own: BOTH_ROWS of 128 or more.
+  const bool both = mb >= BOTH_ROWS;
   const int rw = ma <= 64 ? 2 : 4;
-  p.rwa = a.dtype != F32 && ma <= 16 ? 0 : rw;
+  p.rwa = both ? -1 : a.dtype != F32 && ma <= 16 ? 0 : rw;
   p.rwb = a.dtype != F32 && mb <= 16 ? 0 : rw;
   const int kc = rw == 4 && a.dtype == F32 ? 32 : 64;
-  p.rows_a = p.rwa ? 32 * rw : (int)ma;
+  p.rows_a = both ? 0 : p.rwa ? 32 * rw : (int)ma;
   p.rows_b = p.rwb ? 32 * rw : p.rwa ? (int)mb : (int)ma;  // (one list: one kind of slot)
-  const int64_t ta = (ma + p.rows_a - 1) / p.rows_a, tb = (mb + p.rows_b - 1) / p.rows_b;
+  const int64_t ta = both ? 0 : (ma + p.rows_a - 1) / p.rows_a,
+                tb = (mb + p.rows_b - 1) / p.rows_b;
   const int ka = p.rwa ? kc : WK, kb = p.rwb ? kc : WK;
-  const int64_t ca = a.G * ta * a.Hkv * ((a.max_prefix + ka - 1) / ka),
-                cb = a.B * tb * a.Hkv * ((a.max_len + kb - 1) / kb + (p.rwb ? 0 : 1));
+  const int64_t pk = ((int64_t)a.max_prefix + ka - 1) / ka,
+                ca = a.G * ta * a.Hkv * (pk + OVER),
+                cb = a.B * tb * a.Hkv *
+                     (((int64_t)a.max_len + kb - 1) / kb + (both ? pk : 0) + (p.rwb ? OVER : 1));
   if (ca + cb >= INT_MAX || (a.G * ta + a.B * tb) * a.Hkv >= INT_MAX / 2) return p;
   p.tiles_a = (int)ta;
   p.tiles_b = (int)tb;
   const int per_cu = a.dtype != F32 || a.D == 64 ? 2 : 1;  // Variant::PER_CU
+  // (no more workgroups than chunks, each list having one at least)
   const int64_t wgs = (p.rwa ? ca : (ca + 3) / 4) + (p.rwb ? cb : (cb + 3) / 4);
   p.grid = (int)std::min<int64_t>(per_cu * std::min(device_cu_count(), 512), wgs);
   p.none = false;
@@ -1294,7 +1468,7 @@ Ws carve(const BranchArgs& a, const Plan& p, void* at) {
   ls.tiles_a = p.tiles_a;
   ls.tiles_b = p.tiles_b;
   ls.item_b = p.rwa ? 0 : (int)ia;
-  ls.compact = p.rwa && a.counts != nullptr && a.B / a.G <= MAX_COMPACT;
+  ls.compact = p.rwa > 0 && a.counts != nullptr && a.B / a.G <= MAX_COMPACT;
   ls.sha = (int2*)take(ia * sizeof(int2));
   ls.shb = (int2*)take(ib * sizeof(int2));
   const size_t slots = ((size_t)(p.rwb ? p.grid : 4 * p.grid) + ls.item_b + ib) * p.rows_b;
@@ -1302,7 +1476,7 @@ Ws carve(const BranchArgs& a, const Plan& p, void* at) {
   ls.mlb = (float*)take(slots * 8);
   ls.oa = ls.ob;
   ls.mla = ls.mlb;
-  if (p.rwa) {
+  if (p.rwa > 0) {
     const size_t more = ((size_t)p.grid + ia) * p.rows_a;
     ls.oa = (float*)take(more * a.D * 4);
     ls.mla = (float*)take(more * 8);
@@ -1339,9 +1513,13 @@ template <typename T, int D>
 int stream_and_merge(const BranchArgs& a, const Ws& w, const Plan& p) {
   int rc;
   if constexpr (std::is_same<T, float>::value) {
-    rc = p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p) : launch_stream<T, D, 4, 4>(a, w, p);
+    rc = p.rwa < 0    ? launch_stream<T, D, -1, 4>(a, w, p)
+         : p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p)
+                      : launch_stream<T, D, 4, 4>(a, w, p);
   } else {
-    if (p.rwa == 0)
+    if (p.rwa < 0)
+      rc = launch_stream<T, D, -1, 4>(a, w, p);
+    else if (p.rwa == 0)
       rc = launch_stream<T, D, 0, 0>(a, w, p);
     else if (p.rwb == 0)
       rc = p.rwa == 2 ? launch_stream<T, D, 2, 0>(a, w, p) : launch_stream<T, D, 4, 0>(a, w, p);
@@ -1349,7 +1527,7 @@ int stream_and_merge(const BranchArgs& a, const Ws& w, const Plan& p) {
       rc = p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p) : launch_stream<T, D, 4, 4>(a, w, p);
   }
   if (rc) return rc;
-  const int64_t items = (int64_t)a.G * a.Hkv * p.tiles_a;
+  const int64_t items = p.rwa < 0 ? (int64_t)a.B * a.Hkv * p.tiles_b : (int64_t)a.G * a.Hkv * p.tiles_a;
   const int64_t workers = p.rwa ? p.grid : 4 * p.grid;
   const int jg = workers > 32 * items ? 8 : workers > 8 * items ? 2 : 1;
   const int rpw = 256 / (D / 4) / jg;  // rows of a workgroup
