@@ -14,6 +14,8 @@ Paths (reference lines in ``kempnerforge/model/attention.py``):
 * decode, one token with a cache (``:169-175,229-231``): ``kf_attn_decode``;
 * prefill with a cache (``:169-175,229-231``): ``kf_kv_cache_append`` then the
   forward over the cache with the reference's top-left causal alignment;
+* several sequences behind one prompt (:class:`BranchKVCache`; no counterpart in the
+  reference): ``kf_attn_branch``, and :func:`reorder_branches` for beams;
 * a tree of drafted tokens with a cache (:func:`begin_tree`; no counterpart in the
   reference): ``kf_attn_tree``, after which :func:`keep_path` makes the accepted
   tokens the cache's next ones;
@@ -103,6 +105,9 @@ class KVCache:
         value = int(value)
         if not 0 <= value <= self.max_seq_len:
             raise ValueError(f"seq_len must lie in [0, {self.max_seq_len}] (got {value})")
+        self._set_level(value)
+
+    def _set_level(self, value: int) -> None:
         self._seq_len = value
         self.lens.fill_(value)
         self.ragged = False
@@ -127,8 +132,8 @@ class KVCache:
         lengths = [int(x) for x in lengths]
         if len(lengths) != self.lens.shape[0]:
             raise ValueError(f"need {self.lens.shape[0]} lengths (got {len(lengths)})")
-        if min(lengths) < 0 or max(lengths) > self.max_seq_len:
-            raise ValueError(f"lengths must lie in [0, {self.max_seq_len}]")
+        if min(lengths) < 0 or max(lengths) > self.k.shape[2]:
+            raise ValueError(f"lengths must lie in [0, {self.k.shape[2]}]")
         self.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
         self._seq_len = max(lengths)
         self.ragged = len(set(lengths)) > 1
@@ -157,6 +162,83 @@ class KVCache:
     def _advance(self, new_len: int) -> None:
         self._seq_len += new_len
         self.lens.add_(new_len)
+
+
+    def branch(self, branches: int, max_new_len: int) -> BranchKVCache:
+        """A cache for ``branches`` sequences behind each of this one's, up to
+        ``max_new_len`` tokens each (:class:`BranchKVCache`)."""
+        return BranchKVCache(self, branches, max_new_len)
+
+
+class BranchKVCache(KVCache):
+    """KV cache of ``branches`` sequences behind each sequence of ``prefix``: beams of a
+    beam search, several samples of a prompt, a batch behind one system prompt.
+
+    The prompt's rows stay in ``prefix`` and are read once for all its branches;
+    ``k``, ``v`` and ``lens`` hold only what comes behind.  Sequence b follows prompt
+    ``b // branches``.  ``prefix`` counts as it is when the branches are made: rows that
+    it gets later are not seen, those that it holds must stay.  ``seq_len`` is the prompt
+    and the branch together (the longest of each), ``lens`` and :meth:`set_lengths` the
+    branch's own tokens.  A model's forward takes any number of tokens a sequence (right
+    padding as with any cache: :meth:`set_lengths` afterwards); no masks, no capture, no
+    trees of drafts.  Prompts of different lengths need the full RoPE tables
+    (:meth:`use_rope_tables`, taken over from ``prefix``)."""
+
+    def __init__(self, prefix: KVCache, branches: int, max_new_len: int) -> None:
+        if isinstance(prefix, BranchKVCache):
+            raise ValueError("branches of branches are not supported")
+        if branches < 1 or max_new_len < 1:
+            raise ValueError(f"branches and max_new_len must be at least 1 (got {branches}, "
+                             f"{max_new_len})")
+        batch, n_kv_heads, _, head_dim = prefix.k.shape
+        super().__init__(batch * branches, max_new_len, n_kv_heads, head_dim, prefix.k.dtype,
+                         prefix.k.device)
+        self.prefix, self.branches = prefix, branches
+        self.prefix_lens, self.prefix_len = prefix.lens.clone(), prefix.seq_len
+        self.prefix_ragged, self.rope_tables = prefix.ragged, prefix.rope_tables
+
+    @property
+    def max_seq_len(self) -> int:
+        return self.prefix_len + self.k.shape[2]
+
+    @property
+    def seq_len(self) -> int:
+        """Prompt and branch together (the longest prompt, the longest branch)."""
+        return self.prefix_len + self._seq_len
+
+    @seq_len.setter
+    def seq_len(self, value: int) -> None:
+        """Rewinds every branch to this many tokens, the prompt's included."""
+        value = int(value)
+        if not self.prefix_len <= value <= self.max_seq_len:
+            raise ValueError(f"seq_len must lie in [{self.prefix_len}, {self.max_seq_len}] "
+                             f"(got {value})")
+        self._set_level(value - self.prefix_len)
+
+    def update(self, k_new, v_new):
+        raise ValueError("a branch's rows lie in two caches: there is no one view of them")
+
+    def _decode_tables(self, cos: torch.Tensor, sin: torch.Tensor):
+        if self.rope_tables is None and self.prefix_ragged:
+            raise ValueError("branches of a ragged KV cache need the full RoPE tables: call "
+                             "use_rope_tables")
+        return super()._decode_tables(cos, sin)
+
+
+def reorder_branches(caches, parents: torch.Tensor) -> None:
+    """Every branch continues another one of its prompt (``parents [prompts, branches]``
+    int32 on the device, what ``ops.beam_select_raw`` returns; -1: left alone): the own
+    rows of all layers' caches (:class:`BranchKVCache`, one per layer) follow, in one
+    launch.  The fill levels are the same for all layers."""
+    first = caches[0]
+    ops.cache_reorder_raw([c.k for c in caches], [c.v for c in caches], first.lens, parents)
+    if first.ragged:  # (otherwise all levels are one)
+        W = parents.shape[1]
+        at = torch.arange(parents.numel(), device=parents.device).view(parents.shape)
+        known = (parents >= 0) & (parents < W)
+        lens = first.lens[torch.where(known, at // W * W + parents, at).view(-1)]
+        for c in caches:
+            c.lens.copy_(lens)
 
 
 def begin_tree(caches, parents: torch.Tensor | None = None,
@@ -251,10 +333,14 @@ class Attention(nn.Module):
         tree = getattr(kv_cache, "tree", None)  # (no cache, or a caller's own kind: none)
         if tree is not None and (masked or self.capture_attention_weights):
             raise ValueError("a tree of drafts takes no doc_ids, no key_padding_mask and no capture")
+        branch = isinstance(kv_cache, BranchKVCache)
+        if branch and (masked or self.capture_attention_weights or tree is not None):
+            raise ValueError("branches take no doc_ids, no key_padding_mask, no capture and no "
+                             "tree of drafts")
         decode = (kv_cache is not None and seq_len == 1 and not masked
                   and not self.capture_attention_weights)
         # decode applies the QK-norm inside its kernels (one eps for both)
-        fuse_norm = ((decode or tree is not None) and self.q_norm is not None
+        fuse_norm = ((decode or branch or tree is not None) and self.q_norm is not None
                      and self.q_norm.eps == self.k_norm.eps)  # type: ignore[union-attr]
         if self.q_norm is not None and not fuse_norm:
             q = self.q_norm(q)
@@ -284,6 +370,17 @@ class Attention(nn.Module):
                                 key_padding_mask=key_padding_mask)
         elif kv_cache is None:
             out = ops.attention(q, k, v, rope_cos, rope_sin, causal=True)
+        elif branch:
+            kv_cache._check_room(seq_len)
+            cos_t, sin_t, row0 = kv_cache._decode_tables(rope_cos, rope_sin)
+            out = ops.branch_decode_raw(
+                q, k, v, kv_cache.prefix.k, kv_cache.prefix.v, kv_cache.prefix_lens, kv_cache.k,
+                kv_cache.v, kv_cache.lens, cos_t, sin_t, rope_row_offset=row0,
+                max_prefix=kv_cache.prefix_len, max_len=kv_cache._seq_len + seq_len,
+                q_norm_weight=self.q_norm.weight if fuse_norm else None,  # type: ignore[union-attr]
+                k_norm_weight=self.k_norm.weight if fuse_norm else None,  # type: ignore[union-attr]
+                norm_eps=self.q_norm.eps if fuse_norm else 1e-5)  # type: ignore[union-attr]
+            kv_cache._advance(seq_len)
         elif tree is not None:
             kv_cache._check_room(seq_len)
             cos_t, sin_t, row0 = kv_cache._decode_tables(rope_cos, rope_sin)

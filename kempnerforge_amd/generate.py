@@ -3,7 +3,7 @@
 ``sample`` and ``generate`` keep the signatures and results of
 ``kempnerforge/model/generate.py:15-124`` (temperature, top-k, top-p sampling;
 prefill, then one token per step through the model with one ``KVCache`` per
-layer).  Two additions, both off by default:
+layer).  Three additions, all off by default:
 
 * ``prompt_lens``: prompts of different lengths in one batch, right-padded in
   ``prompt_tokens``.  The prefill runs on the padded batch, then every layer's
@@ -16,6 +16,12 @@ layer).  Two additions, both off by default:
   token); every N steps keeps the GPU queue full, and the output is cut at the
   step where the last sequence finished, so it is the same as the reference's
   (up to N - 1 decode steps are computed and discarded).
+
+* ``num_samples``: several continuations of each prompt.  The prompt is prefilled and
+  its keys and values are kept and read once for all of them (``BranchKVCache``).
+
+``beam_generate`` (no counterpart in the reference) keeps the most likely continuations
+of each prompt, likewise behind one copy of it.
 
 ``speculative_generate`` (no counterpart in the reference) emits tokens of the same
 distribution several at a time: a smaller model drafts a chain or a tree of them,
@@ -34,7 +40,7 @@ import contextlib
 import torch
 
 from kempnerforge_amd import ops
-from kempnerforge_amd.attention import KVCache, begin_tree, keep_path
+from kempnerforge_amd.attention import KVCache, begin_tree, keep_path, reorder_branches
 from kempnerforge_amd.position import precompute_rope_frequencies
 
 
@@ -76,6 +82,24 @@ def _rope_tables(model, total_len: int, device):
     return cos.to(device), sin.to(device)
 
 
+def _prefill(model, prompt_tokens, prompt_lens, rows: int, total_len: int):
+    """Caches of ``rows`` tokens that hold the prompts, and the logits behind each."""
+    cfg, device = model.config, prompt_tokens.device
+    batch = prompt_tokens.shape[0]
+    dtype = next(model.parameters()).dtype
+    caches = [KVCache(batch, rows, cfg.n_kv_heads, cfg.head_dim, dtype, device)
+              for _ in range(cfg.n_layers)]
+    logits = model(prompt_tokens, kv_caches=caches)
+    if prompt_lens is None:
+        return caches, logits[:, -1, :]
+    last = torch.tensor([n - 1 for n in prompt_lens], device=device)
+    cos, sin = _rope_tables(model, total_len, device)
+    for c in caches:
+        c.set_lengths(prompt_lens)
+        c.use_rope_tables(cos, sin)
+    return caches, logits[torch.arange(batch, device=device), last]
+
+
 @torch.no_grad()
 def generate(
     model,
@@ -88,8 +112,10 @@ def generate(
     eos_token_id: int | None = None,
     prompt_lens: list[int] | None = None,
     eos_check_every: int = 1,
+    num_samples: int = 1,
 ) -> torch.Tensor:
-    """Prompt plus generated tokens, ``(batch, prompt_len + generated)``.
+    """Prompt plus generated tokens, ``(batch * num_samples, prompt_len + generated)``
+    (a prompt's samples one after the other).
 
     Without ``prompt_lens`` this is the reference's ``generate``
     (``kempnerforge/model/generate.py:59-124``).  With it, sequence ``b``'s
@@ -99,6 +125,8 @@ def generate(
     """
     if eos_check_every < 1:
         raise ValueError("eos_check_every must be >= 1")
+    if num_samples < 1:
+        raise ValueError("num_samples must be >= 1")
     was_training = model.training
     model.eval()
     device = prompt_tokens.device
@@ -114,20 +142,16 @@ def generate(
         prompt_lens = [int(n) for n in prompt_lens]
         if len(prompt_lens) != batch or min(prompt_lens) < 1 or max(prompt_lens) > prompt_len:
             raise ValueError("prompt_lens needs one length in [1, prompt_len] per sequence")
-    dtype = next(model.parameters()).dtype
-    caches = [KVCache(batch, total_len, cfg.n_kv_heads, cfg.head_dim, dtype, device)
-              for _ in range(cfg.n_layers)]
-
-    logits = model(prompt_tokens, kv_caches=caches)
-    if prompt_lens is None:
-        next_logits = logits[:, -1, :]
-    else:
-        last = torch.tensor([n - 1 for n in prompt_lens], device=device)
-        next_logits = logits[torch.arange(batch, device=device), last]
-        cos, sin = _rope_tables(model, total_len, device)
-        for c in caches:
-            c.set_lengths(prompt_lens)
-            c.use_rope_tables(cos, sin)
+    caches, next_logits = _prefill(model, prompt_tokens, prompt_lens,
+                                   prompt_len if num_samples > 1 else total_len, total_len)
+    if num_samples > 1 and max_new_tokens > 0:
+        caches = [c.branch(num_samples, max_new_tokens) for c in caches]
+    if num_samples > 1:
+        next_logits = next_logits.repeat_interleave(num_samples, dim=0)
+        prompt_tokens = prompt_tokens.repeat_interleave(num_samples, dim=0)
+        batch *= num_samples
+        if prompt_lens is not None:
+            prompt_lens = [n for n in prompt_lens for _ in range(num_samples)]
 
     generated = []
     done = torch.zeros(batch, dtype=torch.bool, device=device)
@@ -161,6 +185,129 @@ def generate(
         out[b, :n] = prompt_tokens[b, :n]
         out[b, n:n + gen.shape[1]] = gen[b]
     return out
+
+
+@torch.no_grad()
+def beam_generate(
+    model,
+    prompt_tokens: torch.Tensor,
+    max_new_tokens: int,
+    *,
+    beams: int = 4,
+    num_return: int = 1,
+    length_penalty: float = 1.0,
+    eos_token_id: int | None = None,
+    prompt_lens: list[int] | None = None,
+    eos_check_every: int = 1,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``num_return`` best continuations of each prompt by beam search: tokens
+    ``(batch, num_return, width)``, best first, and their scores ``(batch, num_return)``
+    float32.
+
+    A continuation's score is its summed log-probability divided by its length (its
+    ``eos_token_id`` counts) to the power of ``length_penalty``.  Each step keeps the
+    ``beams`` most likely unfinished continuations of each prompt; one that ends, and is
+    among the ``beams`` best of all the step's, is set aside with its score, the best
+    ``beams`` of these are kept, and after ``max_new_tokens`` the unfinished ones join
+    them.  The search ends early where no unfinished one can reach the worst of
+    ``beams`` finished ones any more (read back every ``eos_check_every`` steps).
+
+    The prompts are prefilled once; their keys and values are read once for all beams
+    (``kf_attn_branch``), the step's candidates picked in one call (``kf_beam_select``),
+    and the beams' own cache rows moved in one launch (``kf_kv_cache_reorder``).
+    ``prompt_lens`` as in :func:`generate`.  Rows hold the prompt, directly followed by
+    the continuation, padded on the right with ``eos_token_id`` (or 0); a continuation
+    that the vocabulary does not give (fewer than ``num_return``) has the score -inf and
+    no tokens."""
+    batch, prompt_len = prompt_tokens.shape
+    if not 1 <= beams <= ops.BEAM_MAX:
+        raise ValueError(f"beams must lie in [1, {ops.BEAM_MAX}] (got {beams})")
+    if not 1 <= num_return <= beams:
+        raise ValueError(f"num_return must lie in [1, beams] (got {num_return})")
+    if max_new_tokens < 1 or eos_check_every < 1:
+        raise ValueError("max_new_tokens and eos_check_every must be >= 1")
+    limit = model.config.max_seq_len
+    if prompt_len + max_new_tokens > limit:
+        raise ValueError(
+            f"prompt ({prompt_len}) + max_new_tokens ({max_new_tokens}) = "
+            f"{prompt_len + max_new_tokens} exceeds model max_seq_len ({limit})"
+        )
+    if prompt_lens is not None:
+        prompt_lens = [int(n) for n in prompt_lens]
+        if len(prompt_lens) != batch or min(prompt_lens) < 1 or max(prompt_lens) > prompt_len:
+            raise ValueError("prompt_lens needs one length in [1, prompt_len] per sequence")
+    with _evaluating(model):
+        scores, rows, lengths = _beam_search(model, prompt_tokens, prompt_lens, max_new_tokens,
+                                             beams, length_penalty, eos_token_id, eos_check_every)
+    scores, best = scores.topk(num_return, dim=1)
+    rows = rows.gather(1, best[..., None].expand(-1, -1, max_new_tokens)).cpu()
+    lengths = lengths.gather(1, best).tolist()
+    starts = prompt_lens if prompt_lens is not None else [prompt_len] * batch
+    pad = eos_token_id if eos_token_id is not None else 0
+    width = max(n + max(row) for n, row in zip(starts, lengths))
+    out = torch.full((batch, num_return, width), pad, dtype=prompt_tokens.dtype)
+    host_prompt = prompt_tokens.cpu()
+    for b, n in enumerate(starts):
+        out[b, :, :n] = host_prompt[b, :n]
+        for r, k in enumerate(lengths[b]):
+            out[b, r, n:n + k] = rows[b, r, :k].to(out.dtype)
+    return out.to(prompt_tokens.device), scores
+
+
+def _beam_search(model, prompt_tokens, prompt_lens, max_new_tokens, beams, length_penalty,
+                 eos_token_id, eos_check_every):
+    """Scores ``[batch, 2 beams]``, tokens and lengths of the finished continuations and
+    of the unfinished ones at the end."""
+    device, (batch, prompt_len) = prompt_tokens.device, prompt_tokens.shape
+    caches, logits = _prefill(model, prompt_tokens, prompt_lens, prompt_len,
+                              prompt_len + max_new_tokens)
+    caches = [c.branch(beams, max_new_tokens) for c in caches]
+    inf = float("inf")
+    scores = torch.zeros(batch, 1, device=device, dtype=torch.float32)
+    rows = torch.zeros(batch, 1, max_new_tokens, dtype=torch.int64, device=device)
+    rank = torch.arange(2 * beams, device=device)
+    done_scores = torch.full((batch, beams), -inf, device=device, dtype=torch.float32)
+    done_rows = torch.zeros(batch, beams, max_new_tokens, dtype=torch.int64, device=device)
+    done_lens = torch.zeros(batch, beams, dtype=torch.int64, device=device)
+    # what an unfinished continuation of summed log-probability s can still reach: s / this
+    longest = float(max_new_tokens) ** length_penalty
+    for step in range(1, max_new_tokens + 1):
+        # (first step: one sequence a prompt)
+        best, parents, tokens = ops.beam_select_raw(
+            logits.reshape(batch, scores.shape[1], -1), scores, select=2 * beams)
+        rows = rows.gather(1, parents.clamp_min(0).long()[..., None].expand(-1, -1, max_new_tokens))
+        rows[:, :, step - 1] = tokens.clamp_min(0)
+        ends = torch.zeros_like(tokens, dtype=torch.bool)
+        if eos_token_id is not None:
+            ends = tokens == eos_token_id
+            ended = torch.where(ends & (rank < beams), best / float(step) ** length_penalty, -inf)
+            done_scores, at = torch.cat([done_scores, ended], 1).topk(beams, dim=1)
+            done_rows = torch.cat([done_rows, rows], 1).gather(
+                1, at[..., None].expand(-1, -1, max_new_tokens))
+            done_lens = torch.cat([done_lens, torch.full_like(tokens, step)], 1).gather(1, at)
+        # the best that go on, in order (at most one candidate a beam ends)
+        live = torch.sort(ends.to(torch.int8), dim=1, stable=True).indices[:, :beams]
+        scores = torch.where(ends, -inf, best).gather(1, live)
+        tokens, parents = tokens.gather(1, live), parents.gather(1, live)
+        rows = rows.gather(1, live[..., None].expand(-1, -1, max_new_tokens))
+        if step == max_new_tokens:
+            break
+        if eos_token_id is not None and step % eos_check_every == 0:
+            reach = scores.amax(1) / (longest if length_penalty >= 0
+                                      else float(step + 1) ** length_penalty)
+            if bool((reach <= done_scores.amin(1)).all()):
+                scores = torch.full_like(scores, -inf)
+                break
+        if step > 1:
+            reorder_branches(caches, parents.contiguous())
+        logits = model(tokens.clamp_min(0).view(-1, 1).to(prompt_tokens.dtype),
+                       kv_caches=caches)[:, -1, :]
+    left = scores / float(step) ** length_penalty
+    lens = torch.where(torch.isinf(left), 0, step).to(torch.int64)
+    done_lens = torch.where(torch.isinf(done_scores), 0, done_lens)
+    return (torch.cat([done_scores, left], 1), torch.cat([done_rows, rows], 1),
+            torch.cat([done_lens, lens], 1))
+
 
 
 def _tree_levels(tree) -> tuple[list[int], list[int], list[int]]:
