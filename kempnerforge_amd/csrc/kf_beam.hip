@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace kf {
 
@@ -412,6 +413,12 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
 // 16 bytes of a row of all its group's sequences, and reads every one that is continued
 // elsewhere before it writes any.  No other thread touches them, so the move needs no
 // second buffer, whatever the parents (cycles, several children of one).
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x),
+                 hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
+
 struct ReorderPtrs {
   char *k[KEEP_CACHES], *v[KEEP_CACHES];
 };
@@ -445,18 +452,28 @@ __global__ __launch_bounds__(256) void cache_reorder_kernel(
     }
   }
   __syncthreads();
+  // (the same for all threads: in scalar registers)
+  using Mask = typename std::conditional<MW <= 32, uint32_t, uint64_t>::type;
+  Mask to[MW];
+  int64_t end_of[MW];
+#pragma unroll
+  for (int w = 0; w < MW; ++w) {
+    to[w] = (Mask)uniform64(kids[w]);
+    end_of[w] = uniform64(last[w]);
+  }
   const int64_t stride = (int64_t)Hkv * Smax * row_units;  // between two sequences
   U* at = (U*)base + ((int64_t)g * W * Hkv + h) * (int64_t)Smax * row_units;
-  const int64_t end = (int64_t)most * row_units;
+  const int64_t end = uniform64((int64_t)most * row_units);
   for (int64_t i = (int64_t)blockIdx.z * 256 + t; i < end; i += (int64_t)gridDim.z * 256) {
     U x[MW];
 #pragma unroll
     for (int w = 0; w < MW; ++w)
-      if (w < W && i < last[w]) x[w] = at[w * stride + i];
+      if (to[w] && i < end_of[w]) x[w] = at[w * stride + i];
 #pragma unroll
     for (int w = 0; w < MW; ++w)
-      if (w < W && i < last[w])
-        for (uint64_t m = kids[w]; m; m &= m - 1) at[__builtin_ctzll(m) * stride + i] = x[w];
+      if (to[w] && i < end_of[w])
+        for (Mask m = to[w]; m; m &= m - 1)
+          at[__builtin_ctzll(m) * stride + i] = x[w];
   }
 }
 
