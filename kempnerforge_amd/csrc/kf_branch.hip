@@ -170,18 +170,20 @@ struct Lists {
 };
 
 // ---- one wavefront a share: up to 16 rows
-// A chunk is 32 keys.  Products on 16 x 16 tiles:
-//   S^T (keys x rows) = K q^T: lane l supplies key (or row) l % 16, dims 8 (l / 16) ..
-//       of each 32
-//   O^T (dims x rows) += V^T P^T: V through the wavefront's LDS and back transposed, P^T
-//       straight from the S registers (lane l holds row l % 16, keys 4 (l / 16) .. of
-//       each 16)
+// A chunk is 32 keys (float32: 16).  Products on 16 x 16 tiles:
+//   S^T (keys x rows) = K q^T: lane l supplies key (or row) l % 16, 16 bytes l / 16 of each
+//       64 of the row
+//   O^T (dims x rows) += V^T P^T: P^T straight from the S registers (lane l holds row l %
+//       16, keys 4 (l / 16) .. of each 16); V through the wavefront's LDS and back
+//       transposed, or (float32) loaded as the operand is: dim l % 16 of each 16 of keys
+//       4 (l / 16) ..
 // The next chunk's rows are loaded while one is computed.
-constexpr int WK = 32;  // keys of a chunk
+template <typename T>
+constexpr int WK = sizeof(T) == 4 ? 16 : 32;  // keys of a chunk
 
 // Entities of the list: (ALL) the groups' prefixes, then the sequences' own rows: the chunks
 // of what is cached, then one of the new tokens (16 at most).
-template <bool ALL>
+template <bool ALL, int WKEYS>
 struct WaveSched {
   const BranchArgs& a;
   int G0, B, C;  // groups in front, entities, chunks
@@ -208,7 +210,7 @@ struct WaveSched {
     return make_int3(__builtin_amdgcn_readlane(x.x, at), __builtin_amdgcn_readlane(x.y, at),
                      __builtin_amdgcn_readlane(x.z, at));
   }
-  static __device__ __forceinline__ int nck(int3 k) { return (k.x + WK - 1) / WK + (k.y > 0); }
+  static __device__ __forceinline__ int nck(int3 k) { return (k.x + WKEYS - 1) / WKEYS + (k.y > 0); }
   __device__ __forceinline__ int chunks(int e) const { return nck(keys(e)) * a.Hkv; }
   // the entity that holds a chunk, and its first one
   __device__ __forceinline__ void locate(int c, int lane, int& e, int& base) const {
@@ -224,15 +226,18 @@ struct WaveSched {
 
 template <typename T, int D>
 struct WaveLds {
-  T v[WK * D];
+  T v[sizeof(T) == 4 ? 4 : WK<T> * D];
 };
 
 template <typename T, int D, bool ALL>
 __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, char* lds,
-                                          const WaveSched<ALL>& sched, int gw, int NW) {
+                                          const WaveSched<ALL, WK<T>>& sched, int gw, int NW) {
   using namespace mfma;
-  constexpr int KT = D / 32, DB = D / 16, KR = D / 8, HALF = D / 2;
-  constexpr int VL = WK * KR / 64;
+  using P = Piece<T>;
+  constexpr bool F32T = sizeof(T) == 4;
+  constexpr int E = P::E, KEYS = WK<T>, NB = KEYS / 16;  // values of 16 bytes, blocks of 16 keys
+  constexpr int KT = D / (4 * E), DB = D / 16, KR = D / E, HALF = D / 2;
+  constexpr int VL = KEYS * KR / 64;
   // P = 2^(s - m + LIFT), m moved only when a score is 2^SLACK above it (as in the tiles below):
   // chunk after chunk nothing crosses lanes
   constexpr bool HALF_P = std::is_same<T, _Float16>::value;
@@ -264,7 +269,7 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
   };
   auto is_prefix = [&](const Cursor& c) { return ALL && c.e < sched.G0; };
   auto is_new = [&](const Cursor& c) { return c.k.y > 0 && c.lc == c.nck - 1; };
-  auto chunk_rows = [&](const Cursor& c) { return is_new(c) ? c.k.y : min(c.k.x - c.lc * WK, WK); };
+  auto chunk_rows = [&](const Cursor& c) { return is_new(c) ? c.k.y : min(c.k.x - c.lc * KEYS, KEYS); };
   // A chunk's row r begins at base + r * stride; rows behind the last repeat it.  The caches
   // are read once a step: non-temporal loads.
   struct Rows {
@@ -276,46 +281,60 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
   // in memory)
   auto rows_of = [&](const Cursor& c, const void* pre, const void* own, const void* fresh) {
     const int64_t b = c.e - sched.G0;
-    int64_t at = (((b * a.Hkv + c.g) * a.Smax + c.lc * WK) * D) * 2;
+    int64_t at = (((b * a.Hkv + c.g) * a.Smax + c.lc * KEYS) * D) * (int)sizeof(T);
     if (is_prefix(c))
       at = ((const char*)pre - (const char*)own) +
-           ((((int64_t)c.e * a.Hkv + c.g) * a.Pmax + c.lc * WK) * D) * 2;
-    if (is_new(c)) at = ((const char*)fresh - (const char*)own) + (b * N * a.Hkv + c.g) * D * 2;
+           ((((int64_t)c.e * a.Hkv + c.g) * a.Pmax + c.lc * KEYS) * D) * (int)sizeof(T);
+    if (is_new(c))
+      at = ((const char*)fresh - (const char*)own) + (b * N * a.Hkv + c.g) * D * (int)sizeof(T);
     Rows r;
     r.base = (const T*)((const char*)own + at);
     r.stride = is_new(c) ? a.Hkv * D : D;
     r.last = chunk_rows(c) - 1;
     return r;
   };
-  u32x4 kreg[2][KT];  // key 16 kb + c16 of the chunk, dims 32 ks + 8 q4 .. + 7
-  u32x4 vreg[VL];     // V row (64 j + lane) / KR, piece (64 j + lane) % KR
+  u32x4 kreg[NB][KT];  // key 16 kb + c16 of the chunk, dims 4 E ks + E q4 ..
+  // V row (64 j + lane) / KR, piece (64 j + lane) % KR; (float32) key 4 q4 + t, dim 16 blk + c16
+  // at t * DB + blk
+  u32x4 vreg[F32T ? 1 : VL];
+  float vf[F32T ? 4 * DB : 1];
   auto load_k = [&](const Cursor& c) {
     const Rows r = rows_of(c, a.k_prefix, a.k_cache, a.k_new);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const uint32_t off = (uint32_t)min(16 * kb + c16, r.last) * r.stride + 8 * q4;
+    for (int kb = 0; kb < NB; ++kb) {
+      const uint32_t off = (uint32_t)min(16 * kb + c16, r.last) * r.stride + E * q4;
 #pragma unroll
       for (int ks = 0; ks < KT; ++ks)
-        kreg[kb][ks] = __builtin_nontemporal_load((const u32x4*)(r.base + off + 32 * ks));
+        kreg[kb][ks] = __builtin_nontemporal_load((const u32x4*)(r.base + off + 4 * E * ks));
     }
   };
   auto load_v = [&](const Cursor& c) {
     const Rows r = rows_of(c, a.v_prefix, a.v_cache, a.v_new);
+    if constexpr (F32T) {
 #pragma unroll
-    for (int j = 0; j < VL; ++j) {
-      const int li = 64 * j + lane;
-      const uint32_t off = (uint32_t)min(li / KR, r.last) * r.stride + li % KR * 8;
-      vreg[j] = __builtin_nontemporal_load((const u32x4*)(r.base + off));
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t off = (uint32_t)min(4 * q4 + t, r.last) * r.stride + c16;
+#pragma unroll
+        for (int blk = 0; blk < DB; ++blk)
+          vf[t * DB + blk] = __builtin_nontemporal_load(r.base + off + 16 * blk);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VL; ++j) {
+        const int li = 64 * j + lane;
+        const uint32_t off = (uint32_t)min(li / KR, r.last) * r.stride + li % KR * 8;
+        vreg[j] = __builtin_nontemporal_load((const u32x4*)(r.base + off));
+      }
     }
   };
   // Pieces of a row (dims d ..) and of its other half, rotated, after the norm if there is one.
   struct Angles {
-    float c[8], s[8];
+    float c[E], s[E];
   };
   auto angles = [&](int64_t trow, int d) {
     Angles g;
 #pragma unroll
-    for (int x = 0; x < 8; x += 4) {
+    for (int x = 0; x < E; x += 4) {
       *(f32x4*)(g.c + x) = *(const f32x4*)(a.cos + trow + d + x);
       *(f32x4*)(g.s + x) = *(const f32x4*)(a.sin + trow + d + x);
     }
@@ -324,13 +343,13 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
   auto rotate = [&](float* f1, float* f2, const Angles& g, int d, const float* nw, float rs) {
     if (nw != nullptr) {
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
+      for (int x = 0; x < E; ++x) {
         f1[x] = f1[x] * rs * nw[d + x];
         f2[x] = f2[x] * rs * nw[d + HALF + x];
       }
     }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < E; ++x) {
       const float y1 = f1[x] * g.c[x] - f2[x] * g.s[x];
       f2[x] = f2[x] * g.c[x] + f1[x] * g.s[x];
       f1[x] = y1;
@@ -340,10 +359,10 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     float ss = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KT; ++ks) {
-      float f[8];
-      unpack8<T>(raw[ks], f);
+      float f[E];
+      P::unpack(raw[ks], f);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) ss += f[x] * f[x];
+      for (int x = 0; x < E; ++x) ss += f[x] * f[x];
     }
     ss += __shfl_xor(ss, 16, 64);
     ss += __shfl_xor(ss, 32, 64);
@@ -358,7 +377,7 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
                                       (4 * (c16 & 1)) * 2);
   const int tr_hs = tr_sw >> 1;
 
-  u32x4 qh[KT], ql[KT];
+  u32x4 qh[KT], ql[F32T ? 1 : KT];
   f32x4 acc[DB];
   float m = -INFINITY, lsum = 0.f;
   int token = 0;  // the lane's row's, of its sequence's new tokens
@@ -382,16 +401,16 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     const int64_t b = pre ? c.e * W + at : c.e - sched.G0;
     token = pre ? tok - at * N : tok;
     const T* qr =
-        (const T*)a.q_new + ((b * N + token) * a.Hq + (int64_t)c.g * n_rep + r % n_rep) * D + 8 * q4;
+        (const T*)a.q_new + ((b * N + token) * a.Hq + (int64_t)c.g * n_rep + r % n_rep) * D + E * q4;
 #pragma unroll
-    for (int ks = 0; ks < KT; ++ks) raw[ks] = *(const u32x4*)(qr + 32 * ks);
+    for (int ks = 0; ks < KT; ++ks) raw[ks] = *(const u32x4*)(qr + 4 * E * ks);
     int64_t pos = (int64_t)c.k.z + c.k.x + token;
     if (pre)
       pos = (int64_t)c.k.x + token +
             (sched.B <= 64 ? __shfl(sched.own.x, (int)b + sched.G0, 64) : a.lens[b]);
     const int64_t trow = table_row(a, pos);
 #pragma unroll
-    for (int ks = 0; ks < KT / 2; ++ks) ang[ks] = angles(trow, 32 * ks + 8 * q4);
+    for (int ks = 0; ks < KT / 2; ++ks) ang[ks] = angles(trow, 4 * E * ks + E * q4);
   };
   auto rotate_q = [&](const u32x4* raw, const Angles* ang) {
     int ln = lane;
@@ -401,21 +420,23 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     const float sc = a.scale * kLog2e;
 #pragma unroll
     for (int ks = 0; ks < KT / 2; ++ks) {
-      float f[2][8];
-      unpack8<T>(raw[ks], f[0]);
-      unpack8<T>(raw[ks + KT / 2], f[1]);
-      rotate(f[0], f[1], ang[ks], 32 * ks + 8 * q4, a.q_norm_w, rs);
+      float f[2][E];
+      P::unpack(raw[ks], f[0]);
+      P::unpack(raw[ks + KT / 2], f[1]);
+      rotate(f[0], f[1], ang[ks], 4 * E * ks + E * q4, a.q_norm_w, rs);
       __builtin_amdgcn_sched_barrier(0);  // (registers)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float hi[8];
 #pragma unroll
-        for (int y = 0; y < 8; ++y) f[x][y] *= sc;
-        qh[ks + x * (KT / 2)] = pack8<T>(f[x]);
-        unpack8<T>(qh[ks + x * (KT / 2)], hi);
+        for (int y = 0; y < E; ++y) f[x][y] *= sc;
+        qh[ks + x * (KT / 2)] = P::pack(f[x]);
+        if constexpr (!F32T) {
+          float hi[E];
+          P::unpack(qh[ks + x * (KT / 2)], hi);
 #pragma unroll
-        for (int y = 0; y < 8; ++y) f[x][y] -= hi[y];
-        ql[ks + x * (KT / 2)] = pack8<T>(f[x]);
+          for (int y = 0; y < E; ++y) f[x][y] -= hi[y];
+          ql[ks + x * (KT / 2)] = P::pack(f[x]);
+        }
       }
     }
     m = -INFINITY;
@@ -453,63 +474,92 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
       const float rs = a.k_norm_w != nullptr ? row_norm(kreg[0]) : 1.f;
       if (c16 < keys) {
         const int64_t trow = table_row(a, (int64_t)cc.k.z + cc.k.x + c16);
-        T* dst = (T*)a.k_cache + (at + c16) * D + 8 * q4;
+        T* dst = (T*)a.k_cache + (at + c16) * D + E * q4;
 #pragma unroll
         for (int ks = 0; ks < KT / 2; ++ks) {
-          float f[2][8];
-          unpack8<T>(kreg[0][ks], f[0]);
-          unpack8<T>(kreg[0][ks + KT / 2], f[1]);
-          rotate(f[0], f[1], angles(trow, 32 * ks + 8 * q4), 32 * ks + 8 * q4, a.k_norm_w, rs);
+          float f[2][E];
+          const int d = 4 * E * ks + E * q4;
+          P::unpack(kreg[0][ks], f[0]);
+          P::unpack(kreg[0][ks + KT / 2], f[1]);
+          rotate(f[0], f[1], angles(trow, d), d, a.k_norm_w, rs);
           __builtin_amdgcn_sched_barrier(0);  // (registers)
-          kreg[0][ks] = pack8<T>(f[0]);
-          kreg[0][ks + KT / 2] = pack8<T>(f[1]);
-          *(u32x4*)(dst + 32 * ks) = kreg[0][ks];
-          *(u32x4*)(dst + 32 * ks + HALF) = kreg[0][ks + KT / 2];
+          kreg[0][ks] = P::pack(f[0]);
+          kreg[0][ks + KT / 2] = P::pack(f[1]);
+          *(u32x4*)(dst + 4 * E * ks) = kreg[0][ks];
+          *(u32x4*)(dst + 4 * E * ks + HALF) = kreg[0][ks + KT / 2];
         }
       }
+      // (one new token: every row sees it)
+      if constexpr (F32T) {
 #pragma unroll
-      for (int j = 0; j < VL / 2; ++j) {
-        const int li = 64 * j + ln, row = li / KR, pc = li % KR;
-        bool fin = true;
-        if (row < keys) {
-          *(u32x4*)((T*)a.v_cache + (at + row) * D + 8 * pc) = vreg[j];
-          float f[8];
-          unpack8<T>(vreg[j], f);
+        for (int t = 0; t < 4; ++t) {
+          const int row = 4 * q4 + t;
+          T* dst = (T*)a.v_cache + (at + row) * D + c16;
+          bool fin = true;
+          if (row < keys)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) fin = fin && finite(f[x]);
+            for (int blk = 0; blk < DB; ++blk) {
+              dst[16 * blk] = vf[t * DB + blk];
+              fin = fin && finite(vf[t * DB + blk]);
+            }
+          const uint64_t x = keys > 1 ? __builtin_amdgcn_ballot_w64(!fin) : 0;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) bad |= (x >> (16 * y) & 0xffff ? 1u : 0u) << (4 * y + t);
         }
-        // (one new token: every row sees it)
-        const uint64_t x = keys > 1 ? __builtin_amdgcn_ballot_w64(!fin) : 0;
+      } else {
 #pragma unroll
-        for (int y = 0; y < 64 / KR; ++y)
-          bad |= (x >> (y * KR) & ((1ull << KR) - 1) ? 1u : 0u) << (64 / KR * j + y);
+        for (int j = 0; j < VL / 2; ++j) {
+          const int li = 64 * j + ln, row = li / KR, pc = li % KR;
+          bool fin = true;
+          if (row < keys) {
+            *(u32x4*)((T*)a.v_cache + (at + row) * D + 8 * pc) = vreg[j];
+            float f[8];
+            unpack8<T>(vreg[j], f);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) fin = fin && finite(f[x]);
+          }
+          const uint64_t x = keys > 1 ? __builtin_amdgcn_ballot_w64(!fin) : 0;
+#pragma unroll
+          for (int y = 0; y < 64 / KR; ++y)
+            bad |= (x >> (y * KR) & ((1ull << KR) - 1) ? 1u : 0u) << (64 / KR * j + y);
+        }
       }
     }
     Cursor ic = cc;
     if (more) next(ic);
-    f32x4 sc[2], sl[2];
+    f32x4 sc[NB], sl[NB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < NB; ++kb) {
       sc[kb] = sl[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KT; ++ks) {
-        sc[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(qh[ks]), sc[kb]);
-        sl[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(ql[ks]), sl[kb]);
+        if constexpr (F32T) {  // (two sums: each waits for its own last product)
+          const f32x4 x = __builtin_bit_cast(f32x4, kreg[kb][ks]),
+                      y = __builtin_bit_cast(f32x4, qh[ks]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f32x4& s = e & 1 ? sl[kb] : sc[kb];
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], s, 0, 0, 0);
+          }
+        } else {
+          sc[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(qh[ks]), sc[kb]);
+          sl[kb] = mfma16<T>(as_bf16x8(kreg[kb][ks]), as_bf16x8(ql[ks]), sl[kb]);
+        }
       }
     }
     if (more) load_k(ic);
     float tmax = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) sc[kb] += sl[kb];
-    if (keys < WK) {  // (a new token sees those before it and itself)
+    for (int kb = 0; kb < NB; ++kb) sc[kb] += sl[kb];
+    if (keys < KEYS) {  // (a new token sees those before it and itself)
       const int limit = fresh ? token + 1 : keys;
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
+      for (int t = 0; t < 4 * NB; ++t)
         sc[t / 4][t % 4] =
             16 * (t / 4) + 4 * q4 + t % 4 < limit ? sc[t / 4][t % 4] : -INFINITY;
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) tmax = fmaxf(tmax, sc[t / 4][t % 4]);
+    for (int t = 0; t < 4 * NB; ++t) tmax = fmaxf(tmax, sc[t / 4][t % 4]);
     if (__builtin_amdgcn_ballot_w64(tmax > m + SLACK || m == -INFINITY)) {
       tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
       tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
@@ -521,37 +571,53 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
       for (int blk = 0; blk < DB; ++blk) acc[blk] *= alpha;
     }
     const float ref = (m == -INFINITY ? 0.f : m) - LIFT;  // (-inf: no key yet)
-    float p[8];
+    float p[4 * NB];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
+    for (int t = 0; t < 4 * NB; ++t) {
       p[t] = fast_exp2(sc[t / 4][t % 4] - ref);
       lsum += p[t];
     }
-    u32x4 ph, pl;
+    if constexpr (F32T) {
+      if (keys < KEYS || bad)  // (rows behind the last, and those of `bad`: 0 x NaN)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint2 u = Tile<T, D>::split2(p[2 * t], p[2 * t + 1]);
-      ph[t] = u.x;
-      pl[t] = u.y;
-    }
-    // V rows into the tile (rows behind the last, and those of `bad`, as zeros)
+        for (int t = 0; t < 4; ++t) {
+          const bool drop = 4 * q4 + t >= keys || (bad >> (4 * q4 + t) & 1);
 #pragma unroll
-    for (int j = 0; j < VL; ++j) {
-      const int li = 64 * j + lane, row = li / KR, pc = li % KR;
-      const bool drop = row >= keys || (bad >> row & 1);
-      *(u32x4*)(lv + (row * KR + (pc ^ swz<KR>(row))) * 8) = drop ? u32x4{0u, 0u, 0u, 0u} : vreg[j];
-    }
-    if (more) load_v(ic);
+          for (int blk = 0; blk < DB; ++blk) vf[t * DB + blk] = drop ? 0.f : vf[t * DB + blk];
+        }
 #pragma unroll
-    for (int blk = 0; blk < DB; ++blk) {
-      const char* base = (const char*)lv + tr_base + (uint32_t)((blk ^ tr_hs) * 32);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)base);
-      const s16x4 hi =
-          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(base + 16 * KR * 16));
-      const bf16x8 vt =
-          __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[blk] = mfma16<T>(vt, as_bf16x8(ph), acc[blk]);
-      acc[blk] = mfma16<T>(vt, as_bf16x8(pl), acc[blk]);
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int blk = 0; blk < DB; ++blk)
+          acc[blk] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[t * DB + blk], p[t], acc[blk], 0, 0, 0);
+      if (more) load_v(ic);
+    } else {
+      u32x4 ph, pl;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint2 u = Tile<T, D>::split2(p[2 * t], p[2 * t + 1]);
+        ph[t] = u.x;
+        pl[t] = u.y;
+      }
+      // V rows into the tile (rows behind the last, and those of `bad`, as zeros)
+#pragma unroll
+      for (int j = 0; j < VL; ++j) {
+        const int li = 64 * j + lane, row = li / KR, pc = li % KR;
+        const bool drop = row >= keys || (bad >> row & 1);
+        *(u32x4*)(lv + (row * KR + (pc ^ swz<KR>(row))) * 8) = drop ? u32x4{0u, 0u, 0u, 0u} : vreg[j];
+      }
+      if (more) load_v(ic);
+#pragma unroll
+      for (int blk = 0; blk < DB; ++blk) {
+        const char* base = (const char*)lv + tr_base + (uint32_t)((blk ^ tr_hs) * 32);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)base);
+        const s16x4 hi =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(base + 16 * KR * 16));
+        const bf16x8 vt =
+            __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[blk] = mfma16<T>(vt, as_bf16x8(ph), acc[blk]);
+        acc[blk] = mfma16<T>(vt, as_bf16x8(pl), acc[blk]);
+      }
     }
     for (uint32_t x = bad; x; x &= x - 1) {  // one by one, for the rows that see them
       const int r = __builtin_ctz(x);
@@ -1234,7 +1300,7 @@ struct Variant {
       RWA == 0  ? 4 * sizeof(WaveLds<T, D>)
       : RWA < 0 ? Sh::LDS
                 : (Sh::LDS > 4 * sizeof(WaveLds<T, D>) ? Sh::LDS : 4 * sizeof(WaveLds<T, D>));
-  static constexpr int PER_CU = sizeof(T) == 2 || D == 64 ? 2 : 1;
+  static constexpr int PER_CU = sizeof(T) == 2 || D == 64 || RWA == 0 ? 2 : 1;
 };
 
 template <typename T, int D, int RWA, int RWB>
@@ -1243,7 +1309,7 @@ __global__ __launch_bounds__(256, (Variant<T, D, RWA, RWB>::PER_CU)) void branch
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, grid = gridDim.x, blk = blockIdx.x;
   if constexpr (RWA == 0) {  // one list for both
-    const WaveSched<true> sched(a, lane);
+    const WaveSched<true, WK<T>> sched(a, lane);
     wave_role<T, D, true>(a, ls, lds, sched, blk * 4 + mfma::wave_id(), min(4 * grid, sched.C));
   } else if constexpr (RWA < 0) {
     constexpr int BKW = bkw_of<T>(RWB);
@@ -1266,9 +1332,9 @@ __global__ __launch_bounds__(256, (Variant<T, D, RWA, RWB>::PER_CU)) void branch
       return min(max(n, 1), grid - 1);
     };
     if constexpr (RWB == 0) {
-      const WaveSched<false> sb(a, lane);
+      const WaveSched<false, WK<T>> sb(a, lane);
       if (sa.C + sb.C >= 4 * grid) sa.count_beginnings();
-      const int na = split((sb.C + 3) / 4, (float)sb.C * WK / Sh::KC);
+      const int na = split((sb.C + 3) / 4, (float)sb.C * WK<T> / Sh::KC);
       if (blk < na)
         tile_role<T, D, RWA, BKW, PREFIX>(a, ls, lds, pre, sbad, sa, blk, na);
       else
@@ -1303,15 +1369,7 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
   const int b = blockIdx.x / a.Hkv, g = blockIdx.x % a.Hkv, grp = b / W;
   const int r = blockIdx.y * RPW + threadIdx.x / (LPR * JG), jg = threadIdx.x / LPR % JG;
   const int col = threadIdx.x % LPR * 4, i = r / n_rep;
-  const Seq s = branch_seq(a, b);
   const bool inside = i < a.N;
-  T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + g * n_rep + r % n_rep) * D + col;
-  T y[4];
-  if (inside && jg == 0 && i >= s.n) {  // a refused sequence, or an unused token
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(s.n < 0 ? NAN : 0.f);
-    __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
-  }
   int first = (b % W) * a.N;  // the sequence's first token in its group's rows
   if (ls.compact) {
     if (threadIdx.x == 0) before = 0;
@@ -1322,21 +1380,29 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
     __syncthreads();
     first = before;
   }
-  bool live = inside && i < s.n;
-  const int ra = (first + i) * n_rep + r % n_rep;
+  // (what the row is made of is asked for beside what says whether it is one)
+  const int rr = inside ? r : 0, ra = (first + rr / n_rep) * n_rep + rr % n_rep;
   const int ia = (grp * a.Hkv + g) * ls.tiles_a + ra / max(ls.rows_a, 1);
-  const int ib = (b * a.Hkv + g) * ls.tiles_b + r / ls.rows_b;
+  const int ib = (b * a.Hkv + g) * ls.tiles_b + rr / ls.rows_b;
+  const int2 sha = ls.tiles_a > 0 ? ls.sha[ia] : int2{0, -1}, shb = ls.shb[ib];
+  const Seq s = branch_seq(a, b);
+  T* dst = (T*)a.out + (((int64_t)b * a.N + i) * a.Hq + g * n_rep + r % n_rep) * D + col;
+  T y[4];
+  if (inside && jg == 0 && i >= s.n) {  // a refused sequence, or an unused token
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(s.n < 0 ? NAN : 0.f);
+    __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), y, sizeof(y));
+  }
+  bool live = inside && i < s.n;
   int na = 0, nb = 0;
   int64_t at = 0, bt = 0;
   if (live) {
     if (s.P > 0 && ls.tiles_a > 0) {
-      const int2 sh = ls.sha[ia];
-      na = sh.y - sh.x + 1;
-      at = ((int64_t)sh.x + ia) * ls.rows_a + ra % ls.rows_a;
+      na = sha.y - sha.x + 1;
+      at = ((int64_t)sha.x + ia) * ls.rows_a + ra % ls.rows_a;
     }
-    const int2 sh = ls.shb[ib];
-    nb = sh.y - sh.x + 1;
-    bt = ((int64_t)sh.x + ib + ls.item_b) * ls.rows_b + r % ls.rows_b;
+    nb = shb.y - shb.x + 1;
+    bt = ((int64_t)shb.x + ib + ls.item_b) * ls.rows_b + rr % ls.rows_b;
   }
   const int ns = na + nb;
   // (one list for both and one worker: it wrote the outputs)
@@ -1418,14 +1484,15 @@ Plan plan_of(const BranchArgs& a) {
   // One list where the sequences' rows fill tiles of their own: BOTH_ROWS of 128 or more.
   const bool both = mb >= BOTH_ROWS;
   const int rw = ma <= 64 ? 2 : 4;
-  p.rwa = both ? -1 : a.dtype != F32 && ma <= 16 ? 0 : rw;
-  p.rwb = a.dtype != F32 && mb <= 16 ? 0 : rw;
+  p.rwa = both ? -1 : ma <= 16 ? 0 : rw;
+  p.rwb = mb <= 16 ? 0 : rw;
   const int kc = rw == 4 && a.dtype == F32 ? 32 : 64;
   p.rows_a = both ? 0 : p.rwa ? 32 * rw : (int)ma;
   p.rows_b = p.rwb ? 32 * rw : p.rwa ? (int)mb : (int)ma;  // (one list: one kind of slot)
   const int64_t ta = both ? 0 : (ma + p.rows_a - 1) / p.rows_a,
                 tb = (mb + p.rows_b - 1) / p.rows_b;
-  const int ka = p.rwa ? kc : WK, kb = p.rwb ? kc : WK;
+  const int wk = a.dtype == F32 ? WK<float> : WK<bf16>;
+  const int ka = p.rwa ? kc : wk, kb = p.rwb ? kc : wk;
   const int64_t pk = ((int64_t)a.max_prefix + ka - 1) / ka,
                 ca = a.G * ta * a.Hkv * (pk + OVER),
                 cb = a.B * tb * a.Hkv *
@@ -1433,7 +1500,7 @@ Plan plan_of(const BranchArgs& a) {
   if (ca + cb >= INT_MAX || (a.G * ta + a.B * tb) * a.Hkv >= INT_MAX / 2) return p;
   p.tiles_a = (int)ta;
   p.tiles_b = (int)tb;
-  const int per_cu = a.dtype != F32 || a.D == 64 ? 2 : 1;  // Variant::PER_CU
+  const int per_cu = a.dtype != F32 || a.D == 64 || p.rwa == 0 ? 2 : 1;  // Variant::PER_CU
   // (no more workgroups than chunks, each list having one at least)
   const int64_t wgs = (p.rwa ? ca : (ca + 3) / 4) + (p.rwb ? cb : (cb + 3) / 4);
   p.grid = (int)std::min<int64_t>(per_cu * std::min(device_cu_count(), 512), wgs);
@@ -1512,20 +1579,14 @@ int launch_stream(const BranchArgs& a, const Ws& w, const Plan& p) {
 template <typename T, int D>
 int stream_and_merge(const BranchArgs& a, const Ws& w, const Plan& p) {
   int rc;
-  if constexpr (std::is_same<T, float>::value) {
-    rc = p.rwa < 0    ? launch_stream<T, D, -1, 4>(a, w, p)
-         : p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p)
-                      : launch_stream<T, D, 4, 4>(a, w, p);
-  } else {
-    if (p.rwa < 0)
-      rc = launch_stream<T, D, -1, 4>(a, w, p);
-    else if (p.rwa == 0)
-      rc = launch_stream<T, D, 0, 0>(a, w, p);
-    else if (p.rwb == 0)
-      rc = p.rwa == 2 ? launch_stream<T, D, 2, 0>(a, w, p) : launch_stream<T, D, 4, 0>(a, w, p);
-    else
-      rc = p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p) : launch_stream<T, D, 4, 4>(a, w, p);
-  }
+  if (p.rwa < 0)
+    rc = launch_stream<T, D, -1, 4>(a, w, p);
+  else if (p.rwa == 0)
+    rc = launch_stream<T, D, 0, 0>(a, w, p);
+  else if (p.rwb == 0)
+    rc = p.rwa == 2 ? launch_stream<T, D, 2, 0>(a, w, p) : launch_stream<T, D, 4, 0>(a, w, p);
+  else
+    rc = p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p) : launch_stream<T, D, 4, 4>(a, w, p);
   if (rc) return rc;
   const int64_t items = p.rwa < 0 ? (int64_t)a.B * a.Hkv * p.tiles_b : (int64_t)a.G * a.Hkv * p.tiles_a;
   const int64_t workers = p.rwa ? p.grid : 4 * p.grid;
