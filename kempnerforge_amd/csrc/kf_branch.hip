@@ -1416,7 +1416,7 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f + (w != 0.f ? w * po[e] : 0.f);
   };
-  constexpr int U = 8;
+  constexpr int U = JG == 1 ? 4 : 8;  // (few partials a row: no loads of the same again)
   for (int j0 = jg; live && j0 < ns; j0 += U * JG) {
     f32x4 po[U];
     float2 ml[U];
