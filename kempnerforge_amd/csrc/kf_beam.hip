@@ -107,8 +107,8 @@ __device__ __forceinline__ void top_order(int K, int n, Out out, const TopLds<V>
   }
 }
 
-// The same, one at a time: each(f) gives f(value, index) for the thread's values; there are
-// K of them.
+// The same, one at a time: each(f) gives f(value, index) for the thread's values (f says
+// whether to go on, here always); there are K of them.
 template <typename V, typename Each, typename Out>
 __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds<V>& lds) {
   const int t = threadIdx.x;
@@ -117,8 +117,9 @@ __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds
   for (int place = 0; place < K; ++place) {
     // the largest value behind (last, after), then the lowest index that has it
     V x = -INFINITY;
-    each([&](V v, int i) {
+    each([&](V v, int i) __attribute__((always_inline)) {
       if (v < last || (v == last && i > after)) x = fmax(x, v);
+      return true;
     });
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) x = fmax(x, __shfl_xor(x, o, 64));
@@ -128,8 +129,9 @@ __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) x = fmax(x, lds.red[w]);
-    each([&](V v, int i) {
+    each([&](V v, int i) __attribute__((always_inline)) {
       if (v == x && (v < last || i > after)) atomicMin(&lds.best, i);
+      return true;
     });
     __syncthreads();
     if (t == 0) out(place, x, lds.best);
@@ -148,8 +150,9 @@ struct Candidate {
   int v;  // -1: none
 };
 
-// Slices of a row of V values, U granules of E a thread.
-int slices_of(int V, int E, int U) { return ((V + E - 1) / E + NT * U - 1) / (NT * U); }
+constexpr int U = 8;  // granules of a thread
+// Slices of a row of V values, in granules of E.
+int slices_of(int V, int E) { return ((V + E - 1) / E + NT * U - 1) / (NT * U); }
 
 // A granule of -inf, and one without its first k values.
 template <typename T>
@@ -182,7 +185,7 @@ constexpr int GRANULES = 256;
 // counted from the row's first value, whatever its alignment (the loads may be unaligned):
 // rows of equal values have equal sums, to the last bit, and their beams' candidates are
 // equals.
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
                                                             SliceSum* __restrict__ sums,
                                                             Candidate* __restrict__ best) {
@@ -321,7 +324,10 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 }
 
 // ------------------------------------------------------------------ pick
-// The candidates are asked for before anything is waited for: each round trip to what
+// A slice's candidates are a list in order.  `parts` threads take the list's places in turn
+// (more than 256 lists: a thread takes several), and leave it at the first that is below the
+// bound, so of slices x K candidates a beam little more than K in all are looked at.  What a
+// thread begins with is asked for before anything is waited for: each round trip to what
 // other compute units wrote costs as much as the rest.
 __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
                                                          const SliceSum* __restrict__ sums,
@@ -331,19 +337,19 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
   __shared__ double score[KF_BEAM_MAX], lse[KF_BEAM_MAX];
   const int g = blockIdx.x, t = threadIdx.x, W = a.W;
   constexpr double L = 1.4426950408889634074;
-  constexpr int R = 4;  // candidates of a thread in registers
-  const int per = slices * a.K, n = W * per;
-  const Candidate* c = best + (int64_t)g * n;
-  Candidate mine[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) mine[r] = c[min(t + r * NT, n - 1)];
+  const int lists = W * slices, parts = max(NT / lists, 1);
+  const Candidate* c = best + (int64_t)g * lists * a.K;
+  // the thread's first list, and its first two places of it
+  const int l0 = t % lists, r0 = t / lists;
+  const Candidate *begin = c + (int64_t)l0 * a.K;
+  const Candidate one = begin[min(r0, a.K - 1)], two = begin[min(r0 + parts, a.K - 1)];
   // a row per group of lanes, all rows at once
   const int lanes = W <= 4 ? 64 : W <= 8 ? 32 : W <= 16 ? 16 : W <= 32 ? 8 : 4;
   {
     const int w = min(t / lanes, W - 1), x = t % lanes;
     const SliceSum* row = sums + ((int64_t)g * W + w) * slices;
     const float sc = a.scores[(int64_t)g * W + w];
-    SliceSum y = row[min(x, slices - 1)];
+    const SliceSum y = row[min(x, slices - 1)];
     const bool live = fabsf(sc) < INFINITY;  // (else what the slices hold was not written)
     double s = 0.0;
     float M = -INFINITY;
@@ -352,11 +358,16 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
       for (int i = x + lanes; i < slices; i += lanes) M = fmaxf(M, row[i].m);
     }
     for (int o = lanes / 2; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    if (live)
-      for (int i = x; i < slices; i += lanes) {
-        if (i != x) y = row[i];
-        s += y.m == M ? y.s : y.s * exp2_64(((double)y.m - (double)M) * L);
+    if (live) {
+      float m = y.m;
+      double e = y.s;
+      for (int i = x; i < slices;) {
+        s += m == M ? e : e * exp2_64(((double)m - (double)M) * L);
+        i += lanes;
+        m = row[min(i, slices - 1)].m;
+        e = row[min(i, slices - 1)].s;
       }
+    }
     for (int o = lanes / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     const bool ok = live && s > 0.0 && s < INFINITY;
     if (x == 0 && t / lanes < W) {
@@ -365,27 +376,44 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
     }
   }
   __syncthreads();
-  auto each = [&](auto f) {
-    auto one = [&](int i, const Candidate& x) {
-      const int w = (int)((unsigned)i / (unsigned)per);
-      const double sc = score[w];
-      if (sc != -INFINITY && x.v >= 0) f(sc + ((double)x.x - lse[w]), w * a.V + x.v);
-    };
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (t + r * NT < n) one(t + r * NT, mine[r]);
-    for (int i = t + R * NT; i < n; i += NT) one(i, c[i]);
+  // f(value, index) for the thread's candidates, list by list, in order; f says whether to
+  // go on in the list.
+  auto walk = [&](auto f) __attribute__((always_inline)) {
+    // (in registers: a choice between the two as they are is made a choice of addresses)
+    float x1 = one.x, x2 = two.x;
+    int v1 = one.v, v2 = two.v;
+    asm("" : "+v"(x1), "+v"(v1), "+v"(x2), "+v"(v2));
+    if (r0 >= parts) return;  // (threads that are too few for another place of every list)
+    for (int l = l0; l < lists; l += NT) {
+      const int w = l / slices;
+      const double sc = score[w], ls = lse[w];
+      if (sc == -INFINITY) continue;  // (what its slices hold was not written)
+      for (int r = r0; r < a.K; r += parts) {
+        const bool again = r != r0;
+        float y = again ? x2 : x1;
+        int v = again ? v2 : v1;
+        if (l != l0 || r > r0 + parts) {
+          const Candidate z = c[(int64_t)l * a.K + r];
+          y = z.x, v = z.v;
+        }
+        if (v < 0 || !f(sc + ((double)y - ls), w * a.V + v)) break;
+      }
+    }
   };
   double own = -INFINITY;
-  each([&](double x, int) { own = fmax(own, x); });
+  walk([&](double x, int) {
+    own = fmax(own, x);
+    return false;
+  });
   lds.top[t] = own;
   if (t == 0) lds.count = 0;
   __syncthreads();
   const double edge = top_bound(a.K, lds);  // (each wavefront by itself: no other barrier)
-  if (own >= edge)
-    each([&](double x, int i) {
-      if (x >= edge) lds.add(x, i);
-    });
+  walk([&](double x, int i) {
+    if (x < edge) return false;
+    lds.add(x, i);
+    return true;
+  });
   __syncthreads();
   const int64_t at = (int64_t)g * a.K;
   auto put = [&](int place, double x, int i) {
@@ -398,7 +426,7 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
   if (m <= CAP) {
     top_order(a.K, m, put, lds);
   } else {
-    top_one_by_one(a.K, each, put, lds);
+    top_one_by_one(a.K, walk, put, lds);
     m = a.K;
   }
   for (int i = m + t; i < a.K; i += NT) {
@@ -479,21 +507,16 @@ __global__ __launch_bounds__(256) void cache_reorder_kernel(
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Granules a thread of the rows kernel: few where many would leave compute units without a
-// workgroup.
-int unit_of(const SelectArgs& a) {
-  return (int64_t)a.G * a.W * slices_of(a.V, a.dtype == F32 ? 4 : 8, 8) >= 512 ? 8 : 4;
-}
-int slices_of(const SelectArgs& a) { return slices_of(a.V, a.dtype == F32 ? 4 : 8, unit_of(a)); }
+int slices_of(const SelectArgs& a) { return slices_of(a.V, a.dtype == F32 ? 4 : 8); }
 
 template <typename T>
 int select_typed(const SelectArgs& a, void* workspace) {
-  const int unit = unit_of(a), slices = slices_of(a);
+  const int slices = slices_of(a);
   SliceSum* sums = (SliceSum*)workspace;
   Candidate* best =
       (Candidate*)((char*)workspace + up256((size_t)a.G * a.W * slices * sizeof(SliceSum)));
-  KF_LAUNCH("select_rows", (unit == 8 ? select_rows_kernel<T, 8> : select_rows_kernel<T, 4>),
-            dim3(a.G * a.W, slices), dim3(NT), 0, a.stream, a, sums, best);
+  KF_LAUNCH("select_rows", select_rows_kernel<T>, dim3(a.G * a.W, slices), dim3(NT), 0, a.stream,
+            a, sums, best);
   KF_CHECK_LAUNCH();
   KF_LAUNCH("select_pick", select_pick_kernel, dim3(a.G), dim3(NT), 0, a.stream, a, sums, best,
             slices);
@@ -504,11 +527,13 @@ int select_typed(const SelectArgs& a, void* workspace) {
 template <typename U>
 int reorder_launch(const ReorderPtrs& p, int n, const int32_t* lens, const int32_t* parents, int W,
                    int B, int Hkv, int Smax, int row_units, hipStream_t stream) {
-  // Rows are spread over workgroups until there are some 16 per compute unit; the
-  // lengths are on the device, so those behind the last row find nothing to do.
+  // Rows are spread over 8192 workgroups and more, 32 a compute unit (32 layers of 8 x 4
+  // beams of 2048 rows: 2.84 ms with 4096, 2.48, 2.41 with 65536).  The lengths are on the
+  // device, so those behind the last row find nothing to do, which more of them would take
+  // long over where a long cache holds few rows.
   const int64_t items = (int64_t)(B / W) * Hkv * 2 * n;
   const int64_t all = ((int64_t)Smax * row_units + 255) / 256;
-  const int64_t split = std::max<int64_t>(1, std::min<int64_t>({all, 4096 / items + 1, 65535}));
+  const int64_t split = std::max<int64_t>(1, std::min<int64_t>({all, 8192 / items + 1, 65535}));
   const dim3 grid((unsigned)(B / W * Hkv), 2 * n, (unsigned)split);
   auto kernel = W <= 4 ? cache_reorder_kernel<U, 4> : cache_reorder_kernel<U, 8>;
   if (W > 8) kernel = cache_reorder_kernel<U, 16>;

@@ -86,6 +86,18 @@ def test_against_64_bits(dtype, G, W, V, K):
     check(x, s, K, call(x, s, K))
 
 
+@pytest.mark.parametrize("dtype,G,W,V,K", [
+    (F32, 1, 64, 40003, 64), (F32, 2, 33, 40003, 128), (BF, 1, 64, 40003, 3), (FH, 1, 3, 131072, 128),
+    (F32, 1, 5, 131072, 40),
+])
+def test_more_slices_than_threads_and_fewer(dtype, G, W, V, K):
+    """A group's slices against the 256 threads that look through their candidates: several
+    a thread, several threads a slice, a number that does not divide them."""
+    announce(f"select slices {dtype} {G} {W} {V} {K}")
+    x, s = inputs(dtype, G, W, V, seed=V + K)
+    check(x, s, K, call(x, s, K))
+
+
 @pytest.mark.parametrize("dtype,fill", [(BF, 0.0), (F32, -3.5), (FH, 2.0)])
 @pytest.mark.parametrize("K", [4, 64])
 def test_equal_values(dtype, fill, K):
