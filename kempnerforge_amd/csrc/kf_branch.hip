@@ -1355,10 +1355,11 @@ __global__ __launch_bounds__(256, (Variant<T, D, RWA, RWB>::PER_CU)) void branch
   }
 }
 
-// The rows of pair (sequence, KV head) blockIdx.x, 16 bytes of a row per thread and
-// blockIdx.y's share of them: the partials of the prefix's and the own rows' workers,
-// rescaled to a common maximum and summed.  JG groups of threads take a row's partials in
-// turn, U at a time, and are joined through LDS.
+// The rows of a pair (sequence, KV head), 16 bytes of a row per thread and RPW rows a
+// workgroup (pairs first: one dimension, as both may be many): the partials of the prefix's
+// and the own rows' workers, rescaled to a common maximum and summed.  JG groups of threads
+// take a row's partials in turn, U at a time, and are joined through LDS.  Bound by the round
+// trips to what other compute units wrote: 4 us of some 5 for a few rows.
 template <typename T, int D, int JG>
 __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists ls) {
   constexpr int LPR = D / 4, RPW = 256 / (LPR * JG);  // lanes of a row, rows of a workgroup
@@ -1366,8 +1367,9 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
   __shared__ float2 xm[JG > 1 ? 256 : 1];
   __shared__ int before;
   const int n_rep = a.Hq / a.Hkv, W = a.B / a.G;
-  const int b = blockIdx.x / a.Hkv, g = blockIdx.x % a.Hkv, grp = b / W;
-  const int r = blockIdx.y * RPW + threadIdx.x / (LPR * JG), jg = threadIdx.x / LPR % JG;
+  const int pairs = a.B * a.Hkv, pair = blockIdx.x % pairs;
+  const int b = pair / a.Hkv, g = pair % a.Hkv, grp = b / W;
+  const int r = blockIdx.x / pairs * RPW + threadIdx.x / (LPR * JG), jg = threadIdx.x / LPR % JG;
   const int col = threadIdx.x % LPR * 4, i = r / n_rep;
   const bool inside = i < a.N;
   int first = (b % W) * a.N;  // the sequence's first token in its group's rows
@@ -1469,8 +1471,22 @@ __global__ __launch_bounds__(256) void branch_merge_kernel(BranchArgs a, Lists l
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // The stream kernel's shape for a call: row waves of the prefixes' tiles and of the own
-// rows' (0: one wavefront a share), or (none) one wavefront a row.
-constexpr int BOTH_ROWS = 96;
+// rows' (0: one wavefront a share), or (none) one wavefront a row.  All times in us, 32 / 8
+// heads of 128 in bfloat16 if nothing else is said:
+//  - Up to 16 rows of a pair: a wavefront a share.  Its list has four times as many shares,
+//    so a wavefront has little to read before the merge: 4 beams behind 1000 keys 13.8, in
+//    tiles 15.2; 8 x 4 behind 4096 in float32 72, 114 (a tile of 64 rows is mostly padding,
+//    and float32's products are slow).  4 x 4 behind 8192 in bfloat16 44, 40.  Beyond 16 rows
+//    a second block of rows a wavefront needs its registers: 16 beams 21, tiles 17.5.
+//  - Tiles of 64 rows up to 64 rows, of 128 beyond: 4 x 12 behind 8192 in float32 138, 203;
+//    in bfloat16, bound by the keys' bytes, they are level (12 behind 4096: 22).  Beyond 64
+//    rows 128 read the keys half as often: 4 x 16 of 64 / 8 heads behind 8192 75, 78.
+//  - Sequences with over 16 rows of their own: one list of their tiles over prefix and cache
+//    (fewer partials to join, none where a tile is one workgroup's), or a list of the group's
+//    tiles over the prefix (whole tiles) beside one of theirs over their own keys.  8 x 16
+//    tokens behind 512 keys and 512 of their own: 28, 34; behind 4096: 48, 40.  4 x 4 x 24
+//    behind 1024 in float32: 108, 88.  So the first where it is no more than a fifth more
+//    chunks of 128 rows.
 struct Plan {
   bool none;
   int rwa, rwb, rows_a, rows_b, tiles_a, tiles_b, grid, workers_a, workers_b;
@@ -1481,23 +1497,26 @@ Plan plan_of(const BranchArgs& a) {
   const int n_rep = a.Hq / a.Hkv, W = a.B / a.G;
   if (a.D != 64 && a.D != 128) return p;
   const int64_t ma = (int64_t)W * a.N * n_rep, mb = (int64_t)a.N * n_rep;
-  // One list where the sequences' rows fill tiles of their own: BOTH_ROWS of 128 or more.
-  const bool both = mb >= BOTH_ROWS;
   const int rw = ma <= 64 ? 2 : 4;
+  const int kc = rw == 4 && a.dtype == F32 ? 32 : 64;
+  auto tiles = [&](int64_t m, int rows) { return (m + rows - 1) / rows; };
+  auto chunks = [&](int n, int keys) { return ((int64_t)n + keys - 1) / keys; };
+  const int64_t pt = chunks(a.max_prefix, kc), ot = chunks(a.max_len, kc);
+  const int64_t na = a.G * tiles(ma, 128), nb = a.B * tiles(mb, 128);
+  const bool both = rw == 4 && mb > 16 &&
+                    nb * (pt + ot + OVER) * 5 <= (na * (pt + OVER) + nb * (ot + OVER)) * 6;
   p.rwa = both ? -1 : ma <= 16 ? 0 : rw;
   p.rwb = mb <= 16 ? 0 : rw;
-  const int kc = rw == 4 && a.dtype == F32 ? 32 : 64;
   p.rows_a = both ? 0 : p.rwa ? 32 * rw : (int)ma;
   p.rows_b = p.rwb ? 32 * rw : p.rwa ? (int)mb : (int)ma;  // (one list: one kind of slot)
-  const int64_t ta = both ? 0 : (ma + p.rows_a - 1) / p.rows_a,
-                tb = (mb + p.rows_b - 1) / p.rows_b;
+  const int64_t ta = both ? 0 : tiles(ma, p.rows_a), tb = tiles(mb, p.rows_b);
   const int wk = a.dtype == F32 ? WK<float> : WK<bf16>;
   const int ka = p.rwa ? kc : wk, kb = p.rwb ? kc : wk;
-  const int64_t pk = ((int64_t)a.max_prefix + ka - 1) / ka,
-                ca = a.G * ta * a.Hkv * (pk + OVER),
+  const int64_t pk = chunks(a.max_prefix, ka), ca = a.G * ta * a.Hkv * (pk + OVER),
                 cb = a.B * tb * a.Hkv *
-                     (((int64_t)a.max_len + kb - 1) / kb + (both ? pk : 0) + (p.rwb ? OVER : 1));
-  if (ca + cb >= INT_MAX || (a.G * ta + a.B * tb) * a.Hkv >= INT_MAX / 2) return p;
+                     (chunks(a.max_len, kb) + (both ? pk : 0) + (p.rwb ? OVER : 1));
+  // (the merge launches 256 threads a pair and more: fewer than 2^32)
+  if (ca + cb >= INT_MAX || (a.G * ta + a.B * tb) * a.Hkv >= 1 << 24) return p;
   p.tiles_a = (int)ta;
   p.tiles_b = (int)tb;
   const int per_cu = a.dtype != F32 || a.D == 64 || p.rwa == 0 ? 2 : 1;  // Variant::PER_CU
@@ -1588,16 +1607,19 @@ int stream_and_merge(const BranchArgs& a, const Ws& w, const Plan& p) {
   else
     rc = p.rwa == 2 ? launch_stream<T, D, 2, 2>(a, w, p) : launch_stream<T, D, 4, 4>(a, w, p);
   if (rc) return rc;
-  const int64_t items = p.rwa < 0 ? (int64_t)a.B * a.Hkv * p.tiles_b : (int64_t)a.G * a.Hkv * p.tiles_a;
+  // The more partials a row has, the more threads take them.  Calls by 1, 2 and 8, in us: 64
+  // shares an item 18.6, 15.7, 13.8 (4 beams behind 1000 keys); 32 28.4, 26.5, 26.6 (8 x 4
+  // behind 1000); 16 64.0, 65.6, 75.0 (4 x 16 behind 8192); 1 145, 161, 227 (questions).
+  const int64_t items = (p.rwa < 0 ? (int64_t)a.B * p.tiles_b : (int64_t)a.G * p.tiles_a) * a.Hkv;
   const int64_t workers = p.rwa ? p.grid : 4 * p.grid;
-  const int jg = workers > 32 * items ? 8 : workers > 8 * items ? 2 : 1;
+  const int jg = workers > 32 * items ? 8 : workers > 16 * items ? 2 : 1;
   const int rpw = 256 / (D / 4) / jg;  // rows of a workgroup
   KF_LAUNCH("branch_merge",
             (jg == 8   ? branch_merge_kernel<T, D, 8>
              : jg == 2 ? branch_merge_kernel<T, D, 2>
                        : branch_merge_kernel<T, D, 1>),
-            dim3(a.B * a.Hkv, (a.N * (a.Hq / a.Hkv) + rpw - 1) / rpw), dim3(256), 0, a.stream, a,
-            w.ls);
+            dim3(a.B * a.Hkv * ((a.N * (a.Hq / a.Hkv) + rpw - 1) / rpw)), dim3(256), 0, a.stream,
+            a, w.ls);
   KF_CHECK_LAUNCH();
   return KF_OK;
 }

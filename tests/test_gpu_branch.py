@@ -120,6 +120,28 @@ def test_long_prefixes(dtype, shape, plens, hi):
     check(dtype, shape, plens, spread(n, hi // 8, hi), None, f"branch long {dtype} {shape}")
 
 
+@pytest.mark.parametrize("dtype,shape,plens,lens,counts", [
+    (BF, (1, 4, 17, 8, 2, 128), [40], [64, 3, 0, 90], None),       # 68 rows of 128, short prefix
+    (BF, (1, 4, 17, 8, 2, 128), [1500], [0, 3, 0, 9], [17, 4, 0, 1]),  # and a long one
+    (BF, (1, 1, 20, 8, 2, 128), [1200], [130], None),              # one sequence, 80 rows
+    (FH, (3, 1, 9, 16, 2, 64), [65, 0, 700], [0, 200, 1], [9, 5, 9]),
+    (BF, (2, 6, 12, 8, 2, 128), [130, 64], spread(12, 0, 70), None),   # 48 rows of 128
+    (F32, (2, 2, 12, 16, 2, 128), [33, 130], [31, 0, 64, 5], [12, 12, 0, 7]),
+    (F32, (1, 3, 24, 8, 2, 64), [900], [0, 4, 31], None),
+])
+def test_tiles_of_prefix_and_own_rows(dtype, shape, plens, lens, counts):
+    """Sequences of 17 rows and more a pair: their own tiles over prefix and cache, or the
+    group's over the prefix and theirs over the cache, as the lengths have it."""
+    check(dtype, shape, plens, lens, counts, f"branch tiles {dtype} {shape} {plens}")
+
+
+def test_many_unused_tokens():
+    """More rows of a pair than a launch's second dimension has places."""
+    announce("branch many tokens")
+    N, plens, lens, counts = 140000, [40], [5], [3]
+    check(BF, (1, 1, N, 8, 1, 64), plens, lens, counts, "branch many tokens")
+
+
 def test_a_branch_is_a_decode_step():
     """One sequence behind its own prompt is kf_attn_decode over a cache that holds both:
     the same value rows, keys that differ by the roundings of the eager rotation (each
