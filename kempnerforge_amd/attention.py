@@ -231,6 +231,10 @@ def reorder_branches(caches, parents: torch.Tensor) -> None:
     rows of all layers' caches (:class:`BranchKVCache`, one per layer) follow, in one
     launch.  The fill levels are the same for all layers."""
     first = caches[0]
+    want = (first.lens.shape[0] // first.branches, first.branches)
+    if tuple(parents.shape) != want:
+        raise ValueError(f"parents must be {list(want)}: a branch continues one of its own prompt "
+                         f"(got {list(parents.shape)})")
     ops.cache_reorder_raw([c.k for c in caches], [c.v for c in caches], first.lens, parents)
     if first.ragged:  # (otherwise all levels are one)
         W = parents.shape[1]

@@ -113,6 +113,16 @@ def test_reorder_moves_the_levels_of_a_ragged_cache(monkeypatch):
     assert all(c.lens.tolist() == [2, 2, 3, 4] for c in caches)
 
 
+@pytest.mark.parametrize("shape", [(1, 4), (4, 1), (2, 1), (4,), (2, 3)])
+def test_reorder_keeps_to_a_prompts_own_branches(monkeypatch, shape):
+    calls = []
+    monkeypatch.setattr(ops, "cache_reorder_raw", lambda *a: calls.append(a))
+    caches = [_prefix().branch(2, 9)]
+    with pytest.raises(ValueError, match="parents must be"):
+        reorder_branches(caches, torch.zeros(shape, dtype=torch.int32))
+    assert not calls
+
+
 # ------------------------------------------------------------------ generation
 @pytest.fixture
 def oracle(monkeypatch):
