@@ -9,8 +9,9 @@
 //            exponentials, and its K largest logits
 //  2. pick   a workgroup per group: the rows' sums joined, then the K largest of the
 //            W x slices x K candidates, in 64 bits
-// Every logit is read once.  HBM bounds the first (32 x 8 rows of 131072), two dependent
-// launches the smallest calls.
+// Every logit is read once.  HBM bounds the first (bfloat16 rows of 131072: 32 x 8 take
+// 16 to 18 us, 4 TB/s, 128 x 8 58, 4.6), two dependent launches the smallest calls (4 rows
+// of 32000: 5.5 and 5 us).
 #include "kf_common.h"
 #include "kf_internal.h"
 #include "kf_mfma.h"
@@ -30,7 +31,8 @@ namespace {
 // The workgroup's values fall into 64 groups (lane l of the four wavefronts); the K-th
 // largest of the groups' maxima is at most the K-th largest value, and few values are
 // above it (64 ln(64 / (64 - K)) of independent ones), so those are gathered and ordered
-// by counting.  From 48 on the 256 threads are the groups.  More than CAP of them (values
+// by counting.  Many of the 64 picked leave many above (all, at 64), which are ordered in
+// their number's square: then the 256 threads are the groups.  More than CAP of them (values
 // that are ordered against the groups, or mostly equal) are taken one at a time.
 constexpr int NT = 256, CAP = 1024;
 
@@ -68,7 +70,9 @@ __device__ __forceinline__ V top_bound(int K, const TopLds<V>& lds) {
   V g[NT / 64], edge = INFINITY;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) g[i] = lds.top[lane + 64 * i];
-  if (K <= 48) {
+  // (The launches of 16 x 16 rows of 131072 in us, by 64 and by 256: rows at 32 21, 38, at 48
+  // 25, 34, at 56 32, 35, at 63 2200, 42; pick at 32 9.5, 14, at 40 11, 15, at 48 23.6, 17.)
+  if (K <= (sizeof(V) == 4 ? 48 : 40)) {
 #pragma unroll
     for (int i = 1; i < NT / 64; ++i) g[0] = fmax(g[0], g[i]);
     int above = 0;
@@ -77,11 +81,14 @@ __device__ __forceinline__ V top_bound(int K, const TopLds<V>& lds) {
     if (above < K) edge = g[0];
   } else {
     int above[NT / 64] = {};
-    for (int j = 0; j < NT; ++j) {
-      const V x = lds.top[j];
 #pragma unroll
-      for (int i = 0; i < NT / 64; ++i) above[i] += x > g[i];
-    }
+    for (int i = 0; i < NT / 64; ++i)
+#pragma unroll
+      for (int j = 0; j < 64; ++j) {
+        const V x = lane_of(g[i], j);
+#pragma unroll
+        for (int k = 0; k < NT / 64; ++k) above[k] += x > g[k];
+      }
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i)
       if (above[i] < K) edge = fmin(edge, g[i]);
@@ -326,7 +333,8 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 // ------------------------------------------------------------------ pick
 // A slice's candidates are a list in order.  `parts` threads take the list's places in turn
 // (more than 256 lists: a thread takes several), and leave it at the first that is below the
-// bound, so of slices x K candidates a beam little more than K in all are looked at.  What a
+// bound, so of slices x K candidates a beam little more than K in all are looked at (8 x 8
+// slices of 16: 8.5 us with the call's launch, 14 when all were).  What a
 // thread begins with is asked for before anything is waited for: each round trip to what
 // other compute units wrote costs as much as the rest.
 __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
@@ -408,13 +416,37 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
   lds.top[t] = own;
   if (t == 0) lds.count = 0;
   __syncthreads();
-  const double edge = top_bound(a.K, lds);  // (each wavefront by itself: no other barrier)
-  walk([&](double x, int i) {
+  double edge = top_bound(a.K, lds);  // (each wavefront by itself: no other barrier)
+  auto gather = [&](double x, int i) {
     if (x < edge) return false;
     lds.add(x, i);
     return true;
-  });
+  };
+  walk(gather);
   __syncthreads();
+  // Where fewer lists than K hold the K largest (few beams' scores are far above the others'),
+  // the lists' beginnings bound little, and up to K candidates of each of those lists pass:
+  // too many from K = 33 on.  Then all candidates are dealt out, 256 at a time, each deal
+  // turned against the last, so that no thread has two of the first places of a few lists.
+  if (lds.count > CAP) {
+    own = -INFINITY;
+#pragma unroll 1
+    for (int r = 0; r * NT < lists * a.K; ++r) {
+      const int i = r * NT + ((t + 79 * r) & (NT - 1));
+      if (i >= lists * a.K) continue;
+      const int w = i / a.K / slices;
+      if (score[w] == -INFINITY) continue;
+      const Candidate x = c[i];
+      if (x.v >= 0) own = fmax(own, score[w] + ((double)x.x - lse[w]));
+    }
+    __syncthreads();
+    lds.top[t] = own;
+    if (t == 0) lds.count = 0;
+    __syncthreads();
+    edge = fmax(edge, top_bound(a.K, lds));
+    walk(gather);
+    __syncthreads();
+  }
   const int64_t at = (int64_t)g * a.K;
   auto put = [&](int place, double x, int i) {
     const int w = (int)((unsigned)i / (unsigned)a.V);

@@ -8,7 +8,16 @@
 // cache.  Softmax statistics and sums are joined over the prefix and the own rows.
 //
 // Rounding: the norm and the rotation of q and k are formed in 32 bits, k is rounded
-// once, where it is stored.
+// once, where it is stored; the products take q and P as two numbers of the type each
+// (hi + lo), so that what is left is the rounding of the output.
+//
+// A prefix's keys are met once by the rows of all its sequences, each sequence's own keys
+// by its rows; both lists of key chunks are shared out over one launch, and a second joins
+// the partials.  Measured, in us (the stream's launch + the merge's), 128 a head:
+//   4 sequences behind 1000 keys, 32 / 8 heads          9 + 5: latency
+//   4 x 16 behind 8192, up to 512 own, 64 / 8 heads    52 + 8: 3.4 TB/s
+//   128 behind 4096, up to 2048 own, 32 / 8 heads     125 + 8: 5.2 TB/s, bound by HBM
+//   8 x up to 200 tokens behind 4096, 32 / 8 heads    122 .. 155 + 17: bound by the products
 #include "kf_common.h"
 #include "kf_internal.h"
 #include "kf_mfma.h"
@@ -177,7 +186,9 @@ struct Lists {
 //       16, keys 4 (l / 16) .. of each 16); V through the wavefront's LDS and back
 //       transposed, or (float32) loaded as the operand is: dim l % 16 of each 16 of keys
 //       4 (l / 16) ..
-// The next chunk's rows are loaded while one is computed.
+// The next chunk's rows are loaded while one is computed.  Bound by the first round trips
+// where shares are few chunks (4 sequences behind 1000 keys: one chunk each), by HBM where
+// they are long: 32 sequences of 8192 own keys stream at 6.0 TB/s.
 template <typename T>
 constexpr int WK = sizeof(T) == 4 ? 16 : 32;  // keys of a chunk
 

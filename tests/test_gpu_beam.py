@@ -98,6 +98,22 @@ def test_more_slices_than_threads_and_fewer(dtype, G, W, V, K):
     check(x, s, K, call(x, s, K))
 
 
+@pytest.mark.parametrize("dtype,W,V,K,ruling", [
+    (BF, 16, 131072, 128, 1), (BF, 16, 131072, 128, 3), (F32, 9, 60001, 128, 2), (FH, 64, 20000, 100, 4),
+    (BF, 16, 131072, 128, 11), (BF, 12, 131072, 41, 2), (F32, 33, 40003, 33, 1),
+])
+def test_few_beams_rule(dtype, W, V, K, ruling):
+    """The scores of some beams are so far above the others' that all are picked of them:
+    many candidates a slice."""
+    announce(f"select ruling {dtype} {W} {V} {K} {ruling}")
+    x, s = inputs(dtype, 2, W, V, seed=V + ruling)
+    s[0, -ruling:] += 60.0
+    s[1, :ruling] += 60.0
+    out = call(x, s, K)
+    assert (out[1][0] >= W - ruling).all() and (out[1][1] < ruling).all()
+    check(x, s, K, out)
+
+
 @pytest.mark.parametrize("dtype,fill", [(BF, 0.0), (F32, -3.5), (FH, 2.0)])
 @pytest.mark.parametrize("K", [4, 64])
 def test_equal_values(dtype, fill, K):
