@@ -420,8 +420,9 @@ int kf_beam_select_workspace_size(int G, int W, int V, int K, int dtype, size_t*
  *       first, equals by the lowest w, then v; rounded to out_scores; parents are the w
  * A score of -inf is a beam that is not in use; one that is not finite otherwise,
  * and a row that is no distribution (NaN, +inf, or -inf throughout), count as
- * such (a largest logit of 2^127 or more counts as +inf).  -inf is a token of no
- * probability: never picked.  Behind the last candidate: score -inf, parent and token -1.  V <= KF_VERIFY_MAX_VOCAB. */
+ * such.  -inf is a token of no probability: never picked; a finite logit can be, the
+ * type's lowest too.  Behind the last candidate: score -inf, parent and token -1.
+ * V <= KF_VERIFY_MAX_VOCAB. */
 int kf_beam_select(const void* logits, int64_t logits_stride_g, int64_t logits_stride_w,
                    const float* scores, float* out_scores, int32_t* parents, int64_t* tokens,
                    void* workspace, size_t workspace_bytes, int G, int W, int V, int K, int dtype,

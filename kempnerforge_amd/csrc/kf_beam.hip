@@ -16,6 +16,7 @@
 #include "kf_internal.h"
 #include "kf_mfma.h"
 #include "kf_row.h"
+#include "kf_stream.h"
 
 #include <algorithm>
 #include <climits>
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 #pragma unroll
     for (int u = 0; u < U; ++u) drop_first<T>(raw[u], v0 + u * NT * E - first(u));
   }
-  float gm[U], m = -INFINITY, ml = 0.f, part = 0.f;
+  float gm[U], m = -INFINITY, ml = 0.f, part = 0.f, slope = kLog2e;
 #pragma unroll
   for (int b = 0; b < U; b += BATCH) {
     const float old = m;
@@ -243,7 +244,10 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
       mfma::settle(raw[u]);  // (kept as they are: unpacked they would take twice the registers)
     }
     const float was = ml;
-    ml = m == -INFINITY ? 0.f : m * kLog2e;
+    // (of values as far out as the lowest one of the type, differences are 2^102 and more,
+    // or none: any slope gives their exponentials, and this one no infinities)
+    slope = fabsf(m) >= 0x1p126f ? 0x1p-20f : kLog2e;
+    ml = m == -INFINITY ? 0.f : m * slope;
     // (moved by the difference of the rounded references, which the terms were taken
     // against)
     if (old != -INFINITY && m > old) part *= fast_exp2(was - ml);
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
       float f[E], x = 0.f;
       Row<T>::unpack(raw[u], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x += fast_exp2(__builtin_fmaf(f[e], kLog2e, -ml));
+      for (int e = 0; e < E; ++e) x += fast_exp2(__builtin_fmaf(f[e], slope, -ml));
       part += x;
       mfma::settle(raw[u]);
     }
@@ -261,7 +265,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
   // One wavefront finds the bound, another the sum: all four would spend on them what they
   // spend on the values.
   lds.top[t] = m;
-  parts[t] = make_float2(part, ml);
+  parts[t] = make_float2(part, m == -INFINITY ? 0.f : __builtin_fmaf(-m, slope, ml));
   if (t == 0) lds.count = hots = 0;
   __syncthreads();
   const int64_t at = (int64_t)blockIdx.x * gridDim.y + blockIdx.y;
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
       if (x == -INFINITY)
         s += p.x != p.x ? p.x : 0.f;
       else
-        s += (double)p.x * exp2_64((x - (double)M) * L + ((double)p.y - x * (double)kLog2e));
+        s += (double)p.x * exp2_64((x - (double)M) * L + (double)p.y);
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -311,21 +315,64 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
   int n = lds.count;
   if (nh <= GRANULES && n <= CAP) {
     top_order(a.K, n, put, lds);
-  } else {
-    top_one_by_one(
-        a.K,
-        [&](auto f) {
+  } else {  // (of E values and more)
+    auto granule = [&](int u, float* f) {
+      u32x4 x;
+      __builtin_memcpy(&x, row + first(u), 16);
+      drop_first<T>(x, v0 + u * NT * E - first(u));
+      Row<T>::unpack(x, f);
+    };
+    auto each = [&](auto g) {
 #pragma unroll 1
-          for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        float f[E];
+        granule(u, f);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (f[e] > -INFINITY) g(f[e], first(u) + e);
+      }
+    };
+    // Mostly equal values (tokens masked by the type's lowest one): the bound is the K-th
+    // largest value itself where fewer than K are above it, and the lowest tokens that have
+    // it follow those.
+    __syncthreads();
+    if (t == 0) lds.count = 0;
+    __syncthreads();
+    each([&](float x, int v) {
+      if (x > edge) lds.add(x, v);
+    });
+    __syncthreads();
+    n = lds.count;
+    if (n < a.K) {
+      top_order(a.K, n, put, lds);
 #pragma unroll 1
-            for (int e = 0; e < E; ++e) {
-              const int v = v0 + u * NT * E + e;
-              const float x = v < a.V ? to_f32(row[v]) : -INFINITY;
-              if (x > -INFINITY) f(x, v);
-            }
-        },
-        put, lds);
-    n = a.K;
+      for (int u = 0; u < U && n < a.K; ++u) {
+        float f[E];
+        granule(u, f);
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += f[e] == edge;
+        const int end = wave_prefix(mine);
+        __syncthreads();
+        if (lane == 63) hot_at[t >> 6] = end;
+        __syncthreads();
+        int place = n + end - mine;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+          place += w < t >> 6 ? hot_at[w] : 0;
+          n += hot_at[w];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (f[e] == edge) {
+            if (place < a.K) put(place, edge, first(u) + e);
+            ++place;
+          }
+      }
+    } else {
+      top_one_by_one(a.K, each, put, lds);
+      n = a.K;
+    }
   }
   for (int i = n + t; i < a.K; i += NT) put(i, -INFINITY, -1);
 }

@@ -128,6 +128,62 @@ def test_equal_values(dtype, fill, K):
     check(x, s, K, (best, parents, tokens))
 
 
+@pytest.mark.parametrize("dtype", [BF, FH, F32])
+@pytest.mark.parametrize("K,allowed", [(8, 3), (16, 0), (128, 60), (48, 47), (5, 5)])
+@pytest.mark.parametrize("lead", [0, 5])
+def test_masked_by_the_lowest_value(dtype, K, allowed, lead):
+    """All tokens but a few hold the type's lowest value (another mask than -inf): they
+    follow those that are left, lowest first; slices of nothing else."""
+    announce(f"select lowest {dtype} {K} {allowed} {lead}")
+    V, G, W = 40003, 2, 2
+    g = torch.Generator().manual_seed(5 + K)
+    x = torch.full((G, W, V), torch.finfo(dtype).min, dtype=dtype)
+    for i in range(G):
+        for w in range(W):
+            at = torch.randperm(V, generator=g)[:allowed]
+            x[i, w, at] = torch.randn(allowed, generator=g).to(dtype)
+    x[1, 0, ::3] = -INF
+    s = torch.tensor([[-0.5, 0.0], [0.0, -0.25]])
+    buf = torch.zeros(G * W * V + lead, dtype=dtype, device=DEV)
+    view = buf[lead:].view(G, W, V)
+    view.copy_(x)
+    best, parents, tokens = (t.cpu() for t in call(view, s, K))
+    want = branch_ref.select(x, s, K)[0]
+    # (the largest are some 3.4e38: the error is relative there)
+    assert torch.isfinite(best).all()
+    assert ((best.double() - want).abs() <= LSE + half_ulp(want, F32)).all()
+    # each beam's tokens: those allowed by value, then masked ones, lowest first
+    for i in range(G):
+        for w in range(W):
+            mine = tokens[i][parents[i] == w]
+            vals = x[i, w].float()[mine]
+            assert (vals[:-1] >= vals[1:]).all() and not torch.isinf(vals).any()
+            low = mine[vals == torch.finfo(dtype).min]
+            order = (x[i, w] == torch.finfo(dtype).min).nonzero()[:, 0]
+            assert torch.equal(low, order[:len(low)])
+            left = int((x[i, w].float() > torch.finfo(dtype).min).sum())
+            assert len(low) == 0 or len(mine) - len(low) == left
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logits_of_any_size(dtype):
+    """Largest logits from 2^100 to the type's largest value, of either sign: all of the
+    probability lies with them."""
+    announce(f"select far out {dtype}")
+    V, top = 20011, torch.finfo(dtype).max
+    for at, far in enumerate((2.0 ** 100, 2.0 ** 126, -(2.0 ** 126), 2.0 ** 127, top, -(2.0 ** 127))):
+        x = torch.full((1, 2, V), -top, dtype=dtype)
+        x[0, 0, 7 + at::911] = far
+        x[0, 1] = torch.randn(V, generator=torch.Generator().manual_seed(at)).to(dtype)
+        n = len(range(7 + at, V, 911))
+        s = torch.tensor([[0.0, -3.0]])
+        best, parents, tokens = (t.cpu() for t in call(x, s, 9))
+        want, wp, wt = branch_ref.select(x, s, 9)
+        assert torch.equal(parents, wp) and torch.equal(tokens, wt), far
+        assert ((best.double() - want).abs() <= LSE + half_ulp(want, F32)).all()
+        assert n > 9 and (parents == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("K,hot", [(16, 10), (48, 40), (100, 40), (3, 2)])
 @pytest.mark.parametrize("lead", [0, 3])
