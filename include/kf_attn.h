@@ -393,10 +393,11 @@ int kf_attn_branch_workspace_size(int G, int B, int N, int Hq, int Hkv, int D, i
  *       on lens[b] + counts[b] (<= Smax)
  *   q_norm_weight, k_norm_weight, norm_eps  as for kf_attn_decode
  * The prefixes may not overlap the caches.  lens is not modified.  Inf and NaN in
- * rows a token does not see do not reach its output.  prefix_lens, lens and counts live on the device, so they cannot be
- * validated before the launch: a sequence with prefix_lens[g] outside 0 ..
- * max_prefix, a count outside 0 .. N, lens[b] + counts[b] beyond max_len, or a
- * table row outside [0, rope_rows) gets NaN outputs and no cache write. */
+ * rows a token does not see do not reach its output.  prefix_lens, lens and counts
+ * live on the device, so they cannot be validated before the launch: a sequence with
+ * prefix_lens[g] outside 0 .. max_prefix, a count outside 0 .. N, lens[b] + counts[b]
+ * beyond max_len, or a table row outside [0, rope_rows) gets NaN outputs and no cache
+ * write. */
 int kf_attn_branch(const void* q_new, const void* k_new, const void* v_new, const void* k_prefix,
                    const void* v_prefix, const int32_t* prefix_lens, void* k_cache, void* v_cache,
                    const int32_t* lens, const int32_t* counts, const float* rope_cos,
