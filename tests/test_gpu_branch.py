@@ -214,9 +214,21 @@ def test_tables_that_start_at_the_new_tokens():
 def test_what_a_token_does_not_see_does_not_reach_it(dtype, N, W, D):
     """Stale rows of the prefix and the caches, unused tokens, later tokens and the other
     sequences hold NaN and Inf."""
-    announce(f"branch masked NaN {dtype} {N} {W} {D}")
+    masked(dtype, N, W, D, 70)
+
+
+@pytest.mark.parametrize("dtype,N,W,D", [(BF, 12, 8, 128), (FH, 12, 8, 64), (F32, 20, 5, 64)])
+@pytest.mark.parametrize("bound", [70, 2000])
+def test_masked_rows_of_both_kinds_of_tiles(dtype, N, W, D, bound):
+    """The same where sequences have tiles of their own: with a short bound on the prefix
+    they walk it themselves, with a long one the group does."""
+    masked(dtype, N, W, D, bound)
+
+
+def masked(dtype, N, W, D, bound):
+    announce(f"branch masked NaN {dtype} {N} {W} {D} {bound}")
     G, Hq, Hkv = 2, 4, 2
-    B, plens, Pmax, Smax = G * W, [45, 64], 100, 40 + N + 30
+    B, plens, Pmax, Smax = G * W, [45, 64], bound + 30, 40 + N + 30
     lens = [(11 * b) % 37 for b in range(B)]
     counts = [N] * B
     counts[-1] = N // 2
@@ -231,11 +243,11 @@ def test_what_a_token_does_not_see_does_not_reach_it(dtype, N, W, D):
     v[0, N - 1, 0, 3] = float("nan")
     k[-1, counts[-1]:], v[-1, counts[-1]:], q[-1, counts[-1]:] = (float("nan"),) * 3
     vc[1, :, 0] = float("inf")
-    out, kcd, vcd = step(*x, plens, lens, 70, 37 + N, counts)
+    out, kcd, vcd = step(*x, plens, lens, bound, 37 + N, counts)
     clean = [t.clone() for t in x]
     for t in clean:
         t[~torch.isfinite(t)] = 1.0
-    o2, k2, v2 = step(*clean, plens, lens, 70, 37 + N, counts)
+    o2, k2, v2 = step(*clean, plens, lens, bound, 37 + N, counts)
     want, mag = reference(*clean, k2, v2, plens, lens, counts)
     got = out.cpu().double()
     for b in range(B):
@@ -258,17 +270,26 @@ def test_what_a_token_does_not_see_does_not_reach_it(dtype, N, W, D):
 def test_refusals_on_the_device(N, W, D):
     """A sequence whose prefix, length, count or tables are out of range gets NaN and no
     cache write; the others are served, those of its group too."""
-    announce(f"branch device refusals {N} {W} {D}")
+    refused(N, W, D, 60)
+
+
+@pytest.mark.parametrize("bound", [60, 2000])
+def test_refusals_in_both_kinds_of_tiles(bound):
+    refused(12, 8, 128, bound)
+
+
+def refused(N, W, D, bound):
+    announce(f"branch device refusals {N} {W} {D} {bound}")
     G, P, L = 4, 50, 20
     B = G * W
-    x = inputs(BF, G, W, N, 4, 2, D, 60, 40)
+    x = inputs(BF, G, W, N, 4, 2, D, bound, 40)
     q, k, v, kp, vp, kc, vc, cos, sin = x
     plens, lens, counts = [P] * G, [L] * B, [N] * B
-    plens[3] = 61                       # beyond max_prefix: the whole group
+    plens[3] = bound + 1                # beyond max_prefix: the whole group
     lens[0], lens[W] = 41 - N, -1       # beyond max_len; negative
     counts[W + 1], counts[2 * W] = N + 1, -1
     bad = {0, W, W + 1, 2 * W, *range(3 * W, 4 * W)}
-    out, kcd, vcd = step(*x, plens, lens, 60, 40, counts)
+    out, kcd, vcd = step(*x, plens, lens, bound, 40, counts)
     good = [b for b in range(B) if b not in bad]
     for b in bad:
         assert torch.isnan(out[b].float()).all(), b
@@ -280,7 +301,7 @@ def test_refusals_on_the_device(N, W, D):
     # tables that end before the last token of the longer sequences
     lens = [L + b % 2 for b in range(B)]
     rows = P + L + N
-    out, kcd, _ = step(*x[:7], cos[:rows], sin[:rows], [P] * G, lens, 60, 40)
+    out, kcd, _ = step(*x[:7], cos[:rows], sin[:rows], [P] * G, lens, bound, 40)
     for b in range(B):
         assert torch.isnan(out[b].float()).all() == (b % 2 == 1), b
         assert b % 2 == 0 or torch.equal(kcd[b].cpu(), kc[b])
