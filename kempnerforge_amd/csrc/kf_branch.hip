@@ -562,7 +562,8 @@ __device__ __forceinline__ void wave_role(const BranchArgs& a, const Lists& ls, 
     float tmax = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) sc[kb] += sl[kb];
-    if (keys < KEYS) {  // (a new token sees those before it and itself)
+    // (a new token sees those before it and itself: 16 of them fill a chunk of float32)
+    if (fresh || keys < KEYS) {
       const int limit = fresh ? token + 1 : keys;
 #pragma unroll
       for (int t = 0; t < 4 * NB; ++t)

@@ -390,3 +390,44 @@ def test_caches_past_32_bit_offsets(N, W):
                                 x[8].to(DEV), rope_row_offset=0, max_prefix=Pw, max_len=Sw)
     want, mag = reference(*x, kc[:, :, :Sw], vc[:, :, :Sw], plens, lens, None)
     check_tree(out, want, mag, BF, D, Pw + Sw, "long caches")
+
+
+SIXTEEN = [
+    # (G, W, N, Hq, Hkv, D), prefix lengths, own lengths, counts: without groups of heads, 16 new
+    # tokens are all the rows that a wavefront takes, and (float32) all the keys of a chunk
+    ((1, 1, 16, 12, 12, 64), [40], [0], None),
+    ((1, 1, 16, 4, 4, 128), [0], [21], None),
+    ((2, 1, 16, 2, 2, 64), [7, 33], [16, 5], [16, 16]),
+    ((1, 3, 16, 4, 4, 64), [50], [17, 0, 3], None),             # beside tiles over the prefix
+    ((2, 2, 16, 4, 4, 128), [31, 64], [0, 9, 16, 40], [16, 3, 16, 0]),
+    ((1, 6, 16, 16, 16, 64), [100], spread(6, 0, 40), [16] * 6),  # 96 rows of one prefix
+    ((1, 5, 16, 2, 2, 128), [90], spread(5, 0, 70), [16, 15, 16, 1, 16]),
+    ((70, 1, 16, 1, 1, 64), [i % 9 for i in range(70)], spread(70, 0, 40), None),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, FH])
+@pytest.mark.parametrize("cfg", SIXTEEN, ids=lambda c: "-".join(
+    map(str, (*c[0], "counts" if c[3] else "all"))))
+def test_as_many_new_tokens_as_a_chunk_has_keys(dtype, cfg):
+    shape, plens, lens, counts = cfg
+    check(dtype, shape, plens, lens, counts, f"branch sixteen {dtype} {cfg}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("W,D", [(1, 64), (1, 128), (3, 64), (5, 128)])
+def test_a_later_one_of_sixteen_tokens_holds_nan(dtype, W, D):
+    """Token 11's key and value and token 15's value are not finite: tokens before 11 do not
+    see them, those from 11 on give NaN."""
+    announce(f"branch sixteen NaN {dtype} {W} {D}")
+    G, N, H, plens = 2, 16, 2, [45, 0]
+    lens = [(11 * b) % 37 for b in range(G * W)]
+    x = inputs(dtype, G, W, N, H, H, D, 45, 60)
+    clean = [t.clone() for t in x]
+    k, v = x[1], x[2]
+    k[:, 11], v[:, 11], v[:, 15] = float("nan"), float("inf"), float("-inf")
+    out, _, _ = step(*x, plens, lens, 45, 60)
+    _, kcd, vcd = step(*clean, plens, lens, 45, 60)
+    want, mag = reference(*clean, kcd, vcd, plens, lens, None)
+    check_tree(out[:, :11], want[:, :11], mag[:, :11], dtype, D, 105, "before the eleventh")
+    assert torch.isnan(out[:, 11:]).all()
