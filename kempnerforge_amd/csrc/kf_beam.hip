@@ -189,7 +189,8 @@ constexpr int GRANULES = 256;
 // Workgroup (row, slice).  Exponentials are float32 instructions of the difference to the
 // thread's maximum so far, x log2 e - m log2 e in one rounding (2^-24 of it, so a term of
 // weight p is off by 2^-24 |ln p|), sums of a thread's values in 32 bits, of the threads' in
-// 64; what m log2 e was rounded by is taken back in 64 bits.  A thread's granules are
+// 64; what m log2 e was rounded by (64 at most, of logits near 2^30) is taken back in 64
+// bits.  A thread's granules are
 // counted from the row's first value, whatever its alignment (the loads may be unaligned):
 // rows of equal values have equal sums, to the last bit, and their beams' candidates are
 // equals.
@@ -244,13 +245,16 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
       mfma::settle(raw[u]);  // (kept as they are: unpacked they would take twice the registers)
     }
     const float was = ml;
-    // (of values as far out as the lowest one of the type, differences are 2^102 and more,
-    // or none: any slope gives their exponentials, and this one no infinities)
-    slope = fabsf(m) >= 0x1p126f ? 0x1p-20f : kLog2e;
-    ml = m == -INFINITY ? 0.f : m * slope;
+    // (Values of 2^30 and more lie 64 and more apart, or not at all, and so do the thread's
+    // maxima on either side of it: any slope of 1 and more gives their exponentials, and with
+    // this one the reference is exact.  A multiple of log2 e is off by half a unit of its last
+    // place, 64 below 2^30 and past what an exponential can hold soon after.)
+    const float other = fabsf(m) >= 0x1p30f ? 1.f : kLog2e;
+    ml = m == -INFINITY ? 0.f : m * other;
     // (moved by the difference of the rounded references, which the terms were taken
     // against)
-    if (old != -INFINITY && m > old) part *= fast_exp2(was - ml);
+    if (old != -INFINITY && m > old) part *= other == slope ? fast_exp2(was - ml) : 0.f;
+    slope = other;
 #pragma unroll
     for (int u = b; u < b + BATCH; ++u) {
       float f[E], x = 0.f;

@@ -3,6 +3,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -182,6 +184,91 @@ def test_logits_of_any_size(dtype):
         assert torch.equal(parents, wp) and torch.equal(tokens, wt), far
         assert ((best.double() - want).abs() <= LSE + half_ulp(want, F32)).all()
         assert n > 9 and (parents == 0).all()
+
+
+# Magnitudes of masks and of favourites that are no powers of two, which a rounded multiple of
+# log2 e is not exact for.
+FAR = [1e4, 1e7, 3e8, 1e9, 1.3e9, 3e9, 1e10, 1e12, 1e15, 1e20, 1e30, 1e37, 3e38]
+
+
+def _far_rows(dtype, V, far, kind, seed):
+    """One row a kind: few tokens allowed (most threads hold nothing else than the mask);
+    a thread's first granules masked, the others not; its last ones; the first by the type's
+    lowest value, the others by the mask but for a few."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(V, generator=g)
+    e = 16 // torch.empty((), dtype=dtype).element_size()
+    late = torch.arange(V) // (256 * 4 * e) % 2 == 1  # granules 4 .. 7 of the threads
+    few = torch.zeros(V, dtype=torch.bool)
+    few[torch.randperm(V, generator=g)[:23]] = True
+    if kind == "few":
+        x[~few] = far
+    elif kind == "first":
+        x[~late] = far
+    elif kind == "last":
+        x[late] = far
+    else:
+        x[~few] = far
+        x[~late & ~few] = torch.finfo(dtype).min
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("kind", ["few", "first", "last", "two masks"])
+@pytest.mark.parametrize("far", FAR)
+def test_masks_of_any_size(dtype, kind, far):
+    """Tokens masked by -far: those that are left are picked in order, whatever the mask,
+    and the masked ones behind them by the lowest token."""
+    announce(f"select mask {dtype} {kind} {far}")
+    V, K = 40003, 40
+    x = torch.stack([_far_rows(dtype, V, -far, kind, 10 * w) for w in range(3)])
+    s = torch.tensor([[-0.3, 0.0, -1.7]])
+    # three beams of one prompt, as many candidates as are left of one
+    check(x[None], s, 20, call(x[None], s, 20))
+    # each by itself, the masked ones among the candidates
+    best, parents, tokens = (t.cpu() for t in call(x[:, None], s.view(3, 1), K))
+    want, wp, wt = branch_ref.select(x[:, None], s.view(3, 1), K)
+    assert torch.equal(parents, wp) and torch.equal(tokens, wt)
+    assert ((best.double() - want).abs() <= LSE + half_ulp(want, F32)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("rest", [0.0, -1.0])
+def test_favourites_of_any_size(dtype, far, rest):
+    """Largest logits of +far beside ordinary ones, or among -far: all of the probability
+    lies with them, and a row of nothing else is the even distribution."""
+    announce(f"select favourites {dtype} {far} {rest}")
+    V, n = 40003, 11
+    g = torch.Generator().manual_seed(int(far) % 1000)
+    x = torch.randn(1, 3, V, generator=g) + rest * far
+    hot = torch.stack([torch.randperm(V, generator=g)[:n] for _ in range(3)])
+    x[0].scatter_(1, hot, far)
+    x[0, 2] = far
+    x = x.to(dtype)
+    for third in (7.0, 9.0):  # (behind the other two's favourites, and in front of them)
+        s = torch.tensor([[-0.25, -0.5, third]])
+        best, parents, tokens = (t.cpu() for t in call(x, s, 2 * n))
+        want, wp, wt = branch_ref.select(x, s, 2 * n)
+        assert torch.equal(parents, wp) and torch.equal(tokens, wt)
+        assert ((best.double() - want).abs() <= LSE + half_ulp(want, F32)).all()
+
+
+@pytest.mark.parametrize("at", [2.0 ** 24, -3e7, 1e8, -1.5e9, 2.0 ** 30 - 64])
+def test_sums_of_far_logits(at):
+    """Logits a few units (of their last place) about one of 2^24 to 2^30: the sums keep the
+    terms that are left.  The reference that the exponentials are taken against is rounded by
+    64 at most, so a term's argument (64 more than it is about) by 2^-18, and what takes the
+    reference's rounding back by 2^-19: 96 2^-24 of a term besides."""
+    announce(f"select far sums {at}")
+    ulp = 2.0 ** (math.frexp(at)[1] - 24)
+    g = torch.Generator().manual_seed(2)
+    x = (at + ulp * torch.randint(-5, 6, (2, 3, 9001), generator=g).double()).float()
+    s = -torch.rand(2, 3, generator=g)
+    best, parents, tokens = (t.cpu() for t in call(x, s, 6))
+    want, wp, wt = branch_ref.select(x, s, 6)
+    assert torch.equal(parents, wp) and torch.equal(tokens, wt)
+    assert ((best.double() - want).abs() <= LSE + 96 * 2.0 ** -24 + half_ulp(want, F32)).all()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
