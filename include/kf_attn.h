@@ -417,8 +417,12 @@ int kf_beam_select_workspace_size(int G, int W, int V, int K, int dtype, size_t*
  *   logits  [G, W, V], row (g, w) at g * logits_stride_g + w * logits_stride_w
  *   scores  [G, W] float32: the beams' summed log-probabilities so far
  *   out_scores [G, K] float32, parents [G, K] int32, tokens [G, K] int64: the K
- *       largest of scores[g][w] + log softmax(logits[g][w])[v], in 64 bits, largest
- *       first, equals by the lowest w, then v; rounded to out_scores; parents are the w
+ *       largest of scores[g][w] + log softmax(logits[g][w])[v], largest first, equals
+ *       by the lowest w, then v; rounded to out_scores; parents are the w
+ * The totals are formed and ordered in 64 bits.  The log of a row's sum comes from
+ * exponentials of 32 bits: it is off by at most 4e-6 (1.4e-7 measured; 1e-5 where the
+ * largest logit is beyond 2^24), so candidates of different beams that are closer than
+ * that can change places, and the last one of K with the next.
  * A score of -inf is a beam that is not in use; one that is not finite otherwise,
  * and a row that is no distribution (NaN, +inf, or -inf throughout), count as
  * such.  -inf is a token of no probability: never picked; a finite logit can be, the

@@ -190,10 +190,13 @@ constexpr int GRANULES = 256;
 // thread's maximum so far, x log2 e - m log2 e in one rounding (2^-24 of it, so a term of
 // weight p is off by 2^-24 |ln p|), sums of a thread's values in 32 bits, of the threads' in
 // 64; what m log2 e was rounded by (64 at most, of logits near 2^30) is taken back in 64
-// bits.  A thread's granules are
-// counted from the row's first value, whatever its alignment (the loads may be unaligned):
-// rows of equal values have equal sums, to the last bit, and their beams' candidates are
-// equals.
+// bits.  Of V <= 2^20 values |log2 p| is 21.5 on average at most, the instruction adds 2^-22,
+// a thread's sums 24 steps of 2^-24: a row's log-sum is off by less than 4e-6 (measured
+// 1.4e-7).  In 64 bits an exponential would take more than all else that a thread does for
+// a value.
+// A thread's granules are counted from the row's first value, whatever its alignment (the
+// loads may be unaligned): rows of equal values have equal sums, to the last bit, and their
+// beams' candidates are equals.
 template <typename T>
 __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
                                                             SliceSum* __restrict__ sums,

@@ -872,10 +872,11 @@ def beam_select_raw(logits, scores, *, select: int):
     ``logits [G,W,V]`` (contiguous values; any strides between rows) are the W beams' of
     each group, ``scores [G,W]`` float32 their summed log-probabilities.  Candidate (w,
     v) has ``scores[g,w] + log softmax(logits[g,w])[v]``; the largest come first, equals
-    by the lowest beam, then token.  A score of -inf (or none: NaN, +inf) is a beam that
-    is not in use, a logit of -inf a token that cannot be picked, and a row that is no
-    distribution (NaN, +inf, -inf throughout) has no candidates.  Behind the last
-    candidate: score -inf, parent and token -1."""
+    by the lowest beam, then token (the log of a row's sum is off by at most 4e-6, so
+    closer candidates of different beams can change places).  A score of -inf (or none:
+    NaN, +inf) is a beam that is not in use, a logit of -inf a token that cannot be
+    picked, and a row that is no distribution (NaN, +inf, -inf throughout) has no
+    candidates.  Behind the last candidate: score -inf, parent and token -1."""
     here = _here(logits)
     if here is not None:
         out = _lib.native().select(logits, scores, select, *here)

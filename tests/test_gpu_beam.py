@@ -271,6 +271,24 @@ def test_sums_of_far_logits(at):
     assert ((best.double() - want).abs() <= LSE + 96 * 2.0 ** -24 + half_ulp(want, F32)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, FH, F32])
+@pytest.mark.parametrize("V", [300, 32000, 131072, 1 << 20])
+def test_how_exact_a_rows_sum_is(dtype, V):
+    """Scores that bring the best candidate's total to zero, so that its rounding hides
+    nothing: it is off by what the log of the row's sum is, 4e-6 at most as the header says
+    (|log2 p| is 21.5 on average at most: LSE with 21.5 for 18.5 is 3.0e-6)."""
+    announce(f"select sums {dtype} {V}")
+    for spread in (0.01, 1.0, 8.0):
+        g = torch.Generator().manual_seed(V)
+        x = (spread * torch.randn(8, 1, V, generator=g)).to(dtype)
+        top = x.double().amax(-1)
+        lse = torch.logsumexp(x.double(), -1)
+        s = (lse - top).float()
+        err = (call(x, s, 1)[0].cpu().double() - (s.double() + top - lse)).abs().max().item()
+        print(f"[sums {dtype} {V} {spread}] off by {err:.2e}", flush=True)
+        assert err <= 4e-6
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("K,hot", [(16, 10), (48, 40), (100, 40), (3, 2)])
 @pytest.mark.parametrize("lead", [0, 3])
