@@ -4,7 +4,8 @@
 // Selection: of W beams with scores s_w and logits x_w over V tokens, the K largest of
 //   t_wv = s_w + x_wv - log sum_u exp x_wu,
 // equals by the lowest w, then v.  Within a beam t rises with x, so a row's K largest
-// logits are all that can be picked of it:
+// logits are all that can be picked of it, and where a beam's score leaves no bits for
+// their differences (equal t), x still has their order:
 //  1. rows   a workgroup per slice of a row: the slice's maximum and sum of
 //            exponentials, and its K largest logits
 //  2. pick   a workgroup per group: the rows' sums joined, then the K largest of the
@@ -19,7 +20,7 @@
 #include "kf_stream.h"
 
 #include <algorithm>
-#include <climits>
+#include <limits>
 #include <type_traits>
 
 namespace kf {
@@ -27,7 +28,8 @@ namespace kf {
 namespace {
 
 // ------------------------------------------------------------------ the K largest
-// of values spread over a workgroup of 256, largest first, equals by the lowest index.
+// of values spread over a workgroup of 256, largest first, equals by the lowest index (of
+// 64-bit values: the lowest key).
 //
 // The workgroup's values fall into 64 groups (lane l of the four wavefronts); the K-th
 // largest of the groups' maxima is at most the K-th largest value, and few values are
@@ -39,12 +41,13 @@ constexpr int NT = 256, CAP = 1024;
 
 template <typename V>
 struct TopLds {
+  using Index = typename std::conditional<sizeof(V) == 4, int, unsigned long long>::type;
   V top[NT];
   V val[CAP];
-  int idx[CAP];
-  int count, best;
+  Index idx[CAP], best;
+  int count;
   V edge, red[NT / 64];
-  __device__ __forceinline__ void add(V x, int i) {
+  __device__ __forceinline__ void add(V x, Index i) {
     const int at = atomicAdd(&count, 1);
     if (at < CAP) {
       val[at] = x;
@@ -104,7 +107,7 @@ template <typename V, typename Out>
 __device__ __forceinline__ void top_order(int K, int n, Out out, const TopLds<V>& lds) {
   for (int a = threadIdx.x; a < n; a += NT) {
     const V x = lds.val[a];
-    const int i = lds.idx[a];
+    const auto i = lds.idx[a];
     int place = 0;
 #pragma unroll 4
     for (int b = 0; b < n; ++b) {
@@ -119,13 +122,14 @@ __device__ __forceinline__ void top_order(int K, int n, Out out, const TopLds<V>
 // whether to go on, here always); there are K of them.
 template <typename V, typename Each, typename Out>
 __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds<V>& lds) {
+  using Index = typename TopLds<V>::Index;
   const int t = threadIdx.x;
   V last = INFINITY;
-  int after = -1;
+  Index after = 0;  // (no value is as large)
   for (int place = 0; place < K; ++place) {
     // the largest value behind (last, after), then the lowest index that has it
     V x = -INFINITY;
-    each([&](V v, int i) __attribute__((always_inline)) {
+    each([&](V v, Index i) __attribute__((always_inline)) {
       if (v < last || (v == last && i > after)) x = fmax(x, v);
       return true;
     });
@@ -133,11 +137,11 @@ __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds
     for (int o = 32; o >= 1; o >>= 1) x = fmax(x, __shfl_xor(x, o, 64));
     __syncthreads();
     if ((t & 63) == 0) lds.red[t >> 6] = x;
-    if (t == 0) lds.best = INT_MAX;
+    if (t == 0) lds.best = std::numeric_limits<Index>::max();
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) x = fmax(x, lds.red[w]);
-    each([&](V v, int i) __attribute__((always_inline)) {
+    each([&](V v, Index i) __attribute__((always_inline)) {
       if (v == x && (v < last || i > after)) atomicMin(&lds.best, i);
       return true;
     });
@@ -385,6 +389,17 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 }
 
 // ------------------------------------------------------------------ pick
+// A candidate's key: its beam, then its logit from the largest down (equal totals of
+// one beam are equal logits, or such as its score leaves no bits for), then its token.
+using Key = TopLds<double>::Index;
+constexpr int VBITS = 20;
+static_assert(KF_VERIFY_MAX_VOCAB <= 1 << VBITS && KF_BEAM_MAX <= 1 << (32 - VBITS), "a key's bits");
+__device__ __forceinline__ Key key_of(int w, float x, int v) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // (-0 and 0 are equals)
+  const uint32_t down = u >> 31 ? u : u ^ 0x7fffffffu;
+  return (Key)w << (32 + VBITS) | (Key)down << VBITS | (Key)v;
+}
+
 // A slice's candidates are a list in order.  `parts` threads take the list's places in turn
 // (more than 256 lists: a thread takes several), and leave it at the first that is below the
 // bound, so of slices x K candidates a beam little more than K in all are looked at (8 x 8
@@ -438,7 +453,7 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
     }
   }
   __syncthreads();
-  // f(value, index) for the thread's candidates, list by list, in order; f says whether to
+  // f(value, key) for the thread's candidates, list by list, in order; f says whether to
   // go on in the list.
   auto walk = [&](auto f) __attribute__((always_inline)) {
     // (in registers: a choice between the two as they are is made a choice of addresses)
@@ -458,12 +473,12 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
           const Candidate z = c[(int64_t)l * a.K + r];
           y = z.x, v = z.v;
         }
-        if (v < 0 || !f(sc + ((double)y - ls), w * a.V + v)) break;
+        if (v < 0 || !f(sc + ((double)y - ls), key_of(w, y, v))) break;
       }
     }
   };
   double own = -INFINITY;
-  walk([&](double x, int) {
+  walk([&](double x, Key) {
     own = fmax(own, x);
     return false;
   });
@@ -471,9 +486,9 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
   if (t == 0) lds.count = 0;
   __syncthreads();
   double edge = top_bound(a.K, lds);  // (each wavefront by itself: no other barrier)
-  auto gather = [&](double x, int i) {
+  auto gather = [&](double x, Key k) {
     if (x < edge) return false;
-    lds.add(x, i);
+    lds.add(x, k);
     return true;
   };
   walk(gather);
@@ -506,11 +521,10 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a,
     __syncthreads();
   }
   const int64_t at = (int64_t)g * a.K;
-  auto put = [&](int place, double x, int i) {
-    const int w = (int)((unsigned)i / (unsigned)a.V);
+  auto put = [&](int place, double x, Key k) {
     a.out_scores[at + place] = (float)x;
-    a.parents[at + place] = w;
-    a.tokens[at + place] = i - w * a.V;
+    a.parents[at + place] = (int)(k >> (32 + VBITS));
+    a.tokens[at + place] = (int64_t)(k & ((1 << VBITS) - 1));
   };
   int m = lds.count;
   if (m <= CAP) {

@@ -352,6 +352,36 @@ def test_scores_far_apart():
     assert torch.equal(tokens[0], x[1, 0].sort(descending=True, stable=True).indices[:6])
 
 
+@pytest.mark.parametrize("dtype", [BF, FH, F32])
+@pytest.mark.parametrize("score", [-1e12, -1e17, -1e30, 2e38])
+@pytest.mark.parametrize("V,K", [(300, 9), (40003, 9), (131072, 40), (40003, 128)])
+def test_scores_that_leave_no_bits_for_logits(dtype, score, V, K):
+    """Beams whose score is so far out (one that took a masked token) that 64 bits do not tell
+    their totals apart: of equal totals the lowest beam's, and of a beam the largest
+    logits, equals by the lowest token, as of any other beam."""
+    announce(f"select absorbed {dtype} {score} {V} {K}")
+    x, _ = inputs(dtype, 3, 3, V, seed=K)
+    s = torch.full((3, 3), -INF)
+    s[0, 1] = score               # one beam
+    s[1, 1:] = score              # two equal ones
+    s[2] = torch.tensor([score * 1.5, 0.0, score])  # behind (in front of) an ordinary one
+    x[2, 1, K // 2:] = -INF
+    best, parents, tokens = (t.cpu() for t in call(x, s, K))
+    order = x.double().sort(dim=-1, descending=True, stable=True).indices
+    if abs(score) >= 1e17:        # (ulp / 2 above any difference of theirs)
+        assert (parents[:2] == 1).all() and torch.equal(tokens[:2], order[:2, 1, :K])
+    n = K // 2
+    if score < 0:
+        assert (parents[2, :n] == 1).all() and torch.equal(tokens[2, :n], order[2, 1, :n])
+        assert (parents[2, n:] == 2).all() and torch.equal(tokens[2, n:], order[2, 2, :K - n])
+    else:
+        assert (parents[2] == 0).all() and torch.equal(tokens[2], order[2, 0, :K])
+    for g, w in ((0, 1), (1, 1), (1, 2)):  # each beam's own, whatever the other's
+        mine = tokens[g][parents[g] == w]
+        assert torch.equal(mine, order[g, w, :len(mine)])
+    assert torch.isfinite(best).all()
+
+
 def test_strided_logits():
     """The last token's logits of every sequence: rows apart, off 16-byte boundaries."""
     announce("select strides")
