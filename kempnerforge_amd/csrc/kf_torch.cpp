@@ -368,15 +368,18 @@ PyObject* branch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyObject* select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   int64_t K, device, stream;
-  if (nargs != 5 || !branches.select || !integer(args[2], &K) || !fits(K) ||
-      !integer(args[3], &device) || !integer(args[4], &stream))
+  if (nargs != 5 || !branches.select || !integer(args[2], &K) || !integer(args[3], &device) ||
+      !integer(args[4], &stream))
     Py_RETURN_NONE;
   const at::Tensor* x = tensor(args[0], device);
   if (!x || x->dim() != 3 || x->stride(2) != 1) Py_RETURN_NONE;
   const int64_t G = x->size(0), W = x->size(1), V = x->size(2);
   const int dt = dtype_of(*x);
   const at::Tensor* scores = tensor(args[1], device, at::kFloat, {G, W});
-  if (dt < 0 || !scores || !fits(G) || !fits(W) || !fits(V)) Py_RETURN_NONE;
+  // (what Python refuses is left to it, so that a mistake raises one exception)
+  if (dt < 0 || !scores || !fits(G) || !fits(V) || W < 1 || W > KF_BEAM_MAX || K < 1 ||
+      K > KF_BEAM_MAX_SELECT)
+    Py_RETURN_NONE;
   size_t need = 0;
   int rc = branches.select_size((int)G, (int)W, (int)V, (int)K, dt, &need);
   if (rc) return PyLong_FromLong(rc);
@@ -415,7 +418,8 @@ PyObject* reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   std::vector<void*> p;
   p.reserve(2 * n);
   if (dt < 0 || !lens || !tensor(args[3], device, at::kInt, {G, W}) || !fits(B) || !fits(G) ||
-      !fits(W) || G * W != B || !fits(k0->size(1)) || !fits(k0->size(2)) || !fits(k0->size(3)) ||
+      W > KF_BEAM_MAX || G * W != B || !fits(k0->size(1)) || !fits(k0->size(2)) ||
+      !fits(k0->size(3)) ||
       !pointers(args[0], n, device, type, k0->sizes(), p) ||
       !pointers(args[1], n, device, type, k0->sizes(), p))
     Py_RETURN_NONE;

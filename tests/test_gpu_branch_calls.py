@@ -110,3 +110,27 @@ def test_a_leaf_that_wants_gradients():
     best, _, _ = ops.beam_select_raw(new(1, 2, 9).requires_grad_(), new(1, 2, dtype=F32), select=2)
     assert not best.requires_grad
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("other", [False, True])
+def test_what_is_out_of_range_raises_the_same_whatever_the_form(other):
+    """Arguments out of their range raise ValueError where the native call meets them too
+    (``other``: tensors that only the checks in Python take)."""
+    announce(f"branch refusals of either form {other}")
+    form = (lambda t: t.t().contiguous().t()) if other else (lambda t: t)
+    scores = form(torch.zeros(2, 3, dtype=F32, device=DEV))
+    x = new(2, 3, 40)
+    for k in (0, -1, ops.BEAM_MAX_SELECT + 1, 1 << 40):
+        with pytest.raises(ValueError, match="select must lie in"):
+            ops.beam_select_raw(x, scores, select=k)
+    with pytest.raises(ValueError, match="64 beams"):
+        ops.beam_select_raw(new(2, 65, 9), form(new(2, 65, dtype=F32)), select=4)
+    with pytest.raises(ValueError, match="beams of a group"):
+        ops.beam_select_raw(new(2, 0, 9), form(new(2, 0, dtype=F32)), select=4)
+    k = new(130, 1, 4, 8)
+    k[:] = 3.0
+    with pytest.raises(ValueError, match="at most 64 beams"):
+        ops.cache_reorder_raw([k], [k.clone()], new(130, dtype=I32),
+                              form(new(2, 65, dtype=I32)))
+    torch.cuda.synchronize()
+    assert (k == 3.0).all()
