@@ -672,8 +672,8 @@ int check_branch(int G, int B, int N, int Hq, int Hkv, int D, int max_prefix, in
   KF_CHECK_ARG(max_prefix >= 0, "max_prefix must not be negative (got %d)", max_prefix);
   KF_CHECK_ARG(B <= 65535, "at most 65535 sequences (got %d)", B);
   // (a workgroup of 256 threads per four rows, fewer than 2^32 threads a launch)
-  KF_CHECK_ARG((int64_t)B * N * Hq < 1 << 26, "B * N * n_heads must be below 2^26 (%d, %d, %d)", B,
-               N, Hq);
+  KF_CHECK_ARG((int64_t)B * N * Hq <= (1 << 26) - 4,
+               "B * N * n_heads must be at most 2^26 - 4 (%d, %d, %d)", B, N, Hq);
   KF_CHECK_ARG((int64_t)max_prefix + max_len <= INT_MAX,
                "max_prefix + max_len exceeds 2^31 (%d, %d)", max_prefix, max_len);
   return KF_OK;

@@ -374,6 +374,19 @@ def test_branch_abi_refusals(change, message):
     assert re.search(message, _lib.load().kf_last_error().decode())
 
 
+@pytest.mark.parametrize("B,N,H,fits", [(2731, 8191, 3, False), (2, (1 << 25) - 1, 1, False),
+                                        (4, (1 << 24) - 1, 1, True)])
+def test_the_most_rows_a_launch_takes(B, N, H, fits):
+    """A workgroup of 256 threads per four rows, and fewer than 2^32 threads: 2^26 - 1 and
+    2^26 - 2 rows are refused before anything is written, 2^26 - 4 are not."""
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    lib, n = _lib.load(), _lib.size_out()
+    rc = lib.kf_attn_branch_workspace_size(1, B, N, H, H, 96, 9, N, 1, ctypes.byref(n))
+    assert (rc == 0) == fits
+    assert fits or "2^26" in lib.kf_last_error().decode()
+
+
 @pytest.mark.parametrize("G,W,V,K,dtype,message", [
     (0, 1, 9, 1, 1, "positive"), (65536, 1, 9, 1, 1, "65535"), (1, 65, 9, 1, 1, "beams"),
     (1, 1, 9, 129, 1, "picked"), (1, 1, (1 << 20) + 1, 1, 1, "vocabulary"), (1, 1, 9, 1, 4, "dtype"),
