@@ -309,6 +309,24 @@ def test_values_ordered_against_the_threads(dtype, K, hot, lead):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("K,hot", [(16, 10), (48, 40), (100, 40), (3, 2)])
+@pytest.mark.parametrize("lead", [0, 3])
+def test_values_of_few_threads(dtype, K, hot, lead):
+    """The same by the places that the threads take: granules counted from a row's first
+    value, whatever its alignment."""
+    announce(f"select hot threads {dtype} {K} {hot} {lead}")
+    V, e = 40000, 16 // torch.empty((), dtype=dtype).element_size()
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(1, 2, V, generator=g)
+    x = torch.where(torch.arange(V) // e % 64 < hot, x.abs() + 8, x).to(dtype)
+    s = torch.tensor([[-0.3, 0.0]])
+    buf = torch.zeros(2 * V + lead + e, dtype=dtype, device=DEV)
+    view = buf[lead:lead + 2 * V].view(1, 2, V)
+    view.copy_(x)
+    check(x, s, K, call(view, s, K))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_beams_without_candidates(dtype):
     """Beams that are not in use, rows that are no distribution, tokens of no
     probability."""
