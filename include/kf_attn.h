@@ -420,11 +420,10 @@ int kf_beam_select_workspace_size(int G, int W, int V, int K, int dtype, size_t*
  *       largest of scores[g][w] + log softmax(logits[g][w])[v], largest first, equals
  *       by the lowest w, then v; rounded to out_scores; parents are the w
  * The totals are formed and ordered in 64 bits.  The log of a row's sum comes from
- * exponentials of 32 bits: it is off by at most 4e-6 (1.4e-7 measured; 1e-5 where the
- * largest logit is beyond 2^24), so candidates of different beams that are closer than
- * that can change places, and the last one of K with the next.  Candidates of one beam
- * cannot: its larger logits come first, equals by the lowest v, also where its score
- * leaves 64 bits no difference between their totals.
+ * exponentials of 32 bits: it is off by at most 4e-6 (1.4e-7 measured), so candidates
+ * of different beams that are closer than that can change places, and the last one of
+ * K with the next.  Candidates of one beam cannot: its larger logits come first, equals
+ * by the lowest v, also where its score leaves 64 bits no difference between their totals.
  * A score of -inf is a beam that is not in use; one that is not finite otherwise,
  * and a row that is no distribution (NaN, +inf, or -inf throughout), count as
  * such.  -inf is a token of no probability: never picked; a finite logit can be, the

@@ -190,12 +190,13 @@ __device__ __forceinline__ void drop_first(u32x4& x, int k) {
 // sums.
 constexpr int GRANULES = 256;
 
-// Workgroup (row, slice).  Exponentials are float32 instructions of the difference to the
-// thread's maximum so far, x log2 e - m log2 e in one rounding (2^-24 of it, so a term of
-// weight p is off by 2^-24 |ln p|), sums of a thread's values in 32 bits, of the threads' in
-// 64; what m log2 e was rounded by (64 at most, of logits near 2^30) is taken back in 64
-// bits.  Of V <= 2^20 values |log2 p| is 21.5 on average at most, the instruction adds 2^-22,
-// a thread's sums 24 steps of 2^-24: a row's log-sum is off by less than 4e-6 (measured
+// Workgroup (row, slice).  Exponentials are float32 instructions of (x - m) log2 e, m the
+// thread's maximum so far, sums of a thread's values in 32 bits, of the threads' in 64.
+// The difference is formed first: its rounding, the product's and log2 e's are 2.25 steps
+// of 2^-24 of it, whatever x (one rounding of x log2 e - m log2 e is as fast, but is off by
+// what m log2 e was rounded by: too much for an exponential from 1e9 on, and a sum that is
+// 1 was not 1).  Of V <= 2^20 values |log2 p| is 21.5 on average at most, the instruction
+// adds 2^-22, a thread's sums 24 steps: a row's log-sum is off by less than 4e-6 (measured
 // 1.4e-7).  In 64 bits an exponential would take more than all else that a thread does for
 // a value.
 // A thread's granules are counted from the row's first value, whatever its alignment (the
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
   __shared__ TopLds<float> lds;
   __shared__ u32x4 hot[GRANULES];
   __shared__ int hot_at[GRANULES], hots;
-  __shared__ float2 parts[NT];
+  __shared__ float parts[NT];
   constexpr int E = Row<T>::E, BATCH = 4;  // granules whose maximum is taken at once
   const int g = blockIdx.x / a.W, w = blockIdx.x % a.W, t = threadIdx.x, lane = t & 63;
   if (!(fabsf(a.scores[blockIdx.x]) < INFINITY)) return;  // a beam that is not in use
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 #pragma unroll
     for (int u = 0; u < U; ++u) drop_first<T>(raw[u], v0 + u * NT * E - first(u));
   }
-  float gm[U], m = -INFINITY, ml = 0.f, part = 0.f, slope = kLog2e;
+  float gm[U], m = -INFINITY, part = 0.f;
 #pragma unroll
   for (int b = 0; b < U; b += BATCH) {
     const float old = m;
@@ -251,23 +252,14 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
       m = fmaxf(m, gm[u]);
       mfma::settle(raw[u]);  // (kept as they are: unpacked they would take twice the registers)
     }
-    const float was = ml;
-    // (Values of 2^30 and more lie 64 and more apart, or not at all, and so do the thread's
-    // maxima on either side of it: any slope of 1 and more gives their exponentials, and with
-    // this one the reference is exact.  A multiple of log2 e is off by half a unit of its last
-    // place, 64 below 2^30 and past what an exponential can hold soon after.)
-    const float other = fabsf(m) >= 0x1p30f ? 1.f : kLog2e;
-    ml = m == -INFINITY ? 0.f : m * other;
-    // (moved by the difference of the rounded references, which the terms were taken
-    // against)
-    if (old != -INFINITY && m > old) part *= other == slope ? fast_exp2(was - ml) : 0.f;
-    slope = other;
+    if (old != -INFINITY && m > old) part *= fast_exp2((old - m) * kLog2e);
+    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = b; u < b + BATCH; ++u) {
       float f[E], x = 0.f;
       Row<T>::unpack(raw[u], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x += fast_exp2(__builtin_fmaf(f[e], slope, -ml));
+      for (int e = 0; e < E; ++e) x += fast_exp2((f[e] - ref) * kLog2e);
       part += x;
       mfma::settle(raw[u]);
     }
@@ -276,7 +268,7 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
   // One wavefront finds the bound, another the sum: all four would spend on them what they
   // spend on the values.
   lds.top[t] = m;
-  parts[t] = make_float2(part, m == -INFINITY ? 0.f : __builtin_fmaf(-m, slope, ml));
+  parts[t] = part;
   if (t == 0) lds.count = hots = 0;
   __syncthreads();
   const int64_t at = (int64_t)blockIdx.x * gridDim.y + blockIdx.y;
@@ -293,11 +285,11 @@ __global__ __launch_bounds__(NT, 4) void select_rows_kernel(SelectArgs a,
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) {
       const double x = lds.top[lane + 64 * i];
-      const float2 p = parts[lane + 64 * i];
+      const float p = parts[lane + 64 * i];
       if (x == -INFINITY)
-        s += p.x != p.x ? p.x : 0.f;
+        s += p != p ? p : 0.f;
       else
-        s += (double)p.x * exp2_64((x - (double)M) * L + (double)p.y);
+        s += (double)p * exp2_64((x - (double)M) * L);
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
