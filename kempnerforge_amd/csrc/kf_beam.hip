@@ -141,10 +141,12 @@ __device__ __forceinline__ void top_one_by_one(int K, Each each, Out out, TopLds
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) x = fmax(x, lds.red[w]);
+    Index mine = std::numeric_limits<Index>::max();
     each([&](V v, Index i) __attribute__((always_inline)) {
-      if (v == x && (v < last || i > after)) atomicMin(&lds.best, i);
+      if (v == x && (v < last || i > after)) mine = min(mine, i);
       return true;
     });
+    if (mine != std::numeric_limits<Index>::max()) atomicMin(&lds.best, mine);
     __syncthreads();
     if (t == 0) out(place, x, lds.best);
     last = x;
