@@ -182,7 +182,9 @@ class BranchKVCache(KVCache):
     branch's own tokens.  A model's forward takes any number of tokens a sequence (right
     padding as with any cache: :meth:`set_lengths` afterwards); no masks, no capture, no
     trees of drafts.  Prompts of different lengths need the full RoPE tables
-    (:meth:`use_rope_tables`, taken over from ``prefix``)."""
+    (:meth:`use_rope_tables`, taken over from ``prefix``).  The kernels are made for heads of
+    64 and 128: others are served a key at a time, as a decode step over copies of the
+    prompt serves them, and many times slower."""
 
     def __init__(self, prefix: KVCache, branches: int, max_new_len: int) -> None:
         if isinstance(prefix, BranchKVCache):

@@ -11,8 +11,8 @@
 //  2. pick   a workgroup per group: the rows' sums joined, then the K largest of the
 //            W x slices x K candidates, in 64 bits
 // Every logit is read once.  HBM bounds the first (bfloat16 rows of 131072: 32 x 8 take
-// 16 to 18 us, 4 TB/s, 128 x 8 58, 4.6), two dependent launches the smallest calls (4 rows
-// of 32000: 5.5 and 5 us).
+// 17.5 us, 3.8 TB/s; 128 x 8 60 with the pick), two dependent launches the smallest calls
+// (4 rows of 32000: 5.8 and 5 us).
 #include "kf_common.h"
 #include "kf_internal.h"
 #include "kf_mfma.h"
@@ -675,7 +675,9 @@ int cache_reorder(void* const* k, void* const* v, int n_caches, const int32_t* l
       low |= (uintptr_t)p.k[c] | (uintptr_t)p.v[c];
     }
     int rc;
-    // (64 registers of 16 bytes are too many: halves of them for wide beams)
+    // (64 registers of 16 bytes are too many: halves of them for wide beams.  32 layers of 64
+    // sequences of 256 rows in groups of 8 and 16 move at 4.5 and 4.3 TB/s, in groups of 17,
+    // 32 and 64 at 2.5, 2.6 and 3.2)
     if (low % 16 == 0 && W <= 16)
       rc = reorder_launch<u32x4>(p, n, lens, parents, W, B, Hkv, Smax, bytes / 16, stream);
     else if (low % 8 == 0)
